@@ -370,15 +370,15 @@ def _plain_verify(st):
         return top + torch.log(torch.exp(y - top).sum(-1, keepdim=True))
 
     y = capped(st.logits)
-    logp = y - log_total(y)  # what is reported: the target's own log probabilities
+    z = y / (c["temperature"] or 1.0)
+    logp = z - log_total(z)  # what is reported: log probabilities of what is sampled from
     draft = st.draft_tokens.long()[at]
     row = first[:, None] + torch.where(real, slot, 0)
     if c["temperature"] == 0:
         best = y.argmax(1)
         good = real & (best[row] == draft)
     else:
-        z = y / c["temperature"]
-        p = torch.exp(z - log_total(z))
+        p = torch.exp(logp)
         if st.draft_logits is not None:
             z = capped(st.draft_logits) / c["temperature"]
             q = torch.exp(z - log_total(z))
@@ -575,7 +575,7 @@ def _exact_verify(st):
                     r = torch.cumsum(w, 0)
                     choice = int((r <= st.u_next[s].double() * r[-1]).sum())
             tokens[s, i] = t if keep else choice
-            lp[s, i] = torch.log_softmax(y, 0)[int(tokens[s, i])]
+            lp[s, i] = torch.log_softmax(y / (c["temperature"] or 1.0), 0)[int(tokens[s, i])]
             if not keep:
                 accepted[s] = i
                 break

@@ -121,7 +121,7 @@ _u64 = ctypes.c_uint64
 _sz = ctypes.c_size_t
 _i32p = ctypes.POINTER(ctypes.c_int32)
 
-# Every symbol include/g4w8a8.h and include/g4decode.h declare, with its ctypes signature
+# Every symbol the headers of include/ declare, with its ctypes signature
 # (restype, argtypes).
 SIGNATURES = {
     "g4_abi_version": (_c_int, []),
@@ -237,6 +237,17 @@ SIGNATURES = {
     "g4_decode_buffer": (_c_int, [_vp, ctypes.c_char_p, ctypes.POINTER(_vp),
                                   ctypes.POINTER(_sz)]),
     "g4_decode_set_stop": (_c_int, [_vp, _c_int]),
+    # include/g4serve.h
+    "g4_paged_prologue": (_c_int, [_vp, _vp, _c_int, _vp, _i64, _c_float, _vp, _i64, _c_float, _vp,
+                                   _i64, _c_float, _c_int, _vp, _vp, _vp, _vp, _c_int, _c_float,
+                                   _vp, _vp]),
+    "g4_kv_read": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _i64, _vp]),
+    "g4_attention_chunk": (_c_int, [_vp, _vp, _vp, _i64, _c_int, _c_float, _c_int, _vp, _sz, _vp,
+                                    _c_int, _c_float, _vp]),
+    "g4_attention_chunk_workspace_bytes": (_sz, [_vp, _vp, _c_int, _c_int]),
+    "g4_verify_drafts": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _i64, _c_float,
+                                  _c_float, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _vp]),
+    "g4_verify_workspace_bytes": (_sz, [_c_int, _c_int, _i64]),
     # include/g4ckpt.h
     "g4_st_parse": (_c_int, [_vp, _sz, _c_int, ctypes.POINTER(_vp)]),
     "g4_st_open": (_c_int, [ctypes.c_char_p, ctypes.POINTER(_vp)]),

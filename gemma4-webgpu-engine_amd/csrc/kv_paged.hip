@@ -12,8 +12,8 @@ int paged_args(const char *who, const g4_kv_pages *P, const g4_chunk *C, PagedAr
         return set_error(G4_ERR_UNSUPPORTED, "%s: head_dim %d (64, 128 and 256 are served)", who, P->head_dim);
     if (P->kv_heads <= 0 || P->num_pages <= 0)
         return set_error(G4_ERR_INVALID, "%s: %d KV heads, %d pages", who, P->kv_heads, P->num_pages);
-    if (P->page_size <= 0 || P->page_size > 4096 || (P->page_size & (P->page_size - 1)))
-        return set_error(G4_ERR_INVALID, "%s: page_size %d is not a power of two up to 4096", who, P->page_size);
+    if (P->page_size < 8 || P->page_size > 4096 || (P->page_size & (P->page_size - 1)))
+        return set_error(G4_ERR_INVALID, "%s: page_size %d is not a power of two from 8 to 4096", who, P->page_size);
     if (!P->k || !P->v) return set_error(G4_ERR_INVALID, "%s needs both page pools", who);
     if (P->kind == G4_KIND_I8 && (!P->k_scales || !P->v_scales))
         return set_error(G4_ERR_INVALID, "%s: int8 pages need their scales", who);

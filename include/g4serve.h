@@ -28,7 +28,7 @@ extern "C" {
  * [page][slot][head][dim], packed.
  * kind G4_KIND_F16: the rows are f16. kind G4_KIND_I8: int8 codes, and k_scales / v_scales hold one
  * f32 per row, [page][head][slot], packed; the row's values are code * scale.
- * head_dim 64, 128 or 256; page_size a power of two up to 4096; k and v 16-byte aligned and the
+ * head_dim 64, 128 or 256; page_size a power of two from 8 to 4096; k and v 16-byte aligned and the
  * strides multiples of 16 bytes.
  */
 typedef struct g4_kv_pages {

@@ -50,8 +50,8 @@ F32_REL = 32 * 2.0 ** -24
     ([(5, 37), (1, 16), (17, 17), (3, 100)], 8, 1, 256, 16, "i8", np.int8),
     ([(5, 37), (0, 9), (33, 64)], 6, 2, 128, 8, "i8", np.float32),
     ([(70, 70), (2, 300)], 4, 4, 64, 32, "f16", np.float16),
-    ([(9, 40), (0, 0), (1, 1)], 8, 8, 128, 1, "f16", np.float32),
-    ([(1, 2 + i) for i in range(130)], 2, 1, 64, 4, "i8", np.float16),
+    ([(9, 40), (0, 0), (1, 1)], 8, 8, 128, 1024, "f16", np.float32),
+    ([(1, 2 + i) for i in range(130)], 2, 1, 64, 8, "i8", np.float16),
 ])
 def test_prologue_norm_rope_store(gpu, lens, heads, kv_heads, dim, page, kind, x):
     b = Batch(lens, kv_heads, dim, page, kind, seed=len(lens)).upload()

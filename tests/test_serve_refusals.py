@@ -54,6 +54,7 @@ def test_cache_and_chunk_refusals(g4):
     expect(g4, lambda: gs.KVPages(*[Fake((4, 16, 2, 128), np.int8)] * 2, *[Fake((4, 16, 2), np.float32)] * 2), 1, "expected [4, 2, 16]")
     expect(g4, lambda: read(pages(shape=(4, 16, 2, 96)), chunk()), 5, "head_dim 96")
     expect(g4, lambda: read(pages(shape=(4, 24, 2, 128)), chunk()), 1, "page_size 24 is not a power of two")
+    expect(g4, lambda: read(pages(shape=(4, 4, 2, 128)), chunk(max_kv=16)), 1, "page_size 4 is not a power of two from 8")
     expect(g4, lambda: read(pages(shape=(4, 8192, 2, 128)), chunk()), 1, "page_size 8192")
     expect(g4, lambda: read(pages(), chunk(max_kv=65)), 1, "4 table pages of 16 slots do not hold max_kv 65")
     expect(g4, lambda: read(pages(), chunk(max_q=0)), 1, "max_q 0")

@@ -26,18 +26,35 @@ typedef float f16x __attribute__((ext_vector_type(16)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 
+// Division of n < 2^31 by a constant of the call, d > 1: (n * mul) >> (31 + log), log = ceil(log2 d) and
+// mul = floor(2^(31 + log) / d) + 1, which is under 2^32 and whose excess over 2^(31 + log) / d is at most
+// 1 <= 2^log / d, too little to carry n / d over a whole number. By the high word of the product, which the
+// scalar unit has too (a 64-bit product would move uniform values to the vector unit).
+struct FastDiv {
+    uint32_t d, mul;
+    int shift;
+    static FastDiv of(int d) {
+        int log = 0;
+        while ((1ll << log) < d) ++log;
+        return {(uint32_t)d, (uint32_t)(((uint64_t)1 << (31 + log)) / d + 1), log - 1};
+    }
+    __device__ __forceinline__ int div(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n, mul) >> shift); }
+    __device__ __forceinline__ int mod(int n) const { return n - div(n) * (int)d; }
+};
+
 struct AttnArgs {
     const _Float16 *q;
     int64_t q_stride;
-    int heads, group;
+    int heads;
+    FastDiv group;
     float scale2;  // scale * log2(e): scores are kept in base 2
     int window;
     void *out;
     int out_kind;
     float in_scale;
-    int splits;
-    float *part_o;   // [tile][split][kv_head][32][D]
-    float2 *part_ml; // [tile][split][kv_head][32]: maximum, sum
+    FastDiv splits;
+    float *part_o;    // [tile][split][kv_head][row of the tile][D]
+    float2 *part_ml;  // [tile][split][kv_head][row of the tile]: maximum, sum
 };
 
 constexpr int kRows = 32, kKeys = 32;
@@ -64,24 +81,26 @@ __device__ __forceinline__ h8 words_h8(uint32_t a, uint32_t b, uint32_t c, uint3
     return __builtin_bit_cast(h8, w);
 }
 
-// Eight int8 codes (two words) as f16: code + 128 in the low bits of 1024.0, less 1152.
+// An int8 code as f16 without arithmetic: the byte code + 128 zero-extended is the subnormal
+// (code + 128) 2^-24, exact, and the matrix products keep subnormals. The 128s come off outside: from the
+// scores as the accumulator's start, -128 2^-24 sum(q), and from the output by the sum of the rounded
+// weights. (Products of at most 2^8 2^8 codes' bits: f32 sums of them lose about what sums of the codes
+// alone would, the bias being three times a typical code.)
+// Eight codes, two words:
 __device__ __forceinline__ h8 codes_h8(uint32_t a, uint32_t b) {
-    const h2 bias = {(_Float16)-1152.0f, (_Float16)-1152.0f};
     a ^= 0x80808080u;
     b ^= 0x80808080u;
-    const uint32_t m = 0x64646464u;
-    return words_h8(h2_bits(bits_h2(__builtin_amdgcn_perm(m, a, 0x04010400u)) + bias),
-                    h2_bits(bits_h2(__builtin_amdgcn_perm(m, a, 0x04030402u)) + bias),
-                    h2_bits(bits_h2(__builtin_amdgcn_perm(m, b, 0x04010400u)) + bias),
-                    h2_bits(bits_h2(__builtin_amdgcn_perm(m, b, 0x04030402u)) + bias));
+    return words_h8(__builtin_amdgcn_perm(0u, a, 0x0c010c00u), __builtin_amdgcn_perm(0u, a, 0x0c030c02u),
+                    __builtin_amdgcn_perm(0u, b, 0x0c010c00u), __builtin_amdgcn_perm(0u, b, 0x0c030c02u));
 }
-
-// Code j of words a and b as a pair of f16.
+// Element j of words a and b as a pair; the codes' signs are flipped already.
 template <int J>
 __device__ __forceinline__ uint32_t code_pair(uint32_t a, uint32_t b) {
-    const h2 bias = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-    const uint32_t x = __builtin_amdgcn_perm(b, a, 0x0c000c00u | ((4 + J) << 16) | J) ^ 0x64806480u;
-    return h2_bits(bits_h2(x) + bias);
+    return __builtin_amdgcn_perm(b, a, 0x0c000c00u | ((4 + J) << 16) | J);
+}
+template <int J, int N>
+__device__ __forceinline__ uint32_t half_pair(const uint32_t (&a)[N], const uint32_t (&b)[N]) {
+    return __builtin_amdgcn_perm(b[J / 2], a[J / 2], J % 2 ? 0x07060302u : 0x05040100u);
 }
 
 // ---- which rows and keys ----------------------------------------------------------------------------
@@ -104,7 +123,7 @@ __device__ __forceinline__ int wave_scan_sum(int v) {
 }
 
 // Tile `id` of the batch: sequences in order, ceil(rows * group / per) tiles each.
-__device__ __forceinline__ Tile find_tile(const PagedArgs &A, int group, int window, int id, int per) {
+__device__ __forceinline__ Tile find_tile(const PagedArgs &A, const FastDiv &group, int window, int id, int per) {
     const int lane = threadIdx.x & 63;
     Tile T{};
     for (int base = 0; base < A.seqs; base += 64) {
@@ -112,7 +131,7 @@ __device__ __forceinline__ Tile find_tile(const PagedArgs &A, int group, int win
         SeqSpan S{0, 0, 0};
         if (base + lane < A.seqs) {
             S = seq_span(A, base + lane);
-            n = (min(S.rows, A.max_q) * group + per - 1) / per;
+            n = (min(S.rows, A.max_q) * (int)group.d + per - 1) / per;
         }
         const int end = wave_scan_sum(n);
         const unsigned long long past = __ballot(end > id);
@@ -122,10 +141,10 @@ __device__ __forceinline__ Tile find_tile(const PagedArgs &A, int group, int win
             T.S.start = __builtin_amdgcn_readlane(S.start, at);
             T.S.rows = __builtin_amdgcn_readlane(S.rows, at);
             T.S.kv = __builtin_amdgcn_readlane(S.kv, at);
-            T.rows = min(T.S.rows, A.max_q) * group;
+            T.rows = min(T.S.rows, A.max_q) * (int)group.d;
             T.first = (id - (__builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(n, at))) * per;
-            const int p0 = T.S.kv - T.S.rows + T.first / group;
-            const int p1 = T.S.kv - T.S.rows + (min(T.first + per, T.rows) - 1) / group;
+            const int p0 = T.S.kv - T.S.rows + group.div(T.first);
+            const int p1 = T.S.kv - T.S.rows + group.div(min(T.first + per, T.rows) - 1);
             T.lo = window ? max(0, p0 - window + 1) & ~(kKeys - 1) : 0;
             T.hi = max(p1 + 1, 0);
             T.live = true;
@@ -136,83 +155,86 @@ __device__ __forceinline__ Tile find_tile(const PagedArgs &A, int group, int win
     return T;
 }
 
-// Key tiles of one split: `n` key tiles cut in runs of `per`, a multiple of `unit`.
-__device__ __forceinline__ int split_tiles(const Tile &T, int splits, int unit) {
-    const int n = (T.hi - T.lo + kKeys - 1) / kKeys;
-    return max((n + splits - 1) / splits + unit - 1, unit) / unit * unit;
+// Key tiles of one split: `n` key tiles cut in runs of `per`, a multiple of `unit` (a power of two).
+__device__ __forceinline__ int split_tiles(const Tile &T, const FastDiv &splits, int unit) {
+    const int n = (unsigned)(T.hi - T.lo + kKeys - 1) / kKeys;
+    return max(splits.div(n + (int)splits.d - 1) + unit - 1, unit) & ~(unit - 1);
 }
 
-__device__ __forceinline__ void attn_put8(const AttnArgs &R, int64_t at, const float (&y)[8]) {
+__device__ __forceinline__ void attn_put4(const AttnArgs &R, int64_t at, float4 y) {
     if (R.out_kind == G4_KIND_F16) {
-        h8 o;
-#pragma unroll
-        for (int n = 0; n < 8; ++n) o[n] = (_Float16)y[n];
-        *reinterpret_cast<h8 *>(static_cast<_Float16 *>(R.out) + at) = o;
+        const h4 o = {(_Float16)y.x, (_Float16)y.y, (_Float16)y.z, (_Float16)y.w};
+        *reinterpret_cast<h4 *>(static_cast<_Float16 *>(R.out) + at) = o;
     } else if (R.out_kind == G4_KIND_I8) {
-        uint2 o{0, 0};
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            o.x |= (uint32_t)(srq_code_i(y[n], R.in_scale) & 255) << (8 * n);
-            o.y |= (uint32_t)(srq_code_i(y[n + 4], R.in_scale) & 255) << (8 * n);
-        }
-        *reinterpret_cast<uint2 *>(static_cast<int8_t *>(R.out) + at) = o;
+        const float s = R.in_scale;
+        *reinterpret_cast<uint32_t *>(static_cast<int8_t *>(R.out) + at) =
+            (srq_code_i(y.x, s) & 255) | (srq_code_i(y.y, s) & 255) << 8 | (srq_code_i(y.z, s) & 255) << 16 |
+            (uint32_t)(srq_code_i(y.w, s) & 255) << 24;
     } else {
-        float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(R.out) + at);
-        o[0] = make_float4(y[0], y[1], y[2], y[3]);
-        o[1] = make_float4(y[4], y[5], y[6], y[7]);
+        *reinterpret_cast<float4 *>(static_cast<float *>(R.out) + at) = y;
     }
 }
 
-// ---- few rows: the waves of a block split the keys -----------------------------------------------------
+// ---- the attention kernel -------------------------------------------------------------------------------
 
-constexpr int kWaves = 4;
+// The block's shape: RT row tiles (32 query rows each) x KG key groups, a wave each. Key group g takes the
+// key tiles g, g + KG, ... of the block's run; the waves of a group share its K and V tiles, which come
+// straight to LDS as the rows stand in the cache, a ring of NS tiles each.
+//  RT 1: a wave waits for its own loads only, and refills the K half of its buffer as soon as the scores
+//        are done and the V half after the output (NS 1);
+//  RT 2, 4: one block barrier per key tile, NS tiles in flight.
+template <int D, int CK, int RT>
+struct Shape {
+    static constexpr int EB = CK == G4_KIND_I8 ? 1 : 2;  // bytes of an element
+    static constexpr int RB = D * EB;                    // of a row
+    static constexpr int HALF = kKeys * RB;              // of a tile's K or V
+    static constexpr int KG = RT == 1 ? 4 : (RT == 2 && RB < 512 ? 4 : 2);
+    static constexpr int NS = RT == 1 ? 1 : 2;
+    static constexpr int WAVES = RT * KG;
+    static constexpr int RING = KG * NS * 2 * HALF;
+    // int8: the scales of a wave's tiles, ks[32] and vs[32] a tile, and one more tile ahead
+    static constexpr int SCALES = CK == G4_KIND_I8 ? WAVES * 2 * 256 : 0;
+    static constexpr int JOIN = WAVES * (D / 8) * 72 * 4;  // a quarter of every wave's output (see the end)
+    // Q's last operands wait in LDS where two waves a SIMD share the registers: output and Q alone take 192 of 256
+    static constexpr int QL = D == 256 && RT > 1 && WAVES == 8 ? 2 : 0;
+    static constexpr int LDS = (RING > JOIN ? RING : JOIN) + SCALES + WAVES * (kRows * 8 + QL * 1024);
+    static constexpr int MIN_WAVES = WAVES == 4 && LDS > 80 * 1024 ? 1 : 2;  // per SIMD: one block a CU, or two
+};
 
-template <int BYTES> struct Words { uint32_t w[BYTES / 4]; };
-template <> struct Words<2> { uint32_t w[1]; };
-
-// BYTES bytes from base + off.
-template <int BYTES>
-__device__ __forceinline__ Words<BYTES> load_words(const char *base, uint32_t off) {
-    Words<BYTES> r;
-    const char *p = base + off;
-    if constexpr (BYTES == 16) {
-        const u32x4 v = *reinterpret_cast<const u32x4 *>(p);
-        r.w[0] = v.x; r.w[1] = v.y; r.w[2] = v.z; r.w[3] = v.w;
-    } else if constexpr (BYTES == 8) {
-        const uint2 v = *reinterpret_cast<const uint2 *>(p);
-        r.w[0] = v.x; r.w[1] = v.y;
-    } else if constexpr (BYTES == 4) {
-        r.w[0] = *reinterpret_cast<const uint32_t *>(p);
-    } else {
-        r.w[0] = *reinterpret_cast<const uint16_t *>(p);
-    }
-    return r;
+// Byte of chunk x (16 bytes) of K row c of a tile: the chunk index is XORed so that a b128 read of one
+// chunk index over 8 consecutive rows hits 8 different bank groups.
+template <int RB>
+__device__ __forceinline__ int k_swizzle(int c) {
+    return RB >= 128 ? c & 7 : (c >> 2) & 1;
 }
 
-// The DPL operands (8 keys each, one per consecutive dim) of eight keys' words.
-template <int D, int CK, int J, int NB>
-__device__ __forceinline__ h8 v_operand(const Words<NB> (&x)[8]) {
-    uint32_t o[4];
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-        if constexpr (CK == G4_KIND_I8)
-            o[p] = code_pair<J % 4>(x[2 * p].w[J / 4], x[2 * p + 1].w[J / 4]);
-        else
-            o[p] = __builtin_amdgcn_perm(x[2 * p + 1].w[J / 2], x[2 * p].w[J / 2], J % 2 ? 0x07060302u : 0x05040100u);
-    }
-    return words_h8(o[0], o[1], o[2], o[3]);
+// 16 (4) bytes per active lane from base + off to LDS at lds + 16 (4) * lane; see the waits in the kernel.
+__device__ __forceinline__ void dma16(const char *base, uint32_t off, uint32_t lds) {
+    // readfirstlane gives an int: its words are unsigned before they are put together
+    const uint32_t b0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)base);
+    const uint32_t b1 = __builtin_amdgcn_readfirstlane((uint32_t)((uintptr_t)base >> 32));
+    const uint64_t b = (uint64_t)b1 << 32 | b0;
+    // 5 wait states: a scalar register that the vector unit wrote (readfirstlane), read as a base address
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(b) : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(const void *src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+                 :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src) : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() {
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
 }
 
-// The halves of a word that are NaN or infinite as f16, as a mask; and 1 in their place, 0 elsewhere.
+// The halves of a word that are NaN or infinite as f16, as a mask.
 __device__ __forceinline__ uint32_t odd_mask(uint32_t x) {
     return ((x & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((x & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
 }
-__device__ __forceinline__ h8 odd_ones(h8 x) {
-    const u32x4 w = __builtin_bit_cast(u32x4, x);
-    return words_h8(odd_mask(w.x) & 0x3c003c00u, odd_mask(w.y) & 0x3c003c00u, odd_mask(w.z) & 0x3c003c00u,
-                    odd_mask(w.w) & 0x3c003c00u);
-}
-
 template <int J, int N, typename F>
 __device__ __forceinline__ void each(F f) {
     if constexpr (J < N) {
@@ -221,347 +243,561 @@ __device__ __forceinline__ void each(F f) {
     }
 }
 
-// Grid (tiles, splits, KV heads), 4 waves: wave w takes key tiles w, w + 4, ... of the split's run. K
-// arrives as the A operand itself (a lane's own key, 16 bytes at a time), V as described above, both a
-// tile ahead of their use as registers allow.
-template <int D, int CK>
-__global__ __launch_bounds__(64 * kWaves, D == 256 ? 1 : 2) void attn_rows_kernel(PagedArgs A, AttnArgs R) {
-    constexpr int KS = D / 16, DPL = D / 32;
-    constexpr int EB = CK == G4_KIND_I8 ? 1 : 2;          // bytes per element
-    constexpr int KL = D * EB / 32;                       // 16-byte K loads of a lane
-    constexpr int VB = DPL * EB;                          // bytes of a V load
-    __shared__ __align__(16) float sc_lds[kWaves][2][kKeys];
-    __shared__ float2 ml_lds[kWaves][kRows];
-    __shared__ float o_lds[kWaves][DPL * 16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Dims of a lane's V operands: UD consecutive ones (4; 2 at head_dim 64) in each of D / (32 UD) blocks of
+// 32 UD dims, so that a half wave reads 32 UD consecutive elements of a row. Operand j = UD u + w is dims
+// 32 UD u + UD i + w over its rows i.
+template <int D> struct VDims {
+    static constexpr int UD = D == 64 ? 2 : 4, U = D / (32 * UD);
+};
+
+// The pages of a key tile's four 8-key groups, below 0 where absent. Named, not an array: an array is
+// indexed in memory, which makes its values per-lane ones.
+struct Pages {
+    int a, b, c, d;
+    __device__ __forceinline__ int of(int g) const {
+        const int lo = g & 1 ? b : a, hi = g & 1 ? d : c;
+        return g & 2 ? hi : lo;
+    }
+};
+
+typedef const __attribute__((address_space(4))) int32_t *ConstI32;  // uniform reads by the scalar unit
+
+template <int D, int CK, int RT>
+__global__ __launch_bounds__((64 * Shape<D, CK, RT>::WAVES), (Shape<D, CK, RT>::MIN_WAVES))
+void attn_kernel(PagedArgs A, AttnArgs R) {
+    using P = Shape<D, CK, RT>;
+    constexpr bool I8 = CK == G4_KIND_I8;
+    constexpr int EB = P::EB, RB = P::RB, KG = P::KG, NS = P::NS, KS = D / 16, DPL = D / 32;
+    constexpr int UD = VDims<D>::UD, U = VDims<D>::U, VB = UD * EB;   // VB: bytes of a lane's read of a V row
+    constexpr int GB = 8 * RB;                                        // bytes of an 8-key group
+    constexpr int NI = GB >= 1024 ? GB / 1024 : 1;                    // loads of a group
+    constexpr int LPR = RB / 16;                                      // lanes of a row
+    constexpr int GW = 4 / RT;                                        // groups that a wave loads
+    constexpr int LOADS = GW * NI;                                    // loads of a wave for a tile's K (or V)
+    __shared__ __align__(1024) char lds[P::LDS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rt = wave % RT, kg = wave / RT;
     const int h = lane >> 5, c = lane & 31;
     const int kvh = blockIdx.z;
-    const Tile T = find_tile(A, R.group, R.window, blockIdx.x, kRows);
+    const Tile T = find_tile(A, R.group, R.window, blockIdx.x, kRows * RT);
     if (!T.live) return;
-    const int per = split_tiles(T, R.splits, kWaves);
+    const int per = split_tiles(T, R.splits, KG);
     const int k0 = T.lo + blockIdx.y * per * kKeys, k1 = min(T.hi, k0 + per * kKeys);
     if (blockIdx.y && k0 >= T.hi) return;
+    const int rounds = (k1 - k0 + KG * kKeys - 1) / (KG * kKeys);  // 0 where there are no keys
+
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    constexpr int SC0 = P::RING > P::JOIN ? P::RING : P::JOIN, ML0 = SC0 + P::SCALES, Q0 = ML0 + P::WAVES * kRows * 8;
+    char *const scales = lds + SC0 + wave * 512;
+    float2 *const ml = reinterpret_cast<float2 *>(lds + ML0);
+
+    // the page of each 8-key group of this key group's tile t (absent: below 0), by the scalar unit
+    const ConstI32 table = (ConstI32)(uintptr_t)(A.table + T.seq * A.table_stride);
+    auto page_at = [&](int p) {
+        const int x = table[__builtin_amdgcn_readfirstlane(max(min(p, T.S.kv - 1), 0)) >> A.page_shift];
+        return (unsigned)x < (unsigned)A.num_pages ? x : -1;
+    };
+    auto pages_of = [&](int t) { return Pages{page_at(t), page_at(t + 8), page_at(t + 16), page_at(t + 24)}; };
+    const int smask = (1 << A.page_shift) - 1;
+    const int64_t load_rows = 64 / LPR * A.slot_stride * EB;  // from one load of a group to the next: 64 / LPR rows
+    auto group_base = [&](const void *pool, int t, int g, int page) {  // an absent group reads page 0
+        const int p0 = max(min(t + 8 * g, T.S.kv - 1), 0) & ~7;
+        return static_cast<const char *>(pool) + EB * ((int64_t)max(page, 0) * A.page_stride +
+               (int64_t)(p0 & smask) * A.slot_stride + (int64_t)kvh * A.head_stride);
+    };
+    // the loop recomputes what hangs on the lane alone (see `fresh`), loads' addresses among it
+    auto load_half = [&](const void *pool, bool swizzle, int t, const Pages &pg, uint32_t at, int lane) {
+        const uint32_t off_row = (uint32_t)(lane / LPR) * (uint32_t)(A.slot_stride * EB);
+#pragma unroll
+        for (int i = 0; i < GW; ++i) {
+            const int g = rt * GW + i;
+            const int page = pg.of(g);
+            const char *base = group_base(pool, t, g, page);
+            if (GB >= 1024 || lane < GB / 16)
+#pragma unroll
+                for (int n = 0; n < NI; ++n) {
+                    const int x = lane % LPR, r = n * (64 / LPR) + lane / LPR;
+                    dma16(base + n * load_rows, off_row + (swizzle ? x ^ k_swizzle<RB>(r) : x) * 16, at + g * GB + n * 1024);
+                }
+        }
+    };
+    auto load_scales = [&](int t, const Pages &pg, int slot, int lane) {  // lane c: ks (half 0) or vs of key c
+        const int c = lane & 31, h = lane >> 5;
+        const int p = max(min(t + c, T.S.kv - 1), 0);
+        const int page = pg.of(c >> 3);
+        dma4((h ? A.vs : A.ks) + scale_offset(A, max(page, 0), p, kvh), lds0 + SC0 + wave * 512 + slot * 256);
+    };
+    auto ring = [&](int slot, int half) { return (uint32_t)(((kg * NS + slot) * 2 + half) * P::HALF); };
+    auto tile_at = [&](int i) { return k0 + (i * KG + kg) * kKeys; };
 
     // this lane's query row
-    const int row = T.first + c;
-    const bool real = row < T.rows;
-    const int token = real ? row / R.group : 0, head = kvh * R.group + (real ? row % R.group : 0);
+    const int first = T.first + rt * kRows;  // of this wave
+    const int row = first + c;
+    const bool real = row < T.rows, active = first < T.rows;
+    const int token = real ? R.group.div(row) : 0, head = kvh * (int)R.group.d + (real ? R.group.mod(row) : 0);
     const int pos = real ? T.S.kv - T.S.rows + token : -1;
-    const int p_first = T.S.kv - T.S.rows + T.first / R.group;  // the tile's first row
-    const int p_last = T.hi - 1;
-    h8 q[KS];
+    const int p_first = T.S.kv - T.S.rows + R.group.div(first);  // the wave's first row, and its last
+    const int p_last = T.S.kv - T.S.rows + R.group.div(max(min(first + kRows, T.rows) - 1, 0));
+
+    Pages pg{-1, -1, -1, -1}, pg_next = pg;
+    if (rounds) {
+        pg = pages_of(tile_at(0));
+        if (I8) load_scales(tile_at(0), pg, 0, lane);
+        load_half(A.k, true, tile_at(0), pg, lds0 + ring(0, 0), lane);
+        load_half(A.v, false, tile_at(0), pg, lds0 + ring(0, 1), lane);
+        if (rounds > 1) pg_next = pages_of(tile_at(1));
+    }
+    constexpr int QL = P::QL;
+    h8 q[KS - QL];
+    char *const q_lds = lds + Q0 + wave * QL * 1024;
+    float q_sum = 0.0f;
     {
         const _Float16 *src = R.q + (int64_t)(T.S.start + token) * R.q_stride + (int64_t)head * D;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            // the k-step's 8 dims of this half, in the order that K's loads give them
-            const int at = CK == G4_KIND_I8 ? 32 * (s / 2) + 16 * h + 8 * (s % 2) : 16 * s + 8 * h;
-            q[s] = *reinterpret_cast<const h8 *>(src + at);
-            if (!real) q[s] = h8{};
+            // the k-step's 8 dims of this half, in the order that K's reads give them
+            const int at = I8 ? 32 * (s / 2) + 16 * h + 8 * (s % 2) : 16 * s + 8 * h;
+            h8 x = *reinterpret_cast<const h8 *>(src + at);
+            if (!real) x = h8{};
+            if (I8)
+#pragma unroll
+                for (int n = 0; n < 8; ++n) q_sum += (float)x[n];
+            if (s < KS - QL) q[s] = x;
+            else *reinterpret_cast<h8 *>(q_lds + (s - (KS - QL)) * 1024 + lane * 16) = x;
         }
+        if (I8) q_sum = other_half_sum(q_sum);
     }
+    const float s_init = I8 ? -q_sum * 0x1p-17f : 0.0f;  // the codes' bias, see codes_h8
 
     f16x o[DPL];
 #pragma unroll
     for (int j = 0; j < DPL; ++j) o[j] = f16x{};
-    float m = -INFINITY, l = 0.0f, vref = 0x1p-100f;  // vref: the power of two of the row's V scales
+    // vref: the power of two of the row's V scales; w_sum: the sum of the rounded weights (int8)
+    float m = -INFINITY, l = 0.0f, vref = 0x1p-100f, w_sum = 0.0f;
 
-    const int step = kWaves * kKeys;
-    int t0 = k0 + wave * kKeys;
-    auto key_pos = [&](int t) { return max(min(t + c, T.S.kv - 1), 0); };
-    auto raw_page = [&](int t) { return A.table[T.seq * A.table_stride + (key_pos(t) >> A.page_shift)]; };
-    u32x4 k[KL];
-    float ks = 1.0f, vs = 1.0f;
-    int page = 0, next_page = 0;
-    const int smask = (1 << A.page_shift) - 1;
-    auto load_k = [&](int t, int pg) {  // this lane's key of tile t (any row of the pool where it is absent)
-        const int p = key_pos(t);
-        const int64_t at = (int64_t)((unsigned)pg < (unsigned)A.num_pages ? pg : 0) * A.page_stride +
-                           (int64_t)(p & smask) * A.slot_stride + (int64_t)kvh * A.head_stride;
-        const char *src = static_cast<const char *>(A.k) + at * EB + 16 * h;
-#pragma unroll
-        for (int i = 0; i < KL; ++i) k[i] = *reinterpret_cast<const u32x4 *>(src + 32 * i);
-        if (CK == G4_KIND_I8) {
-            const int64_t sa = scale_offset(A, (unsigned)pg < (unsigned)A.num_pages ? pg : 0, p, kvh);
-            ks = A.ks[sa];
-            vs = A.vs[sa];
-        }
-    };
-    if (t0 < k1) {
-        page = raw_page(t0);
-        load_k(t0, page);
-        if (t0 + step < k1) next_page = raw_page(t0 + step);
-    }
-    for (; t0 < k1; t0 += step) {
-        // keys of the tile that exist
-        const bool there = t0 + c < T.S.kv && (unsigned)page < (unsigned)A.num_pages;
-        const uint32_t keys = (uint32_t)__ballot(there);
-        Words<VB> v[2][8];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int pg = __builtin_amdgcn_readlane(page, 8 * g);
-            const int p0 = max(min(t0 + 8 * g, T.S.kv - 1), 0) & ~7;
-            const int64_t at = (int64_t)((unsigned)pg < (unsigned)A.num_pages ? pg : 0) * A.page_stride +
-                               (int64_t)(p0 & smask) * A.slot_stride + (int64_t)kvh * A.head_stride;
-            const char *base = static_cast<const char *>(A.v) + at * EB;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                v[g / 2][(g % 2) * 4 + i] = load_words<VB>(base, (uint32_t)((4 * h + i) * A.slot_stride * EB) + c * VB);
-        }
-        f4 kss[4], vss[4];
-        if (CK == G4_KIND_I8) {
-            if (lane < kKeys) {
-                sc_lds[wave][0][c] = ks * R.scale2;
-                sc_lds[wave][1][c] = vs;
+    const int lane_ = lane;
+    for (int i = 0; i < rounds; ++i) {
+        // A fresh copy of the lane index: addresses and masks that hang on it are worked out again each time
+        // (a few instructions); kept across the loop they would not fit beside the output and Q.
+        int lane = lane_;
+        float bias0 = s_init;
+        asm volatile("" : "+v"(lane), "+v"(bias0));
+        const int h = lane >> 5, c = lane & 31;
+        const int t0 = tile_at(i), slot = NS == 1 ? 0 : i % NS;
+        // which keys of the tile exist (scalar)
+        uint32_t keys = T.S.kv - t0 >= 32 ? 0xffffffffu : (T.S.kv > t0 ? (1u << (T.S.kv - t0)) - 1 : 0u);
+        if (t0 >= k1) keys = 0;
+        keys &= (pg.a < 0 ? 0u : 0xffu) | (pg.b < 0 ? 0u : 0xff00u) | (pg.c < 0 ? 0u : 0xff0000u) | (pg.d < 0 ? 0u : 0xff000000u);
+        const bool more = i + 1 < rounds;
+        if (RT == 1) {
+            wait_loads<LOADS>();  // K and the scales are here, V may be on its way
+        } else {
+            wait_loads<0>();
+            wait_lds();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (more) {  // the other buffer was last read before the barrier
+                if (I8) load_scales(tile_at(i + 1), pg_next, (i + 1) & 1, lane);
+                load_half(A.k, true, tile_at(i + 1), pg_next, lds0 + ring((i + 1) % NS, 0), lane);
+                load_half(A.v, false, tile_at(i + 1), pg_next, lds0 + ring((i + 1) % NS, 1), lane);
             }
         }
-        f16x sacc = {};
+        const bool skip = !active || !keys || t0 > p_last || (R.window && t0 + kKeys - 1 <= p_first - R.window);
+        f16x x;
+        if (!skip) {
+            // chunk 2 n + h of the lane's row, swizzled: the chunk's low three bits, so an XOR of the address
+            const uint32_t kb = ring(slot, 0) + c * RB + (h ^ k_swizzle<RB>(c)) * 16;
+            constexpr int KC = RB / 32 < 4 ? RB / 32 : 4;
 #pragma unroll
-        for (int i = 0; i < KL; ++i) {
-            if constexpr (CK == G4_KIND_I8) {
-                sacc = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_h8(k[i].x, k[i].y), q[2 * i], sacc, 0, 0, 0);
-                sacc = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_h8(k[i].z, k[i].w), q[2 * i + 1], sacc, 0, 0, 0);
-            } else {
-                sacc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, k[i]), q[i], sacc, 0, 0, 0);
+            for (int r = 0; r < 16; ++r) x[r] = bias0;
+            auto q_at = [&](int s) {
+                return s < KS - QL ? q[s < KS - QL ? s : 0]
+                                   : *reinterpret_cast<const h8 *>(q_lds + (s - (KS - QL)) * 1024 + lane * 16);
+            };
+#pragma unroll
+            for (int n = 0; n < RB / 32; ++n) {
+                const u32x4 k = *reinterpret_cast<const u32x4 *>(lds + (kb ^ (n % KC * 32)) + n / KC * KC * 32);
+                if constexpr (I8) {
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_h8(k.x, k.y), q_at(2 * n), x, 0, 0, 0);
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_h8(k.z, k.w), q_at(2 * n + 1), x, 0, 0, 0);
+                } else {
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, k), q_at(n), x, 0, 0, 0);
+                }
             }
-        }
-        if (CK == G4_KIND_I8) {
+            const char *sc = scales + (i & 1) * 256;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                kss[g] = *reinterpret_cast<const f4 *>(&sc_lds[wave][0][8 * g + 4 * h]);
-                vss[g] = *reinterpret_cast<const f4 *>(&sc_lds[wave][1][8 * g + 4 * h]);
+                f4 ks = {};
+                if (I8) {
+                    ks = *reinterpret_cast<const f4 *>(sc + (8 * g + 4 * h) * 4) * (R.scale2 * 0x1p24f);
+                }
+#pragma unroll
+                for (int n = 0; n < 4; ++n) x[4 * g + n] *= I8 ? ks[n] : R.scale2;
             }
         }
-        if (t0 + step < k1) {
-            page = next_page;
-            load_k(t0 + step, page);
-            if (t0 + 2 * step < k1) next_page = raw_page(t0 + 2 * step);
-        }
-        float x[16];
-        const bool edge = t0 + kKeys - 1 > p_first || (R.window && t0 <= p_last - R.window);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = sacc[r] * (CK == G4_KIND_I8 ? kss[r / 4][r % 4] : R.scale2);
-        uint32_t seen = 0xffff;  // bit r: this row sees the key of register r
-        if (edge || keys != 0xffffffffu) {
-            seen = 0;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int kk = 8 * (r / 4) + 4 * h + r % 4, j = t0 + kk;
-                const bool ok = (keys >> kk & 1) && j <= pos && (!R.window || j > pos - R.window);
-                seen |= (uint32_t)ok << r;
-                x[r] = ok ? x[r] : -INFINITY;
-            }
-        }
-        float top = x[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
-        top = other_half_max(top);
-        if (__any(top > m + kLazy || (m == -INFINITY && top > -INFINITY))) {
-            const float mn = fmaxf(m, top);
-            const float a = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-            l *= a;
-#pragma unroll
-            for (int j = 0; j < DPL; ++j) o[j] *= a;
-            m = mn;
-        }
-        const float mu = m == -INFINITY ? 0.0f : m;
-        float vinv = 1.0f;
-        if (CK == G4_KIND_I8) {
-            // the largest finite scale that the row sees
-            float vtop = 0.0f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float a = fabsf(vss[r / 4][r % 4]);
-                vtop = fmaxf(vtop, (seen >> r & 1) && a < INFINITY ? a : 0.0f);
-            }
-            vtop = other_half_max(vtop);
-            if (__any(vtop > vref)) {
-                const float to = fmaxf(vref, pow2_above(vtop)), f = vref / to;
-                vref = to;
-#pragma unroll
-                for (int j = 0; j < DPL; ++j) o[j] *= f;
-            }
-            vinv = 1.0f / vref;
+        if (RT == 1 && more) {
+            wait_lds();
+            if (I8) load_scales(tile_at(i + 1), pg_next, (i + 1) & 1, lane);
+            load_half(A.k, true, tile_at(i + 1), pg_next, lds0 + ring(0, 0), lane);
         }
         h8 p[2];
-        float sum = 0.0f;
+        uint32_t seen = 0xffffffffu;  // bit 8 g + n: this row sees the key of register 4 g + n
+        bool edge = false;
+        if (!skip) {
+            edge = t0 + kKeys - 1 > p_first || (R.window && t0 <= p_last - R.window) || keys != 0xffffffffu;
+            if (edge) {
+                const int hi = pos - t0, lo = R.window ? pos - R.window - t0 : -1;  // keys lo + 1 .. hi of the tile
+                seen = hi < 0 ? 0u : (hi >= 31 ? keys : keys & ((2u << hi) - 1));
+                if (lo >= 0) seen = lo >= 31 ? 0u : seen & ~((2u << lo) - 1);
+                seen >>= 4 * h;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float e = __builtin_amdgcn_exp2f(x[r] - mu);
-            sum += e;
-            float w = e;
-            if (CK == G4_KIND_I8) {
-                w = e * (vss[r / 4][r % 4] * vinv);
-                if (!(seen >> r & 1)) w = 0.0f;  // a masked scale may be anything
-            }
-            p[r / 8][r % 8] = (_Float16)w;
-        }
-        l += sum;
-        if (CK == G4_KIND_F16 && (edge || keys != 0xffffffffu)) {
-            // absent keys hold anything: their V counts as zero. A NaN or an infinity at a key that some rows
-            // see and others do not is kept out of the product and put into the rows that see it.
-            uint32_t odd = 0;
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int kk = 8 * g + 4 * h + i;
-                    const bool ok = keys >> kk & 1;
-                    Words<VB> &y = v[g / 2][(g % 2) * 4 + i];
-#pragma unroll
-                    for (int n = 0; n < (VB + 3) / 4; ++n) {
-                        y.w[n] = ok ? y.w[n] : 0u;
-                        odd |= odd_mask(y.w[n]);
-                    }
+                for (int r = 0; r < 16; ++r) {
+                    const bool ok = seen >> (8 * (r / 4) + r % 4) & 1;
+                    x[r] = ok ? x[r] : -INFINITY;
                 }
-            if (__any(odd)) {
-                h8 one[2];
+            }
+            float top = x[0];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) one[r / 8][r % 8] = (seen >> r & 1) ? (_Float16)1.0f : (_Float16)0.0f;
-                each<0, DPL>([&](auto J) {
-                    f16x n = {};
-                    n = __builtin_amdgcn_mfma_f32_32x32x16_f16(odd_ones(v_operand<D, CK, J.value>(v[0])), one[0], n, 0, 0, 0);
-                    n = __builtin_amdgcn_mfma_f32_32x32x16_f16(odd_ones(v_operand<D, CK, J.value>(v[1])), one[1], n, 0, 0, 0);
+            for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
+            top = other_half_max(top);
+            float vtop = 0.0f;  // the largest V scale that the row sees
+            uint32_t v_scales = (i & 1) * 256 + 128 + 16 * h;
+            if (I8) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (n[r] > 0.0f) o[J.value][r] = __builtin_nanf("");
-                });
+                for (int g = 0; g < 4; ++g) {
+                    f4 y = *reinterpret_cast<const f4 *>(scales + v_scales + 32 * g);
+                    if (edge)
 #pragma unroll
-                for (int s = 0; s < 2; ++s)
+                        for (int n = 0; n < 4; ++n) y[n] = seen >> (8 * g + n) & 1 ? y[n] : 0.0f;
+                    vtop = fmaxf(vtop, fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
+                }
+                vtop = other_half_max(vtop);
+                asm volatile("" : "+v"(v_scales));  // read again below rather than kept
+            }
+            if (__any(top > m + kLazy || (m == -INFINITY && top > -INFINITY) || (I8 && vtop > vref))) {
+                const float mn = fmaxf(m, top);
+                const float a = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+                float f = a;
+                if (I8) {
+                    const float to = fmaxf(vref, pow2_above(vtop));
+                    f *= vref / to;
+                    w_sum *= f;
+                    vref = to;
+                }
+                l *= a;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
+                for (int j = 0; j < DPL; ++j) o[j] *= f;
+                m = mn;
+            }
+            const float mu = m == -INFINITY ? 0.0f : m, vinv = I8 ? 1.0f / vref : 1.0f;
 #pragma unroll
-                        for (int n = 0; n < (VB + 3) / 4; ++n) v[s][i].w[n] &= ~odd_mask(v[s][i].w[n]);
+            for (int g = 0; g < 4; ++g) {
+                f4 y = {};
+                if (I8) y = *reinterpret_cast<const f4 *>(scales + v_scales + 32 * g) * vinv;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const int r = 4 * g + n;
+                    const float e = __builtin_amdgcn_exp2f(x[r] - mu);
+                    l += e;
+                    p[r / 8][r % 8] = (_Float16)(I8 ? e * y[n] : e);
+                }
+            }
+            if (I8 && edge) {  // a masked scale may be anything, NaN included
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const int b = 8 * (k / 2) + 2 * (k % 2);  // bits of registers 2 k and 2 k + 1
+                    u32x4 w = __builtin_bit_cast(u32x4, p[k / 4]);
+                    w[k % 4] &= (seen >> b & 1 ? 0xffffu : 0u) | (seen >> b & 2 ? 0xffff0000u : 0u);
+                    p[k / 4] = __builtin_bit_cast(h8, w);
+                }
+            }
+            if (I8) {
+                const h2 one = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    w_sum = __builtin_amdgcn_fdot2(h2{p[r / 4][2 * (r % 4)], p[r / 4][2 * (r % 4) + 1]}, one, w_sum, false);
             }
         }
+        if (RT == 1) {  // V is here, the next K and scales may be on their way
+            if (more) wait_loads<LOADS + (I8 ? 1 : 0)>();
+            else wait_loads<0>();
+        }
+        if (!skip) {
+            char *const tile = lds + ring(slot, 1);
+            bool odd = false;
+            if (!I8 && edge) {
+                // Absent keys hold anything: their rows are cleared (by every wave that shares the tile, with
+                // the same zeros). Then whether the tile has a NaN or an infinity: exponent bits all ones.
+                for (uint32_t gone = ~keys; gone; gone &= gone - 1)
+                    if (lane < LPR) *reinterpret_cast<u32x4 *>(tile + (__ffs(gone) - 1) * RB + lane * 16) = u32x4{};
+                uint32_t any = 0;
+#pragma unroll 4
+                for (int n = 0; n < P::HALF / 1024; ++n) {
+                    const u32x4 y = *reinterpret_cast<const u32x4 *>(tile + n * 1024 + lane * 16);
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-            each<0, DPL>([&](auto J) {
-                o[J.value] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_operand<D, CK, J.value>(v[s]), p[s], o[J.value], 0, 0, 0);
-            });
+                    for (int w = 0; w < 4; ++w) any |= (y[w] & 0x7fff7fffu) + 0x04000400u;
+                }
+                odd = __any(any & 0x80008000u);
+            }
+            const char *vb = tile + c * VB + 4 * h * RB;
+            // the lane's dims of block u, of the 8 keys of k-step s
+            auto v_words = [&](int s, int u, uint32_t (&v)[8][(VB + 3) / 4]) {
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    const char *at = vb + (16 * s + 8 * (n / 4) + n % 4) * RB + u * 32 * VB;
+                    if constexpr (VB == 8) {
+                        const uint2 y = *reinterpret_cast<const uint2 *>(at);
+                        v[n][0] = y.x;
+                        v[n][1] = y.y;
+                    } else if constexpr (VB == 4) {
+                        v[n][0] = *reinterpret_cast<const uint32_t *>(at);
+                    } else {
+                        v[n][0] = *reinterpret_cast<const uint16_t *>(at);
+                    }
+                    if (I8) v[n][0] ^= 0x80808080u;
+                }
+            };
+            auto v_operand = [&](auto W, const uint32_t (&v)[8][(VB + 3) / 4]) {
+                constexpr int w = decltype(W)::value;
+                if constexpr (I8)
+                    return words_h8(code_pair<w>(v[0][0], v[1][0]), code_pair<w>(v[2][0], v[3][0]),
+                                    code_pair<w>(v[4][0], v[5][0]), code_pair<w>(v[6][0], v[7][0]));
+                else
+                    return words_h8(half_pair<w>(v[0], v[1]), half_pair<w>(v[2], v[3]), half_pair<w>(v[4], v[5]),
+                                    half_pair<w>(v[6], v[7]));
+            };
+            if (odd) {
+                // A NaN or an infinity at a key that some rows see and others do not is kept out of the
+                // product (below) and put into the rows that see it, a key at a time.
+#pragma unroll 1
+                for (int kk = 0; kk < kKeys; ++kk) {
+                    const int j = t0 + kk;
+                    const bool sees = (keys >> kk & 1) && j <= pos && (!R.window || j > pos - R.window);
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const int d = 32 * UD * u + UD * (8 * (r / 4) + 4 * h + r % 4);
+#pragma unroll
+                            for (int w = 0; w < UD; ++w) {
+                                const uint32_t x = *reinterpret_cast<const uint16_t *>(tile + kk * RB + (d + w) * 2);
+                                if (sees && (x & 0x7c00u) == 0x7c00u) o[u * UD + w][r] = __builtin_nanf("");
+                            }
+                            __builtin_amdgcn_sched_barrier(0);  // a few loads at a time: the registers are full
+                        }
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    uint32_t v[8][(VB + 3) / 4];
+                    v_words(s, u, v);
+                    if (odd)
+#pragma unroll
+                        for (int n = 0; n < 8; ++n)
+#pragma unroll
+                            for (int w = 0; w < (VB + 3) / 4; ++w) v[n][w] &= ~odd_mask(v[n][w]);
+                    each<0, UD>([&](auto W) {
+                        f16x &acc = o[u * UD + decltype(W)::value];
+                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_operand(W, v), p[s], acc, 0, 0, 0);
+                    });
+                }
+        }
+        pg = pg_next;
+        if (more) {
+            if (RT == 1) {
+                wait_lds();
+                load_half(A.v, false, tile_at(i + 1), pg, lds0 + ring(0, 1), lane);
+            }
+            if (i + 2 < rounds) pg_next = pages_of(tile_at(i + 2));
+        }
     }
     l = other_half_sum(l);
+    if (I8) w_sum = other_half_sum(w_sum);
 
-    // the four waves' parts: relative to the block's maximum, then each wave adds a quarter of the dims
-    if (h == 0) ml_lds[wave][c] = make_float2(m, l);
+    // The key groups' parts of a row, relative to their common maximum, summed in LDS a quarter of the
+    // registers at a time: registers 4 ph .. 4 ph + 3 of the operands of block u are dims
+    // 32 UD u + UD (8 ph + 4 h + 0..3) + 0..UD-1, 8 UD consecutive ones over both halves.
+    if (h == 0) ml[wave * kRows + c] = make_float2(m, l);
     __syncthreads();
-    float top = ml_lds[0][c].x;
+    float f;
+    {
+        float top = -INFINITY;
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = fmaxf(top, ml_lds[w][c].x);
-    const float mu = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f;
+        for (int g = 0; g < KG; ++g) top = fmaxf(top, ml[(g * RT + rt) * kRows + c].x);
+        f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
+        if (I8) f *= vref * 0x1p24f;
+    }
+    const float bias = I8 ? w_sum * 0x1p-17f : 0.0f;
+    float *const part = reinterpret_cast<float *>(lds);
+    // summing: 2 UD threads a row of 8 UD dims each (4 dims a thread), 64 / (2 UD) rows a wave and round
+    constexpr int TPR = 2 * UD, RPW = 64 / TPR;
+    const bool whole = R.splits.d == 1;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) total += ml_lds[w][c].y * __builtin_amdgcn_exp2f(ml_lds[w][c].x - mu);
-    const float f = __builtin_amdgcn_exp2f(m - mu) * (CK == G4_KIND_I8 ? vref : 1.0f);
+    for (int ph = 0; ph < 4; ++ph) {
+        if (ph) __syncthreads();
 #pragma unroll
-    for (int j = 0; j < DPL; ++j)
+        for (int j = 0; j < DPL; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o_lds[wave][j * 16 + r][lane] = o[j][r] * f;
-    __syncthreads();
-    if (!real) return;
-    const bool whole = R.splits == 1;
-    const float inv = whole ? (total == 0.0f ? 0.0f : 1.0f / total) : 1.0f;
-    const int64_t slot = (((int64_t)blockIdx.x * R.splits + blockIdx.y) * A.kv_heads + kvh) * kRows + c;
-    // register r = 4 wave + i of every operand j: dims DPL (8 wave + 4 h + i) + j, consecutive over i and j
-    float y[4 * DPL];
+            for (int n = 0; n < 4; ++n)
+                part[(wave * DPL * 4 + j * 4 + n) * 72 + lane] = (o[j][4 * ph + n] - bias) * f;
+        __syncthreads();
+        // wave kg of row tile rt: rows kg * RPW .. of each KG * RPW
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int b = 0; b < kRows / (KG * RPW > kRows ? kRows : KG * RPW); ++b) {
+            const int rr = (b * KG + kg) * RPW + lane / TPR;
+            if (rr >= kRows || first + rr >= T.rows) continue;
+            // this thread's 4 dims of a block: element e of its 8 UD is half hh, register nn, operand w
+            float y[U][4];
 #pragma unroll
-        for (int j = 0; j < DPL; ++j) {
-            float a = 0.0f;
+            for (int e = 0; e < 4; ++e) {
+                const int el = (lane % TPR) * 4 + e, hh = el / (4 * UD), nn = el / UD % 4, w = el % UD;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) a += o_lds[w][j * 16 + 4 * wave + i][lane];
-            y[i * DPL + j] = a * inv;
-        }
-    const int d0 = DPL * (8 * wave + 4 * h);
+                for (int u = 0; u < U; ++u) {
+                    float a = 0.0f;
 #pragma unroll
-    for (int b = 0; b < 4 * DPL; b += 8) {
-        const float z[8] = {y[b], y[b + 1], y[b + 2], y[b + 3], y[b + 4], y[b + 5], y[b + 6], y[b + 7]};
-        if (whole) {
-            attn_put8(R, ((int64_t)(T.S.start + token) * R.heads + head) * D + d0 + b, z);
-        } else {
-            float4 *dst = reinterpret_cast<float4 *>(R.part_o + slot * D + d0 + b);
-            dst[0] = make_float4(z[0], z[1], z[2], z[3]);
-            dst[1] = make_float4(z[4], z[5], z[6], z[7]);
+                    for (int g = 0; g < KG; ++g)
+                        a += part[((g * RT + rt) * DPL * 4 + (u * UD + w) * 4 + nn) * 72 + hh * 32 + rr];
+                    y[u][e] = a;
+                }
+            }
+            float top = -INFINITY, total = 0.0f;
+#pragma unroll
+            for (int g = 0; g < KG; ++g) top = fmaxf(top, ml[(g * RT + rt) * kRows + rr].x);
+#pragma unroll
+            for (int g = 0; g < KG; ++g) {
+                const float2 x = ml[(g * RT + rt) * kRows + rr];
+                total += x.y * __builtin_amdgcn_exp2f(x.x - (top == -INFINITY ? 0.0f : top));
+            }
+            const int64_t slot = (((int64_t)blockIdx.x * R.splits.d + blockIdx.y) * A.kv_heads + kvh) * (kRows * RT) + rt * kRows + rr;
+            const int d = 8 * UD * ph + (lane % TPR) * 4, grow = first + rr;
+            const int64_t out = ((int64_t)(T.S.start + R.group.div(grow)) * R.heads + kvh * (int)R.group.d + R.group.mod(grow)) * D;
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float4 z = make_float4(y[u][0], y[u][1], y[u][2], y[u][3]);
+                if (whole)
+                    attn_put4(R, out + 32 * UD * u + d, make_float4(z.x * inv, z.y * inv, z.z * inv, z.w * inv));
+                else
+                    *reinterpret_cast<float4 *>(R.part_o + slot * D + 32 * UD * u + d) = z;
+            }
+            if (!whole && ph == 0 && lane % TPR == 0) R.part_ml[slot] = make_float2(top, total);
         }
     }
-    if (!whole && wave == 0 && h == 0) R.part_ml[slot] = make_float2(top, total);
 }
 
 // ---- the parts of a split row joined -----------------------------------------------------------------
 
-// Grid (tiles, KV heads, 32 / rows of a block): a thread sums 8 dims of one row over the splits, in order.
-template <int D>
-__global__ __launch_bounds__(256) void attn_join_kernel(PagedArgs A, AttnArgs R, int unit) {
-    constexpr int TR = D / 8, RB = 256 / TR;  // threads of a row, rows of a block
-    const int t = threadIdx.x, c = blockIdx.z * RB + t / TR, d = (t % TR) * 8, kvh = blockIdx.y;
-    const Tile T = find_tile(A, R.group, R.window, blockIdx.x, kRows);
-    if (!T.live) return;
-    const int row = T.first + c;
-    if (c >= kRows || row >= T.rows) return;
+// Grid (tiles, row blocks, KV heads): D / 4 threads a row, G groups of them taking the splits in turn.
+template <int D, int G>
+__global__ __launch_bounds__(256) void attn_join_kernel(PagedArgs A, AttnArgs R, int tile_rows, int unit) {
+    constexpr int TR = D / 4, RBK = 256 / (TR * G);
+    __shared__ float4 os[G > 1 ? 256 : 1];
+    __shared__ float2 mls[G > 1 ? 256 : 1];
+    const int t = threadIdx.x, d = (t % TR) * 4, g = t / TR % G, kvh = blockIdx.z;
+    const int rr = blockIdx.y * RBK + t / (TR * G);
+    const Tile T = find_tile(A, R.group, R.window, blockIdx.x, tile_rows);
+    if (!T.live || T.first + (int)blockIdx.y * RBK >= T.rows) return;
+    const int row = T.first + rr;
+    const bool real = rr < tile_rows && row < T.rows;
     const int per = split_tiles(T, R.splits, unit);
-    const int n = max(1, ((T.hi - T.lo + kKeys - 1) / kKeys + per - 1) / per);
-    const int64_t stride = (int64_t)A.kv_heads * kRows;
-    const int64_t slot = ((int64_t)blockIdx.x * R.splits * A.kv_heads + kvh) * kRows + c;
-    float top = -INFINITY;
-    for (int s = 0; s < n; ++s) top = fmaxf(top, R.part_ml[slot + s * stride].x);
-    const float mu = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f, y[8] = {};
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-        const float2 ml = R.part_ml[slot + s * stride];
-        const float4 *src = reinterpret_cast<const float4 *>(R.part_o + (slot + s * stride) * D + d);
-        const float4 a = src[0], b = src[1];
-        const float f = __builtin_amdgcn_exp2f(ml.x - mu);
-        total += ml.y * f;
-        y[0] += a.x * f; y[1] += a.y * f; y[2] += a.z * f; y[3] += a.w * f;
-        y[4] += b.x * f; y[5] += b.y * f; y[6] += b.z * f; y[7] += b.w * f;
-    }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const int n = real ? max(1, ((T.hi - T.lo + kKeys - 1) / kKeys + per - 1) / per) : 0;
+    const int64_t stride = (int64_t)A.kv_heads * tile_rows;
+    const int64_t slot = ((int64_t)blockIdx.x * R.splits.d * A.kv_heads + kvh) * tile_rows + rr;
+    float m = -INFINITY, l = 0.0f;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [&](float pm, float pl, float4 a) {
+        const float mn = fmaxf(m, pm), mu = mn == -INFINITY ? 0.0f : mn;
+        const float fo = __builtin_amdgcn_exp2f(m - mu), fn = __builtin_amdgcn_exp2f(pm - mu);
+        l = l * fo + pl * fn;
+        y.x = y.x * fo + a.x * fn;
+        y.y = y.y * fo + a.y * fn;
+        y.z = y.z * fo + a.z * fn;
+        y.w = y.w * fo + a.w * fn;
+        m = mn;
+    };
+    for (int s = g; s < n; s += 4 * G) {  // four splits' loads at a time
+        float2 pm[4];
+        float4 a[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] *= inv;
-    const int token = row / R.group, head = kvh * R.group + row % R.group;
-    attn_put8(R, ((int64_t)(T.S.start + token) * R.heads + head) * D + d, y);
+        for (int i = 0; i < 4; ++i) {
+            const int64_t at = slot + min(s + i * G, n - 1) * stride;
+            pm[i] = R.part_ml[at];
+            a[i] = *reinterpret_cast<const float4 *>(R.part_o + at * D + d);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s + i * G < n) add(pm[i].x, pm[i].y, a[i]);
+    }
+    if (G > 1) {
+        os[t] = y;
+        mls[t] = make_float2(m, l);
+        __syncthreads();
+        if (g) return;
+#pragma unroll
+        for (int i = 1; i < G; ++i) add(mls[t + i * TR].x, mls[t + i * TR].y, os[t + i * TR]);
+    }
+    if (!real) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    attn_put4(R, ((int64_t)(T.S.start + R.group.div(row)) * R.heads + kvh * (int)R.group.d + R.group.mod(row)) * D + d,
+              make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
 }
 
 // ---- host ---------------------------------------------------------------------------------------------
 
 struct AttnPlan {
-    int64_t tiles;  // upper bound over the batch
-    int splits;
+    int rt;         // row tiles of a block
+    int64_t tiles;  // blocks' row ranges, an upper bound over the batch
+    int splits, key_groups;
     size_t bytes;
 };
 
-// Enough splits for two blocks a CU (one block leaves a CU idle while it joins its waves), no split
-// under one round of the block's waves.
-static AttnPlan attn_plan(const PagedArgs &A, int head_dim, int heads, int window) {
-    const int group = heads / A.kv_heads;
+static int key_groups(int rt, int row_bytes) { return rt == 1 ? 4 : (rt == 2 && row_bytes < 512 ? 4 : 2); }
+
+static AttnPlan attn_plan(const PagedArgs &A, const g4_kv_pages *pages, int heads, int window) {
+    const int group = heads / A.kv_heads, d = pages->head_dim;
     AttnPlan P;
-    const int64_t per_seq = ((int64_t)A.max_q * group + kRows - 1) / kRows;
-    P.tiles = std::min(per_seq * A.seqs, (int64_t)A.tokens * group / kRows + A.seqs);
+    const int64_t most = (int64_t)A.max_q * group;  // rows of a sequence
+    P.rt = most <= kRows ? 1 : (most <= 2 * kRows ? 2 : 4);
+    P.key_groups = key_groups(P.rt, pages->kind == G4_KIND_I8 ? d : 2 * d);
+    const int rows = kRows * P.rt;
+    P.tiles = std::min((most + rows - 1) / rows * A.seqs, (int64_t)A.tokens * group / rows + A.seqs);
     int64_t keys = A.max_kv;
-    if (window) keys = std::min<int64_t>(keys, (int64_t)window + kKeys + kRows / group + 1);
-    const int64_t rounds = (keys + kWaves * kKeys - 1) / (kWaves * kKeys);
-    const int64_t want = 2 * (int64_t)device_cu_count();
+    if (window) keys = std::min<int64_t>(keys, (int64_t)window + kKeys + rows / group + 1);
+    const int64_t rounds = (keys + P.key_groups * kKeys - 1) / (P.key_groups * kKeys);
+    const int64_t want = (P.rt == 1 ? 2 : 1) * (int64_t)device_cu_count();
     const int64_t blocks = P.tiles * A.kv_heads;
     P.splits = (int)std::max<int64_t>(1, std::min<int64_t>({rounds, (want + blocks - 1) / blocks, 64}));
-    const int64_t slots = P.tiles * P.splits * A.kv_heads * kRows;
-    P.bytes = P.splits == 1 ? 16 : (size_t)slots * (head_dim * sizeof(float) + sizeof(float2));
+    const int64_t slots = P.tiles * P.splits * A.kv_heads * rows;
+    P.bytes = P.splits == 1 ? 16 : (size_t)slots * (d * sizeof(float) + sizeof(float2));
     return P;
 }
 
-template <int D>
-static int launch_attn(const PagedArgs &A, const AttnArgs &R, const AttnPlan &P, int ck, hipStream_t stream) {
-    const dim3 grid((unsigned)P.tiles, P.splits, A.kv_heads);
-    if (ck == G4_KIND_F16)
-        hipLaunchKernelGGL((attn_rows_kernel<D, G4_KIND_F16>), grid, dim3(64 * kWaves), 0, stream, A, R);
-    else
-        hipLaunchKernelGGL((attn_rows_kernel<D, G4_KIND_I8>), grid, dim3(64 * kWaves), 0, stream, A, R);
-    G4_LAUNCHED("attn_rows_kernel");
+template <int D, int CK, int RT>
+static void launch_rows(const PagedArgs &A, const AttnArgs &R, const AttnPlan &P, hipStream_t stream) {
+    static_assert(Shape<D, CK, RT>::LDS <= 160 * 1024, "LDS of a CU");
+    hipLaunchKernelGGL((attn_kernel<D, CK, RT>), dim3((unsigned)P.tiles, P.splits, A.kv_heads),
+                       dim3(64 * Shape<D, CK, RT>::WAVES), 0, stream, A, R);
+}
+
+template <int D, int CK>
+static int launch_attn(const PagedArgs &A, const AttnArgs &R, const AttnPlan &P, hipStream_t stream) {
+    if (P.rt == 1) launch_rows<D, CK, 1>(A, R, P, stream);
+    else if (P.rt == 2) launch_rows<D, CK, 2>(A, R, P, stream);
+    else launch_rows<D, CK, 4>(A, R, P, stream);
+    G4_LAUNCHED("attn_kernel");
     if (P.splits > 1) {
-        constexpr int rb = 256 / (D / 8);
-        hipLaunchKernelGGL(attn_join_kernel<D>, dim3((unsigned)P.tiles, A.kv_heads, (kRows + rb - 1) / rb), dim3(256), 0,
-                           stream, A, R, kWaves);
+        const int rows = kRows * P.rt;
+        if (P.splits >= 8) {
+            constexpr int rb = 256 / (D / 4 * 4);
+            hipLaunchKernelGGL((attn_join_kernel<D, 4>), dim3((unsigned)P.tiles, rows / rb, A.kv_heads), dim3(256), 0,
+                               stream, A, R, rows, P.key_groups);
+        } else {
+            constexpr int rb = 256 / (D / 4);
+            hipLaunchKernelGGL((attn_join_kernel<D, 1>), dim3((unsigned)P.tiles, rows / rb, A.kv_heads), dim3(256), 0,
+                               stream, A, R, rows, P.key_groups);
+        }
         G4_LAUNCHED("attn_join_kernel");
     }
     return G4_OK;
@@ -589,7 +825,7 @@ size_t g4_attention_chunk_workspace_bytes(const g4_kv_pages *pages, const g4_chu
                                           int window) {
     PagedArgs A;
     if (attn_check(pages, chunk, heads, window, &A)) return 0;
-    return attn_plan(A, pages->head_dim, heads, window).bytes;
+    return attn_plan(A, pages, heads, window).bytes;
 }
 
 int g4_attention_chunk(const g4_kv_pages *pages, const g4_chunk *chunk, const void *q, int64_t q_stride,
@@ -607,16 +843,20 @@ int g4_attention_chunk(const g4_kv_pages *pages, const g4_chunk *chunk, const vo
         return set_error(G4_ERR_INVALID, "attention-chunk: q_stride must hold a row and be a multiple of 8");
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15)
         return set_error(G4_ERR_INVALID, "attention-chunk: q, the output and the workspace must be 16-byte aligned");
-    const AttnPlan P = attn_plan(A, pages->head_dim, heads, window);
+    const AttnPlan P = attn_plan(A, pages, heads, window);
     if (workspace_bytes < P.bytes)
         return set_error(G4_ERR_INVALID, "attention-chunk: workspace %zu B < %zu B", workspace_bytes, P.bytes);
     float *part_o = static_cast<float *>(workspace);
-    const AttnArgs R{static_cast<const _Float16 *>(q), q_stride ? q_stride : qw, heads, heads / A.kv_heads,
-                     scale * 1.44269504088896340736f, window, out, out_kind, in_scale, P.splits, part_o,
-                     reinterpret_cast<float2 *>(part_o + P.tiles * P.splits * A.kv_heads * kRows * pages->head_dim)};
-    if (pages->head_dim == 64) return launch_attn<64>(A, R, P, pages->kind, as_stream(stream));
-    if (pages->head_dim == 128) return launch_attn<128>(A, R, P, pages->kind, as_stream(stream));
-    return launch_attn<256>(A, R, P, pages->kind, as_stream(stream));
+    const AttnArgs R{static_cast<const _Float16 *>(q), q_stride ? q_stride : qw, heads,
+                     FastDiv::of(heads / A.kv_heads),                     scale * 1.44269504088896340736f, window, out, out_kind, in_scale, FastDiv::of(P.splits), part_o,
+                     reinterpret_cast<float2 *>(part_o + P.tiles * P.splits * A.kv_heads * kRows * P.rt * pages->head_dim)};
+    const bool i8 = pages->kind == G4_KIND_I8;
+    hipStream_t st = as_stream(stream);
+    switch (pages->head_dim) {
+        case 64: return i8 ? launch_attn<64, G4_KIND_I8>(A, R, P, st) : launch_attn<64, G4_KIND_F16>(A, R, P, st);
+        case 128: return i8 ? launch_attn<128, G4_KIND_I8>(A, R, P, st) : launch_attn<128, G4_KIND_F16>(A, R, P, st);
+        default: return i8 ? launch_attn<256, G4_KIND_I8>(A, R, P, st) : launch_attn<256, G4_KIND_F16>(A, R, P, st);
+    }
 }
 
 }  // extern "C"

@@ -13,9 +13,11 @@
 //    DPL i + j. No LDS transposes anything.
 // The softmax keeps a running maximum (base 2) and sum in f32; the maximum moves, and the output is
 // rescaled, only when a score passes it by more than 2^8, so weights reach 2^8 at most and are rounded to
-// f16 (11 bits; the sum adds them unrounded). int8 rows: codes are exact in f16; K's scale multiplies the
+// f16 (11 bits; an f16 cache's sum adds the rounded ones, an int8 cache's the exact ones, whose weights
+// are rounded with V's scale in them). int8 rows: codes are exact in f16; K's scale multiplies the
 // score, V's the weight, taken relative to a power of two above the largest scale that the row has seen,
-// which scales the row's output (f16 would not hold scales of every size).
+// which scales the row's output and sum (f16 would not hold scales of every size) and enters the weights
+// by their exponent.
 #include "g4_paged.h"
 #include <algorithm>
 #include <cmath>
@@ -47,7 +49,11 @@ struct AttnArgs {
     int64_t q_stride;
     int heads;
     FastDiv group;
-    float scale2;  // scale * log2(e): scores are kept in base 2
+    // Scores are kept as the products give them; the base-2 exponent is score * scale2, scale2 > 0. A
+    // negative scale turns Q's signs over; lazy is kLazy / scale2.
+    float scale2, lazy;
+    uint32_t q_sign;  // 0x80008000: Q is turned over
+    uint32_t page_bytes, slot_bytes;
     int window;
     void *out;
     int out_kind;
@@ -69,9 +75,20 @@ __device__ __forceinline__ float other_half_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// The next power of two above a scale (2^120 and more: 2^121).
+// The next power of two above a scale (2^99 and more: 2^100), and a power of two's exponent.
 __device__ __forceinline__ float pow2_above(float v) {
-    return __uint_as_float((__float_as_uint(fminf(v, 0x1p120f)) & 0x7f800000u) + 0x00800000u);
+    return __uint_as_float((__float_as_uint(fminf(v, 0x1p99f)) & 0x7f800000u) + 0x00800000u);
+}
+__device__ __forceinline__ float pow2_log(float v) { return (float)((int)(__float_as_uint(v) >> 23) - 127); }
+
+// The maximum over lanes 0..31, with lanes 32..63 holding the same values.
+__device__ __forceinline__ float half_max(float v) {
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, false)));   // lane ^ 1
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, false)));   // ^ 2
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, false)));  // 7 -
+    v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, false)));  // 15 -
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 __device__ __forceinline__ h2 bits_h2(uint32_t x) { return __builtin_bit_cast(h2, x); }
@@ -196,7 +213,8 @@ struct Shape {
     static constexpr int SCALES = CK == G4_KIND_I8 ? WAVES * 2 * 256 : 0;
     static constexpr int JOIN = WAVES * (D / 8) * 72 * 4;  // a quarter of every wave's output (see the end)
     // Q's last operands wait in LDS where two waves a SIMD share the registers: output and Q alone take 192 of 256
-    static constexpr int QL = D == 256 && RT > 1 && WAVES == 8 ? 2 : 0;
+    static constexpr int QL = D != 256 ? 0 : (WAVES == 8 ? 3 : (RT == 1 && CK == G4_KIND_I8 ? 3 : 0));
+    static constexpr bool TIGHT = D == 256 && CK == G4_KIND_F16 && WAVES == 8;  // no registers for V's reads ahead
     static constexpr int LDS = (RING > JOIN ? RING : JOIN) + SCALES + WAVES * (kRows * 8 + QL * 1024);
     static constexpr int MIN_WAVES = WAVES == 4 && LDS > 80 * 1024 ? 1 : 2;  // per SIMD: one block a CU, or two
 };
@@ -293,21 +311,23 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
 
     // the page of each 8-key group of this key group's tile t (absent: below 0), by the scalar unit
     const ConstI32 table = (ConstI32)(uintptr_t)(A.table + T.seq * A.table_stride);
+    const int last = T.S.kv - 1;  // >= 0 where there are rounds
     auto page_at = [&](int p) {
-        const int x = table[__builtin_amdgcn_readfirstlane(max(min(p, T.S.kv - 1), 0)) >> A.page_shift];
+        const int x = table[min(p, max(last, 0)) >> A.page_shift];
         return (unsigned)x < (unsigned)A.num_pages ? x : -1;
     };
     auto pages_of = [&](int t) { return Pages{page_at(t), page_at(t + 8), page_at(t + 16), page_at(t + 24)}; };
     const int smask = (1 << A.page_shift) - 1;
-    const int64_t load_rows = 64 / LPR * A.slot_stride * EB;  // from one load of a group to the next: 64 / LPR rows
-    auto group_base = [&](const void *pool, int t, int g, int page) {  // an absent group reads page 0
-        const int p0 = max(min(t + 8 * g, T.S.kv - 1), 0) & ~7;
-        return static_cast<const char *>(pool) + EB * ((int64_t)max(page, 0) * A.page_stride +
-               (int64_t)(p0 & smask) * A.slot_stride + (int64_t)kvh * A.head_stride);
+    const char *const k_pool = static_cast<const char *>(A.k) + (int64_t)kvh * A.head_stride * EB;
+    const char *const v_pool = static_cast<const char *>(A.v) + (int64_t)kvh * A.head_stride * EB;
+    const uint32_t load_rows = 64 / LPR * R.slot_bytes;  // from one load of a group to the next: 64 / LPR rows
+    auto group_base = [&](const char *pool, int t, int g, int page) {  // an absent group reads page 0
+        const int slot = min(t + 8 * g, max(last, 0)) & smask & ~7;
+        return pool + ((uint64_t)(uint32_t)max(page, 0) * R.page_bytes + (uint32_t)slot * R.slot_bytes);
     };
     // the loop recomputes what hangs on the lane alone (see `fresh`), loads' addresses among it
-    auto load_half = [&](const void *pool, bool swizzle, int t, const Pages &pg, uint32_t at, int lane) {
-        const uint32_t off_row = (uint32_t)(lane / LPR) * (uint32_t)(A.slot_stride * EB);
+    auto load_half = [&](const char *pool, bool swizzle, int t, const Pages &pg, uint32_t at, int lane) {
+        const uint32_t off_row = (uint32_t)(lane / LPR) * R.slot_bytes;
 #pragma unroll
         for (int i = 0; i < GW; ++i) {
             const int g = rt * GW + i;
@@ -323,7 +343,7 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
     };
     auto load_scales = [&](int t, const Pages &pg, int slot, int lane) {  // lane c: ks (half 0) or vs of key c
         const int c = lane & 31, h = lane >> 5;
-        const int p = max(min(t + c, T.S.kv - 1), 0);
+        const int p = min(t + c, max(last, 0));
         const int page = pg.of(c >> 3);
         dma4((h ? A.vs : A.ks) + scale_offset(A, max(page, 0), p, kvh), lds0 + SC0 + wave * 512 + slot * 256);
     };
@@ -343,8 +363,8 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
     if (rounds) {
         pg = pages_of(tile_at(0));
         if (I8) load_scales(tile_at(0), pg, 0, lane);
-        load_half(A.k, true, tile_at(0), pg, lds0 + ring(0, 0), lane);
-        load_half(A.v, false, tile_at(0), pg, lds0 + ring(0, 1), lane);
+        load_half(k_pool, true, tile_at(0), pg, lds0 + ring(0, 0), lane);
+        load_half(v_pool, false, tile_at(0), pg, lds0 + ring(0, 1), lane);
         if (rounds > 1) pg_next = pages_of(tile_at(1));
     }
     constexpr int QL = P::QL;
@@ -358,7 +378,11 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
             // the k-step's 8 dims of this half, in the order that K's reads give them
             const int at = I8 ? 32 * (s / 2) + 16 * h + 8 * (s % 2) : 16 * s + 8 * h;
             h8 x = *reinterpret_cast<const h8 *>(src + at);
-            if (!real) x = h8{};
+            const uint32_t sign = R.q_sign;
+            u32x4 y = __builtin_bit_cast(u32x4, x);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) y[n] = real ? y[n] ^ sign : 0u;
+            x = __builtin_bit_cast(h8, y);
             if (I8)
 #pragma unroll
                 for (int n = 0; n < 8; ++n) q_sum += (float)x[n];
@@ -373,7 +397,8 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
 #pragma unroll
     for (int j = 0; j < DPL; ++j) o[j] = f16x{};
     // vref: the power of two of the row's V scales; w_sum: the sum of the rounded weights (int8)
-    float m = -INFINITY, l = 0.0f, vref = 0x1p-100f, w_sum = 0.0f;
+    // off: the exponents' offset, -m scale2 - log2(vref); l is in units of vref too
+    float m = -INFINITY, l = 0.0f, vref = 0x1p-100f, w_sum = 0.0f, off = I8 ? 100.0f : 0.0f;
 
     const int lane_ = lane;
     for (int i = 0; i < rounds; ++i) {
@@ -398,8 +423,8 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
             asm volatile("" ::: "memory");
             if (more) {  // the other buffer was last read before the barrier
                 if (I8) load_scales(tile_at(i + 1), pg_next, (i + 1) & 1, lane);
-                load_half(A.k, true, tile_at(i + 1), pg_next, lds0 + ring((i + 1) % NS, 0), lane);
-                load_half(A.v, false, tile_at(i + 1), pg_next, lds0 + ring((i + 1) % NS, 1), lane);
+                load_half(k_pool, true, tile_at(i + 1), pg_next, lds0 + ring((i + 1) % NS, 0), lane);
+                load_half(v_pool, false, tile_at(i + 1), pg_next, lds0 + ring((i + 1) % NS, 1), lane);
             }
         }
         const bool skip = !active || !keys || t0 > p_last || (R.window && t0 + kKeys - 1 <= p_first - R.window);
@@ -410,35 +435,45 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
             constexpr int KC = RB / 32 < 4 ? RB / 32 : 4;
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = bias0;
-            auto q_at = [&](int s) {
-                return s < KS - QL ? q[s < KS - QL ? s : 0]
-                                   : *reinterpret_cast<const h8 *>(q_lds + (s - (KS - QL)) * 1024 + lane * 16);
+            // K's reads run two products ahead (and no further: the scheduling barriers keep the compiler from
+            // either gathering them, for which there are no registers, or waiting for each)
+            constexpr int NK = RB / 32, AHEAD = 2;
+            u32x4 k[NK];
+            h8 q_last[QL > 0 ? QL : 1];
+            auto read_k = [&](int n) {
+                k[n] = *reinterpret_cast<const u32x4 *>(lds + (kb ^ (n % KC * 32)) + n / KC * KC * 32);
             };
 #pragma unroll
-            for (int n = 0; n < RB / 32; ++n) {
-                const u32x4 k = *reinterpret_cast<const u32x4 *>(lds + (kb ^ (n % KC * 32)) + n / KC * KC * 32);
+            for (int n = 0; n < AHEAD && n < NK; ++n) read_k(n);
+            f4 ks[4];
+#pragma unroll
+            for (int n = 0; n < NK; ++n) {
+                if (n + AHEAD < NK) read_k(n + AHEAD);
+                if (QL && n == (KS - QL) / (I8 ? 2 : 1) - 1)  // a step before the first that needs one
+#pragma unroll
+                    for (int s = 0; s < QL; ++s) q_last[s] = *reinterpret_cast<const h8 *>(q_lds + s * 1024 + lane * 16);
+                if (I8 && n + 1 == NK)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        ks[g] = *reinterpret_cast<const f4 *>(scales + (i & 1) * 256 + (8 * g + 4 * h) * 4);
+                __builtin_amdgcn_sched_barrier(0);
+                auto q_at = [&](int s) { return s < KS - QL ? q[s < KS - QL ? s : 0] : q_last[s < KS - QL ? 0 : s - (KS - QL)]; };
                 if constexpr (I8) {
-                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_h8(k.x, k.y), q_at(2 * n), x, 0, 0, 0);
-                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_h8(k.z, k.w), q_at(2 * n + 1), x, 0, 0, 0);
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_h8(k[n].x, k[n].y), q_at(2 * n), x, 0, 0, 0);
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_h8(k[n].z, k[n].w), q_at(2 * n + 1), x, 0, 0, 0);
                 } else {
-                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, k), q_at(n), x, 0, 0, 0);
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, k[n]), q_at(n), x, 0, 0, 0);
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            const char *sc = scales + (i & 1) * 256;
+            if (I8)
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                f4 ks = {};
-                if (I8) {
-                    ks = *reinterpret_cast<const f4 *>(sc + (8 * g + 4 * h) * 4) * (R.scale2 * 0x1p24f);
-                }
-#pragma unroll
-                for (int n = 0; n < 4; ++n) x[4 * g + n] *= I8 ? ks[n] : R.scale2;
-            }
+                for (int r = 0; r < 16; ++r) x[r] *= ks[r / 4][r % 4];
         }
         if (RT == 1 && more) {
             wait_lds();
             if (I8) load_scales(tile_at(i + 1), pg_next, (i + 1) & 1, lane);
-            load_half(A.k, true, tile_at(i + 1), pg_next, lds0 + ring(0, 0), lane);
+            load_half(k_pool, true, tile_at(i + 1), pg_next, lds0 + ring(0, 0), lane);
         }
         h8 p[2];
         uint32_t seen = 0xffffffffu;  // bit 8 g + n: this row sees the key of register 4 g + n
@@ -463,42 +498,43 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
             float vtop = 0.0f;  // the largest V scale that the row sees
             uint32_t v_scales = (i & 1) * 256 + 128 + 16 * h;
             if (I8) {
+                if (edge) {
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    f4 y = *reinterpret_cast<const f4 *>(scales + v_scales + 32 * g);
-                    if (edge)
+                    for (int g = 0; g < 4; ++g) {
+                        const f4 y = *reinterpret_cast<const f4 *>(scales + v_scales + 32 * g);
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) y[n] = seen >> (8 * g + n) & 1 ? y[n] : 0.0f;
-                    vtop = fmaxf(vtop, fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))));
+                        for (int n = 0; n < 4; ++n) vtop = fmaxf(vtop, seen >> (8 * g + n) & 1 ? fabsf(y[n]) : 0.0f);
+                    }
+                    vtop = other_half_max(vtop);
+                } else {  // every key: a lane each
+                    vtop = half_max(fabsf(*reinterpret_cast<const float *>(scales + (i & 1) * 256 + 128 + 4 * c)));
                 }
-                vtop = other_half_max(vtop);
                 asm volatile("" : "+v"(v_scales));  // read again below rather than kept
             }
-            if (__any(top > m + kLazy || (m == -INFINITY && top > -INFINITY) || (I8 && vtop > vref))) {
+            if (__any(top > m + R.lazy || (m == -INFINITY && top > -INFINITY) || (I8 && vtop > vref))) {
                 const float mn = fmaxf(m, top);
-                const float a = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-                float f = a;
+                float f = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * R.scale2);
                 if (I8) {
                     const float to = fmaxf(vref, pow2_above(vtop));
                     f *= vref / to;
                     w_sum *= f;
                     vref = to;
                 }
-                l *= a;
+                l *= f;
 #pragma unroll
                 for (int j = 0; j < DPL; ++j) o[j] *= f;
                 m = mn;
+                off = (m == -INFINITY ? 0.0f : -m * R.scale2) - (I8 ? pow2_log(vref) : 0.0f);
             }
-            const float mu = m == -INFINITY ? 0.0f : m, vinv = I8 ? 1.0f / vref : 1.0f;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 f4 y = {};
-                if (I8) y = *reinterpret_cast<const f4 *>(scales + v_scales + 32 * g) * vinv;
+                if (I8) y = *reinterpret_cast<const f4 *>(scales + v_scales + 32 * g);
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
                     const int r = 4 * g + n;
-                    const float e = __builtin_amdgcn_exp2f(x[r] - mu);
-                    l += e;
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], R.scale2, off));
+                    if (I8) l += e;
                     p[r / 8][r % 8] = (_Float16)(I8 ? e * y[n] : e);
                 }
             }
@@ -511,12 +547,12 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
                     p[k / 4] = __builtin_bit_cast(h8, w);
                 }
             }
-            if (I8) {
-                const h2 one = {(_Float16)1.0f, (_Float16)1.0f};
+            // the sum of the rounded weights: the row's sum (f16), or what takes the codes' bias off (int8)
+            const h2 one = {(_Float16)1.0f, (_Float16)1.0f};
+            float &sum = I8 ? w_sum : l;
 #pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    w_sum = __builtin_amdgcn_fdot2(h2{p[r / 4][2 * (r % 4)], p[r / 4][2 * (r % 4) + 1]}, one, w_sum, false);
-            }
+            for (int r = 0; r < 8; ++r)
+                sum = __builtin_amdgcn_fdot2(h2{p[r / 4][2 * (r % 4)], p[r / 4][2 * (r % 4) + 1]}, one, sum, false);
         }
         if (RT == 1) {  // V is here, the next K and scales may be on their way
             if (more) wait_loads<LOADS + (I8 ? 1 : 0)>();
@@ -587,34 +623,40 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
                         }
                 }
             }
+            uint32_t v[2 * U + 1][8][(VB + 3) / 4];  // V's reads, one step ahead
+            if (!P::TIGHT) v_words(0, 0, v[0]);
+            each<0, 2 * U>([&](auto Step) {
+                constexpr int step = decltype(Step)::value, ss = step / U, u = step % U;
+                constexpr int next = P::TIGHT ? step : step + 1;
+                if (next < 2 * U) v_words(next / U, next % U, v[next]);
+                __builtin_amdgcn_sched_barrier(0);
+                if (odd)
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+                    for (int n = 0; n < 8; ++n)
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    uint32_t v[8][(VB + 3) / 4];
-                    v_words(s, u, v);
-                    if (odd)
-#pragma unroll
-                        for (int n = 0; n < 8; ++n)
-#pragma unroll
-                            for (int w = 0; w < (VB + 3) / 4; ++w) v[n][w] &= ~odd_mask(v[n][w]);
-                    each<0, UD>([&](auto W) {
-                        f16x &acc = o[u * UD + decltype(W)::value];
-                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_operand(W, v), p[s], acc, 0, 0, 0);
-                    });
-                }
+                        for (int w = 0; w < (VB + 3) / 4; ++w) v[step][n][w] &= ~odd_mask(v[step][n][w]);
+                each<0, UD>([&](auto W) {
+                    f16x &acc = o[u * UD + decltype(W)::value];
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_operand(W, v[step]), p[ss], acc, 0, 0, 0);
+                });
+                __builtin_amdgcn_sched_barrier(0);
+            });
         }
         pg = pg_next;
         if (more) {
             if (RT == 1) {
                 wait_lds();
-                load_half(A.v, false, tile_at(i + 1), pg, lds0 + ring(0, 1), lane);
+                load_half(v_pool, false, tile_at(i + 1), pg, lds0 + ring(0, 1), lane);
             }
             if (i + 2 < rounds) pg_next = pages_of(tile_at(i + 2));
         }
     }
     l = other_half_sum(l);
-    if (I8) w_sum = other_half_sum(w_sum);
+    if (I8) {
+        w_sum = other_half_sum(w_sum);
+        l *= vref;
+    }
+    m *= R.scale2;  // from here on in exponents
 
     // The key groups' parts of a row, relative to their common maximum, summed in LDS a quarter of the
     // registers at a time: registers 4 ph .. 4 ph + 3 of the operands of block u are dims
@@ -810,8 +852,8 @@ static int attn_check(const g4_kv_pages *pages, const g4_chunk *chunk, int heads
     if (window < 0) return set_error(G4_ERR_INVALID, "attention-chunk: window %d", window);
     if ((int64_t)A->tokens * heads > ((int64_t)1 << 30) || A->kv_heads > 65535)
         return set_error(G4_ERR_UNSUPPORTED, "attention-chunk: more than 2^30 query rows, or 65535 KV heads");
-    if (A->slot_stride > ((int64_t)1 << 27))
-        return set_error(G4_ERR_UNSUPPORTED, "attention-chunk: slots more than 2^27 elements apart");
+    if (A->page_stride > INT32_MAX || A->slot_stride * pages->page_size > INT32_MAX)
+        return set_error(G4_ERR_UNSUPPORTED, "attention-chunk: pages, or a page's slots, 2^31 or more elements apart");
     return G4_OK;
 }
 
@@ -836,6 +878,7 @@ int g4_attention_chunk(const g4_kv_pages *pages, const g4_chunk *chunk, const vo
     if (!q || !out || !workspace) return set_error(G4_ERR_INVALID, "attention-chunk needs q, an output and a workspace");
     if (out_kind != G4_KIND_F16 && out_kind != G4_KIND_F32 && out_kind != G4_KIND_I8)
         return set_error(G4_ERR_INVALID, "attention-chunk: outputs are f16, f32 or int8 codes, got kind %d", out_kind);
+    if (!std::isfinite(scale)) return set_error(G4_ERR_INVALID, "attention-chunk: scale must be finite");
     if (out_kind == G4_KIND_I8 && in_scale == 0.0f)
         return set_error(G4_ERR_INVALID, "attention-chunk: int8 codes need the consumer's inScale");
     const int64_t qw = (int64_t)heads * pages->head_dim;
@@ -847,10 +890,26 @@ int g4_attention_chunk(const g4_kv_pages *pages, const g4_chunk *chunk, const vo
     if (workspace_bytes < P.bytes)
         return set_error(G4_ERR_INVALID, "attention-chunk: workspace %zu B < %zu B", workspace_bytes, P.bytes);
     float *part_o = static_cast<float *>(workspace);
-    const AttnArgs R{static_cast<const _Float16 *>(q), q_stride ? q_stride : qw, heads,
-                     FastDiv::of(heads / A.kv_heads),                     scale * 1.44269504088896340736f, window, out, out_kind, in_scale, FastDiv::of(P.splits), part_o,
-                     reinterpret_cast<float2 *>(part_o + P.tiles * P.splits * A.kv_heads * kRows * P.rt * pages->head_dim)};
     const bool i8 = pages->kind == G4_KIND_I8;
+    const int eb = i8 ? 1 : 2;
+    AttnArgs R{};
+    R.q = static_cast<const _Float16 *>(q);
+    R.q_stride = q_stride ? q_stride : qw;
+    R.heads = heads;
+    R.group = FastDiv::of(heads / A.kv_heads);
+    // a scale of 0 as one too small to matter, so that a masked score stays minus infinity
+    R.scale2 = std::max(std::fabs(scale) * 1.44269504088896340736f, 0x1p-100f) * (i8 ? 0x1p24f : 1.0f);
+    R.lazy = kLazy / R.scale2;
+    R.q_sign = scale < 0.0f ? 0x80008000u : 0u;
+    R.page_bytes = (uint32_t)(A.page_stride * eb);
+    R.slot_bytes = (uint32_t)(A.slot_stride * eb);
+    R.window = window;
+    R.out = out;
+    R.out_kind = out_kind;
+    R.in_scale = in_scale;
+    R.splits = FastDiv::of(P.splits);
+    R.part_o = part_o;
+    R.part_ml = reinterpret_cast<float2 *>(part_o + P.tiles * P.splits * A.kv_heads * kRows * P.rt * pages->head_dim);
     hipStream_t st = as_stream(stream);
     switch (pages->head_dim) {
         case 64: return i8 ? launch_attn<64, G4_KIND_I8>(A, R, P, st) : launch_attn<64, G4_KIND_F16>(A, R, P, st);

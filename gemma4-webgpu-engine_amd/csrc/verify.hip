@@ -1,11 +1,13 @@
 // Verification of drafted tokens against the target's logits (include/g4serve.h): the speculative
 // sampling rule with given random numbers, or the greedy one.
 //
-// Three launches: (1) every row's maximum and sum of exp by parts of kPart logits; (2) per sequence the
-// decisions, and the sums of the weights that the next token is drawn from, by parts; (3) per sequence
-// the part and then the logit where the running sum passes u_next of the total. Greedy runs (1) and (3).
-// A token is the one of 262144 whose running sum passes a given point, so sums that are 1e-7 off would
-// often name its neighbour: weights and sums are held in 64 bits.
+// Launches: (1) every row's maximum and sum of exp, by parts of kPart logits; (2) a block per sequence
+// joins its rows' parts, judges the drafts and writes all outputs but the drawn token (greedy: that too, and
+// no more launches); (3) the weights that the token is drawn from, summed by units of kUnit logits; (4) a
+// block per sequence finds the unit and then the logit where the running sum passes u_next of the total.
+//
+// A drawn token is the one of up to 262144 whose running sum passes a given point: sums that are 1e-7 off
+// would often name its neighbour. So exponents and sums are held in 64 bits and 2^f is good to 1e-12.
 #include "g4_internal.h"
 #include "../../include/g4serve.h"
 #include <cmath>
@@ -13,6 +15,8 @@
 namespace g4 {
 
 constexpr int kPart = 8192, kVerThreads = 256, kPerThread = kPart / kVerThreads;
+constexpr int kUnit = 2048, kUnitPer = kUnit / kVerThreads;
+constexpr int kJudgeWaves = 16;
 constexpr int kMaxDrafts = 63;
 
 struct PartStat {
@@ -21,18 +25,24 @@ struct PartStat {
     int index;   // of the first maximum
 };
 
+// What the draw of a sequence needs.
+struct Draw {
+    double p_top, p_sum, q_top, q_sum;  // y(max) and sum of exp((y - top) / T) of the two rows; sum 0: no weight
+    int taken, refused;                 // drafts taken; whether the next one was refused
+};
+
 struct VerifyArgs {
     const float *logits, *draft_logits;
     const int32_t *draft_tokens, *draft_start;
-    int seqs, drafts, max_drafts, parts;
+    int seqs, drafts, max_drafts, parts, units;
     int64_t vocab;
     double cap, inv_t;
-    int greedy;
+    double inv_cap2;
+    int greedy, vec;  // vec: rows may be read 16 bytes at a time
     const float *u, *u_next;
-    PartStat *stats;   // [drafts + seqs (+ drafts)][parts]
-    double *weights;   // [seqs][parts]
-    double *norms;     // [seqs][4]: y(max) and sum of the p row, of the q row
-    int *chosen;       // [seqs][2]: drafts taken, whether one was refused
+    PartStat *stats;  // [drafts + seqs (+ drafts)][parts]
+    double *weights;  // [seqs][units]
+    Draw *draws;      // [seqs]
     int32_t *tokens, *accepted;
     float *logprobs;
 };
@@ -49,15 +59,89 @@ __device__ __forceinline__ double weight(float x, double top, const VerifyArgs &
     return y == top ? 1.0 : exp((y - top) * A.inv_t);
 }
 
+// weight() for the bulk of a row. 2^z: z = n + f, |f| <= 1/2, a polynomial in f (fitted on Chebyshev nodes,
+// relative error 1.1e-12) and n into the exponent. The softcap of |x| <= cap / 2 as x + x t P(t), t =
+// (x / cap)^2 (fitted likewise, 8e-14 t x off); past that the definition. 13 operations of the 64-bit unit a
+// logit, about what its 4 bytes cost to read; 24 with the softcap.
+struct RowScale {
+    double top, slope, base;  // 2^(y slope + base)
+};
+__device__ __forceinline__ RowScale row_scale(double top, const VerifyArgs &A) {
+    const double slope = A.inv_t * 1.4426950408889634074;
+    return {top, slope, -top * slope};
+}
+__device__ __forceinline__ double bulk_weight(float x, const RowScale &S, const VerifyArgs &A) {
+    double y = x;
+    if (A.cap != 0.0) {
+        const double t = y * y * A.inv_cap2;
+        double c = 0.00039943422382545215;
+        c = __builtin_fma(c, t, -0.0013843999024647944);
+        c = __builtin_fma(c, t, 0.0035776163994480498);
+        c = __builtin_fma(c, t, -0.008861575554686911);
+        c = __builtin_fma(c, t, 0.021869384578835853);
+        c = __builtin_fma(c, t, -0.053968250756296965);
+        c = __builtin_fma(c, t, 0.1333333332954187);
+        c = __builtin_fma(c, t, -0.3333333333332598);
+        y = t <= 0.25 ? __builtin_fma(y, t * c, y) : softcap64(x, A.cap);
+    }
+    if (y == S.top) return 1.0;
+    double z = __builtin_fma(y, S.slope, S.base);
+    z = z > -1000.0 ? z : -1000.0;  // too small to count, and the exponent stays normal; a NaN too (infinite rows)
+    const double n = __builtin_rint(z), f = z - n;
+    double e = 1.3259689002093833e-06;
+    e = __builtin_fma(e, f, 1.531008106933654e-05);
+    e = __builtin_fma(e, f, 0.00015403433582607232);
+    e = __builtin_fma(e, f, 0.0013333450560096254);
+    e = __builtin_fma(e, f, 0.009618129194093111);
+    e = __builtin_fma(e, f, 0.05550410941217064);
+    e = __builtin_fma(e, f, 0.24022650695640319);
+    e = __builtin_fma(e, f, 0.6931471805459295);
+    e = __builtin_fma(e, f, 1.0000000000000135);
+    return __longlong_as_double(__double_as_longlong(e) + ((int64_t)(int)n << 52));
+}
+
 __device__ __forceinline__ float clean(float x) { return x == x ? x : -INFINITY; }
 
-__device__ __forceinline__ double shfl_xor64(double v, int m) { return __shfl_xor(v, m); }
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+    for (int s = 32; s; s >>= 1) v += __shfl_xor(v, s);
+    return v;
+}
 
 __device__ __forceinline__ void first_max(float &m, int &at, float om, int oat) {
     if (om > m || (om == m && oat < at)) {
         m = om;
         at = oat;
     }
+}
+
+// N values of a thread from a row's range of `n` logits at x (past its end: no weight): 16 bytes at a time
+// (element j is 1024 (j / 4) + 4 t + j % 4 of the range) or one (256 j + t).
+__device__ __forceinline__ int element(int j, int vec) {
+    return vec ? (j / 4) * 4 * kVerThreads + 4 * (int)threadIdx.x + j % 4 : j * kVerThreads + (int)threadIdx.x;
+}
+template <int N>
+__device__ __forceinline__ void load_range(const float *x, int n, int vec, float (&v)[N]) {
+    if (vec) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const int i = element(j, 1);
+            float4 y = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            if (i < n) y = *reinterpret_cast<const float4 *>(x + i);  // n is a multiple of 4 here
+            v[j] = y.x;
+            v[j + 1] = y.y;
+            v[j + 2] = y.z;
+            v[j + 3] = y.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int i = element(j, 0);
+            v[j] = i < n ? x[i] : -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = clean(v[j]);
 }
 
 // Grid (parts, rows): part blockIdx.x of row blockIdx.y, the target's rows first.
@@ -69,20 +153,15 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs A)
     const float *x = row < targets ? A.logits + row * A.vocab : A.draft_logits + (int64_t)(row - targets) * A.vocab;
     const int64_t base = (int64_t)part * kPart;
     const int n = (int)(A.vocab - base < kPart ? A.vocab - base : kPart);
-    x += base;
     float v[kPerThread];
+    load_range(x + base, n, A.vec, v);
     float m = -INFINITY;
     int at = INT32_MAX;
-#pragma unroll
-    for (int j = 0; j < kPerThread; ++j) {
-        const int i = j * kVerThreads + t;
-        v[j] = i < n ? clean(x[i]) : -INFINITY;
-    }
 #pragma unroll
     for (int j = 0; j < kPerThread; ++j)
         if (v[j] > m) {
             m = v[j];
-            at = j * kVerThreads + t;
+            at = element(j, A.vec);
         }
 #pragma unroll
     for (int s = 32; s; s >>= 1) first_max(m, at, __shfl_xor(m, s), __shfl_xor(at, s));
@@ -97,13 +176,11 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs A)
     for (int w = 1; w < 4; ++w) first_max(m, at, ms[w], is[w]);
     double sum = 0.0;
     if (m > -INFINITY) {
-        const double top = softcap64(m, A.cap);
+        const RowScale S = row_scale(softcap64(m, A.cap), A);
 #pragma unroll
-        for (int j = 0; j < kPerThread; ++j)
-            if (j * kVerThreads + t < n && v[j] > -INFINITY) sum += weight(v[j], top, A);
+        for (int j = 0; j < kPerThread; ++j) sum += v[j] > -INFINITY ? bulk_weight(v[j], S, A) : 0.0;
     }
-#pragma unroll
-    for (int s = 32; s; s >>= 1) sum += shfl_xor64(sum, s);
+    sum = wave_sum64(sum);
     if ((t & 63) == 0) ss[t >> 6] = sum;
     __syncthreads();
     if (t == 0)
@@ -112,31 +189,32 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs A)
 }
 
 struct RowStat {
-    double top, sum;  // y(max), sum of exp((y - top) / T); sum 0: no weight
+    double top, sum;
     int index;
 };
 
 // A row's statistics from its parts, by one wave (the same in every lane).
 __device__ __forceinline__ RowStat row_stat(const VerifyArgs &A, int row) {
     const PartStat *p = A.stats + (int64_t)row * A.parts;
+    const int lane = threadIdx.x & 63;
+    const PartStat mine = p[min(lane, A.parts - 1)];  // the first 64 parts are read once
     float m = -INFINITY;
     int at = INT32_MAX;
-    for (int c = threadIdx.x & 63; c < A.parts; c += 64) first_max(m, at, p[c].max, p[c].index < 0 ? INT32_MAX : p[c].index);
+    for (int c = lane; c < A.parts; c += 64) {
+        const PartStat s = c == lane ? mine : p[c];
+        first_max(m, at, s.max, s.index < 0 ? INT32_MAX : s.index);
+    }
 #pragma unroll
     for (int s = 32; s; s >>= 1) first_max(m, at, __shfl_xor(m, s), __shfl_xor(at, s));
     if (!(m > -INFINITY)) return {0.0, 0.0, -1};
     const double top = softcap64(m, A.cap);
     double sum = 0.0;
-    for (int c = threadIdx.x & 63; c < A.parts; c += 64)
-        if (p[c].max > -INFINITY) sum += p[c].sum * weight(p[c].max, top, A);
-#pragma unroll
-    for (int s = 32; s; s >>= 1) sum += shfl_xor64(sum, s);
-    return {top, sum, at};
+    for (int c = lane; c < A.parts; c += 64) {
+        const PartStat s = c == lane ? mine : p[c];
+        if (s.max > -INFINITY) sum += s.sum * weight(s.max, top, A);
+    }
+    return {top, wave_sum64(sum), at};
 }
-
-struct Decision {
-    int taken, refused, count, start;
-};
 
 __device__ __forceinline__ void draft_span(const VerifyArgs &A, int seq, int *start, int *count) {
     const int a = min(max(A.draft_start[seq], 0), A.drafts);
@@ -145,164 +223,157 @@ __device__ __forceinline__ void draft_span(const VerifyArgs &A, int seq, int *st
     *count = min(b - a, A.max_drafts);
 }
 
-// Every draft of the sequence judged, one wave a draft at a time; the block agrees through LDS.
-__device__ __forceinline__ Decision decide(const VerifyArgs &A, int seq, unsigned long long *good_lds) {
+// log p of a token of target row `row`.
+__device__ __forceinline__ float log_p(const VerifyArgs &A, int row, int token, const RowStat &P) {
+    const double y = softcap64(A.logits[row * A.vocab + token], A.cap);
+    return (float)((y == P.top ? 0.0 : (y - P.top) * A.inv_t) - log(P.sum));
+}
+
+// One block per sequence: a wave joins one row's parts at a time, then lane i of the first wave judges
+// draft i.
+__global__ __launch_bounds__(64 * kJudgeWaves) void verify_judge_kernel(VerifyArgs A) {
+    __shared__ RowStat ps[kMaxDrafts + 1], qs[kMaxDrafts + 1];
+    const int seq = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int start, count;
     draft_span(A, seq, &start, &count);
-    const int wave = threadIdx.x >> 6;
-    if (threadIdx.x < 4) good_lds[threadIdx.x] = 0;
+    const int tasks = count + 1 + (A.draft_logits ? count : 0);
+    for (int i = wave; i < tasks; i += kJudgeWaves) {
+        const bool target = i <= count;
+        const int r = target ? i : i - count - 1;
+        const RowStat S = row_stat(A, target ? start + seq + r : A.drafts + A.seqs + start + r);
+        if (lane == 0) (target ? ps : qs)[r] = S;
+    }
     __syncthreads();
-    unsigned long long good = 0;
-    for (int i = wave; i < count; i += 4) {
-        const int tok = A.draft_tokens[start + i], row = start + seq + i;
-        const RowStat P = row_stat(A, row);
-        bool ok = false;
-        if (tok >= 0 && tok < A.vocab && P.sum > 0.0) {
+    if (wave) return;
+    const int row = start + seq + lane;
+    int token = -1;
+    bool ok = false;
+    RowStat P{0.0, 0.0, -1};
+    if (lane < count) {
+        token = A.draft_tokens[start + lane];
+        P = ps[lane];
+        if (token >= 0 && token < A.vocab && P.sum > 0.0) {
             if (A.greedy) {
-                ok = P.index == tok;
+                ok = P.index == token;
             } else {
-                const float xp = clean(A.logits[row * A.vocab + tok]);
+                const float xp = clean(A.logits[row * A.vocab + token]);
                 const double p = xp > -INFINITY ? weight(xp, P.top, A) / P.sum : 0.0;
                 double q = 1.0;
                 if (A.draft_logits) {
-                    const RowStat Q = row_stat(A, A.drafts + A.seqs + start + i);
-                    const float xq = clean(A.draft_logits[(int64_t)(start + i) * A.vocab + tok]);
+                    const RowStat Q = qs[lane];
+                    const float xq = clean(A.draft_logits[(int64_t)(start + lane) * A.vocab + token]);
                     q = Q.sum > 0.0 && xq > -INFINITY ? weight(xq, Q.top, A) / Q.sum : 0.0;
                 }
-                ok = (double)A.u[start + i] * q < p;
+                ok = (double)A.u[start + lane] * q < p;
             }
         }
-        if (ok) good |= 1ull << i;
     }
-    if ((threadIdx.x & 63) == 0) good_lds[wave] = good;
-    __syncthreads();
-    good = good_lds[0] | good_lds[1] | good_lds[2] | good_lds[3];
-    const int taken = min(__ffsll((long long)~good) - 1, count);
-    return {taken, taken < count, count, start};
+    const unsigned long long good = __ballot(ok);
+    const int taken = min(__ffsll((long long)~good) - 1, count);  // bit 63 of good is never set: count <= 63
+    int32_t *out = A.tokens + (int64_t)seq * (A.max_drafts + 1);
+    float *lp = A.logprobs ? A.logprobs + (int64_t)seq * (A.max_drafts + 1) : nullptr;
+    if (lane <= A.max_drafts && lane != taken) {
+        out[lane] = lane < taken ? token : -1;
+        if (lp) lp[lane] = lane < taken ? log_p(A, row, token, P) : 0.0f;
+    }
+    if (lane) return;
+    const bool refused = taken < count;
+    const RowStat S = ps[taken];
+    A.accepted[seq] = taken;
+    if (A.greedy) {
+        out[taken] = S.index;
+        if (lp) lp[taken] = S.index >= 0 ? log_p(A, start + seq + taken, S.index, S) : 0.0f;
+        return;
+    }
+    const RowStat Q = refused && A.draft_logits ? qs[taken] : RowStat{0.0, 0.0, -1};
+    A.draws[seq] = {S.top, S.sum, Q.top, Q.sum, taken, refused};
 }
 
 // The distribution that the next token comes from: max(p - q, 0), with q a row, one token, or nothing.
 struct Source {
     const float *p, *q;
-    double p_top, p_inv, q_top, q_inv;
+    RowScale ps, qs;
+    double p_inv, q_inv;
     int64_t point;  // q is 1 here (-1: nowhere)
 };
 
-__device__ __forceinline__ double source_weight(const VerifyArgs &A, const Source &S, int64_t i) {
-    const float xp = clean(S.p[i]);
-    double w = xp > -INFINITY ? weight(xp, S.p_top, A) * S.p_inv : 0.0;
+__device__ __forceinline__ Source source_of(const VerifyArgs &A, int seq, int start, const Draw &D, bool less) {
+    Source S;
+    S.p = A.logits + (int64_t)(start + seq + D.taken) * A.vocab;
+    S.q = less && A.draft_logits ? A.draft_logits + (int64_t)(start + D.taken) * A.vocab : nullptr;
+    S.ps = row_scale(D.p_top, A);
+    S.qs = row_scale(D.q_top, A);
+    S.p_inv = D.p_sum > 0.0 ? 1.0 / D.p_sum : 0.0;
+    S.q_inv = D.q_sum > 0.0 ? 1.0 / D.q_sum : 0.0;
+    S.point = less && !A.draft_logits ? A.draft_tokens[start + D.taken] : -1;
+    return S;
+}
+
+__device__ __forceinline__ double source_weight(const VerifyArgs &A, const Source &S, int64_t i, float xp, float xq) {
+    double w = xp > -INFINITY ? bulk_weight(xp, S.ps, A) * S.p_inv : 0.0;
     if (S.q) {
-        const float xq = clean(S.q[i]);
-        if (xq > -INFINITY) w -= weight(xq, S.q_top, A) * S.q_inv;
+        if (xq > -INFINITY) w -= bulk_weight(xq, S.qs, A) * S.q_inv;
     } else if (i == S.point) {
         w -= 1.0;
     }
     return w > 0.0 ? w : 0.0;
 }
 
-__device__ __forceinline__ Source source_of(const VerifyArgs &A, int seq, int start, int taken, bool refused,
-                                            double p_top, double p_sum, double q_top, double q_sum) {
-    Source S;
-    S.p = A.logits + (int64_t)(start + seq + taken) * A.vocab;
-    S.q = refused && A.draft_logits ? A.draft_logits + (int64_t)(start + taken) * A.vocab : nullptr;
-    S.p_top = p_top;
-    S.p_inv = p_sum > 0.0 ? 1.0 / p_sum : 0.0;
-    S.q_top = q_top;
-    S.q_inv = q_sum > 0.0 ? 1.0 / q_sum : 0.0;
-    S.point = refused && !A.draft_logits ? A.draft_tokens[start + taken] : -1;
-    return S;
-}
-
-// Grid (parts, seqs): the decisions, and part blockIdx.x's sum of the weights to draw from. Part 0
-// writes the outputs of the drafts taken.
-__global__ __launch_bounds__(kVerThreads) void verify_weights_kernel(VerifyArgs A) {
-    __shared__ unsigned long long good[4];
-    __shared__ double ss[4];
-    const int t = threadIdx.x, part = blockIdx.x, seq = blockIdx.y;
-    const Decision D = decide(A, seq, good);
-    const RowStat P = row_stat(A, D.start + seq + D.taken);
-    RowStat Q{0.0, 0.0, -1};
-    if (D.refused && A.draft_logits) Q = row_stat(A, A.drafts + A.seqs + D.start + D.taken);
-    const Source S = source_of(A, seq, D.start, D.taken, D.refused, P.top, P.sum, Q.top, Q.sum);
-    const int64_t base = (int64_t)part * kPart;
+// The block's thread's weights of a unit, in the element order of load_range; returns their sum.
+__device__ __forceinline__ double unit_weights(const VerifyArgs &A, const Source &S, int64_t base, double (&w)[kUnitPer]) {
+    float xp[kUnitPer], xq[kUnitPer] = {};
+    const int n = (int)(A.vocab - base < kUnit ? A.vocab - base : kUnit);
+    load_range(S.p + base, n, A.vec, xp);
+    if (S.q) load_range(S.q + base, n, A.vec, xq);
     double sum = 0.0;
-#pragma unroll 4
-    for (int j = 0; j < kPerThread; ++j) {
-        const int64_t i = base + j * kVerThreads + t;
-        if (i < A.vocab) sum += source_weight(A, S, i);
-    }
 #pragma unroll
-    for (int s = 32; s; s >>= 1) sum += shfl_xor64(sum, s);
-    if ((t & 63) == 0) ss[t >> 6] = sum;
+    for (int j = 0; j < kUnitPer; ++j) {
+        w[j] = source_weight(A, S, base + element(j, A.vec), xp[j], xq[j]);
+        sum += w[j];
+    }
+    return sum;
+}
+
+__device__ __forceinline__ double block_sum64(double sum, double *lds) {
+    sum = wave_sum64(sum);
     __syncthreads();
-    if (t == 0) {
-        A.weights[(int64_t)seq * A.parts + part] = (ss[0] + ss[1]) + (ss[2] + ss[3]);
-        if (part == 0) {
-            double *n = A.norms + 4 * seq;
-            n[0] = P.top;
-            n[1] = P.sum;
-            n[2] = Q.top;
-            n[3] = Q.sum;
-            A.chosen[2 * seq] = D.taken;
-            A.chosen[2 * seq + 1] = D.refused;
-        }
-    }
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    return (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
-// The tokens and log probabilities of a sequence but the drawn one, one wave a draft at a time.
-__device__ __forceinline__ void put_taken(const VerifyArgs &A, int seq, int start, int taken) {
-    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, lane = threadIdx.x & 63;
-    int32_t *out = A.tokens + (int64_t)seq * (A.max_drafts + 1);
-    float *lp = A.logprobs ? A.logprobs + (int64_t)seq * (A.max_drafts + 1) : nullptr;
-    for (int i = wave; i < taken; i += waves) {
-        const int tok = A.draft_tokens[start + i];
-        const RowStat P = row_stat(A, start + seq + i);
-        if (lane == 0) {
-            out[i] = tok;
-            if (lp) {
-                const double y = softcap64(A.logits[(int64_t)(start + seq + i) * A.vocab + tok], A.cap);
-                lp[i] = (float)((y == P.top ? 0.0 : (y - P.top) * A.inv_t) - log(P.sum));
-            }
-        }
-    }
-    for (int i = taken + 1 + threadIdx.x; i <= A.max_drafts; i += blockDim.x) {
-        out[i] = -1;
-        if (lp) lp[i] = 0.0f;
-    }
+// Grid (units, seqs): unit blockIdx.x's sum of the weights to draw from.
+__global__ __launch_bounds__(kVerThreads) void verify_weights_kernel(VerifyArgs A) {
+    __shared__ double ss[4];
+    const int seq = blockIdx.y;
+    int start, count;
+    draft_span(A, seq, &start, &count);
+    const Draw D = A.draws[seq];
+    const Source S = source_of(A, seq, start, D, D.refused);
+    double w[kUnitPer];
+    const double sum = block_sum64(unit_weights(A, S, (int64_t)blockIdx.x * kUnit, w), ss);
+    if (threadIdx.x == 0) A.weights[(int64_t)seq * A.units + blockIdx.x] = sum;
 }
 
-__device__ __forceinline__ void put_drawn(const VerifyArgs &A, int seq, int start, int taken, int token, double top,
-                                          double sum) {
-    A.tokens[(int64_t)seq * (A.max_drafts + 1) + taken] = token;
-    A.accepted[seq] = taken;
-    if (!A.logprobs) return;
-    double lp = 0.0;
-    if (token >= 0) {
-        const double y = softcap64(A.logits[(int64_t)(start + seq + taken) * A.vocab + token], A.cap);
-        lp = (y == top ? 0.0 : (y - top) * A.inv_t) - log(sum);
-    }
-    A.logprobs[(int64_t)seq * (A.max_drafts + 1) + taken] = (float)lp;
-}
-
-__global__ __launch_bounds__(kVerThreads) void verify_greedy_kernel(VerifyArgs A) {
-    __shared__ unsigned long long good[4];
-    const int seq = blockIdx.x;
-    const Decision D = decide(A, seq, good);
-    put_taken(A, seq, D.start, D.taken);
-    const RowStat P = row_stat(A, D.start + seq + D.taken);
-    if (threadIdx.x == 0) put_drawn(A, seq, D.start, D.taken, P.index, P.top, P.sum);
-}
-
-// The first of the block's kPart weights from `base` on whose running sum exceeds `target`; the last
-// one with any weight where rounding leaves none (-1: no weight at all). Same in every thread.
-__device__ __forceinline__ int64_t pick(const VerifyArgs &A, const Source &S, int64_t base, double target, double *ws,
-                                        int *first, int *last) {
+// The first weight of the unit at `base` whose running sum exceeds `target`; the last one with any weight
+// where rounding leaves none (-1: no weight at all). Same in every thread.
+__device__ __forceinline__ int64_t pick(const VerifyArgs &A, const Source &S, int64_t base, double target, double *w_lds,
+                                        double *ws, int *first, int *last) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    double w[kPerThread], sum = 0.0;
-    const int64_t at = base + (int64_t)t * kPerThread;
+    double w[kUnitPer];
+    unit_weights(A, S, base, w);
+    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kPerThread; ++j) {
-        w[j] = at + j < A.vocab ? source_weight(A, S, at + j) : 0.0;
+    for (int j = 0; j < kUnitPer; ++j) w_lds[element(j, A.vec)] = w[j];  // to token order
+    if (t == 0) {
+        *first = INT32_MAX;
+        *last = -1;
+    }
+    __syncthreads();
+    double sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < kUnitPer; ++j) {
+        w[j] = w_lds[t * kUnitPer + j];
         sum += w[j];
     }
     double run = sum;  // of the threads up to this one
@@ -311,20 +382,16 @@ __device__ __forceinline__ int64_t pick(const VerifyArgs &A, const Source &S, in
         const double o = __shfl_up(run, s);
         if (lane >= s) run += o;
     }
-    if (t == 0) {
-        *first = INT32_MAX;
-        *last = -1;
-    }
     if (lane == 63) ws[wave] = run;
     __syncthreads();
     for (int v = 0; v < wave; ++v) run += ws[v];
     double before = run - sum;
     int hit = INT32_MAX, any = -1;
 #pragma unroll
-    for (int j = 0; j < kPerThread; ++j) {
+    for (int j = 0; j < kUnitPer; ++j) {
         before += w[j];
         if (w[j] > 0.0) {
-            any = t * kPerThread + j;
+            any = t * kUnitPer + j;
             if (hit == INT32_MAX && before > target) hit = any;
         }
     }
@@ -332,62 +399,64 @@ __device__ __forceinline__ int64_t pick(const VerifyArgs &A, const Source &S, in
     if (any >= 0) atomicMax(last, any);
     __syncthreads();
     const int f = *first, l = *last;
-    __syncthreads();
     return f != INT32_MAX ? base + f : (l >= 0 ? base + l : -1);
 }
 
-// One block per sequence: the part where the running sum of the parts passes the target, then the logit.
+// One block per sequence: the unit where the running sum of the units passes the target, then the logit.
 __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs A) {
-    __shared__ double ws[4];
+    __shared__ double w_lds[kUnit], ws[4];
     __shared__ int first, last;
-    const int seq = blockIdx.x;
+    const int seq = blockIdx.x, lane = threadIdx.x & 63;
     int start, count;
     draft_span(A, seq, &start, &count);
-    const int taken = A.chosen[2 * seq];
-    bool refused = A.chosen[2 * seq + 1];
-    const double *n = A.norms + 4 * seq, *w = A.weights + (int64_t)seq * A.parts;
-    put_taken(A, seq, start, taken);
-    double total = 0.0;
-    for (int c = 0; c < A.parts; ++c) total += w[c];
-    int64_t token = -1;
+    const Draw D = A.draws[seq];
+    const double *w = A.weights + (int64_t)seq * A.units;
     const double u = A.u_next[seq];
+    // every wave by itself: the total, then the first unit that takes the running sum past u of it
+    double total = 0.0;
+    for (int c0 = 0; c0 < A.units; c0 += 64) total += c0 + lane < A.units ? w[c0 + lane] : 0.0;
+    total = wave_sum64(total);
+    int64_t token = -1;
     if (total > 0.0) {
-        const Source S = source_of(A, seq, start, taken, refused, n[0], n[1], n[2], n[3]);
-        double before = 0.0, target = u * total;
-        int part = -1;
-        double part_before = 0.0;
-        for (int c = 0; c < A.parts; ++c) {
-            if (w[c] > 0.0) {
-                part = c;
-                part_before = before;
-                if (before + w[c] > target) break;
-            }
-            before += w[c];
-        }
-        token = pick(A, S, (int64_t)part * kPart, target - part_before, ws, &first, &last);
-    } else if (refused && n[1] > 0.0) {
-        // p and q are the same everywhere: the draw is from p, whose sum of weights is 1
-        const Source S = source_of(A, seq, start, taken, false, n[0], n[1], 0.0, 0.0);
-        double before = 0.0;
-        for (int c = 0; c < A.parts; ++c) {
-            const int64_t base = (int64_t)c * kPart;
-            double sum = 0.0;
-            for (int j = 0; j < kPerThread; ++j) {
-                const int64_t i = base + j * kVerThreads + threadIdx.x;
-                if (i < A.vocab) sum += source_weight(A, S, i);
-            }
+        const double target = u * total;
+        double before = 0.0, unit_before = 0.0;
+        int unit = -1;
+        for (int c0 = 0; c0 < A.units; c0 += 64) {
+            const double x = c0 + lane < A.units ? w[c0 + lane] : 0.0;
+            double run = x;
 #pragma unroll
-            for (int s = 32; s; s >>= 1) sum += shfl_xor64(sum, s);
-            if ((threadIdx.x & 63) == 0) ws[threadIdx.x >> 6] = sum;
-            __syncthreads();
-            sum = (ws[0] + ws[1]) + (ws[2] + ws[3]);
-            __syncthreads();
-            if (sum > 0.0) token = pick(A, S, base, u - before, ws, &first, &last);
+            for (int s = 1; s < 64; s <<= 1) {
+                const double o = __shfl_up(run, s);
+                if (lane >= s) run += o;
+            }
+            const unsigned long long some = __ballot(x > 0.0), past = __ballot(x > 0.0 && before + run > target);
+            if (some) {  // the first past the target, or the last with any weight so far
+                const int at = past ? __ffsll((long long)past) - 1 : 63 - __clzll((long long)some);
+                unit = c0 + at;
+                unit_before = before + __shfl(run - x, at);
+            }
+            if (past) break;
+            before += __shfl(run, 63);
+        }
+        token = pick(A, source_of(A, seq, start, D, D.refused), (int64_t)unit * kUnit, target - unit_before, w_lds, ws,
+                     &first, &last);
+    } else if (D.refused && D.p_sum > 0.0) {
+        // p and q are the same everywhere: the draw is from p, whose sum of weights is 1
+        const Source S = source_of(A, seq, start, D, false);
+        double before = 0.0;
+        for (int c = 0; c < A.units; ++c) {
+            double x[kUnitPer];
+            const double sum = block_sum64(unit_weights(A, S, (int64_t)c * kUnit, x), ws);
+            if (sum > 0.0) token = pick(A, S, (int64_t)c * kUnit, u - before, w_lds, ws, &first, &last);
             if (before + sum > u) break;
             before += sum;
         }
     }
-    if (threadIdx.x == 0) put_drawn(A, seq, start, taken, (int)token, n[0], n[1]);
+    if (threadIdx.x) return;
+    A.tokens[(int64_t)seq * (A.max_drafts + 1) + D.taken] = (int)token;
+    if (A.logprobs)
+        A.logprobs[(int64_t)seq * (A.max_drafts + 1) + D.taken] =
+            token >= 0 ? log_p(A, start + seq + D.taken, (int)token, RowStat{D.p_top, D.p_sum, -1}) : 0.0f;
 }
 
 static int64_t verify_rows(int seqs, int drafts) { return 2 * (int64_t)drafts + seqs; }
@@ -401,8 +470,8 @@ extern "C" {
 size_t g4_verify_workspace_bytes(int seqs, int drafts, int64_t vocab) {
     if (seqs <= 0 || drafts < 0 || vocab <= 0 || vocab > INT32_MAX) return 0;
     const size_t parts = (size_t)((vocab + kPart - 1) / kPart);
-    return (size_t)verify_rows(seqs, drafts) * parts * sizeof(PartStat) + (size_t)seqs * parts * sizeof(double) +
-           (size_t)seqs * (4 * sizeof(double) + 2 * sizeof(int));
+    const size_t units = (size_t)((vocab + kUnit - 1) / kUnit);
+    return (size_t)verify_rows(seqs, drafts) * parts * sizeof(PartStat) + (size_t)seqs * (units * sizeof(double) + sizeof(Draw));
 }
 
 int g4_verify_drafts(const float *logits, const float *draft_logits, const int32_t *draft_tokens,
@@ -440,28 +509,28 @@ int g4_verify_drafts(const float *logits, const float *draft_logits, const int32
     A.drafts = drafts;
     A.max_drafts = max_drafts;
     A.parts = (int)((vocab + kPart - 1) / kPart);
+    A.units = (int)((vocab + kUnit - 1) / kUnit);
     A.vocab = vocab;
     A.cap = cap;
+    A.inv_cap2 = cap > 0.0f ? 1.0 / ((double)cap * cap) : 0.0;
+    A.vec = vocab % 4 == 0 && (((uintptr_t)logits | (uintptr_t)draft_logits) & 15) == 0;
     A.inv_t = greedy ? 1.0 : 1.0 / (double)temperature;
     A.greedy = greedy;
     A.u = u;
     A.u_next = u_next;
     A.stats = static_cast<PartStat *>(workspace);
     A.weights = reinterpret_cast<double *>(A.stats + verify_rows(seqs, drafts) * A.parts);
-    A.norms = A.weights + (int64_t)seqs * A.parts;
-    A.chosen = reinterpret_cast<int *>(A.norms + 4 * (int64_t)seqs);
+    A.draws = reinterpret_cast<Draw *>(A.weights + (int64_t)seqs * A.units);
     A.tokens = tokens;
     A.accepted = accepted;
     A.logprobs = logprobs;
     hipStream_t s = as_stream(stream);
     hipLaunchKernelGGL(verify_stats_kernel, dim3(A.parts, (unsigned)rows), dim3(kVerThreads), 0, s, A);
     G4_LAUNCHED("verify_stats_kernel");
-    if (greedy) {
-        hipLaunchKernelGGL(verify_greedy_kernel, dim3(seqs), dim3(kVerThreads), 0, s, A);
-        G4_LAUNCHED("verify_greedy_kernel");
-        return G4_OK;
-    }
-    hipLaunchKernelGGL(verify_weights_kernel, dim3(A.parts, seqs), dim3(kVerThreads), 0, s, A);
+    hipLaunchKernelGGL(verify_judge_kernel, dim3(seqs), dim3(64 * kJudgeWaves), 0, s, A);
+    G4_LAUNCHED("verify_judge_kernel");
+    if (greedy) return G4_OK;
+    hipLaunchKernelGGL(verify_weights_kernel, dim3(A.units, seqs), dim3(kVerThreads), 0, s, A);
     G4_LAUNCHED("verify_weights_kernel");
     hipLaunchKernelGGL(verify_pick_kernel, dim3(seqs), dim3(kVerThreads), 0, s, A);
     G4_LAUNCHED("verify_pick_kernel");

@@ -8,6 +8,7 @@ by the library, which raises G4Error. Everything computes in the HIP library.
 from __future__ import annotations
 
 import ctypes
+import sys
 
 import g4w8a8 as g4
 
@@ -15,6 +16,8 @@ _vp = ctypes.c_void_p
 _KIND_NAMES = {"float32": g4.KIND_F32, "float16": g4.KIND_F16, "int8": g4.KIND_I8,
                "int32": g4.KIND_I32, "uint8": None}
 _kinds = {}  # dtype object -> kind, filled as dtypes are met
+_X_KINDS = (g4.KIND_F32, g4.KIND_F16, g4.KIND_I8)
+_F32, _I32, _F16 = (g4.KIND_F32,), (g4.KIND_I32,), (g4.KIND_F16,)
 
 
 def _kind(x):
@@ -27,50 +30,49 @@ def _kind(x):
         return _kinds.setdefault(x.dtype, _KIND_NAMES[name])
 
 
-def _address(x, what):
+def _device() -> int:
+    """The current device, which torch tensors have to be on (asked once a call)."""
+    torch = sys.modules.get("torch")
+    return torch.cuda.current_device() if torch is not None and torch.cuda.is_initialized() else 0
+
+
+def _address(x, what, device):
     """The device address of a buffer or tensor. A host tensor, or one of another device than the
     current one, is refused: its address means nothing to a kernel launched here."""
     try:
         p = x.data_ptr()
     except AttributeError:
-        p = x.ptr
-        if not p:
-            raise g4.G4Error(1, f"{what} has no device memory")
-        return p
-    if not x.is_cuda:
-        raise g4.G4Error(1, f"{what} is not in device memory")
-    if x.get_device() != _current_device():
-        raise g4.G4Error(1, f"{what} is on another device than the current one")
+        if not x.ptr:
+            raise g4.G4Error(1, f"{what} has no device memory") from None
+        return x.ptr
+    if x.get_device() != device:
+        raise g4.G4Error(1, f"{what} is on another device than the current one" if x.is_cuda else
+                         f"{what} is not in device memory")
     return p
 
 
-def _current_device():
-    import torch
-    return torch.cuda.current_device()
-
-
-def _packed(x, what, kinds=None, shape=None):
-    """(address, kind) of a contiguous operand of one of `kinds`, with the sizes of `shape` (None: any)."""
-    kind = _kind(x)
-    if kinds is not None and kind not in kinds:
+def _packed(x, what, kinds, shape, device):
+    """The address of a contiguous operand of one of `kinds` and of `shape`."""
+    if _kind(x) not in kinds:
         raise g4.G4Error(1, f"{what} cannot be {x.dtype}")
-    if shape is not None:
-        got = tuple(x.shape)
-        if len(got) != len(shape) or any(w is not None and w != n for w, n in zip(shape, got)):
-            raise g4.G4Error(1, f"{what} has shape {list(got)}, expected "
-                                f"{['any' if w is None else w for w in shape]}")
-    if hasattr(x, "is_contiguous") and not x.is_contiguous():
+    if x.shape != shape:
+        raise g4.G4Error(1, f"{what} has shape {list(x.shape)}, expected {list(shape)}")
+    try:
+        packed = x.is_contiguous()
+    except AttributeError:  # a DeviceBuffer is
+        packed = not hasattr(x, "stride")
+    if not packed:
         raise g4.G4Error(1, f"{what} must be contiguous")
-    return _address(x, what), kind
+    return _address(x, what, device)
 
 
-def _rows(x, what, kinds, heads, dim, tokens):
+def _rows(x, what, kinds, heads, dim, tokens, device):
     """(address, kind, elements between tokens) of a [tokens][heads][dim] operand, whose tokens may
     lie apart (part of a wider projection's output)."""
     kind = _kind(x)
     if kind not in kinds:
         raise g4.G4Error(1, f"{what} cannot be {x.dtype}")
-    if tuple(x.shape) != (tokens, heads, dim):
+    if x.shape != (tokens, heads, dim):
         raise g4.G4Error(1, f"{what} has shape {list(x.shape)}, expected {[tokens, heads, dim]}")
     stride = heads * dim
     if hasattr(x, "stride"):
@@ -79,7 +81,7 @@ def _rows(x, what, kinds, heads, dim, tokens):
             raise g4.G4Error(1, f"{what}: a token's heads must be packed, and its tokens apart")
         if tokens > 1:
             stride = st[0]
-    return _address(x, what), kind, stride
+    return _address(x, what, device), kind, stride
 
 
 class KVPagesStruct(ctypes.Structure):
@@ -121,14 +123,14 @@ class KVPages:
         page_stride, slot, head = strides[0], *(reversed(strides[1:]) if heads_first else strides[1:])
         self.buffers = (k, v, k_scales, v_scales)
         self.kind, self.kv_heads, self.head_dim, self.page_size = kind, heads, dim, slots
-        s = [None, None]
+        s, device = [None, None], _device()
         if kind == g4.KIND_I8:
             if k_scales is None or v_scales is None:
                 raise g4.G4Error(1, "int8 pages need their scales")
-            s = [_packed(x, "page scales", (g4.KIND_F32,), (pages, heads, slots))[0] for x in (k_scales, v_scales)]
+            s = [_packed(x, "page scales", _F32, (pages, heads, slots), device) for x in (k_scales, v_scales)]
         elif k_scales is not None or v_scales is not None:
             raise g4.G4Error(1, "f16 pages have no scales")
-        self.c = KVPagesStruct(_address(k, "k pages"), _address(v, "v pages"), s[0], s[1], kind, pages, slots,
+        self.c = KVPagesStruct(_address(k, "k pages", device), _address(v, "v pages", device), s[0], s[1], kind, pages, slots,
                                heads, dim, page_stride, slot, head)
         self.ref = ctypes.byref(self.c)
 
@@ -150,18 +152,14 @@ class Chunk:
             stride = st[0] if seqs > 1 else width
         if _kind(page_table) != g4.KIND_I32:
             raise g4.G4Error(1, f"page_table cannot be {page_table.dtype}")
-        i32 = (g4.KIND_I32,)
+        device = _device()
         self.buffers = (q_start, kv_len, page_table)
         self.seqs, self.tokens, self.max_q, self.max_kv = seqs, int(tokens), int(max_q), int(max_kv)
         self.c = ChunkStruct(seqs, self.tokens, self.max_q, self.max_kv,
-                             _packed(q_start, "q_start", i32, (seqs + 1,))[0],
-                             _packed(kv_len, "kv_len", i32, (seqs,))[0],
-                             _address(page_table, "page_table"), width, stride)
+                             _packed(q_start, "q_start", _I32, (seqs + 1,), device),
+                             _packed(kv_len, "kv_len", _I32, (seqs,), device),
+                             _address(page_table, "page_table", device), width, stride)
         self.ref = ctypes.byref(self.c)
-
-
-_X_KINDS = (g4.KIND_F32, g4.KIND_F16, g4.KIND_I8)
-_F32, _I32, _F16 = (g4.KIND_F32,), (g4.KIND_I32,), (g4.KIND_F16,)
 
 
 def paged_prologue(pages, chunk, q, k, v, q_out, q_gain=None, k_gain=None, cos=None, sin=None, eps=1e-6,
@@ -170,7 +168,7 @@ def paged_prologue(pages, chunk, q, k, v, q_out, q_gain=None, k_gain=None, cos=N
     q [tokens][heads][head_dim], k and v [tokens][kv_heads][head_dim], of one type (f32, f16, or int8
     codes times q_scale / k_scale / v_scale, each x_scale where not given); their tokens may lie apart.
     q and q_out None: only the store; k and v None: only the queries."""
-    d, t = pages.head_dim, chunk.tokens
+    d, t, device = pages.head_dim, chunk.tokens, _device()
     kind, heads = None, 0
     qa = ka = va = (None, None, 0)
     qo = None
@@ -180,26 +178,28 @@ def paged_prologue(pages, chunk, q, k, v, q_out, q_gain=None, k_gain=None, cos=N
         raise g4.G4Error(1, "paged-prologue needs q and q_out together")
     if q is not None:
         heads = int(q.shape[1])
-        qa = _rows(q, "q", _X_KINDS, heads, d, t)
-        qo = _packed(q_out, "q_out", _F16, (t, heads, d))[0]
+        qa = _rows(q, "q", _X_KINDS, heads, d, t, device)
+        qo = _packed(q_out, "q_out", _F16, (t, heads, d), device)
         kind = qa[1]
     if k is not None:
-        ka = _rows(k, "k", _X_KINDS, pages.kv_heads, d, t)
-        va = _rows(v, "v", _X_KINDS, pages.kv_heads, d, t)
+        ka = _rows(k, "k", _X_KINDS, pages.kv_heads, d, t, device)
+        va = _rows(v, "v", _X_KINDS, pages.kv_heads, d, t, device)
         if va[1] != ka[1] or kind not in (None, ka[1]):
             raise g4.G4Error(1, "paged-prologue: q, k and v must be of one type")
         kind = ka[1]
-    gains = [None if g is None else _packed(g, n, _F32, (d,))[0] for g, n in ((q_gain, "q_gain"), (k_gain, "k_gain"))]
-    tabs, positions = [None, None], 0
+    qg = None if q_gain is None else _packed(q_gain, "q_gain", _F32, (d,), device)
+    kg = None if k_gain is None else _packed(k_gain, "k_gain", _F32, (d,), device)
+    tab_c, tab_s, positions = None, None, 0
     if cos is not None or sin is not None:
         if cos is None or sin is None:
             raise g4.G4Error(1, "paged-prologue needs cos and sin together")
         positions = int(cos.shape[0])
-        tabs = [_packed(x, n, _F32, (positions, d // 2))[0] for x, n in ((cos, "cos"), (sin, "sin"))]
+        tab_c = _packed(cos, "cos", _F32, (positions, d // 2), device)
+        tab_s = _packed(sin, "sin", _F32, (positions, d // 2), device)
     st = g4.lib().g4_paged_prologue(
         pages.ref, chunk.ref, g4.KIND_F32 if kind is None else kind, qa[0], qa[2],
         x_scale if q_scale is None else q_scale, ka[0], ka[2], x_scale if k_scale is None else k_scale, va[0], va[2],
-        x_scale if v_scale is None else v_scale, heads, gains[0], gains[1], tabs[0], tabs[1], positions, eps, qo, stream)
+        x_scale if v_scale is None else v_scale, heads, qg, kg, tab_c, tab_s, positions, eps, qo, stream)
     if st:
         g4._check(st)
 
@@ -208,21 +208,20 @@ def kv_read(pages, chunk, k_out, v_out, stream=None):
     """g4_kv_read: the chunk's rows back from the cache, f32 or f16, to [tokens][kv_heads][head_dim],
     or to [seqs][rows][kv_heads][head_dim] with rows >= max_q (row i of a sequence at [s][i]; the rest
     is left as it was). k_out or v_out may be None."""
-    kinds, at, stride = [], [], 0
+    device, kinds, at = _device(), [], []
     for x, what in ((k_out, "k_out"), (v_out, "v_out")):
         if x is None:
             at.append(None)
             continue
         if len(x.shape) == 4:
-            if x.shape[1] < min(chunk.max_q, chunk.tokens):
-                raise g4.G4Error(1, f"{what} holds {x.shape[1]} rows a sequence, max_q is {chunk.max_q}")
-            want = (chunk.seqs, None, pages.kv_heads, pages.head_dim)
-            mine = int(x.shape[1]) * pages.kv_heads * pages.head_dim
+            rows = int(x.shape[1])
+            if rows < min(chunk.max_q, chunk.tokens):
+                raise g4.G4Error(1, f"{what} holds {rows} rows a sequence, max_q is {chunk.max_q}")
+            want = (chunk.seqs, rows, pages.kv_heads, pages.head_dim)
         else:
-            want, mine = (chunk.tokens, pages.kv_heads, pages.head_dim), 0
-        p, kind = _packed(x, what, (g4.KIND_F32, g4.KIND_F16), want)
-        at.append(p)
-        kinds.append((kind, mine))
+            rows, want = 0, (chunk.tokens, pages.kv_heads, pages.head_dim)
+        at.append(_packed(x, what, (g4.KIND_F32, g4.KIND_F16), want, device))
+        kinds.append((_kind(x), rows * pages.kv_heads * pages.head_dim))
     if not kinds or kinds[0] != kinds[-1]:
         raise g4.G4Error(1, "kv-read needs k_out and v_out of one type and layout, or one of them")
     st = g4.lib().g4_kv_read(pages.ref, chunk.ref, at[0], at[1], kinds[0][0], kinds[0][1], stream)
@@ -240,11 +239,11 @@ def attention_chunk_workspace_bytes(pages, chunk, heads, window=0) -> int:
 def attention_chunk(pages, chunk, q, out, workspace, scale=1.0, window=0, in_scale=0.0, stream=None):
     """g4_attention_chunk: causal attention of the chunk's rows over the cache. q f16 [tokens][heads]
     [head_dim] (tokens may lie apart); out f16, f32, or int8 codes on in_scale, packed."""
-    heads = int(q.shape[1])
-    qp, _, stride = _rows(q, "q", _F16, heads, pages.head_dim, chunk.tokens)
-    op, kind = _packed(out, "out", _X_KINDS, (chunk.tokens, heads, pages.head_dim))
+    heads, device = int(q.shape[1]), _device()
+    qp, _, stride = _rows(q, "q", _F16, heads, pages.head_dim, chunk.tokens, device)
+    op = _packed(out, "out", _X_KINDS, (chunk.tokens, heads, pages.head_dim), device)
     st = g4.lib().g4_attention_chunk(pages.ref, chunk.ref, qp, stride, heads, scale, window,
-                                     _address(workspace, "workspace"), workspace.nbytes, op, kind, in_scale, stream)
+                                     _address(workspace, "workspace", device), workspace.nbytes, op, _kind(out), in_scale, stream)
     if st:
         g4._check(st)
 
@@ -262,17 +261,18 @@ def verify_drafts(logits, draft_logits, draft_tokens, draft_start, u, u_next, to
     draft_logits f32 [drafts][vocab] or None, draft_tokens int32 [drafts], draft_start int32 [seqs + 1],
     u f32 [drafts] and u_next f32 [seqs] in [0, 1) (None when greedy); tokens int32 and logprobs f32 (or
     None) [seqs][max_drafts + 1] and accepted int32 [seqs] out."""
+    device = _device()
     seqs, drafts = int(draft_start.shape[0]) - 1, int(draft_tokens.shape[0])
     vocab, width = int(logits.shape[1]), int(tokens.shape[1])
     st = g4.lib().g4_verify_drafts(
-        _packed(logits, "logits", _F32, (drafts + seqs, vocab))[0],
-        None if draft_logits is None else _packed(draft_logits, "draft_logits", _F32, (drafts, vocab))[0],
-        _packed(draft_tokens, "draft_tokens", _I32, (drafts,))[0], _packed(draft_start, "draft_start", _I32, (seqs + 1,))[0],
-        seqs, drafts, width - 1, vocab, cap, temperature,
-        None if u is None else _packed(u, "u", _F32, (drafts,))[0],
-        None if u_next is None else _packed(u_next, "u_next", _F32, (seqs,))[0],
-        _address(workspace, "workspace"), workspace.nbytes, _packed(tokens, "tokens", _I32, (seqs, width))[0],
-        _packed(accepted, "accepted", _I32, (seqs,))[0],
-        None if logprobs is None else _packed(logprobs, "logprobs", _F32, (seqs, width))[0], stream)
+        _packed(logits, "logits", _F32, (drafts + seqs, vocab), device),
+        None if draft_logits is None else _packed(draft_logits, "draft_logits", _F32, (drafts, vocab), device),
+        _packed(draft_tokens, "draft_tokens", _I32, (drafts,), device),
+        _packed(draft_start, "draft_start", _I32, (seqs + 1,), device), seqs, drafts, width - 1, vocab, cap, temperature,
+        None if u is None else _packed(u, "u", _F32, (drafts,), device),
+        None if u_next is None else _packed(u_next, "u_next", _F32, (seqs,), device),
+        _address(workspace, "workspace", device), workspace.nbytes, _packed(tokens, "tokens", _I32, (seqs, width), device),
+        _packed(accepted, "accepted", _I32, (seqs,), device),
+        None if logprobs is None else _packed(logprobs, "logprobs", _F32, (seqs, width), device), stream)
     if st:
         g4._check(st)

@@ -29,8 +29,8 @@ def probabilities(x, cap, t):
 
 
 def verify(logits, draft_logits, drafts, start, u, u_next, max_drafts, cap, t):
-    """(tokens, accepted, logprobs, margin): margin is how near a decision came to going the other way, in
-    probability."""
+    """(tokens, accepted, logprobs, margin): margin is how near a decision came to going the other way: of a
+    draft in parts of its probability, of a draw in parts of the total."""
     t = float(np.float32(t))
     seqs = len(start) - 1
     tokens = np.full((seqs, max_drafts + 1), -1, np.int32)
@@ -57,7 +57,7 @@ def verify(logits, draft_logits, drafts, start, u, u_next, max_drafts, cap, t):
                         q[d] = 1.0
                     take = inside and float(u[a + i]) * q[d] < p[d]
                     if inside and (q[d] or p[d]):  # 0 < 0 is decided exactly
-                        margin = min(margin, abs(float(u[a + i]) * q[d] - p[d]))
+                        margin = min(margin, abs(float(u[a + i]) * q[d] - p[d]) / max(q[d], p[d]))
                 if take:
                     tokens[s, i], lp[s, i] = d, logp[d]
                     accepted[s] = i + 1
@@ -100,17 +100,18 @@ def case(counts, vocab, seed, blur=0.7, spread=3.0):
     return logits, draft_logits, drafts, start, r.random(n).astype(np.float32), r.random(len(counts)).astype(np.float32)
 
 
-# Sums of 64-bit weights of relative error 2^-50: far under any margin that random inputs come to. f32
-# log probabilities: half a step of the value, and 2^-45 before it.
+# Weights of relative error 2^-39 and 64-bit sums: a decision whose margin is over 2^-34 of the total is the
+# same.
+# f32 log probabilities: half a step of the value, and 2^-38 before it.
 def check(c, max_drafts, cap, t, drafter=True):
     logits, dl, drafts, start, u, un = c
     dl = dl if drafter else None
     want = verify(logits, dl, drafts, start, u, un, max_drafts, cap, t)
-    assert t == 0 or want[3] > 2.0 ** -44  # the inputs decide, not the last bits
+    assert t == 0 or want[3] > 2.0 ** -32  # the inputs decide, not the last bits
     got = run(logits, dl, drafts, start, u, un, max_drafts, cap, t)
     assert np.array_equal(got[1], want[1])
     assert np.array_equal(got[0], want[0])
-    assert (np.abs(got[2] - want[2]) <= np.abs(want[2]) * 2.0 ** -24 * 1.01 + 2.0 ** -40).all()
+    assert (np.abs(got[2] - want[2]) <= np.abs(want[2]) * 2.0 ** -24 * 1.01 + 2.0 ** -36).all()
     return got
 
 

@@ -14,7 +14,10 @@
 // The softmax keeps a running maximum (base 2) and sum in f32; the maximum moves, and the output is
 // rescaled, only when a score passes it by more than 2^8, so weights reach 2^8 at most and are rounded to
 // f16 (11 bits; an f16 cache's sum adds the rounded ones, an int8 cache's the exact ones, whose weights
-// are rounded with V's scale in them). int8 rows: codes are exact in f16; K's scale multiplies the
+// are rounded with V's scale in them). int8 rows: the scores are integer products of K's codes
+// with Q as 16-bit fixed point of the row's largest magnitude, in two 8-bit digits (v_mfma_i32_32x32x32_i8 twice:
+// the matrix time of one f16 product and none of the conversion, 96 vector operations a tile; an element of Q
+// is off by 2^-17 of the largest at most, where f16 holds one of an eighth of it to 2^-15); K's scale multiplies the
 // score, V's the weight, taken relative to a power of two above the largest scale that the row has seen,
 // which scales the row's output and sum (f16 would not hold scales of every size) and enters the weights
 // by their exponent.
@@ -26,7 +29,8 @@ namespace g4 {
 
 typedef float f16x __attribute__((ext_vector_type(16)));
 typedef float f4 __attribute__((ext_vector_type(4)));
-typedef float f2 __attribute__((ext_vector_type(2)));
+typedef int i16x __attribute__((ext_vector_type(16)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 // Division of n < 2^31 by a constant of the call, d > 1: (n * mul) >> (31 + log), log = ceil(log2 d) and
 // mul = floor(2^(31 + log) / d) + 1, which is under 2^32 and whose excess over 2^(31 + log) / d is at most
@@ -50,8 +54,8 @@ struct AttnArgs {
     int heads;
     FastDiv group;
     // Scores are kept as the products give them; the base-2 exponent is score * scale2, scale2 > 0. A
-    // negative scale turns Q's signs over; lazy is kLazy / scale2.
-    float scale2, lazy;
+    // negative scale turns Q's signs over.
+    float scale2;
     uint32_t q_sign;  // 0x80008000: Q is turned over
     uint32_t page_bytes, slot_bytes;
     int window;
@@ -98,18 +102,10 @@ __device__ __forceinline__ h8 words_h8(uint32_t a, uint32_t b, uint32_t c, uint3
     return __builtin_bit_cast(h8, w);
 }
 
-// An int8 code as f16 without arithmetic: the byte code + 128 zero-extended is the subnormal
-// (code + 128) 2^-24, exact, and the matrix products keep subnormals. The 128s come off outside: from the
-// scores as the accumulator's start, -128 2^-24 sum(q), and from the output by the sum of the rounded
-// weights. (Products of at most 2^8 2^8 codes' bits: f32 sums of them lose about what sums of the codes
-// alone would, the bias being three times a typical code.)
-// Eight codes, two words:
-__device__ __forceinline__ h8 codes_h8(uint32_t a, uint32_t b) {
-    a ^= 0x80808080u;
-    b ^= 0x80808080u;
-    return words_h8(__builtin_amdgcn_perm(0u, a, 0x0c010c00u), __builtin_amdgcn_perm(0u, a, 0x0c030c02u),
-                    __builtin_amdgcn_perm(0u, b, 0x0c010c00u), __builtin_amdgcn_perm(0u, b, 0x0c030c02u));
-}
+// A V code as f16 without arithmetic: the byte code + 128 zero-extended is the subnormal (code + 128) 2^-24,
+// exact, and the matrix products keep subnormals. The 128s come off the output at the end, by the sum of the
+// rounded weights. (Products of at most 2^8 2^8 codes' bits: f32 sums of them lose about what sums of the
+// codes alone would, the bias being three times a typical code.)
 // Element j of words a and b as a pair; the codes' signs are flipped already.
 template <int J>
 __device__ __forceinline__ uint32_t code_pair(uint32_t a, uint32_t b) {
@@ -178,17 +174,24 @@ __device__ __forceinline__ int split_tiles(const Tile &T, const FastDiv &splits,
     return max(splits.div(n + (int)splits.d - 1) + unit - 1, unit) & ~(unit - 1);
 }
 
-__device__ __forceinline__ void attn_put4(const AttnArgs &R, int64_t at, float4 y) {
-    if (R.out_kind == G4_KIND_F16) {
-        const h4 o = {(_Float16)y.x, (_Float16)y.y, (_Float16)y.z, (_Float16)y.w};
-        *reinterpret_cast<h4 *>(static_cast<_Float16 *>(R.out) + at) = o;
-    } else if (R.out_kind == G4_KIND_I8) {
-        const float s = R.in_scale;
-        *reinterpret_cast<uint32_t *>(static_cast<int8_t *>(R.out) + at) =
-            (srq_code_i(y.x, s) & 255) | (srq_code_i(y.y, s) & 255) << 8 | (srq_code_i(y.z, s) & 255) << 16 |
-            (uint32_t)(srq_code_i(y.w, s) & 255) << 24;
+// N times 4 values to elements at(n), rounded or quantised as the output's kind says.
+template <int N, typename F>
+__device__ __forceinline__ void attn_put(void *out, int kind, float in_scale, const float4 (&y)[N], F at) {
+    if (kind == G4_KIND_F32) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) *reinterpret_cast<float4 *>(static_cast<float *>(out) + at(n)) = y[n];
+    } else if (kind == G4_KIND_F16) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const h4 o = {(_Float16)y[n].x, (_Float16)y[n].y, (_Float16)y[n].z, (_Float16)y[n].w};
+            *reinterpret_cast<h4 *>(static_cast<_Float16 *>(out) + at(n)) = o;
+        }
     } else {
-        *reinterpret_cast<float4 *>(static_cast<float *>(R.out) + at) = y;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            *reinterpret_cast<uint32_t *>(static_cast<int8_t *>(out) + at(n)) =
+                (srq_code_i(y[n].x, in_scale) & 255) | (srq_code_i(y[n].y, in_scale) & 255) << 8 |
+                (srq_code_i(y[n].z, in_scale) & 255) << 16 | (uint32_t)(srq_code_i(y[n].w, in_scale) & 255) << 24;
     }
 }
 
@@ -199,22 +202,26 @@ __device__ __forceinline__ void attn_put4(const AttnArgs &R, int64_t at, float4 
 // straight to LDS as the rows stand in the cache, a ring of NS tiles each.
 //  RT 1: a wave waits for its own loads only, and refills the K half of its buffer as soon as the scores
 //        are done and the V half after the output (NS 1);
-//  RT 2, 4: one block barrier per key tile, NS tiles in flight.
+//  RT 2, 4: two block barriers a key tile, one before the softmax and one after it, and waves 4..7 one barrier
+//        behind waves 0..3: of the two waves that share a SIMD, one has the matrix unit (a tile's output and
+//        the next tile's scores) while the other has the vector unit. K comes two tiles ahead and V one.
 template <int D, int CK, int RT>
 struct Shape {
     static constexpr int EB = CK == G4_KIND_I8 ? 1 : 2;  // bytes of an element
     static constexpr int RB = D * EB;                    // of a row
     static constexpr int HALF = kKeys * RB;              // of a tile's K or V
-    static constexpr int KG = RT == 1 ? 4 : (RT == 2 && RB < 512 ? 4 : 2);
+    static constexpr int KG = RT == 1 || (RT == 2 && CK == G4_KIND_I8) ? 4 : 2;
     static constexpr int NS = RT == 1 ? 1 : 2;
     static constexpr int WAVES = RT * KG;
     static constexpr int RING = KG * NS * 2 * HALF;
-    // int8: the scales of a wave's tiles, ks[32] and vs[32] a tile, and one more tile ahead
-    static constexpr int SCALES = CK == G4_KIND_I8 ? WAVES * 2 * 256 : 0;
-    static constexpr int JOIN = WAVES * (D / 8) * 72 * 4;  // a quarter of every wave's output (see the end)
+    // int8: the scales of a key group's tiles, for each 8 keys K's and then V's; they come with K
+    static constexpr int NSC = NS + 1, SCALES = CK == G4_KIND_I8 ? KG * NSC * 256 : 0;
+    // quarters of every wave's output that are joined at a time (see the end): as many as the ring holds
+    static constexpr int PH = WAVES * D * 128 <= RING ? 4 : (WAVES * D * 64 <= RING ? 2 : 1);
+    static constexpr int JOIN = WAVES * D * 32 * PH;
     // Q's last operands wait in LDS where two waves a SIMD share the registers: output and Q alone take 192 of 256
-    static constexpr int QL = D != 256 ? 0 : (WAVES == 8 ? 3 : (RT == 1 && CK == G4_KIND_I8 ? 3 : 0));
-    static constexpr bool TIGHT = D == 256 && CK == G4_KIND_F16 && WAVES == 8;  // no registers for V's reads ahead
+    static constexpr int QL = D == 256 && (CK == G4_KIND_I8 || RT == 4) ? 3 : 0;
+    static constexpr bool TIGHT = D == 256 && CK == G4_KIND_F16 && RT == 4;  // no registers for V's reads ahead
     static constexpr int LDS = (RING > JOIN ? RING : JOIN) + SCALES + WAVES * (kRows * 8 + QL * 1024);
     static constexpr int MIN_WAVES = WAVES == 4 && LDS > 80 * 1024 ? 1 : 2;  // per SIMD: one block a CU, or two
 };
@@ -236,9 +243,18 @@ __device__ __forceinline__ void dma16(const char *base, uint32_t off, uint32_t l
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2"
                  :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off), "s"(b) : "memory", "m0");
 }
+template <int LANES>
 __device__ __forceinline__ void dma4(const void *src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
-                 :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src) : "memory", "m0");
+    // the first LANES lanes, by the mask rather than by a branch (the wave is whole here)
+    uint64_t all;
+    if constexpr (LANES == 64)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+                     :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src) : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, exec\n\ts_mov_b64 exec, %3\n\ts_nop 0\n\t"
+                     "global_load_lds_dword %2, off\n\ts_mov_b64 exec, %0"
+                     : "=&s"(all)
+                     : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src), "s"((1ull << LANES) - 1) : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void wait_loads() {
@@ -268,24 +284,20 @@ template <int D> struct VDims {
     static constexpr int UD = D == 64 ? 2 : 4, U = D / (32 * UD);
 };
 
-// The pages of a key tile's four 8-key groups, below 0 where absent. Named, not an array: an array is
-// indexed in memory, which makes its values per-lane ones.
-struct Pages {
-    int a, b, c, d;
-    __device__ __forceinline__ int of(int g) const {
-        const int lo = g & 1 ? b : a, hi = g & 1 ? d : c;
-        return g & 2 ? hi : lo;
-    }
+// What a wave needs to load its 8-key groups of a key tile: bytes to the group in the pools, and in the
+// scales' (int8); there: which of the tile's four groups have a page, a bit each.
+template <int GW>
+struct Next {
+    uint64_t off[GW], row[GW];
+    uint32_t there;
 };
-
-typedef const __attribute__((address_space(4))) int32_t *ConstI32;  // uniform reads by the scalar unit
 
 template <int D, int CK, int RT>
 __global__ __launch_bounds__((64 * Shape<D, CK, RT>::WAVES), (Shape<D, CK, RT>::MIN_WAVES))
 void attn_kernel(PagedArgs A, AttnArgs R) {
     using P = Shape<D, CK, RT>;
     constexpr bool I8 = CK == G4_KIND_I8;
-    constexpr int EB = P::EB, RB = P::RB, KG = P::KG, NS = P::NS, KS = D / 16, DPL = D / 32;
+    constexpr int EB = P::EB, RB = P::RB, KG = P::KG, NS = P::NS, KS = D / 16, DPL = D / 32, NK = RB / 32;  // NK: K reads of a lane
     constexpr int UD = VDims<D>::UD, U = VDims<D>::U, VB = UD * EB;   // VB: bytes of a lane's read of a V row
     constexpr int GB = 8 * RB;                                        // bytes of an 8-key group
     constexpr int NI = GB >= 1024 ? GB / 1024 : 1;                    // loads of a group
@@ -306,49 +318,69 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
 
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
     constexpr int SC0 = P::RING > P::JOIN ? P::RING : P::JOIN, ML0 = SC0 + P::SCALES, Q0 = ML0 + P::WAVES * kRows * 8;
-    char *const scales = lds + SC0 + wave * 512;
+    char *const scales = lds + SC0 + kg * P::NSC * 256;
     float2 *const ml = reinterpret_cast<float2 *>(lds + ML0);
 
-    // the page of each 8-key group of this key group's tile t (absent: below 0), by the scalar unit
-    const ConstI32 table = (ConstI32)(uintptr_t)(A.table + T.seq * A.table_stride);
-    const int last = T.S.kv - 1;  // >= 0 where there are rounds
-    auto page_at = [&](int p) {
-        const int x = table[min(p, max(last, 0)) >> A.page_shift];
-        return (unsigned)x < (unsigned)A.num_pages ? x : -1;
+    // Pages: lane l looks up 8-key group l % 4 of the key group's tile 16 w + l / 4, 16 tiles at a time and
+    // a tile ahead; a tile's four pages are then register reads (a scalar load per tile would be waited
+    // for with the tile's LDS reads: they share a counter).
+    const int last = max(T.S.kv - 1, 0);
+    const int32_t *const table = A.table + T.seq * A.table_stride;
+    auto tile_at = [&](int i) { return k0 + (i * KG + kg) * kKeys; };
+    auto look_up = [&](int w) {
+        return table[min(tile_at(16 * w + lane / 4) + 8 * (lane % 4), last) >> A.page_shift];
     };
-    auto pages_of = [&](int t) { return Pages{page_at(t), page_at(t + 8), page_at(t + 16), page_at(t + 24)}; };
     const int smask = (1 << A.page_shift) - 1;
     const char *const k_pool = static_cast<const char *>(A.k) + (int64_t)kvh * A.head_stride * EB;
     const char *const v_pool = static_cast<const char *>(A.v) + (int64_t)kvh * A.head_stride * EB;
     const uint32_t load_rows = 64 / LPR * R.slot_bytes;  // from one load of a group to the next: 64 / LPR rows
-    auto group_base = [&](const char *pool, int t, int g, int page) {  // an absent group reads page 0
-        const int slot = min(t + 8 * g, max(last, 0)) & smask & ~7;
-        return pool + ((uint64_t)(uint32_t)max(page, 0) * R.page_bytes + (uint32_t)slot * R.slot_bytes);
-    };
-    // the loop recomputes what hangs on the lane alone (see `fresh`), loads' addresses among it
-    auto load_half = [&](const char *pool, bool swizzle, int t, const Pages &pg, uint32_t at, int lane) {
-        const uint32_t off_row = (uint32_t)(lane / LPR) * R.slot_bytes;
+    int page_v = 0;      // the pages of 16 tiles, or once the last of them is read out the next 16, not yet checked
+    uint64_t there = 0;  // bit l: lane l's is one
+    auto next_tile = [&](int j) {  // for j = 0, 1, ... in turn
+        if ((j & 15) == 0) {
+            there = __ballot((unsigned)page_v < (unsigned)A.num_pages);
+            page_v = (unsigned)page_v < (unsigned)A.num_pages ? page_v : 0;  // an absent group reads page 0
+        }
+        const int l = (j & 15) * 4;
+        Next<GW> N;
+        N.there = (uint32_t)(there >> l) & 15;
 #pragma unroll
         for (int i = 0; i < GW; ++i) {
-            const int g = rt * GW + i;
-            const int page = pg.of(g);
-            const char *base = group_base(pool, t, g, page);
+            const uint32_t page = __builtin_amdgcn_readlane(page_v, l + rt * GW + i);
+            const uint32_t at = min(tile_at(j) + 8 * (rt * GW + i), last) & smask & ~7;
+            N.off[i] = (uint64_t)page * R.page_bytes + at * R.slot_bytes;
+            N.row[i] = (((uint64_t)page * A.kv_heads + kvh) << A.page_shift) + at;
+        }
+        if ((j & 15) == 15) page_v = look_up(j / 16 + 1);
+        return N;
+    };
+    // the loop recomputes what hangs on the lane alone (see `fresh`), loads' addresses among it
+    auto load_half = [&](const char *pool, bool swizzle, const Next<GW> &N, uint32_t at, uint32_t lane) {
+        const uint32_t off_row = lane / LPR * R.slot_bytes, x = lane % LPR;
+#pragma unroll
+        for (int i = 0; i < GW; ++i) {
+            const char *base = pool + N.off[i];
             if (GB >= 1024 || lane < GB / 16)
 #pragma unroll
                 for (int n = 0; n < NI; ++n) {
-                    const int x = lane % LPR, r = n * (64 / LPR) + lane / LPR;
-                    dma16(base + n * load_rows, off_row + (swizzle ? x ^ k_swizzle<RB>(r) : x) * 16, at + g * GB + n * 1024);
+                    const int r = n * (64 / LPR) + lane / LPR;
+                    dma16(base + n * load_rows, off_row + (swizzle ? x ^ k_swizzle<RB>(r) : x) * 16,
+                          at + (rt * GW + i) * GB + n * 1024);
                 }
         }
     };
-    auto load_scales = [&](int t, const Pages &pg, int slot, int lane) {  // lane c: ks (half 0) or vs of key c
-        const int c = lane & 31, h = lane >> 5;
-        const int p = min(t + c, max(last, 0));
-        const int page = pg.of(c >> 3);
-        dma4((h ? A.vs : A.ks) + scale_offset(A, max(page, 0), p, kvh), lds0 + SC0 + wave * 512 + slot * 256);
+    // The scales of the wave's groups: lane 16 i + n is key n of group rt GW + i, of K (n < 8) or V.
+    auto load_scales = [&](const Next<GW> &N, int slot, uint32_t lane) {
+        uint64_t row = N.row[0];
+#pragma unroll
+        for (int i = 1; i < GW; ++i) {
+            uint64_t r = N.row[i];
+            asm volatile("" : "+s"(r));  // a value: or the array is kept in memory and indexed by the lane
+            row = lane >> 4 == (uint32_t)i ? r : row;
+        }
+        dma4<16 * GW>((lane & 8 ? A.vs : A.ks) + row + (lane & 7), lds0 + SC0 + (kg * P::NSC + slot) * 256 + rt * GW * 64);
     };
     auto ring = [&](int slot, int half) { return (uint32_t)(((kg * NS + slot) * 2 + half) * P::HALF); };
-    auto tile_at = [&](int i) { return k0 + (i * KG + kg) * kKeys; };
 
     // this lane's query row
     const int first = T.first + rt * kRows;  // of this wave
@@ -358,129 +390,266 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
     const int pos = real ? T.S.kv - T.S.rows + token : -1;
     const int p_first = T.S.kv - T.S.rows + R.group.div(first);  // the wave's first row, and its last
     const int p_last = T.S.kv - T.S.rows + R.group.div(max(min(first + kRows, T.rows) - 1, 0));
+    const int t_inner = R.window ? p_last - R.window + 1 : 0;  // the first key that every row of the wave sees
 
-    Pages pg{-1, -1, -1, -1}, pg_next = pg;
+    // of the tile whose V is loaded next; and the bits `there` of the tiles i and i + 1
+    Next<GW> ahead{};
+    uint32_t there0 = 0, there1 = 0;
     if (rounds) {
-        pg = pages_of(tile_at(0));
-        if (I8) load_scales(tile_at(0), pg, 0, lane);
-        load_half(k_pool, true, tile_at(0), pg, lds0 + ring(0, 0), lane);
-        load_half(v_pool, false, tile_at(0), pg, lds0 + ring(0, 1), lane);
-        if (rounds > 1) pg_next = pages_of(tile_at(1));
-    }
-    constexpr int QL = P::QL;
-    h8 q[KS - QL];
-    char *const q_lds = lds + Q0 + wave * QL * 1024;
-    float q_sum = 0.0f;
-    {
-        const _Float16 *src = R.q + (int64_t)(T.S.start + token) * R.q_stride + (int64_t)head * D;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            // the k-step's 8 dims of this half, in the order that K's reads give them
-            const int at = I8 ? 32 * (s / 2) + 16 * h + 8 * (s % 2) : 16 * s + 8 * h;
-            h8 x = *reinterpret_cast<const h8 *>(src + at);
-            const uint32_t sign = R.q_sign;
-            u32x4 y = __builtin_bit_cast(u32x4, x);
-#pragma unroll
-            for (int n = 0; n < 4; ++n) y[n] = real ? y[n] ^ sign : 0u;
-            x = __builtin_bit_cast(h8, y);
-            if (I8)
-#pragma unroll
-                for (int n = 0; n < 8; ++n) q_sum += (float)x[n];
-            if (s < KS - QL) q[s] = x;
-            else *reinterpret_cast<h8 *>(q_lds + (s - (KS - QL)) * 1024 + lane * 16) = x;
+        page_v = look_up(0);
+        const Next<GW> N = next_tile(0);
+        there0 = N.there;
+        if (I8) load_scales(N, 0, lane);
+        load_half(k_pool, true, N, lds0 + ring(0, 0), lane);
+        if (RT > 1 && rounds > 1) {
+            ahead = next_tile(1);
+            there1 = ahead.there;
+            if (I8) load_scales(ahead, 1, lane);
+            load_half(k_pool, true, ahead, lds0 + ring(1, 0), lane);
         }
-        if (I8) q_sum = other_half_sum(q_sum);
+        if (RT == 1) ahead = N;
+        if (RT > 1 || !I8) load_half(v_pool, false, N, lds0 + ring(0, 1), lane);
     }
-    const float s_init = I8 ? -q_sum * 0x1p-17f : 0.0f;  // the codes' bias, see codes_h8
+    auto lds_sync = [&]() {  // LDS writes and reads of the block's waves are done; loads may be on their way
+        wait_lds();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    constexpr int QL = P::QL;
+    u32x4 q[KS - QL];
+    char *const q_lds = lds + Q0 + wave * QL * 1024;
+    float sc = R.scale2;  // exponents are score * sc
+    {
+        auto put_q = [&](int s, u32x4 x) {
+            if (s < KS - QL) q[s < KS - QL ? s : 0] = x;
+            else *reinterpret_cast<u32x4 *>(q_lds + (s - (KS - QL)) * 1024 + lane * 16) = x;
+        };
+        // a lane without a row takes the sequence's first: nothing of it is kept
+        const _Float16 *src = R.q + (int64_t)(T.S.start + token) * R.q_stride + (int64_t)head * D;
+        if constexpr (I8) {
+            // In steps of 32 dims, shared out among the key groups' waves of a row tile, which exchange them in the V
+            // halves of the ring's last slot (RT 1 loads V after this)
+            static_assert(RT <= 2, "the V halves of four key groups hold two row tiles' Q");
+            constexpr int QN = NK > KG ? NK / KG : 1;
+            const int s0 = kg * QN;
+            u32x4 x[2 * QN] = {};
+            uint32_t top = 0;  // of the row's magnitudes, as f16 bits
+            if (s0 < NK) {
+#pragma unroll
+                for (int s = 0; s < 2 * QN; ++s)  // the dims of this half in the order that K's reads give them
+                    x[s] = *reinterpret_cast<const u32x4 *>(src + 32 * (s0 + s / 2) + 16 * h + 8 * (s % 2));
+#pragma unroll
+                for (int s = 0; s < 2 * QN; ++s)
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const u16x2 y = __builtin_bit_cast(u16x2, x[s][n] & 0x7fff7fffu);
+                        top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top), y));
+                    }
+            }
+            top = max(top & 0xffff, top >> 16);
+            const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+            top = max(both[0], both[1]);
+            if (h == 0) ml[wave * kRows + c].x = __uint_as_float(top);
+            lds_sync();
+#pragma unroll
+            for (int g = 0; g < KG; ++g) top = max(top, __float_as_uint(ml[(g * RT + rt) * kRows + c].x));
+            const float amax = (float)bits_h2(top)[0];
+            const float inv = top ? (R.q_sign ? -32512.0f : 32512.0f) / amax : 0.0f;
+            sc = fmaxf(R.scale2 * (amax / 32512.0f), 0x1p-100f);
+            if (top >= 0x7c00u) sc = __builtin_nanf("");  // a NaN or an infinity in Q
+            auto stage = [&](int at) {  // of the row tile's KS operands
+                const int e = rt * KS + at;
+                return lds + ring(NS - 1, 1) + (e / (KS / 2) - kg) * (NS * 2 * P::HALF) + e % (KS / 2) * 1024 + lane * 16;
+            };
+            // n = RNE(32512 q / amax); n + 128 stands in the low 16 bits of 1.5 2^23 + 128 + n: the second byte is
+            // the high digit, the low byte less 128 the low one
+            if (s0 < NK)
+#pragma unroll
+                for (int s = 0; s < QN; ++s) {
+                    u32x4 hi, lo;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t n[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            n[i] = __float_as_uint(__builtin_fmaf((float)bits_h2(x[2 * s + w / 2][w % 2 * 2 + i / 2])[i % 2], inv, 0x1.8p23f + 128.0f));
+                        const uint32_t a = __builtin_amdgcn_perm(n[1], n[0], 0x05010400u), b = __builtin_amdgcn_perm(n[3], n[2], 0x05010400u);
+                        lo[w] = __builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u;
+                        hi[w] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+                    }
+                    *reinterpret_cast<u32x4 *>(stage(2 * (s0 + s))) = hi;
+                    *reinterpret_cast<u32x4 *>(stage(2 * (s0 + s) + 1)) = lo;
+                }
+            lds_sync();
+#pragma unroll
+            for (int s = 0; s < KS; ++s) put_q(s, *reinterpret_cast<const u32x4 *>(stage(s)));
+            lds_sync();
+            if (RT == 1 && rounds) load_half(v_pool, false, ahead, lds0 + ring(0, 1), lane);
+        } else {
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                u32x4 x = *reinterpret_cast<const u32x4 *>(src + 16 * s + 8 * h);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) x[n] ^= R.q_sign;
+                put_q(s, x);
+            }
+        }
+    }
 
     f16x o[DPL];
 #pragma unroll
     for (int j = 0; j < DPL; ++j) o[j] = f16x{};
     // vref: the power of two of the row's V scales; w_sum: the sum of the rounded weights (int8)
     // off: the exponents' offset, -m scale2 - log2(vref); l is in units of vref too
-    float m = -INFINITY, l = 0.0f, vref = 0x1p-100f, w_sum = 0.0f, off = I8 ? 100.0f : 0.0f;
+    // v_low: the least vref of the wave's rows (a lane without a row keeps out of it)
+    float m = -INFINITY, l = 0.0f, vref = real ? 0x1p-100f : 0x1p100f, v_low = 0x1p-100f, w_sum = 0.0f, off = I8 ? 100.0f : 0.0f;
 
     const int lane_ = lane;
+    constexpr int KC = NK < 4 ? NK : 4, AHEAD = D == 256 && I8 && RT == 1 ? 1 : 2;
+    u32x4 k_first[RT > 1 ? AHEAD : 1];  // the tile's first K reads, made in the tile before (RT > 1)
+    int slot = 0, sc_slot = 0;
+    auto barrier = [&]() {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    auto k_read = [&](int at, int lane, int n) {
+        // chunk 2 n + h of the lane's row, swizzled: the chunk's low three bits, so an XOR of the address
+        const int c = lane & 31, kb = at + c * RB + ((lane >> 5) ^ k_swizzle<RB>(c)) * 16;
+        return *reinterpret_cast<const u32x4 *>(lds + (kb ^ (n % KC * 32)) + n / KC * KC * 32);
+    };
+    if (RT > 1 && rounds) {
+        wait_loads<0>();
+        barrier();
+        if (P::WAVES > 4 && wave >= 4) barrier();
+#pragma unroll
+        for (int n = 0; n < AHEAD && n < NK; ++n) k_first[n] = k_read(ring(0, 0), lane, n);
+    }
+    // Active: a wave with rows. One without only takes its part in the loads. (Two loops, not a branch inside: the
+    // output would be merged where the branch ends, and there are no registers for the copies.)
+    auto run = [&](auto Active) {
     for (int i = 0; i < rounds; ++i) {
         // A fresh copy of the lane index: addresses and masks that hang on it are worked out again each time
         // (a few instructions); kept across the loop they would not fit beside the output and Q.
         int lane = lane_;
-        float bias0 = s_init;
-        asm volatile("" : "+v"(lane), "+v"(bias0));
+        asm volatile("" : "+v"(lane));
         const int h = lane >> 5, c = lane & 31;
-        const int t0 = tile_at(i), slot = NS == 1 ? 0 : i % NS;
-        // which keys of the tile exist (scalar)
-        uint32_t keys = T.S.kv - t0 >= 32 ? 0xffffffffu : (T.S.kv > t0 ? (1u << (T.S.kv - t0)) - 1 : 0u);
-        if (t0 >= k1) keys = 0;
-        keys &= (pg.a < 0 ? 0u : 0xffu) | (pg.b < 0 ? 0u : 0xff00u) | (pg.c < 0 ? 0u : 0xff0000u) | (pg.d < 0 ? 0u : 0xff000000u);
+        const int t0 = tile_at(i);
+        const int sc_next = sc_slot + 1 == P::NSC ? 0 : sc_slot + 1, sc_after = sc_next + 1 == P::NSC ? 0 : sc_next + 1;
         const bool more = i + 1 < rounds;
-        if (RT == 1) {
-            wait_loads<LOADS>();  // K and the scales are here, V may be on its way
-        } else {
-            wait_loads<0>();
-            wait_lds();
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            if (more) {  // the other buffer was last read before the barrier
-                if (I8) load_scales(tile_at(i + 1), pg_next, (i + 1) & 1, lane);
-                load_half(k_pool, true, tile_at(i + 1), pg_next, lds0 + ring((i + 1) % NS, 0), lane);
-                load_half(v_pool, false, tile_at(i + 1), pg_next, lds0 + ring((i + 1) % NS, 1), lane);
-            }
-        }
-        const bool skip = !active || !keys || t0 > p_last || (R.window && t0 + kKeys - 1 <= p_first - R.window);
+        if (RT == 1) wait_loads<LOADS>();  // K and the scales are here, V may be on its way
+        // K's reads run two steps ahead (one where registers are short; no further: the scheduling barriers keep the compiler from either
+        // gathering them, for which there are no registers, or waiting for each)
+        constexpr int KB = AHEAD + 1;
+        u32x4 k[KB];
+#pragma unroll
+        for (int n = 0; n < AHEAD && n < NK; ++n)
+            k[n] = RT > 1 ? k_first[n] : k_read(ring(slot, 0), lane, n);
         f16x x;
-        if (!skip) {
-            // chunk 2 n + h of the lane's row, swizzled: the chunk's low three bits, so an XOR of the address
-            const uint32_t kb = ring(slot, 0) + c * RB + (h ^ k_swizzle<RB>(c)) * 16;
-            constexpr int KC = RB / 32 < 4 ? RB / 32 : 4;
+        uint32_t v[2 * U + 1][8][(VB + 3) / 4];  // V's reads, one step ahead
+        char *const tile = lds + ring(slot, 1);
+        const char *vb = tile + c * VB + 4 * h * RB;
+        // the lane's dims of block u, of the 8 keys of k-step s
+        auto v_words = [&](int s, int u, uint32_t (&v)[8][(VB + 3) / 4]) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = bias0;
-            // K's reads run two products ahead (and no further: the scheduling barriers keep the compiler from
-            // either gathering them, for which there are no registers, or waiting for each)
-            constexpr int NK = RB / 32, AHEAD = 2;
-            u32x4 k[NK];
-            h8 q_last[QL > 0 ? QL : 1];
-            auto read_k = [&](int n) {
-                k[n] = *reinterpret_cast<const u32x4 *>(lds + (kb ^ (n % KC * 32)) + n / KC * KC * 32);
-            };
-#pragma unroll
-            for (int n = 0; n < AHEAD && n < NK; ++n) read_k(n);
-            f4 ks[4];
-#pragma unroll
-            for (int n = 0; n < NK; ++n) {
-                if (n + AHEAD < NK) read_k(n + AHEAD);
-                if (QL && n == (KS - QL) / (I8 ? 2 : 1) - 1)  // a step before the first that needs one
-#pragma unroll
-                    for (int s = 0; s < QL; ++s) q_last[s] = *reinterpret_cast<const h8 *>(q_lds + s * 1024 + lane * 16);
-                if (I8 && n + 1 == NK)
-#pragma unroll
-                    for (int g = 0; g < 4; ++g)
-                        ks[g] = *reinterpret_cast<const f4 *>(scales + (i & 1) * 256 + (8 * g + 4 * h) * 4);
-                __builtin_amdgcn_sched_barrier(0);
-                auto q_at = [&](int s) { return s < KS - QL ? q[s < KS - QL ? s : 0] : q_last[s < KS - QL ? 0 : s - (KS - QL)]; };
-                if constexpr (I8) {
-                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_h8(k[n].x, k[n].y), q_at(2 * n), x, 0, 0, 0);
-                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(codes_h8(k[n].z, k[n].w), q_at(2 * n + 1), x, 0, 0, 0);
+            for (int n = 0; n < 8; ++n) {
+                const char *at = vb + (16 * s + 8 * (n / 4) + n % 4) * RB + u * 32 * VB;
+                if constexpr (VB == 8) {
+                    const uint2 y = *reinterpret_cast<const uint2 *>(at);
+                    v[n][0] = y.x;
+                    v[n][1] = y.y;
+                } else if constexpr (VB == 4) {
+                    v[n][0] = *reinterpret_cast<const uint32_t *>(at);
                 } else {
-                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, k[n]), q_at(n), x, 0, 0, 0);
+                    v[n][0] = *reinterpret_cast<const uint16_t *>(at);
                 }
-                __builtin_amdgcn_sched_barrier(0);
             }
+        };
+        // RT 1, between the products: the K half is free for the next tile; V has landed
+        auto refill_k = [&]() {
+            if (RT != 1 || !more) return;
+            wait_lds();
+            ahead = next_tile(i + 1);
+            if (I8) load_scales(ahead, sc_next, lane);
+            load_half(k_pool, true, ahead, lds0 + ring(0, 0), lane);
+        };
+        auto wait_v = [&]() {
+            if (RT != 1) return;
+            if (more) wait_loads<LOADS + (I8 ? 1 : 0)>();  // the next K and scales may be on their way
+            else wait_loads<0>();
+        };
+        // RT > 1, between the scores and the softmax: every wave is done with this tile's K and the last one's V,
+        // whose places the next loads take; and after the softmax: the loads made a tile ago have landed
+        auto scores_done = [&]() {
+            if (RT == 1) return;
+            barrier();
+            if (more) load_half(v_pool, false, ahead, lds0 + ring(slot ^ 1, 1), lane);
+            if (i + 2 < rounds) {
+                ahead = next_tile(i + 2);
+                if (I8) load_scales(ahead, sc_after, lane);
+                load_half(k_pool, true, ahead, lds0 + ring(slot, 0), lane);
+            }
+        };
+        auto softmax_done = [&]() {
+            if (RT == 1) return;
+            if (i + 2 < rounds) wait_loads<2 * LOADS + (I8 ? 1 : 0)>();
+            else if (more) wait_loads<LOADS>();
+            else wait_loads<0>();
+            barrier();
+        };
+        if constexpr (decltype(Active)::value) {
+            u32x4 q_last[QL > 0 ? QL : 1];
+            auto read_q_last = [&]() {
+#pragma unroll
+                for (int s = 0; s < QL; ++s) q_last[s] = *reinterpret_cast<const u32x4 *>(q_lds + s * 1024 + lane * 16);
+            };
+            auto q_at = [&](int s) { return s < KS - QL ? q[s < KS - QL ? s : 0] : q_last[s < KS - QL ? 0 : s - (KS - QL)]; };
+            f4 ks[4];
+            if constexpr (I8) {
+                // codes times Q's high digits and low ones, 256 times the first and the second put together
+                i16x a = {}, b = {};
+#pragma unroll
+                for (int n = 0; n < NK; ++n) {
+                    if (n + AHEAD < NK) k[(n + AHEAD) % KB] = k_read(ring(slot, 0), lane, n + AHEAD);
+                    if (QL && n == (KS - QL) / 2 - 1) read_q_last();  // a step before the first that needs one
+                    __builtin_amdgcn_sched_barrier(0);
+                    const v4i kn = __builtin_bit_cast(v4i, k[n % KB]);
+                    a = __builtin_amdgcn_mfma_i32_32x32x32_i8(kn, __builtin_bit_cast(v4i, q_at(2 * n)), a, 0, 0, 0);
+                    b = __builtin_amdgcn_mfma_i32_32x32x32_i8(kn, __builtin_bit_cast(v4i, q_at(2 * n + 1)), b, 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) a[r] = (int)(((uint32_t)a[r] << 8) + (uint32_t)b[r]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    ks[g] = *reinterpret_cast<const f4 *>(scales + sc_slot * 256 + 64 * g + 16 * h);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = (float)a[r];
+            } else {
+                x = f16x{};
+#pragma unroll
+                for (int n = 0; n < NK; ++n) {
+                    if (n + AHEAD < NK) k[(n + AHEAD) % KB] = k_read(ring(slot, 0), lane, n + AHEAD);
+                    if (QL && n == KS - QL - 1) read_q_last();
+                    __builtin_amdgcn_sched_barrier(0);
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, k[n % KB]), __builtin_bit_cast(h8, q_at(n)), x, 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            scores_done();
             if (I8)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) x[r] *= ks[r / 4][r % 4];
-        }
-        if (RT == 1 && more) {
-            wait_lds();
-            if (I8) load_scales(tile_at(i + 1), pg_next, (i + 1) & 1, lane);
-            load_half(k_pool, true, tile_at(i + 1), pg_next, lds0 + ring(0, 0), lane);
-        }
-        h8 p[2];
-        uint32_t seen = 0xffffffffu;  // bit 8 g + n: this row sees the key of register 4 g + n
-        bool edge = false;
-        if (!skip) {
-            edge = t0 + kKeys - 1 > p_first || (R.window && t0 <= p_last - R.window) || keys != 0xffffffffu;
+            refill_k();
+            h8 p[2];
+            uint32_t seen = 0xffffffffu;  // bit 8 g + n: this row sees the key of register 4 g + n
+            uint32_t keys = 0xffffffffu;  // that exist (scalar)
+            const bool edge = t0 < t_inner || t0 > p_first - (kKeys - 1) || there0 != 15;
             if (edge) {
+                keys = T.S.kv - t0 >= 32 ? 0xffffffffu : (T.S.kv > t0 ? (1u << (T.S.kv - t0)) - 1 : 0u);
+                if (t0 >= k1) keys = 0;
+                keys &= (there0 * 0x00204081u & 0x01010101u) * 0xffu;  // bits to bytes
                 const int hi = pos - t0, lo = R.window ? pos - R.window - t0 : -1;  // keys lo + 1 .. hi of the tile
                 seen = hi < 0 ? 0u : (hi >= 31 ? keys : keys & ((2u << hi) - 1));
                 if (lo >= 0) seen = lo >= 31 ? 0u : seen & ~((2u << lo) - 1);
@@ -491,49 +660,50 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
                     x[r] = ok ? x[r] : -INFINITY;
                 }
             }
+            asm volatile("" : "+v"(seen));  // opaque: or what follows is made twice, with and without a mask
             float top = x[0];
 #pragma unroll
             for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
             top = other_half_max(top);
-            float vtop = 0.0f;  // the largest V scale that the row sees
-            uint32_t v_scales = (i & 1) * 256 + 128 + 16 * h;
-            if (I8) {
-                if (edge) {
+            // V's scales, lane c key c's: those above the least vref of the wave lead to the closer look below
+            uint32_t v_scales = sc_slot * 256 + 32 + 16 * h;
+            float v_mine = 0.0f;
+            if (I8) v_mine = fabsf(*reinterpret_cast<const float *>(scales + sc_slot * 256 + (c >> 3) * 64 + 32 + (c & 7) * 4));
+            float vto = vref;
+            if (I8 && __any(v_mine > v_low)) {
+                float vtop = 0.0f;  // the largest scale that the row sees
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const f4 y = *reinterpret_cast<const f4 *>(scales + v_scales + 32 * g);
+                for (int g = 0; g < 4; ++g) {
+                    const f4 y = *reinterpret_cast<const f4 *>(scales + v_scales + 64 * g);
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) vtop = fmaxf(vtop, seen >> (8 * g + n) & 1 ? fabsf(y[n]) : 0.0f);
-                    }
-                    vtop = other_half_max(vtop);
-                } else {  // every key: a lane each
-                    vtop = half_max(fabsf(*reinterpret_cast<const float *>(scales + (i & 1) * 256 + 128 + 4 * c)));
+                    for (int n = 0; n < 4; ++n) vtop = fmaxf(vtop, seen >> (8 * g + n) & 1 ? fabsf(y[n]) : 0.0f);
                 }
-                asm volatile("" : "+v"(v_scales));  // read again below rather than kept
+                vtop = other_half_max(vtop);
+                if (vtop > vref) vto = pow2_above(vtop);
+                v_low = -half_max(-vto);
             }
-            if (__any(top > m + R.lazy || (m == -INFINITY && top > -INFINITY) || (I8 && vtop > vref))) {
+            if (__any((top - m) * sc > kLazy || (I8 && vto > vref))) {
                 const float mn = fmaxf(m, top);
-                float f = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * R.scale2);
+                float f = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * sc);
                 if (I8) {
-                    const float to = fmaxf(vref, pow2_above(vtop));
-                    f *= vref / to;
+                    f *= vref / vto;
                     w_sum *= f;
-                    vref = to;
+                    vref = vto;
                 }
                 l *= f;
 #pragma unroll
                 for (int j = 0; j < DPL; ++j) o[j] *= f;
                 m = mn;
-                off = (m == -INFINITY ? 0.0f : -m * R.scale2) - (I8 ? pow2_log(vref) : 0.0f);
+                off = (m == -INFINITY ? 0.0f : -m * sc) - (I8 ? pow2_log(vref) : 0.0f);
             }
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 f4 y = {};
-                if (I8) y = *reinterpret_cast<const f4 *>(scales + v_scales + 32 * g);
+                if (I8) y = *reinterpret_cast<const f4 *>(scales + v_scales + 64 * g);
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
                     const int r = 4 * g + n;
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], R.scale2, off));
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r], sc, off));
                     if (I8) l += e;
                     p[r / 8][r % 8] = (_Float16)(I8 ? e * y[n] : e);
                 }
@@ -553,13 +723,8 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
 #pragma unroll
             for (int r = 0; r < 8; ++r)
                 sum = __builtin_amdgcn_fdot2(h2{p[r / 4][2 * (r % 4)], p[r / 4][2 * (r % 4) + 1]}, one, sum, false);
-        }
-        if (RT == 1) {  // V is here, the next K and scales may be on their way
-            if (more) wait_loads<LOADS + (I8 ? 1 : 0)>();
-            else wait_loads<0>();
-        }
-        if (!skip) {
-            char *const tile = lds + ring(slot, 1);
+            wait_v();
+            softmax_done();
             bool odd = false;
             if (!I8 && edge) {
                 // Absent keys hold anything: their rows are cleared (by every wave that shares the tile, with
@@ -575,24 +740,6 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
                 }
                 odd = __any(any & 0x80008000u);
             }
-            const char *vb = tile + c * VB + 4 * h * RB;
-            // the lane's dims of block u, of the 8 keys of k-step s
-            auto v_words = [&](int s, int u, uint32_t (&v)[8][(VB + 3) / 4]) {
-#pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                    const char *at = vb + (16 * s + 8 * (n / 4) + n % 4) * RB + u * 32 * VB;
-                    if constexpr (VB == 8) {
-                        const uint2 y = *reinterpret_cast<const uint2 *>(at);
-                        v[n][0] = y.x;
-                        v[n][1] = y.y;
-                    } else if constexpr (VB == 4) {
-                        v[n][0] = *reinterpret_cast<const uint32_t *>(at);
-                    } else {
-                        v[n][0] = *reinterpret_cast<const uint16_t *>(at);
-                    }
-                    if (I8) v[n][0] ^= 0x80808080u;
-                }
-            };
             auto v_operand = [&](auto W, const uint32_t (&v)[8][(VB + 3) / 4]) {
                 constexpr int w = decltype(W)::value;
                 if constexpr (I8)
@@ -623,13 +770,15 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
                         }
                 }
             }
-            uint32_t v[2 * U + 1][8][(VB + 3) / 4];  // V's reads, one step ahead
             if (!P::TIGHT) v_words(0, 0, v[0]);
             each<0, 2 * U>([&](auto Step) {
                 constexpr int step = decltype(Step)::value, ss = step / U, u = step % U;
                 constexpr int next = P::TIGHT ? step : step + 1;
                 if (next < 2 * U) v_words(next / U, next % U, v[next]);
                 __builtin_amdgcn_sched_barrier(0);
+                if (I8)
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) v[step][n][0] ^= 0x80808080u;
                 if (odd)
 #pragma unroll
                     for (int n = 0; n < 8; ++n)
@@ -642,25 +791,37 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
                 __builtin_amdgcn_sched_barrier(0);
             });
         }
-        pg = pg_next;
-        if (more) {
-            if (RT == 1) {
-                wait_lds();
-                load_half(v_pool, false, tile_at(i + 1), pg, lds0 + ring(0, 1), lane);
-            }
-            if (i + 2 < rounds) pg_next = pages_of(tile_at(i + 2));
+        if constexpr (decltype(Active)::value) {
+            if (RT > 1)
+#pragma unroll
+                for (int n = 0; n < AHEAD && n < NK; ++n) k_first[n] = k_read(ring(slot ^ 1, 0), lane, n);
+        } else {
+            scores_done();
+            softmax_done();
+        }
+        if (RT > 1) slot ^= 1;
+        sc_slot = sc_next;
+        there0 = RT > 1 ? there1 : ahead.there;
+        there1 = ahead.there;
+        if (RT == 1 && more) {
+            wait_lds();
+            load_half(v_pool, false, ahead, lds0 + ring(0, 1), lane);
         }
     }
+    };
+    if (RT == 1 || active) run(std::integral_constant<bool, true>{});
+    else run(std::integral_constant<bool, false>{});
+    if (RT > 1 && P::WAVES > 4 && wave < 4 && rounds) barrier();
     l = other_half_sum(l);
     if (I8) {
         w_sum = other_half_sum(w_sum);
         l *= vref;
     }
-    m *= R.scale2;  // from here on in exponents
+    m *= sc;  // from here on in exponents
 
-    // The key groups' parts of a row, relative to their common maximum, summed in LDS a quarter of the
+    // The key groups' parts of a row, relative to their common maximum, summed in LDS PH quarters of the
     // registers at a time: registers 4 ph .. 4 ph + 3 of the operands of block u are dims
-    // 32 UD u + UD (8 ph + 4 h + 0..3) + 0..UD-1, 8 UD consecutive ones over both halves.
+    // 32 UD u + UD (8 ph + 4 h + 0..3) + 0..UD-1, UD chunks of 4 in a row on either half.
     if (h == 0) ml[wave * kRows + c] = make_float2(m, l);
     __syncthreads();
     float f;
@@ -671,60 +832,74 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
         f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
         if (I8) f *= vref * 0x1p24f;
     }
-    const float bias = I8 ? w_sum * 0x1p-17f : 0.0f;
-    float *const part = reinterpret_cast<float *>(lds);
-    // summing: 2 UD threads a row of 8 UD dims each (4 dims a thread), 64 / (2 UD) rows a wave and round
-    constexpr int TPR = 2 * UD, RPW = 64 / TPR;
+    const float bias = I8 ? -(w_sum * 0x1p-17f) * f : 0.0f;
+    constexpr int PH = P::PH;
+    // chunk e of half h of row c in block u and quarter ph; the XOR spreads a row's chunks over the banks
+    auto chunk = [&](int wave, int ph, int u, int e, int h, int c) {
+        return lds + ((((wave * PH + ph) * U + u) * UD + e) * 64 + h * 32 + (c ^ (e + UD * h))) * 16;
+    };
+    // summing: 2 UD threads a row, a chunk each, 64 / (2 UD) rows a wave; the KG waves of a row tile share its rows
+    constexpr int TPR = 2 * UD, RPW = 64 / TPR, GROUPS = kRows / RPW, GPW = GROUPS > KG ? GROUPS / KG : 1;
+    const int e_sum = lane % UD, h_sum = lane / UD & 1;
     const bool whole = R.splits.d == 1;
+    const int kind = whole ? R.out_kind : G4_KIND_F32;
+    bool live[GPW];
+    float inv[GPW];
+    int64_t to[GPW];  // of this thread's first chunk, in elements
 #pragma unroll
-    for (int ph = 0; ph < 4; ++ph) {
-        if (ph) __syncthreads();
+    for (int i = 0; i < GPW; ++i) {
+        const int group = kg * GPW + i, rr = group % GROUPS * RPW + lane / TPR, grow = first + rr;
+        live[i] = group < GROUPS && grow < T.rows;
+        float top = -INFINITY, total = 0.0f;
+        float2 x[KG];
 #pragma unroll
-        for (int j = 0; j < DPL; ++j)
+        for (int g = 0; g < KG; ++g) {
+            x[g] = ml[(g * RT + rt) * kRows + rr];
+            top = fmaxf(top, x[g].x);
+        }
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
-                part[(wave * DPL * 4 + j * 4 + n) * 72 + lane] = (o[j][4 * ph + n] - bias) * f;
-        __syncthreads();
-        // wave kg of row tile rt: rows kg * RPW .. of each KG * RPW
+        for (int g = 0; g < KG; ++g) total += x[g].y * __builtin_amdgcn_exp2f(x[g].x - (top == -INFINITY ? 0.0f : top));
+        if (whole) {
+            inv[i] = total == 0.0f ? 0.0f : 1.0f / total;
+            to[i] = ((int64_t)(T.S.start + R.group.div(grow)) * R.heads + kvh * (int)R.group.d + R.group.mod(grow)) * D;
+        } else {
+            inv[i] = 1.0f;
+            to[i] = (((int64_t)blockIdx.x * R.splits.d + blockIdx.y) * A.kv_heads + kvh) * (kRows * RT) + rt * kRows + rr;
+            if (live[i] && lane % TPR == 0) R.part_ml[to[i]] = make_float2(top, total);
+            to[i] *= D;
+        }
+        to[i] += lane % TPR * 4;
+    }
+    void *const dst = whole ? R.out : R.part_o;
 #pragma unroll
-        for (int b = 0; b < kRows / (KG * RPW > kRows ? kRows : KG * RPW); ++b) {
-            const int rr = (b * KG + kg) * RPW + lane / TPR;
-            if (rr >= kRows || first + rr >= T.rows) continue;
-            // this thread's 4 dims of a block: element e of its 8 UD is half hh, register nn, operand w
-            float y[U][4];
+    for (int ph0 = 0; ph0 < 4; ph0 += PH) {
+        if (ph0) __syncthreads();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int el = (lane % TPR) * 4 + e, hh = el / (4 * UD), nn = el / UD % 4, w = el % UD;
+        for (int ph = 0; ph < PH; ++ph)
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    float a = 0.0f;
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                    for (int g = 0; g < KG; ++g)
-                        a += part[((g * RT + rt) * DPL * 4 + (u * UD + w) * 4 + nn) * 72 + hh * 32 + rr];
-                    y[u][e] = a;
+                for (int e = 0; e < UD; ++e) {
+                    f4 y;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        y[k] = __builtin_fmaf(o[u * UD + (4 * e + k) % UD][4 * (ph0 + ph) + (4 * e + k) / UD], f, bias);
+                    *reinterpret_cast<f4 *>(chunk(wave, ph, u, e, h, c)) = y;
                 }
-            }
-            float top = -INFINITY, total = 0.0f;
+        __syncthreads();
 #pragma unroll
-            for (int g = 0; g < KG; ++g) top = fmaxf(top, ml[(g * RT + rt) * kRows + rr].x);
+        for (int i = 0; i < GPW; ++i) {
+            if (!live[i]) continue;
+            const int rr = (kg * GPW + i) % GROUPS * RPW + lane / TPR;
+            float4 y[PH * U];
 #pragma unroll
-            for (int g = 0; g < KG; ++g) {
-                const float2 x = ml[(g * RT + rt) * kRows + rr];
-                total += x.y * __builtin_amdgcn_exp2f(x.x - (top == -INFINITY ? 0.0f : top));
-            }
-            const int64_t slot = (((int64_t)blockIdx.x * R.splits.d + blockIdx.y) * A.kv_heads + kvh) * (kRows * RT) + rt * kRows + rr;
-            const int d = 8 * UD * ph + (lane % TPR) * 4, grow = first + rr;
-            const int64_t out = ((int64_t)(T.S.start + R.group.div(grow)) * R.heads + kvh * (int)R.group.d + R.group.mod(grow)) * D;
-            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            for (int n = 0; n < PH * U; ++n) {
+                f4 a = {};
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const float4 z = make_float4(y[u][0], y[u][1], y[u][2], y[u][3]);
-                if (whole)
-                    attn_put4(R, out + 32 * UD * u + d, make_float4(z.x * inv, z.y * inv, z.z * inv, z.w * inv));
-                else
-                    *reinterpret_cast<float4 *>(R.part_o + slot * D + 32 * UD * u + d) = z;
+                for (int g = 0; g < KG; ++g) a += *reinterpret_cast<const f4 *>(chunk(g * RT + rt, n / U, n % U, e_sum, h_sum, rr));
+                y[n] = make_float4(a[0] * inv[i], a[1] * inv[i], a[2] * inv[i], a[3] * inv[i]);
             }
-            if (!whole && ph == 0 && lane % TPR == 0) R.part_ml[slot] = make_float2(top, total);
+            attn_put<PH * U>(dst, kind, R.in_scale, y, [&](int n) { return to[i] + 32 * UD * (n % U) + 8 * UD * (ph0 + n / U); });
         }
     }
 }
@@ -782,8 +957,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(PagedArgs A, AttnArgs R,
     }
     if (!real) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    attn_put4(R, ((int64_t)(T.S.start + R.group.div(row)) * R.heads + kvh * (int)R.group.d + R.group.mod(row)) * D + d,
-              make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+    const int64_t to = ((int64_t)(T.S.start + R.group.div(row)) * R.heads + kvh * (int)R.group.d + R.group.mod(row)) * D + d;
+    const float4 z[1] = {make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv)};
+    attn_put<1>(R.out, R.out_kind, R.in_scale, z, [&](int) { return to; });
 }
 
 // ---- host ---------------------------------------------------------------------------------------------
@@ -795,14 +971,33 @@ struct AttnPlan {
     size_t bytes;
 };
 
-static int key_groups(int rt, int row_bytes) { return rt == 1 ? 4 : (rt == 2 && row_bytes < 512 ? 4 : 2); }
+// Blocks of one row tile need no barrier and run two to a CU; blocks of more share each key tile's loads. Of
+// 256 tokens' rows or more at group 4 or 8 (us):
+//   int8, head_dim 64, 128: 1 always (2048 tokens, 32 heads on 8, 4096 keys: 140 and 214; two or four row tiles
+//     a block: 152..171 and 254..261).
+//   int8, head_dim 256: 2 (8 heads on 1; 8192 tokens on their own: 381, one: 398, four: 415; 2048 tokens on 8192
+//     keys: 166, 181, 170).
+//   f16: 4 where that leaves every second CU a block at least, for splitting the keys further costs more than
+//     it brings (head_dim 256, 8 heads on 1, 8192 tokens: 402, two: 580, one: 555; 2048 on 8192 keys: 171, 245,
+//     226; head_dim 128, 32 heads on 8, 2048 tokens on 4096 keys: 181, 196, 197). With fewer blocks 2 at head_dim
+//     256 (512 tokens, window 512: 21, four: 28, one: 27), which one block a CU is left of anyway, and else 1
+//     (300 tokens, 16 heads on 4, head_dim 128: 20, two: 26, four: 22).
+static int row_tiles(bool i8, int d, int64_t rows, int64_t blocks4) {
+    if (rows <= kRows) return 1;
+    if (!i8 && blocks4 * 2 >= device_cu_count()) return 4;
+    return d == 256 ? 2 : 1;
+}
+
+static int key_groups(int rt, bool i8) { return rt == 1 || (rt == 2 && i8) ? 4 : 2; }
 
 static AttnPlan attn_plan(const PagedArgs &A, const g4_kv_pages *pages, int heads, int window) {
     const int group = heads / A.kv_heads, d = pages->head_dim;
     AttnPlan P;
     const int64_t most = (int64_t)A.max_q * group;  // rows of a sequence
-    P.rt = most <= kRows ? 1 : (most <= 2 * kRows ? 2 : 4);
-    P.key_groups = key_groups(P.rt, pages->kind == G4_KIND_I8 ? d : 2 * d);
+    const bool i8 = pages->kind == G4_KIND_I8;
+    const int64_t tiles4 = std::min((most + 127) / 128 * A.seqs, (int64_t)A.tokens * group / 128 + A.seqs);
+    P.rt = row_tiles(i8, d, most, tiles4 * A.kv_heads);
+    P.key_groups = key_groups(P.rt, i8);
     const int rows = kRows * P.rt;
     P.tiles = std::min((most + rows - 1) / rows * A.seqs, (int64_t)A.tokens * group / rows + A.seqs);
     int64_t keys = A.max_kv;
@@ -825,9 +1020,13 @@ static void launch_rows(const PagedArgs &A, const AttnArgs &R, const AttnPlan &P
 
 template <int D, int CK>
 static int launch_attn(const PagedArgs &A, const AttnArgs &R, const AttnPlan &P, hipStream_t stream) {
+    if constexpr (CK == G4_KIND_F16) {
+        if (P.rt == 4) launch_rows<D, CK, 4>(A, R, P, stream);
+    }
+    if constexpr (D == 256) {
+        if (P.rt == 2) launch_rows<D, CK, 2>(A, R, P, stream);
+    }
     if (P.rt == 1) launch_rows<D, CK, 1>(A, R, P, stream);
-    else if (P.rt == 2) launch_rows<D, CK, 2>(A, R, P, stream);
-    else launch_rows<D, CK, 4>(A, R, P, stream);
     G4_LAUNCHED("attn_kernel");
     if (P.splits > 1) {
         const int rows = kRows * P.rt;
@@ -898,8 +1097,7 @@ int g4_attention_chunk(const g4_kv_pages *pages, const g4_chunk *chunk, const vo
     R.heads = heads;
     R.group = FastDiv::of(heads / A.kv_heads);
     // a scale of 0 as one too small to matter, so that a masked score stays minus infinity
-    R.scale2 = std::max(std::fabs(scale) * 1.44269504088896340736f, 0x1p-100f) * (i8 ? 0x1p24f : 1.0f);
-    R.lazy = kLazy / R.scale2;
+    R.scale2 = std::max(std::fabs(scale) * 1.44269504088896340736f, 0x1p-100f);
     R.q_sign = scale < 0.0f ? 0x80008000u : 0u;
     R.page_bytes = (uint32_t)(A.page_stride * eb);
     R.slot_bytes = (uint32_t)(A.slot_stride * eb);

@@ -108,7 +108,8 @@ def attention(b, q, scale, window):
     of their own from the rounding to f16; one under 2^-14 of the row's largest loses up to 2^-25 of that.
     A weight is relative to a running maximum whose factor exp(m - m') is applied once more in f32. Sums
     of n terms in f32 lose (n + 8) 2^-24 of the sum of magnitudes. ds is the f32 dot product's (dim + 4)
-    2^-24 of its magnitudes, and exp's few 2^-24."""
+    2^-24 of its magnitudes, and exp's few 2^-24; with an int8 cache an element of q may be off by half a step
+    of 2^-15 of the row's largest (32512 steps) too, so a score by that times the sum of |k|."""
     heads = q.shape[1]
     out = np.zeros(q.shape)
     bound = np.zeros(q.shape)
@@ -137,6 +138,9 @@ def attention(b, q, scale, window):
             sl = np.s_[b.start[s]:b.start[s + 1], h]
             out[sl] = p @ vv
             ds = (mag.max(1, keepdims=True, initial=0) * (b.dim + 4) + 16) * 2.0 ** -24
+            if b.kind == "i8":
+                ds = ds + np.abs(qq).max(1, keepdims=True, initial=0) / 65024 * \
+                    np.abs(kk).sum(1).max(initial=0) * abs(scale)
             n = seen.sum(1, keepdims=True)
             spread = p @ np.abs(vv)
             vmax = np.abs(vv).max(initial=0)

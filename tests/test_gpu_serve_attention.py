@@ -96,6 +96,32 @@ def test_absent_pages_and_empty_rows(gpu, lens, absent, kind):
     check(b, 8, window=20)
 
 
+@pytest.mark.parametrize("window", [0, 1, 40, 150])
+@pytest.mark.parametrize("dim,kind,kv_heads", [(256, "i8", 2), (256, "f16", 2), (64, "f16", 128), (128, "f16", 128),
+                                               (256, "f16", 128)])
+def test_blocks_of_more_row_tiles(gpu, dim, kind, kv_heads, window):
+    """Row counts around 32, 64 and 128, ends inside pages and key tiles, pages let go of."""
+    lens = [(33, 35), (140, 300)] if kv_heads > 2 else [(33, 35), (64, 64), (140, 300), (0, 9), (129, 130), (1, 77)]
+    check(Batch(lens, kv_heads, dim, 16, kind, seed=window + dim, absent=[(0, 1), (1, 0), (1, 2)]), kv_heads, window)
+
+
+@pytest.mark.parametrize("dim,kv_heads", [(256, 1), (64, 128), (256, 128)])
+def test_masked_contents_in_blocks_of_more_row_tiles(gpu, dim, kv_heads):
+    """NaN and infinities in the last two tokens' V: rows before them untouched, rows that see them not finite."""
+    m = 70
+    def batch():
+        return Batch([(m, m + 30)], kv_heads, dim, 16, "f16", seed=dim)
+    b = batch()
+    for p, x in ((m + 28, np.inf), (m + 29, np.nan)):
+        b.v[b.table[0, p // 16], p % 16, :, ::3] = x
+    q = queries(b.upload(), kv_heads)
+    got = run(b, q, 0, 0.1).astype(np.float64)
+    want, bound = attention(batch(), q, float(np.float32(0.1)), 0)
+    assert (np.abs(got - want) <= to_kind(want, bound, np.float16))[:m - 2].all()
+    assert not np.isfinite(got[m - 1, :, ::3]).any()
+    assert np.isfinite(got[m - 1, :, 1::3]).all()
+
+
 @pytest.mark.parametrize("kind", ["i8", "f16"])
 def test_rows_without_positions(gpu, kind):
     """More rows than positions: the rows in front see nothing and give zeros. Rows behind the last

@@ -38,6 +38,7 @@ struct VerifyArgs {
     int64_t vocab;
     double cap, inv_t;
     double inv_cap2;
+    float half_cap;  // a little less than half the cap
     int greedy, vec;  // vec: rows may be read 16 bytes at a time
     const float *u, *u_next;
     PartStat *stats;  // [drafts + seqs (+ drafts)][parts]
@@ -60,44 +61,60 @@ __device__ __forceinline__ double weight(float x, double top, const VerifyArgs &
 }
 
 // weight() for the bulk of a row. 2^z: z = n + f, |f| <= 1/2, a polynomial in f (fitted on Chebyshev nodes,
-// relative error 1.1e-12) and n into the exponent. The softcap of |x| <= cap / 2 as x + x t P(t), t =
-// (x / cap)^2 (fitted likewise, 8e-14 t x off); past that the definition. 13 operations of the 64-bit unit a
-// logit, about what its 4 bytes cost to read; 24 with the softcap.
+// relative error 1.1e-12) and n into the exponent: 14 operations of the 64-bit unit a logit, about what its 4
+// bytes cost to read. The softcap of |x| <= cap / 2 as x + x t P(t), t = (x / cap)^2 (fitted likewise, 8e-14
+// t x off): 11 more; past that the definition.
 struct RowScale {
-    double top, slope, base;  // 2^(y slope + base)
+    double top, slope;  // 2^((y - top) slope)
 };
 __device__ __forceinline__ RowScale row_scale(double top, const VerifyArgs &A) {
-    const double slope = A.inv_t * 1.4426950408889634074;
-    return {top, slope, -top * slope};
+    return {top, A.inv_t * 1.4426950408889634074};
 }
+// a b + k with k in scalar registers (the compiler would copy it to vector ones first, two moves a step).
+__device__ __forceinline__ double fma_k(double a, double b, double k) {
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(k));
+    return r;
+}
+__device__ __forceinline__ double near_cap(double x, const VerifyArgs &A) {
+    const double t = x * x * A.inv_cap2;
+    double c = 0.00039943422382545215;
+    c = fma_k(c, t, -0.0013843999024647944);
+    c = fma_k(c, t, 0.0035776163994480498);
+    c = fma_k(c, t, -0.008861575554686911);
+    c = fma_k(c, t, 0.021869384578835853);
+    c = fma_k(c, t, -0.053968250756296965);
+    c = fma_k(c, t, 0.1333333332954187);
+    c = fma_k(c, t, -0.3333333333332598);
+    return __builtin_fma(x, t * c, x);
+}
+// 2^z; below 2^-1000 that (too small to count, and the exponent stays normal), and for a NaN.
+__device__ __forceinline__ double pow2(double z) {
+    z = z > -1000.0 ? z : -1000.0;
+    const double r = z + 0x1.8p52;  // n in the low word
+    const double f = z - (r - 0x1.8p52);
+    double e = 1.3259689002093833e-06;
+    e = fma_k(e, f, 1.531008106933654e-05);
+    e = fma_k(e, f, 0.00015403433582607232);
+    e = fma_k(e, f, 0.0013333450560096254);
+    e = fma_k(e, f, 0.009618129194093111);
+    e = fma_k(e, f, 0.05550410941217064);
+    e = fma_k(e, f, 0.24022650695640319);
+    e = fma_k(e, f, 0.6931471805459295);
+    e = fma_k(e, f, 1.0000000000000135);
+    return __hiloint2double(__double2hiint(e) + (int)((uint32_t)__double2loint(r) << 20), __double2loint(e));
+}
+// |x| past what near_cap is good for, -infinity (no weight) not included
+__device__ __forceinline__ bool is_far(float x, const VerifyArgs &A) { return fabsf(x) > A.half_cap && x > -INFINITY; }
+template <bool CAP>
 __device__ __forceinline__ double bulk_weight(float x, const RowScale &S, const VerifyArgs &A) {
     double y = x;
-    if (A.cap != 0.0) {
-        const double t = y * y * A.inv_cap2;
-        double c = 0.00039943422382545215;
-        c = __builtin_fma(c, t, -0.0013843999024647944);
-        c = __builtin_fma(c, t, 0.0035776163994480498);
-        c = __builtin_fma(c, t, -0.008861575554686911);
-        c = __builtin_fma(c, t, 0.021869384578835853);
-        c = __builtin_fma(c, t, -0.053968250756296965);
-        c = __builtin_fma(c, t, 0.1333333332954187);
-        c = __builtin_fma(c, t, -0.3333333333332598);
-        y = t <= 0.25 ? __builtin_fma(y, t * c, y) : softcap64(x, A.cap);
+    if (CAP) {
+        y = near_cap(y, A);
+        if (is_far(x, A)) y = softcap64(x, A.cap);
     }
-    if (y == S.top) return 1.0;
-    double z = __builtin_fma(y, S.slope, S.base);
-    z = z > -1000.0 ? z : -1000.0;  // too small to count, and the exponent stays normal; a NaN too (infinite rows)
-    const double n = __builtin_rint(z), f = z - n;
-    double e = 1.3259689002093833e-06;
-    e = __builtin_fma(e, f, 1.531008106933654e-05);
-    e = __builtin_fma(e, f, 0.00015403433582607232);
-    e = __builtin_fma(e, f, 0.0013333450560096254);
-    e = __builtin_fma(e, f, 0.009618129194093111);
-    e = __builtin_fma(e, f, 0.05550410941217064);
-    e = __builtin_fma(e, f, 0.24022650695640319);
-    e = __builtin_fma(e, f, 0.6931471805459295);
-    e = __builtin_fma(e, f, 1.0000000000000135);
-    return __longlong_as_double(__double_as_longlong(e) + ((int64_t)(int)n << 52));
+    const double e = pow2((y - S.top) * S.slope);
+    return !CAP && x == INFINITY ? 1.0 : e;  // the maximum then too
 }
 
 __device__ __forceinline__ float clean(float x) { return x == x ? x : -INFINITY; }
@@ -145,47 +162,60 @@ __device__ __forceinline__ void load_range(const float *x, int n, int vec, float
 }
 
 // Grid (parts, rows): part blockIdx.x of row blockIdx.y, the target's rows first.
+template <bool CAP>
 __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs A) {
     __shared__ float ms[4];
-    __shared__ int is[4];
     __shared__ double ss[4];
+    __shared__ int first;
     const int t = threadIdx.x, part = blockIdx.x, row = blockIdx.y, targets = A.drafts + A.seqs;
     const float *x = row < targets ? A.logits + row * A.vocab : A.draft_logits + (int64_t)(row - targets) * A.vocab;
     const int64_t base = (int64_t)part * kPart;
     const int n = (int)(A.vocab - base < kPart ? A.vocab - base : kPart);
     float v[kPerThread];
     load_range(x + base, n, A.vec, v);
-    float m = -INFINITY;
-    int at = INT32_MAX;
+    float mine = v[0];
 #pragma unroll
-    for (int j = 0; j < kPerThread; ++j)
-        if (v[j] > m) {
-            m = v[j];
-            at = element(j, A.vec);
-        }
+    for (int j = 1; j < kPerThread; ++j) mine = fmaxf(mine, v[j]);
+    float m = mine;
 #pragma unroll
-    for (int s = 32; s; s >>= 1) first_max(m, at, __shfl_xor(m, s), __shfl_xor(at, s));
-    if ((t & 63) == 0) {
-        ms[t >> 6] = m;
-        is[t >> 6] = at;
-    }
+    for (int s = 32; s; s >>= 1) m = fmaxf(m, __shfl_xor(m, s));
+    if ((t & 63) == 0) ms[t >> 6] = m;
+    if (t == 0) first = INT32_MAX;
     __syncthreads();
-    m = ms[0];
-    at = is[0];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) first_max(m, at, ms[w], is[w]);
+    m = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
     double sum = 0.0;
     if (m > -INFINITY) {
-        const RowScale S = row_scale(softcap64(m, A.cap), A);
+        if (mine == m) {  // few threads: the first of the maximum's places
+            int at = INT32_MAX;
 #pragma unroll
-        for (int j = 0; j < kPerThread; ++j) sum += v[j] > -INFINITY ? bulk_weight(v[j], S, A) : 0.0;
+            for (int j = kPerThread - 1; j >= 0; --j) at = v[j] == m ? element(j, A.vec) : at;
+            atomicMin(&first, at);
+        }
+        if (!CAP && m == INFINITY) {
+#pragma unroll
+            for (int j = 0; j < kPerThread; ++j) sum += v[j] == m ? 1.0 : 0.0;
+        } else {
+            const RowScale S = row_scale(softcap64(m, A.cap), A);
+            uint32_t far = 0;  // elements left out here
+#pragma unroll
+            for (int j = 0; j < kPerThread; ++j) {
+                double z = ((CAP ? near_cap(v[j], A) : (double)v[j]) - S.top) * S.slope;
+                if (CAP) {
+                    const bool f = is_far(v[j], A);
+                    far |= f ? 1u << j : 0u;
+                    z = f ? -1000.0 : z;
+                }
+                sum += pow2(z);
+            }
+            for (; far; far &= far - 1) sum += weight(x[base + element(__ffs(far) - 1, A.vec)], S.top, A);
+        }
     }
     sum = wave_sum64(sum);
     if ((t & 63) == 0) ss[t >> 6] = sum;
     __syncthreads();
     if (t == 0)
         A.stats[(int64_t)row * A.parts + part] = {(ss[0] + ss[1]) + (ss[2] + ss[3]), m,
-                                                  at == INT32_MAX ? -1 : (int)(base + at)};
+                                                  first == INT32_MAX ? -1 : (int)(base + first)};
 }
 
 struct RowStat {
@@ -309,10 +339,11 @@ __device__ __forceinline__ Source source_of(const VerifyArgs &A, int seq, int st
     return S;
 }
 
+template <bool CAP>
 __device__ __forceinline__ double source_weight(const VerifyArgs &A, const Source &S, int64_t i, float xp, float xq) {
-    double w = xp > -INFINITY ? bulk_weight(xp, S.ps, A) * S.p_inv : 0.0;
+    double w = xp > -INFINITY ? bulk_weight<CAP>(xp, S.ps, A) * S.p_inv : 0.0;
     if (S.q) {
-        if (xq > -INFINITY) w -= bulk_weight(xq, S.qs, A) * S.q_inv;
+        if (xq > -INFINITY) w -= bulk_weight<CAP>(xq, S.qs, A) * S.q_inv;
     } else if (i == S.point) {
         w -= 1.0;
     }
@@ -320,6 +351,7 @@ __device__ __forceinline__ double source_weight(const VerifyArgs &A, const Sourc
 }
 
 // The block's thread's weights of a unit, in the element order of load_range; returns their sum.
+template <bool CAP>
 __device__ __forceinline__ double unit_weights(const VerifyArgs &A, const Source &S, int64_t base, double (&w)[kUnitPer]) {
     float xp[kUnitPer], xq[kUnitPer] = {};
     const int n = (int)(A.vocab - base < kUnit ? A.vocab - base : kUnit);
@@ -328,7 +360,7 @@ __device__ __forceinline__ double unit_weights(const VerifyArgs &A, const Source
     double sum = 0.0;
 #pragma unroll
     for (int j = 0; j < kUnitPer; ++j) {
-        w[j] = source_weight(A, S, base + element(j, A.vec), xp[j], xq[j]);
+        w[j] = source_weight<CAP>(A, S, base + element(j, A.vec), xp[j], xq[j]);
         sum += w[j];
     }
     return sum;
@@ -343,6 +375,7 @@ __device__ __forceinline__ double block_sum64(double sum, double *lds) {
 }
 
 // Grid (units, seqs): unit blockIdx.x's sum of the weights to draw from.
+template <bool CAP>
 __global__ __launch_bounds__(kVerThreads) void verify_weights_kernel(VerifyArgs A) {
     __shared__ double ss[4];
     const int seq = blockIdx.y;
@@ -351,17 +384,18 @@ __global__ __launch_bounds__(kVerThreads) void verify_weights_kernel(VerifyArgs 
     const Draw D = A.draws[seq];
     const Source S = source_of(A, seq, start, D, D.refused);
     double w[kUnitPer];
-    const double sum = block_sum64(unit_weights(A, S, (int64_t)blockIdx.x * kUnit, w), ss);
+    const double sum = block_sum64(unit_weights<CAP>(A, S, (int64_t)blockIdx.x * kUnit, w), ss);
     if (threadIdx.x == 0) A.weights[(int64_t)seq * A.units + blockIdx.x] = sum;
 }
 
 // The first weight of the unit at `base` whose running sum exceeds `target`; the last one with any weight
 // where rounding leaves none (-1: no weight at all). Same in every thread.
+template <bool CAP>
 __device__ __forceinline__ int64_t pick(const VerifyArgs &A, const Source &S, int64_t base, double target, double *w_lds,
                                         double *ws, int *first, int *last) {
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     double w[kUnitPer];
-    unit_weights(A, S, base, w);
+    unit_weights<CAP>(A, S, base, w);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kUnitPer; ++j) w_lds[element(j, A.vec)] = w[j];  // to token order
@@ -403,6 +437,7 @@ __device__ __forceinline__ int64_t pick(const VerifyArgs &A, const Source &S, in
 }
 
 // One block per sequence: the unit where the running sum of the units passes the target, then the logit.
+template <bool CAP>
 __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs A) {
     __shared__ double w_lds[kUnit], ws[4];
     __shared__ int first, last;
@@ -438,7 +473,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs A) 
             if (past) break;
             before += __shfl(run, 63);
         }
-        token = pick(A, source_of(A, seq, start, D, D.refused), (int64_t)unit * kUnit, target - unit_before, w_lds, ws,
+        token = pick<CAP>(A, source_of(A, seq, start, D, D.refused), (int64_t)unit * kUnit, target - unit_before, w_lds, ws,
                      &first, &last);
     } else if (D.refused && D.p_sum > 0.0) {
         // p and q are the same everywhere: the draw is from p, whose sum of weights is 1
@@ -446,8 +481,8 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs A) 
         double before = 0.0;
         for (int c = 0; c < A.units; ++c) {
             double x[kUnitPer];
-            const double sum = block_sum64(unit_weights(A, S, (int64_t)c * kUnit, x), ws);
-            if (sum > 0.0) token = pick(A, S, (int64_t)c * kUnit, u - before, w_lds, ws, &first, &last);
+            const double sum = block_sum64(unit_weights<CAP>(A, S, (int64_t)c * kUnit, x), ws);
+            if (sum > 0.0) token = pick<CAP>(A, S, (int64_t)c * kUnit, u - before, w_lds, ws, &first, &last);
             if (before + sum > u) break;
             before += sum;
         }
@@ -457,6 +492,20 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs A) 
     if (A.logprobs)
         A.logprobs[(int64_t)seq * (A.max_drafts + 1) + D.taken] =
             token >= 0 ? log_p(A, start + seq + D.taken, (int)token, RowStat{D.p_top, D.p_sum, -1}) : 0.0f;
+}
+
+template <bool CAP>
+static int launch_verify(const VerifyArgs &A, unsigned rows, hipStream_t s) {
+    hipLaunchKernelGGL(verify_stats_kernel<CAP>, dim3(A.parts, rows), dim3(kVerThreads), 0, s, A);
+    G4_LAUNCHED("verify_stats_kernel");
+    hipLaunchKernelGGL(verify_judge_kernel, dim3(A.seqs), dim3(64 * kJudgeWaves), 0, s, A);
+    G4_LAUNCHED("verify_judge_kernel");
+    if (A.greedy) return G4_OK;
+    hipLaunchKernelGGL(verify_weights_kernel<CAP>, dim3(A.units, A.seqs), dim3(kVerThreads), 0, s, A);
+    G4_LAUNCHED("verify_weights_kernel");
+    hipLaunchKernelGGL(verify_pick_kernel<CAP>, dim3(A.seqs), dim3(kVerThreads), 0, s, A);
+    G4_LAUNCHED("verify_pick_kernel");
+    return G4_OK;
 }
 
 static int64_t verify_rows(int seqs, int drafts) { return 2 * (int64_t)drafts + seqs; }
@@ -513,6 +562,7 @@ int g4_verify_drafts(const float *logits, const float *draft_logits, const int32
     A.vocab = vocab;
     A.cap = cap;
     A.inv_cap2 = cap > 0.0f ? 1.0 / ((double)cap * cap) : 0.0;
+    A.half_cap = 0.4999999f * cap;
     A.vec = vocab % 4 == 0 && (((uintptr_t)logits | (uintptr_t)draft_logits) & 15) == 0;
     A.inv_t = greedy ? 1.0 : 1.0 / (double)temperature;
     A.greedy = greedy;
@@ -525,16 +575,7 @@ int g4_verify_drafts(const float *logits, const float *draft_logits, const int32
     A.accepted = accepted;
     A.logprobs = logprobs;
     hipStream_t s = as_stream(stream);
-    hipLaunchKernelGGL(verify_stats_kernel, dim3(A.parts, (unsigned)rows), dim3(kVerThreads), 0, s, A);
-    G4_LAUNCHED("verify_stats_kernel");
-    hipLaunchKernelGGL(verify_judge_kernel, dim3(seqs), dim3(64 * kJudgeWaves), 0, s, A);
-    G4_LAUNCHED("verify_judge_kernel");
-    if (greedy) return G4_OK;
-    hipLaunchKernelGGL(verify_weights_kernel, dim3(A.units, seqs), dim3(kVerThreads), 0, s, A);
-    G4_LAUNCHED("verify_weights_kernel");
-    hipLaunchKernelGGL(verify_pick_kernel, dim3(seqs), dim3(kVerThreads), 0, s, A);
-    G4_LAUNCHED("verify_pick_kernel");
-    return G4_OK;
+    return cap > 0.0f ? launch_verify<true>(A, (unsigned)rows, s) : launch_verify<false>(A, (unsigned)rows, s);
 }
 
 }  // extern "C"

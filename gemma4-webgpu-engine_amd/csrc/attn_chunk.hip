@@ -1,26 +1,32 @@
 // Causal attention of a chunk of new tokens over the paged cache (include/g4serve.h).
 //
 // Query rows are (token, query head of the group) pairs, 32 to a tile, tokens first, so that every head
-// on one KV head shares its loads. Both products run on v_mfma_f32_32x32x16_f16 in the transposed order
+// on one KV head shares its loads. Both products run on the 32x32 matrix instructions in the transposed order
 //   S^T = K Q^T   (A: 32 keys, B: 32 query rows)       O^T += V^T P^T   (A: 32 dims, B: 32 query rows)
 // whose result lane holds one query row (lane % 32) and 16 of the keys: a row's softmax is per-lane
 // arithmetic and one exchange with lane ^ 32, and the weights are the second product's B operand where
 // they stand. The order of the k index of a product is free as long as both operands agree on it; the
 // layouts below use that twice:
 //  - P: lane half h holds, for k-step t of 16 keys, keys 16 t + 4 h + 0..3 and 16 t + 8 + 4 h + 0..3;
-//  - V: a lane loads DPL = D / 32 consecutive dims of each of these eight keys (a whole row per half
-//    wave) and byte-permutes them into DPL operands of eight keys each, the row i of operand j being dim
-//    DPL i + j. No LDS transposes anything.
+//  - V: a lane reads UD consecutive dims of each of these eight keys and byte-permutes them into UD operands
+//    of eight keys each. No LDS transposes anything.
 // The softmax keeps a running maximum (base 2) and sum in f32; the maximum moves, and the output is
 // rescaled, only when a score passes it by more than 2^8, so weights reach 2^8 at most and are rounded to
 // f16 (11 bits; an f16 cache's sum adds the rounded ones, an int8 cache's the exact ones, whose weights
-// are rounded with V's scale in them). int8 rows: the scores are integer products of K's codes
-// with Q as 16-bit fixed point of the row's largest magnitude, in two 8-bit digits (v_mfma_i32_32x32x32_i8 twice:
-// the matrix time of one f16 product and none of the conversion, 96 vector operations a tile; an element of Q
-// is off by 2^-17 of the largest at most, where f16 holds one of an eighth of it to 2^-15); K's scale multiplies the
-// score, V's the weight, taken relative to a power of two above the largest scale that the row has seen,
-// which scales the row's output and sum (f16 would not hold scales of every size) and enters the weights
-// by their exponent.
+// are rounded with V's scale in them).
+// int8 rows: the scores are integer products of K's codes with Q as 16-bit fixed point of the row's largest
+// magnitude, in two 8-bit digits (v_mfma_i32_32x32x32_i8 twice: the matrix time of one f16 product, K read
+// once and not converted, which took 96 vector operations a tile). An element of Q is off by 2^-16 of the
+// row's largest at most, K's codes not at all. K's scale multiplies the score, V's the weight, taken relative
+// to a power of two above the largest scale that the row has seen, which scales the row's output and sum (f16
+// would not hold scales of every size) and enters the weights by their exponent. V's codes are f16 subnormals.
+//
+// What bounds it. Many rows: of a key tile's 32 products of 32 cycles a wave and its 330 other vector
+// operations of 4, a SIMD's two waves overlap most, but the two streams share the issue; 2048 tokens on 8192
+// keys, 8 heads of 256, int8: 162 us, 743 TFLOP/s, 0.62 of what a large f16 product reaches (8192 tokens on
+// their own: 381 us; f16: 402 us). Few rows: reading the cache (32 single tokens on 16384 keys, f16: 94 us,
+// 5.7 TB/s), and below that a block's way from its arguments to the first keys and from its last to memory,
+// 4 us each: 4 tokens on 4096 keys take 9.8 us and their join 4.4.
 #include "g4_paged.h"
 #include <algorithm>
 #include <cmath>
@@ -201,10 +207,11 @@ __device__ __forceinline__ void attn_put(void *out, int kind, float in_scale, co
 // key tiles g, g + KG, ... of the block's run; the waves of a group share its K and V tiles, which come
 // straight to LDS as the rows stand in the cache, a ring of NS tiles each.
 //  RT 1: a wave waits for its own loads only, and refills the K half of its buffer as soon as the scores
-//        are done and the V half after the output (NS 1);
+//        are done and the V half after the output (NS 1).
 //  RT 2, 4: two block barriers a key tile, one before the softmax and one after it, and waves 4..7 one barrier
 //        behind waves 0..3: of the two waves that share a SIMD, one has the matrix unit (a tile's output and
-//        the next tile's scores) while the other has the vector unit. K comes two tiles ahead and V one.
+//        the next tile's scores) while the other has the vector unit. K comes two tiles ahead and V one. In
+//        step, 8192 tokens took 447 us for 381 (int8, RT 2) and 436 for 402 (f16, RT 4), head_dim 128 221 for 181.
 template <int D, int CK, int RT>
 struct Shape {
     static constexpr int EB = CK == G4_KIND_I8 ? 1 : 2;  // bytes of an element
@@ -297,7 +304,8 @@ __global__ __launch_bounds__((64 * Shape<D, CK, RT>::WAVES), (Shape<D, CK, RT>::
 void attn_kernel(PagedArgs A, AttnArgs R) {
     using P = Shape<D, CK, RT>;
     constexpr bool I8 = CK == G4_KIND_I8;
-    constexpr int EB = P::EB, RB = P::RB, KG = P::KG, NS = P::NS, KS = D / 16, DPL = D / 32, NK = RB / 32;  // NK: K reads of a lane
+    constexpr int EB = P::EB, RB = P::RB, KG = P::KG, NS = P::NS, KS = D / 16, DPL = D / 32;
+    constexpr int NK = RB / 32;                                       // K reads of a lane
     constexpr int UD = VDims<D>::UD, U = VDims<D>::U, VB = UD * EB;   // VB: bytes of a lane's read of a V row
     constexpr int GB = 8 * RB;                                        // bytes of an 8-key group
     constexpr int NI = GB >= 1024 ? GB / 1024 : 1;                    // loads of a group
@@ -378,7 +386,8 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
             asm volatile("" : "+s"(r));  // a value: or the array is kept in memory and indexed by the lane
             row = lane >> 4 == (uint32_t)i ? r : row;
         }
-        dma4<16 * GW>((lane & 8 ? A.vs : A.ks) + row + (lane & 7), lds0 + SC0 + (kg * P::NSC + slot) * 256 + rt * GW * 64);
+        dma4<16 * GW>((lane & 8 ? A.vs : A.ks) + row + (lane & 7),
+                      lds0 + SC0 + (kg * P::NSC + slot) * 256 + rt * GW * 64);
     };
     auto ring = [&](int slot, int half) { return (uint32_t)(((kg * NS + slot) * 2 + half) * P::HALF); };
 
@@ -455,7 +464,7 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
             for (int g = 0; g < KG; ++g) top = max(top, __float_as_uint(ml[(g * RT + rt) * kRows + c].x));
             const float amax = (float)bits_h2(top)[0];
             const float inv = top ? (R.q_sign ? -32512.0f : 32512.0f) / amax : 0.0f;
-            sc = fmaxf(R.scale2 * (amax / 32512.0f), 0x1p-100f);
+            sc = fmaxf(R.scale2 * (amax / 32512.0f), 0x1p-126f);
             if (top >= 0x7c00u) sc = __builtin_nanf("");  // a NaN or an infinity in Q
             auto stage = [&](int at) {  // of the row tile's KS operands
                 const int e = rt * KS + at;
@@ -472,8 +481,10 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
                         uint32_t n[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            n[i] = __float_as_uint(__builtin_fmaf((float)bits_h2(x[2 * s + w / 2][w % 2 * 2 + i / 2])[i % 2], inv, 0x1.8p23f + 128.0f));
-                        const uint32_t a = __builtin_amdgcn_perm(n[1], n[0], 0x05010400u), b = __builtin_amdgcn_perm(n[3], n[2], 0x05010400u);
+                            n[i] = __float_as_uint(__builtin_fmaf(
+                                (float)bits_h2(x[2 * s + w / 2][w % 2 * 2 + i / 2])[i % 2], inv, 0x1.8p23f + 128.0f));
+                        const uint32_t a = __builtin_amdgcn_perm(n[1], n[0], 0x05010400u);
+                        const uint32_t b = __builtin_amdgcn_perm(n[3], n[2], 0x05010400u);
                         lo[w] = __builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u;
                         hi[w] = __builtin_amdgcn_perm(b, a, 0x07060302u);
                     }
@@ -502,7 +513,8 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
     // vref: the power of two of the row's V scales; w_sum: the sum of the rounded weights (int8)
     // off: the exponents' offset, -m scale2 - log2(vref); l is in units of vref too
     // v_low: the least vref of the wave's rows (a lane without a row keeps out of it)
-    float m = -INFINITY, l = 0.0f, vref = real ? 0x1p-100f : 0x1p100f, v_low = 0x1p-100f, w_sum = 0.0f, off = I8 ? 100.0f : 0.0f;
+    float m = -INFINITY, l = 0.0f, w_sum = 0.0f, off = I8 ? 100.0f : 0.0f;
+    float vref = real ? 0x1p-100f : 0x1p100f, v_low = 0x1p-100f;
 
     const int lane_ = lane;
     constexpr int KC = NK < 4 ? NK : 4, AHEAD = D == 256 && I8 && RT == 1 ? 1 : 2;
@@ -535,11 +547,12 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
         asm volatile("" : "+v"(lane));
         const int h = lane >> 5, c = lane & 31;
         const int t0 = tile_at(i);
-        const int sc_next = sc_slot + 1 == P::NSC ? 0 : sc_slot + 1, sc_after = sc_next + 1 == P::NSC ? 0 : sc_next + 1;
+        const int sc_next = sc_slot + 1 == P::NSC ? 0 : sc_slot + 1;
+        const int sc_after = sc_next + 1 == P::NSC ? 0 : sc_next + 1;
         const bool more = i + 1 < rounds;
         if (RT == 1) wait_loads<LOADS>();  // K and the scales are here, V may be on its way
-        // K's reads run two steps ahead (one where registers are short; no further: the scheduling barriers keep the compiler from either
-        // gathering them, for which there are no registers, or waiting for each)
+        // K's reads run two steps ahead (one where registers are short); the scheduling barriers keep the compiler
+        // from gathering them, for which there are no registers, and from waiting for each
         constexpr int KB = AHEAD + 1;
         u32x4 k[KB];
 #pragma unroll
@@ -633,7 +646,8 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
                     if (n + AHEAD < NK) k[(n + AHEAD) % KB] = k_read(ring(slot, 0), lane, n + AHEAD);
                     if (QL && n == KS - QL - 1) read_q_last();
                     __builtin_amdgcn_sched_barrier(0);
-                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, k[n % KB]), __builtin_bit_cast(h8, q_at(n)), x, 0, 0, 0);
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, k[n % KB]),
+                                                               __builtin_bit_cast(h8, q_at(n)), x, 0, 0, 0);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -668,7 +682,7 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
             // V's scales, lane c key c's: those above the least vref of the wave lead to the closer look below
             uint32_t v_scales = sc_slot * 256 + 32 + 16 * h;
             float v_mine = 0.0f;
-            if (I8) v_mine = fabsf(*reinterpret_cast<const float *>(scales + sc_slot * 256 + (c >> 3) * 64 + 32 + (c & 7) * 4));
+            if (I8) v_mine = fabsf(*reinterpret_cast<const float *>(scales + sc_slot * 256 + (c >> 3) * 64 + 32 + c % 8 * 4));
             float vto = vref;
             if (I8 && __any(v_mine > v_low)) {
                 float vtop = 0.0f;  // the largest scale that the row sees
@@ -896,10 +910,12 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
             for (int n = 0; n < PH * U; ++n) {
                 f4 a = {};
 #pragma unroll
-                for (int g = 0; g < KG; ++g) a += *reinterpret_cast<const f4 *>(chunk(g * RT + rt, n / U, n % U, e_sum, h_sum, rr));
+                for (int g = 0; g < KG; ++g)
+                    a += *reinterpret_cast<const f4 *>(chunk(g * RT + rt, n / U, n % U, e_sum, h_sum, rr));
                 y[n] = make_float4(a[0] * inv[i], a[1] * inv[i], a[2] * inv[i], a[3] * inv[i]);
             }
-            attn_put<PH * U>(dst, kind, R.in_scale, y, [&](int n) { return to[i] + 32 * UD * (n % U) + 8 * UD * (ph0 + n / U); });
+            attn_put<PH * U>(dst, kind, R.in_scale, y,
+                             [&](int n) { return to[i] + 32 * UD * (n % U) + 8 * UD * (ph0 + n / U); });
         }
     }
 }
@@ -957,9 +973,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(PagedArgs A, AttnArgs R,
     }
     if (!real) return;
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int64_t to = ((int64_t)(T.S.start + R.group.div(row)) * R.heads + kvh * (int)R.group.d + R.group.mod(row)) * D + d;
+    const int64_t orow = (int64_t)(T.S.start + R.group.div(row)) * R.heads + kvh * (int)R.group.d + R.group.mod(row);
     const float4 z[1] = {make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv)};
-    attn_put<1>(R.out, R.out_kind, R.in_scale, z, [&](int) { return to; });
+    attn_put<1>(R.out, R.out_kind, R.in_scale, z, [&](int) { return orow * D + d; });
 }
 
 // ---- host ---------------------------------------------------------------------------------------------
@@ -971,17 +987,16 @@ struct AttnPlan {
     size_t bytes;
 };
 
-// Blocks of one row tile need no barrier and run two to a CU; blocks of more share each key tile's loads. Of
-// 256 tokens' rows or more at group 4 or 8 (us):
-//   int8, head_dim 64, 128: 1 always (2048 tokens, 32 heads on 8, 4096 keys: 140 and 214; two or four row tiles
-//     a block: 152..171 and 254..261).
-//   int8, head_dim 256: 2 (8 heads on 1; 8192 tokens on their own: 381, one: 398, four: 415; 2048 tokens on 8192
-//     keys: 166, 181, 170).
-//   f16: 4 where that leaves every second CU a block at least, for splitting the keys further costs more than
-//     it brings (head_dim 256, 8 heads on 1, 8192 tokens: 402, two: 580, one: 555; 2048 on 8192 keys: 171, 245,
-//     226; head_dim 128, 32 heads on 8, 2048 tokens on 4096 keys: 181, 196, 197). With fewer blocks 2 at head_dim
-//     256 (512 tokens, window 512: 21, four: 28, one: 27), which one block a CU is left of anyway, and else 1
-//     (300 tokens, 16 heads on 4, head_dim 128: 20, two: 26, four: 22).
+// Row tiles of a block (kRows rows of a sequence or fewer: 1). Blocks of one need no barrier and run two to a
+// CU where LDS holds two; blocks of more share each key tile's loads. Measured with 1, 2 and 4 (us):
+//   int8, head_dim 64 and 128: 1. 2048 tokens, 32 heads on 8, on 4096 keys: 140, 171, 152 and 214, 261, 254.
+//   int8, head_dim 256: 2. 8 heads on 1: 8192 tokens on their own 398, 381, 415; 2048 on 8192 keys 181, 166, 170
+//     (four split the keys in two); 100 on 1100 keys 19, 20, 28; 16 x 64 tokens 30, 28, 42.
+//   f16: 4 where that gives every second CU a block, so that the keys are split in two at most, for the parts'
+//     way through memory costs more from there on. head_dim 256, 8 heads on 1: 8192 tokens 555, 580, 402; 2048 on
+//     8192 keys 226, 245, 168; head_dim 128, 2048 tokens, 32 heads on 8, 197, 196, 181; head_dim 64 111, 116, 103.
+//   f16 otherwise: 2 at head_dim 256, where LDS holds one block a CU anyway (512 tokens, window 512, 27, 20,
+//     28; 16 x 64 tokens 40, 29, 40), else 1 (300 tokens, 16 heads on 4, head_dim 128: 20, 26, 22).
 static int row_tiles(bool i8, int d, int64_t rows, int64_t blocks4) {
     if (rows <= kRows) return 1;
     if (!i8 && blocks4 * 2 >= device_cu_count()) return 4;
@@ -1051,6 +1066,8 @@ static int attn_check(const g4_kv_pages *pages, const g4_chunk *chunk, int heads
     if (window < 0) return set_error(G4_ERR_INVALID, "attention-chunk: window %d", window);
     if ((int64_t)A->tokens * heads > ((int64_t)1 << 30) || A->kv_heads > 65535)
         return set_error(G4_ERR_UNSUPPORTED, "attention-chunk: more than 2^30 query rows, or 65535 KV heads");
+    if (A->max_kv > 1 << 30)
+        return set_error(G4_ERR_UNSUPPORTED, "attention-chunk: max_kv %d is over 2^30 positions", A->max_kv);
     if (A->page_stride > INT32_MAX || A->slot_stride * pages->page_size > INT32_MAX)
         return set_error(G4_ERR_UNSUPPORTED, "attention-chunk: pages, or a page's slots, 2^31 or more elements apart");
     return G4_OK;
@@ -1077,7 +1094,8 @@ int g4_attention_chunk(const g4_kv_pages *pages, const g4_chunk *chunk, const vo
     if (!q || !out || !workspace) return set_error(G4_ERR_INVALID, "attention-chunk needs q, an output and a workspace");
     if (out_kind != G4_KIND_F16 && out_kind != G4_KIND_F32 && out_kind != G4_KIND_I8)
         return set_error(G4_ERR_INVALID, "attention-chunk: outputs are f16, f32 or int8 codes, got kind %d", out_kind);
-    if (!std::isfinite(scale)) return set_error(G4_ERR_INVALID, "attention-chunk: scale must be finite");
+    if (!std::isfinite(scale * 2.0f))
+        return set_error(G4_ERR_INVALID, "attention-chunk: the scale must be finite and below 2^127");
     if (out_kind == G4_KIND_I8 && in_scale == 0.0f)
         return set_error(G4_ERR_INVALID, "attention-chunk: int8 codes need the consumer's inScale");
     const int64_t qw = (int64_t)heads * pages->head_dim;
@@ -1097,7 +1115,7 @@ int g4_attention_chunk(const g4_kv_pages *pages, const g4_chunk *chunk, const vo
     R.heads = heads;
     R.group = FastDiv::of(heads / A.kv_heads);
     // a scale of 0 as one too small to matter, so that a masked score stays minus infinity
-    R.scale2 = std::max(std::fabs(scale) * 1.44269504088896340736f, 0x1p-100f);
+    R.scale2 = std::max(std::fabs(scale) * 1.44269504088896340736f, 0x1p-126f);
     R.q_sign = scale < 0.0f ? 0x80008000u : 0u;
     R.page_bytes = (uint32_t)(A.page_stride * eb);
     R.slot_bytes = (uint32_t)(A.slot_stride * eb);

@@ -113,8 +113,9 @@ __device__ __forceinline__ double bulk_weight(float x, const RowScale &S, const 
         y = near_cap(y, A);
         if (is_far(x, A)) y = softcap64(x, A.cap);
     }
-    const double e = pow2((y - S.top) * S.slope);
-    return !CAP && x == INFINITY ? 1.0 : e;  // the maximum then too
+    const double z = (y - S.top) * S.slope;
+    const double e = z > -1000.0 ? pow2(z) : 0.0;  // under 2^-1000 of the largest: none
+    return !CAP && x == INFINITY ? 1.0 : e;
 }
 
 __device__ __forceinline__ float clean(float x) { return x == x ? x : -INFINITY; }
@@ -352,7 +353,8 @@ __device__ __forceinline__ double source_weight(const VerifyArgs &A, const Sourc
 
 // The block's thread's weights of a unit, in the element order of load_range; returns their sum.
 template <bool CAP>
-__device__ __forceinline__ double unit_weights(const VerifyArgs &A, const Source &S, int64_t base, double (&w)[kUnitPer]) {
+__device__ __forceinline__ double unit_weights(const VerifyArgs &A, const Source &S, int64_t base,
+                                               double (&w)[kUnitPer]) {
     float xp[kUnitPer], xq[kUnitPer] = {};
     const int n = (int)(A.vocab - base < kUnit ? A.vocab - base : kUnit);
     load_range(S.p + base, n, A.vec, xp);

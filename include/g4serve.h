@@ -107,9 +107,13 @@ int g4_kv_read(const g4_kv_pages *pages, const g4_chunk *chunk, void *k_out, voi
  * multiple of kv_heads (query heads h * heads / kv_heads .. share KV head h). out [tokens][heads]
  * [head_dim], packed: G4_KIND_F16, G4_KIND_F32, or G4_KIND_I8: the consumer's input codes on in_scale
  * (quant.ts:309-334 srqCodes). A row that sees no key is zeros.
- * Products are of f16 values (int8 codes are exact in f16) added up in f32; softmax weights are rounded
- * to f16, their sum is not. A masked position's contents, NaN included, change nothing; a NaN or an
- * infinity that a row sees makes that row's outputs non-finite.
+ * f16 rows: products of f16 values, added up in f32; a weight is rounded to f16 (relative to a maximum
+ * within 2^8 of the row's), and the softmax's sum adds the rounded ones. int8 rows: q enters the scores as
+ * 16-bit fixed point of the row's largest magnitude (off by 2^-16 of that at most) and the codes exactly;
+ * a weight is rounded to f16 with V's scale in it (scales up to 2^99 in magnitude). A masked position's
+ * contents, NaN included, change nothing. Of what a row sees: a NaN or an infinity in V, and a score that is NaN or
+ * +infinity, make its outputs non-finite; a score of -infinity has no weight.
+ * page_stride and page_size * slot_stride below 2^31 elements; |scale| below 2^127.
  * workspace: g4_attention_chunk_workspace_bytes(...) bytes, 16-byte aligned.
  */
 int g4_attention_chunk(const g4_kv_pages *pages, const g4_chunk *chunk, const void *q, int64_t q_stride,

@@ -181,6 +181,10 @@ def test_ends_of_the_random_numbers(gpu):
         assert (got[1] == 3).all()
     un[:] = 0
     assert (run(logits, dl, drafts, start, u, un, 3, 0.0, 1.0)[0][:, 3] == 100).all()
+    logits[[3, 7], 8500] = np.inf  # the others weigh nothing beside it
+    assert (run(logits, dl, drafts, start, u, un, 3, 0.0, 1.0)[0][:, 3] == 8500).all()
+    logits[[3, 7], 8500], logits[[3, 7], 100:8500] = 3000, -3000
+    assert (run(logits, dl, drafts, start, u, un, 3, 0.0, 1.0)[0][:, 3] == 8500).all()
 
 
 def test_nan_infinite_and_empty_rows(gpu):

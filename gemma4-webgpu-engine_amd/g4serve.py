@@ -51,6 +51,13 @@ def _address(x, what, device):
     return p
 
 
+def _call_device(pages, chunk) -> int:
+    device = _device()
+    if pages.device != device or chunk.device != device:
+        raise g4.G4Error(1, "the pages or the chunk are on another device than the current one")
+    return device
+
+
 def _packed(x, what, kinds, shape, device):
     """The address of a contiguous operand of one of `kinds` and of `shape`."""
     if _kind(x) not in kinds:
@@ -123,15 +130,16 @@ class KVPages:
         page_stride, slot, head = strides[0], *(reversed(strides[1:]) if heads_first else strides[1:])
         self.buffers = (k, v, k_scales, v_scales)
         self.kind, self.kv_heads, self.head_dim, self.page_size = kind, heads, dim, slots
-        s, device = [None, None], _device()
+        s = [None, None]
+        device = self.device = _device()
         if kind == g4.KIND_I8:
             if k_scales is None or v_scales is None:
                 raise g4.G4Error(1, "int8 pages need their scales")
             s = [_packed(x, "page scales", _F32, (pages, heads, slots), device) for x in (k_scales, v_scales)]
         elif k_scales is not None or v_scales is not None:
             raise g4.G4Error(1, "f16 pages have no scales")
-        self.c = KVPagesStruct(_address(k, "k pages", device), _address(v, "v pages", device), s[0], s[1], kind, pages, slots,
-                               heads, dim, page_stride, slot, head)
+        self.c = KVPagesStruct(_address(k, "k pages", device), _address(v, "v pages", device), s[0], s[1], kind,
+                               pages, slots, heads, dim, page_stride, slot, head)
         self.ref = ctypes.byref(self.c)
 
 
@@ -152,7 +160,7 @@ class Chunk:
             stride = st[0] if seqs > 1 else width
         if _kind(page_table) != g4.KIND_I32:
             raise g4.G4Error(1, f"page_table cannot be {page_table.dtype}")
-        device = _device()
+        device = self.device = _device()
         self.buffers = (q_start, kv_len, page_table)
         self.seqs, self.tokens, self.max_q, self.max_kv = seqs, int(tokens), int(max_q), int(max_kv)
         self.c = ChunkStruct(seqs, self.tokens, self.max_q, self.max_kv,
@@ -168,7 +176,7 @@ def paged_prologue(pages, chunk, q, k, v, q_out, q_gain=None, k_gain=None, cos=N
     q [tokens][heads][head_dim], k and v [tokens][kv_heads][head_dim], of one type (f32, f16, or int8
     codes times q_scale / k_scale / v_scale, each x_scale where not given); their tokens may lie apart.
     q and q_out None: only the store; k and v None: only the queries."""
-    d, t, device = pages.head_dim, chunk.tokens, _device()
+    d, t, device = pages.head_dim, chunk.tokens, _call_device(pages, chunk)
     kind, heads = None, 0
     qa = ka = va = (None, None, 0)
     qo = None
@@ -208,7 +216,7 @@ def kv_read(pages, chunk, k_out, v_out, stream=None):
     """g4_kv_read: the chunk's rows back from the cache, f32 or f16, to [tokens][kv_heads][head_dim],
     or to [seqs][rows][kv_heads][head_dim] with rows >= max_q (row i of a sequence at [s][i]; the rest
     is left as it was). k_out or v_out may be None."""
-    device, kinds, at = _device(), [], []
+    device, kinds, at = _call_device(pages, chunk), [], []
     for x, what in ((k_out, "k_out"), (v_out, "v_out")):
         if x is None:
             at.append(None)
@@ -239,11 +247,12 @@ def attention_chunk_workspace_bytes(pages, chunk, heads, window=0) -> int:
 def attention_chunk(pages, chunk, q, out, workspace, scale=1.0, window=0, in_scale=0.0, stream=None):
     """g4_attention_chunk: causal attention of the chunk's rows over the cache. q f16 [tokens][heads]
     [head_dim] (tokens may lie apart); out f16, f32, or int8 codes on in_scale, packed."""
-    heads, device = int(q.shape[1]), _device()
+    heads, device = int(q.shape[1]), _call_device(pages, chunk)
     qp, _, stride = _rows(q, "q", _F16, heads, pages.head_dim, chunk.tokens, device)
     op = _packed(out, "out", _X_KINDS, (chunk.tokens, heads, pages.head_dim), device)
     st = g4.lib().g4_attention_chunk(pages.ref, chunk.ref, qp, stride, heads, scale, window,
-                                     _address(workspace, "workspace", device), workspace.nbytes, op, _kind(out), in_scale, stream)
+                                     _address(workspace, "workspace", device), workspace.nbytes, op, _kind(out),
+                                     in_scale, stream)
     if st:
         g4._check(st)
 

@@ -135,6 +135,20 @@ def test_attention_refusals(g4):
     expect(g4, lambda: g4._check(g4.lib().g4_attention_chunk(p.ref, c.ref, 0x1000, 0, 4, 1.0, 0, 0x1000, 1 << 24, 0x1000, 3, 0.0, None)), 1, "got kind 3")
 
 
+def test_attention_limits(g4, monkeypatch):
+    p, q, ws = pages(), Fake((6, 4, 128), np.float16), Fake((1 << 24,), np.uint8)
+    call = lambda p=p, c=chunk(), **kw: gs.attention_chunk(p, c, q, q, ws, **kw)
+    for scale in (float("inf"), float("nan"), 2.0 ** 127):
+        expect(g4, lambda: call(scale=scale), 1, "below 2^127")
+    wide = Strided((4, 16, 2, 128), np.float16, (1 << 31, 256, 128, 1))
+    expect(g4, lambda: call(p=gs.KVPages(wide, wide)), 5, "2^31 or more elements apart")
+    long = gs.Chunk(Fake((3,), np.int32), Fake((2,), np.int32), Fake((2, (1 << 26) + 1), np.int32), 6, 4, (1 << 30) + 1)
+    expect(g4, lambda: call(c=long), 5, "over 2^30 positions")
+    monkeypatch.setattr(gs, "_device", lambda: 1)
+    for f in (call, lambda: gs.kv_read(p, chunk(), q, None), lambda: gs.paged_prologue(p, chunk(), q, None, None, q)):
+        expect(g4, f, 1, "on another device than the current one")
+
+
 def test_verify_refusals(g4):
     f = Fake
     base = dict(logits=f((5, 100), np.float32), draft_logits=f((3, 100), np.float32), draft_tokens=f((3,), np.int32),

@@ -58,7 +58,7 @@ struct AttnArgs {
     const _Float16 *q;
     int64_t q_stride;
     int heads;
-    FastDiv group;
+    FastDiv group, per_seq;
     // Scores are kept as the products give them; the base-2 exponent is score * scale2, scale2 > 0. A
     // negative scale turns Q's signs over.
     float scale2;
@@ -141,36 +141,48 @@ __device__ __forceinline__ int wave_scan_sum(int v) {
     return v;
 }
 
-// Tile `id` of the batch: sequences in order, ceil(rows * group / per) tiles each.
-__device__ __forceinline__ Tile find_tile(const PagedArgs &A, const FastDiv &group, int window, int id, int per) {
-    const int lane = threadIdx.x & 63;
+// The tile of block `id`: tile id % per_seq of sequence id / per_seq; or with per_seq 0, where the grid has no
+// room for every sequence's most, the id-th of all: sequences in order, ceil(rows * group / per) tiles each,
+// looked for 64 sequences at a time.
+__device__ __forceinline__ Tile find_tile(const PagedArgs &A, const FastDiv &group, const FastDiv &per_seq, int window,
+                                          int id, int per) {
     Tile T{};
-    for (int base = 0; base < A.seqs; base += 64) {
-        int n = 0;
-        SeqSpan S{0, 0, 0};
-        if (base + lane < A.seqs) {
-            S = seq_span(A, base + lane);
-            n = (min(S.rows, A.max_q) * (int)group.d + per - 1) / per;
+    int at = 0;
+    if (per_seq.d) {
+        T.seq = per_seq.div(id);
+        at = per_seq.mod(id);
+        T.S = seq_span(A, T.seq);
+        T.rows = min(T.S.rows, A.max_q) * (int)group.d;
+        T.live = at * per < T.rows;
+    } else {
+        const int lane = threadIdx.x & 63;
+        for (int base = 0; base < A.seqs && !T.live; base += 64) {
+            int n = 0;
+            SeqSpan S{0, 0, 0};
+            if (base + lane < A.seqs) {
+                S = seq_span(A, base + lane);
+                n = (min(S.rows, A.max_q) * (int)group.d + per - 1) / per;
+            }
+            const int end = wave_scan_sum(n);
+            const unsigned long long past = __ballot(end > id);
+            if (past) {
+                const int l = __ffsll((long long)past) - 1;
+                T.seq = base + l;
+                T.S.start = __builtin_amdgcn_readlane(S.start, l);
+                T.S.rows = __builtin_amdgcn_readlane(S.rows, l);
+                T.S.kv = __builtin_amdgcn_readlane(S.kv, l);
+                T.rows = min(T.S.rows, A.max_q) * (int)group.d;
+                at = id - (__builtin_amdgcn_readlane(end, l) - __builtin_amdgcn_readlane(n, l));
+                T.live = true;
+            }
+            id -= __builtin_amdgcn_readlane(end, 63);
         }
-        const int end = wave_scan_sum(n);
-        const unsigned long long past = __ballot(end > id);
-        if (past) {
-            const int at = __ffsll((long long)past) - 1;
-            T.seq = base + at;
-            T.S.start = __builtin_amdgcn_readlane(S.start, at);
-            T.S.rows = __builtin_amdgcn_readlane(S.rows, at);
-            T.S.kv = __builtin_amdgcn_readlane(S.kv, at);
-            T.rows = min(T.S.rows, A.max_q) * (int)group.d;
-            T.first = (id - (__builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(n, at))) * per;
-            const int p0 = T.S.kv - T.S.rows + group.div(T.first);
-            const int p1 = T.S.kv - T.S.rows + group.div(min(T.first + per, T.rows) - 1);
-            T.lo = window ? max(0, p0 - window + 1) & ~(kKeys - 1) : 0;
-            T.hi = max(p1 + 1, 0);
-            T.live = true;
-            return T;
-        }
-        id -= __builtin_amdgcn_readlane(end, 63);
     }
+    T.first = at * per;
+    const int p0 = T.S.kv - T.S.rows + group.div(T.first);
+    const int p1 = T.S.kv - T.S.rows + group.div(max(min(T.first + per, T.rows) - 1, 0));
+    T.lo = window ? max(0, p0 - window + 1) & ~(kKeys - 1) : 0;
+    T.hi = max(p1 + 1, 0);
     return T;
 }
 
@@ -317,7 +329,7 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
     const int rt = wave % RT, kg = wave / RT;
     const int h = lane >> 5, c = lane & 31;
     const int kvh = blockIdx.z;
-    const Tile T = find_tile(A, R.group, R.window, blockIdx.x, kRows * RT);
+    const Tile T = find_tile(A, R.group, R.per_seq, R.window, blockIdx.x, kRows * RT);
     if (!T.live) return;
     const int per = split_tiles(T, R.splits, KG);
     const int k0 = T.lo + blockIdx.y * per * kKeys, k1 = min(T.hi, k0 + per * kKeys);
@@ -930,7 +942,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(PagedArgs A, AttnArgs R,
     __shared__ float2 mls[G > 1 ? 256 : 1];
     const int t = threadIdx.x, d = (t % TR) * 4, g = t / TR % G, kvh = blockIdx.z;
     const int rr = blockIdx.y * RBK + t / (TR * G);
-    const Tile T = find_tile(A, R.group, R.window, blockIdx.x, tile_rows);
+    const Tile T = find_tile(A, R.group, R.per_seq, R.window, blockIdx.x, tile_rows);
     if (!T.live || T.first + (int)blockIdx.y * RBK >= T.rows) return;
     const int row = T.first + rr;
     const bool real = rr < tile_rows && row < T.rows;
@@ -983,6 +995,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(PagedArgs A, AttnArgs R,
 struct AttnPlan {
     int rt;         // row tiles of a block
     int64_t tiles;  // blocks' row ranges, an upper bound over the batch
+    int per_seq;    // tiles is this many for every sequence (0: less)
     int splits, key_groups;
     size_t bytes;
 };
@@ -1014,7 +1027,9 @@ static AttnPlan attn_plan(const PagedArgs &A, const g4_kv_pages *pages, int head
     P.rt = row_tiles(i8, d, most, tiles4 * A.kv_heads);
     P.key_groups = key_groups(P.rt, i8);
     const int rows = kRows * P.rt;
-    P.tiles = std::min((most + rows - 1) / rows * A.seqs, (int64_t)A.tokens * group / rows + A.seqs);
+    const int64_t per_seq = (most + rows - 1) / rows, ragged = (int64_t)A.tokens * group / rows + A.seqs;
+    P.per_seq = per_seq * A.seqs <= ragged ? (int)per_seq : 0;
+    P.tiles = std::min(per_seq * A.seqs, ragged);
     int64_t keys = A.max_kv;
     if (window) keys = std::min<int64_t>(keys, (int64_t)window + kKeys + rows / group + 1);
     const int64_t rounds = (keys + P.key_groups * kKeys - 1) / (P.key_groups * kKeys);
@@ -1114,6 +1129,7 @@ int g4_attention_chunk(const g4_kv_pages *pages, const g4_chunk *chunk, const vo
     R.q_stride = q_stride ? q_stride : qw;
     R.heads = heads;
     R.group = FastDiv::of(heads / A.kv_heads);
+    if (P.per_seq) R.per_seq = FastDiv::of(P.per_seq);
     // a scale of 0 as one too small to matter, so that a masked score stays minus infinity
     R.scale2 = std::max(std::fabs(scale) * 1.44269504088896340736f, 0x1p-126f);
     R.q_sign = scale < 0.0f ? 0x80008000u : 0u;

@@ -1003,16 +1003,20 @@ struct AttnPlan {
 // Row tiles of a block (kRows rows of a sequence or fewer: 1). Blocks of one need no barrier and run two to a
 // CU where LDS holds two; blocks of more share each key tile's loads. Measured with 1, 2 and 4 (us):
 //   int8, head_dim 64 and 128: 1. 2048 tokens, 32 heads on 8, on 4096 keys: 140, 171, 152 and 214, 261, 254.
-//   int8, head_dim 256: 2. 8 heads on 1: 8192 tokens on their own 398, 381, 415; 2048 on 8192 keys 181, 166, 170
-//     (four split the keys in two); 100 on 1100 keys 19, 20, 28; 16 x 64 tokens 30, 28, 42.
+//   int8, head_dim 256, 8 heads on 1: 2 where a block then has 4096 keys or more of its own, else 1. 8192 tokens on
+//     their own 398, 381, 415; 2048 on 8192 keys 181, 164, 170 (four split the keys in two); 4096 on their own 122,
+//     123; 300 on 8300 keys 46, 60; 64 x 64 tokens on up to 2064 keys 62, 80; 32 x 8 on up to 4096 28, 28, on up
+//     to 16008 59, 56; 1000 tokens, window 512, 30, 37, 47; 100 on 1100 keys 18, 20, 28.
 //   f16: 4 where that gives every second CU a block, so that the keys are split in two at most, for the parts'
 //     way through memory costs more from there on. head_dim 256, 8 heads on 1: 8192 tokens 555, 580, 402; 2048 on
 //     8192 keys 226, 245, 168; head_dim 128, 2048 tokens, 32 heads on 8, 197, 196, 181; head_dim 64 111, 116, 103.
 //   f16 otherwise: 2 at head_dim 256, where LDS holds one block a CU anyway (512 tokens, window 512, 27, 20,
 //     28; 16 x 64 tokens 40, 29, 40), else 1 (300 tokens, 16 heads on 4, head_dim 128: 20, 26, 22).
-static int row_tiles(bool i8, int d, int64_t rows, int64_t blocks4) {
+static int row_tiles(bool i8, int d, int64_t rows, int64_t keys, int64_t blocks2, int64_t blocks4) {
+    const int64_t cus = device_cu_count();
     if (rows <= kRows) return 1;
-    if (!i8 && blocks4 * 2 >= device_cu_count()) return 4;
+    if (i8) return d == 256 && keys * std::min(blocks2, cus) >= 4096 * cus ? 2 : 1;
+    if (blocks4 * 2 >= cus) return 4;
     return d == 256 ? 2 : 1;
 }
 
@@ -1023,15 +1027,22 @@ static AttnPlan attn_plan(const PagedArgs &A, const g4_kv_pages *pages, int head
     AttnPlan P;
     const int64_t most = (int64_t)A.max_q * group;  // rows of a sequence
     const bool i8 = pages->kind == G4_KIND_I8;
-    const int64_t tiles4 = std::min((most + 127) / 128 * A.seqs, (int64_t)A.tokens * group / 128 + A.seqs);
-    P.rt = row_tiles(i8, d, most, tiles4 * A.kv_heads);
+    auto tiles = [&](int rows, bool *even) {  // of `rows` rows, at most; even: that is every sequence's most
+        const int64_t each = (most + rows - 1) / rows * A.seqs, ragged = (int64_t)A.tokens * group / rows + A.seqs;
+        if (even) *even = each <= ragged;
+        return std::min(each, ragged);
+    };
+    auto keys_of = [&](int rows) -> int64_t {
+        return window ? std::min<int64_t>(A.max_kv, (int64_t)window + kKeys + rows / group + 1) : A.max_kv;
+    };
+    P.rt = row_tiles(i8, d, most, keys_of(2 * kRows), tiles(2 * kRows, nullptr) * A.kv_heads,
+                     tiles(4 * kRows, nullptr) * A.kv_heads);
     P.key_groups = key_groups(P.rt, i8);
     const int rows = kRows * P.rt;
-    const int64_t per_seq = (most + rows - 1) / rows, ragged = (int64_t)A.tokens * group / rows + A.seqs;
-    P.per_seq = per_seq * A.seqs <= ragged ? (int)per_seq : 0;
-    P.tiles = std::min(per_seq * A.seqs, ragged);
-    int64_t keys = A.max_kv;
-    if (window) keys = std::min<int64_t>(keys, (int64_t)window + kKeys + rows / group + 1);
+    bool even;
+    P.tiles = tiles(rows, &even);
+    P.per_seq = even ? (int)((most + rows - 1) / rows) : 0;
+    const int64_t keys = keys_of(rows);
     const int64_t rounds = (keys + P.key_groups * kKeys - 1) / (P.key_groups * kKeys);
     const int64_t want = (P.rt == 1 ? 2 : 1) * (int64_t)device_cu_count();
     const int64_t blocks = P.tiles * A.kv_heads;

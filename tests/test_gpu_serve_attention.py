@@ -105,6 +105,28 @@ def test_blocks_of_more_row_tiles(gpu, dim, kind, kv_heads, window):
     check(Batch(lens, kv_heads, dim, 16, kind, seed=window + dim, absent=[(0, 1), (1, 0), (1, 2)]), kv_heads, window)
 
 
+@pytest.mark.parametrize("window", [0, 4000])
+def test_int8_blocks_of_two_row_tiles(gpu, window):
+    """Many blocks of 4096 keys or more (by the bounds; most sequences are short), one sequence past the window."""
+    lens = [(33, 35), (64, 64), (65, 140), (0, 9), (40, 4200), (1, 77), (33, 300), (50, 90), (60, 61)]
+    check(Batch(lens, 32, 256, 16, "i8", seed=window, absent=[(2, 1), (4, 0), (4, 240), (6, 18)], max_kv=4224), 32, window)
+
+
+def test_int8_masked_scales_in_blocks_of_two_row_tiles(gpu):
+    m = 70
+    def batch():
+        return Batch([(m, m + 30)], 128, 256, 16, "i8", seed=5, max_kv=4100)
+    b = batch()
+    for p, x in ((m + 28, np.inf), (m + 29, np.nan)):
+        page = b.table[0, p // 16]
+        b.ks[page, :, p % 16], b.vs[page, :, p % 16] = x, x
+    q = queries(b.upload(), 128)
+    got = run(b, q, 0, 0.1).astype(np.float64)
+    want, bound = attention(batch(), q, float(np.float32(0.1)), 0)
+    assert (np.abs(got - want) <= to_kind(want, bound, np.float16))[:m - 2].all()
+    assert not np.isfinite(got[m - 1]).any()
+
+
 @pytest.mark.parametrize("dim,kv_heads", [(256, 1), (64, 128), (256, 128)])
 def test_masked_contents_in_blocks_of_more_row_tiles(gpu, dim, kv_heads):
     """NaN and infinities in the last two tokens' V: rows before them untouched, rows that see them not finite."""

@@ -59,6 +59,7 @@ struct AttnArgs {
     int64_t q_stride;
     int heads;
     FastDiv group, per_seq;
+    bool by_xcd;
     // Scores are kept as the products give them; the base-2 exponent is score * scale2, scale2 > 0. A
     // negative scale turns Q's signs over.
     float scale2;
@@ -141,16 +142,20 @@ __device__ __forceinline__ int wave_scan_sum(int v) {
     return v;
 }
 
-// The tile of block `id`: tile id % per_seq of sequence id / per_seq; or with per_seq 0, where the grid has no
+// The tile of block `id`: tile id % per_seq of sequence id / per_seq (by_xcd: of each eight blocks in a row one
+// takes the next tile of each of eight sequences, so that a sequence's tiles run on one XCD, whose L2 they share:
+// 32 x 8 tokens of 8 heads on up to 16008 keys 53 us for 59, on up to 4096 26.4 for 27.5); or with per_seq 0, where the grid has no
 // room for every sequence's most, the id-th of all: sequences in order, ceil(rows * group / per) tiles each,
 // looked for 64 sequences at a time.
-__device__ __forceinline__ Tile find_tile(const PagedArgs &A, const FastDiv &group, const FastDiv &per_seq, int window,
-                                          int id, int per) {
+__device__ __forceinline__ Tile find_tile(const PagedArgs &A, const FastDiv &group, const FastDiv &per_seq, bool by_xcd,
+                                          int window, int id, int per) {
     Tile T{};
     int at = 0;
     if (per_seq.d) {
-        T.seq = per_seq.div(id);
-        at = per_seq.mod(id);
+        const int n = by_xcd ? id >> 3 : id;
+        T.seq = by_xcd ? per_seq.div(n) * 8 + (id & 7) : per_seq.div(n);
+        at = per_seq.mod(n);
+        if (T.seq >= A.seqs) return T;
         T.S = seq_span(A, T.seq);
         T.rows = min(T.S.rows, A.max_q) * (int)group.d;
         T.live = at * per < T.rows;
@@ -329,7 +334,7 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
     const int rt = wave % RT, kg = wave / RT;
     const int h = lane >> 5, c = lane & 31;
     const int kvh = blockIdx.z;
-    const Tile T = find_tile(A, R.group, R.per_seq, R.window, blockIdx.x, kRows * RT);
+    const Tile T = find_tile(A, R.group, R.per_seq, R.by_xcd, R.window, blockIdx.x, kRows * RT);
     if (!T.live) return;
     const int per = split_tiles(T, R.splits, KG);
     const int k0 = T.lo + blockIdx.y * per * kKeys, k1 = min(T.hi, k0 + per * kKeys);
@@ -942,7 +947,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(PagedArgs A, AttnArgs R,
     __shared__ float2 mls[G > 1 ? 256 : 1];
     const int t = threadIdx.x, d = (t % TR) * 4, g = t / TR % G, kvh = blockIdx.z;
     const int rr = blockIdx.y * RBK + t / (TR * G);
-    const Tile T = find_tile(A, R.group, R.per_seq, R.window, blockIdx.x, tile_rows);
+    const Tile T = find_tile(A, R.group, R.per_seq, R.by_xcd, R.window, blockIdx.x, tile_rows);
     if (!T.live || T.first + (int)blockIdx.y * RBK >= T.rows) return;
     const int row = T.first + rr;
     const bool real = rr < tile_rows && row < T.rows;
@@ -996,6 +1001,7 @@ struct AttnPlan {
     int rt;         // row tiles of a block
     int64_t tiles;  // blocks' row ranges, an upper bound over the batch
     int per_seq;    // tiles is this many for every sequence (0: less)
+    bool by_xcd;
     int splits, key_groups;
     size_t bytes;
 };
@@ -1005,8 +1011,8 @@ struct AttnPlan {
 //   int8, head_dim 64 and 128: 1. 2048 tokens, 32 heads on 8, on 4096 keys: 140, 171, 152 and 214, 261, 254.
 //   int8, head_dim 256, 8 heads on 1: 2 where a block then has 4096 keys or more of its own, else 1. 8192 tokens on
 //     their own 398, 381, 415; 2048 on 8192 keys 181, 164, 170 (four split the keys in two); 4096 on their own 122,
-//     123; 300 on 8300 keys 46, 60; 64 x 64 tokens on up to 2064 keys 62, 80; 32 x 8 on up to 4096 28, 28, on up
-//     to 16008 59, 56; 1000 tokens, window 512, 30, 37, 47; 100 on 1100 keys 18, 20, 28.
+//     123; 300 on 8300 keys 46, 60; 64 x 64 tokens on up to 2064 keys 62, 80; 32 x 8 on up to 4096 28, 28;
+//     1000 tokens, window 512, 30, 37, 47; 100 on 1100 keys 18, 20, 28.
 //   f16: 4 where that gives every second CU a block, so that the keys are split in two at most, for the parts'
 //     way through memory costs more from there on. head_dim 256, 8 heads on 1: 8192 tokens 555, 580, 402; 2048 on
 //     8192 keys 226, 245, 168; head_dim 128, 2048 tokens, 32 heads on 8, 197, 196, 181; head_dim 64 111, 116, 103.
@@ -1042,6 +1048,8 @@ static AttnPlan attn_plan(const PagedArgs &A, const g4_kv_pages *pages, int head
     bool even;
     P.tiles = tiles(rows, &even);
     P.per_seq = even ? (int)((most + rows - 1) / rows) : 0;
+    P.by_xcd = P.per_seq > 1 && A.seqs >= 8;
+    if (P.by_xcd) P.tiles = P.per_seq * (((int64_t)A.seqs + 7) & ~7);
     const int64_t keys = keys_of(rows);
     const int64_t rounds = (keys + P.key_groups * kKeys - 1) / (P.key_groups * kKeys);
     const int64_t want = (P.rt == 1 ? 2 : 1) * (int64_t)device_cu_count();
@@ -1141,6 +1149,7 @@ int g4_attention_chunk(const g4_kv_pages *pages, const g4_chunk *chunk, const vo
     R.heads = heads;
     R.group = FastDiv::of(heads / A.kv_heads);
     if (P.per_seq) R.per_seq = FastDiv::of(P.per_seq);
+    R.by_xcd = P.by_xcd;
     // a scale of 0 as one too small to matter, so that a masked score stays minus infinity
     R.scale2 = std::max(std::fabs(scale) * 1.44269504088896340736f, 0x1p-126f);
     R.q_sign = scale < 0.0f ? 0x80008000u : 0u;

@@ -186,81 +186,93 @@ __global__ __launch_bounds__(256) void paged_prologue_kernel(PagedArgs A, Prolog
 
 // ---- the read-back ------------------------------------------------------------------------------------
 
-// Grid (blocks of kReadTokens rows, 2): y picks K or V. A wave looks the block's rows up at once (their
-// sequences by ballots over the ends), then threads move 8 elements each.
-constexpr int kReadTokens = 16;
+// A block takes kReadTokens rows: a wave looks them up at once (the first one's sequence by ballots over the
+// ends, the others' from there on), then threads move units of 8 elements, K's and V's of kReadBatch at a time.
+constexpr int kReadTokens = 16, kReadBatch = 4;
 
 template <int CK, int OK>
 __global__ __launch_bounds__(256) void kv_read_kernel(PagedArgs A, int d_shift, void *k_out, void *v_out,
                                                       int64_t seq_stride) {
-    __shared__ int64_t src_at[kReadTokens], dst_at[kReadTokens];
-    __shared__ int pos_at[kReadTokens], page_at[kReadTokens];
+    __shared__ int64_t src_at[kReadTokens], dst_at[kReadTokens], scale_at[kReadTokens];  // src_at < 0: absent
     const int t = threadIdx.x;
-    const bool is_v = blockIdx.y;
-    void *out = is_v ? v_out : k_out;
-    if (!out) return;
     const int row0 = blockIdx.x * kReadTokens;
     const int64_t width = (int64_t)A.kv_heads << d_shift;
     if (t < 64) {
-        int seq = A.seqs;
-        for (int j = 0; j < kReadTokens; ++j) {
-            const int s = seq_of_row(A, row0 + j);
-            if (t == j) seq = s;
-        }
+        int seq = seq_of_row(A, row0);
         if (t < kReadTokens) {
-            int64_t dst = -1;
-            int page = -1, pos = 0;
-            if (seq < A.seqs && row0 + t < A.tokens) {
+            const int row = row0 + t;
+            while (seq < A.seqs && A.q_start[seq + 1] <= row) ++seq;
+            int64_t dst = -1, src = -1;
+            if (seq < A.seqs && row < A.tokens) {
                 const SeqSpan S = seq_span(A, seq);
-                const int i = row0 + t - S.start;
-                pos = S.kv - S.rows + i;
+                const int i = row - S.start, pos = S.kv - S.rows + i;
                 if (i >= 0 && i < min(S.rows, A.max_q)) {
-                    dst = seq_stride ? seq * seq_stride + i * width : (int64_t)(row0 + t) * width;
-                    page = pos >= 0 ? page_of(A, seq, pos) : -1;
+                    dst = seq_stride ? seq * seq_stride + i * width : (int64_t)row * width;
+                    const int page = pos >= 0 ? page_of(A, seq, pos) : -1;
+                    if (page >= 0) {
+                        src = row_offset(A, page, pos, 0);
+                        scale_at[t] = scale_offset(A, page, pos, 0);
+                    }
                 }
             }
             dst_at[t] = dst;
-            page_at[t] = page;
-            pos_at[t] = pos;
-            src_at[t] = page >= 0 ? row_offset(A, page, pos, 0) : 0;
+            src_at[t] = src;
         }
     }
     __syncthreads();
-    const int d = 1 << d_shift;
-    const int units = kReadTokens * (int)(width >> 3);
-    for (int u = t; u < units; u += 256) {
-        const int j = u / (int)(width >> 3);
-        const int64_t dst = dst_at[j];
-        if (dst < 0) continue;
-        const int e = (u % (int)(width >> 3)) * 8, head = e >> d_shift;
-        const int page = page_at[j];
-        float y[8] = {};
-        if (page >= 0) {
-            const int64_t at = src_at[j] + head * A.head_stride + (e & (d - 1));
-            if (CK == G4_KIND_F16) {
-                const h8 x = *reinterpret_cast<const h8 *>(static_cast<const _Float16 *>(is_v ? A.v : A.k) + at);
+    const int d = 1 << d_shift, per = (int)(width >> 3);  // units of 8 elements, of a token
+    const int units = kReadTokens * per;
+    constexpr int EB = CK == G4_KIND_F16 ? 2 : 1;
+    for (int u0 = t; u0 < units; u0 += 256 * kReadBatch) {
+        int64_t to[kReadBatch];
+        uint4 x[2][kReadBatch];
+        float s[2][kReadBatch];
 #pragma unroll
-                for (int n = 0; n < 8; ++n) y[n] = (float)x[n];
-            } else {
-                const uint2 x = *reinterpret_cast<const uint2 *>(static_cast<const int8_t *>(is_v ? A.v : A.k) + at);
-                const float s = (is_v ? A.vs : A.ks)[scale_offset(A, page, pos_at[j], head)];
+        for (int b = 0; b < kReadBatch; ++b) {
+            const int u = min(u0 + 256 * b, units - 1), j = u / per, e = (u - j * per) * 8, head = e >> d_shift;
+            to[b] = u0 + 256 * b < units ? dst_at[j] : -1;
+            const int64_t src = src_at[j];
+            const int64_t at = (src + head * A.head_stride + (e & (d - 1))) * EB;
+            const int64_t sat = CK == G4_KIND_I8 && src >= 0 ? scale_at[j] + ((int64_t)head << A.page_shift) : 0;
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    y[n] = (float)(int8_t)(x.x >> (8 * n)) * s;
-                    y[n + 4] = (float)(int8_t)(x.y >> (8 * n)) * s;
+            for (int w = 0; w < 2; ++w) {
+                x[w][b] = make_uint4(0, 0, 0, 0);
+                s[w][b] = 0.0f;
+                if (to[b] < 0 || src < 0 || !(w ? v_out : k_out)) continue;
+                const char *p = static_cast<const char *>(w ? A.v : A.k) + at;
+                if (CK == G4_KIND_F16) {
+                    x[w][b] = *reinterpret_cast<const uint4 *>(p);
+                } else {
+                    const uint2 y = *reinterpret_cast<const uint2 *>(p);
+                    x[w][b].x = y.x;
+                    x[w][b].y = y.y;
+                    s[w][b] = (w ? A.vs : A.ks)[sat];
                 }
             }
+            if (to[b] >= 0) to[b] += e;
         }
-        if (OK == G4_KIND_F16) {
-            h8 o;
 #pragma unroll
-            for (int n = 0; n < 8; ++n) o[n] = (_Float16)y[n];
-            *reinterpret_cast<h8 *>(static_cast<_Float16 *>(out) + dst + e) = o;
-        } else {
-            float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(out) + dst + e);
-            o[0] = make_float4(y[0], y[1], y[2], y[3]);
-            o[1] = make_float4(y[4], y[5], y[6], y[7]);
-        }
+        for (int b = 0; b < kReadBatch; ++b)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                void *out = w ? v_out : k_out;
+                if (to[b] < 0 || !out) continue;
+                float y[8];
+#pragma unroll
+                for (int n = 0; n < 8; ++n)
+                    y[n] = CK == G4_KIND_F16 ? (float)__builtin_bit_cast(h8, x[w][b])[n]
+                                             : (float)(int8_t)((n < 4 ? x[w][b].x : x[w][b].y) >> (8 * (n % 4))) * s[w][b];
+                if (OK == G4_KIND_F16) {
+                    h8 o;
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) o[n] = (_Float16)y[n];
+                    *reinterpret_cast<h8 *>(static_cast<_Float16 *>(out) + to[b]) = o;
+                } else {
+                    float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(out) + to[b]);
+                    o[0] = make_float4(y[0], y[1], y[2], y[3]);
+                    o[1] = make_float4(y[4], y[5], y[6], y[7]);
+                }
+            }
     }
 }
 
@@ -332,7 +344,7 @@ int g4_kv_read(const g4_kv_pages *pages, const g4_chunk *chunk, void *k_out, voi
     const int64_t unit = out_kind == G4_KIND_F16 ? 8 : 4;
     if (seq_stride && (seq_stride % unit || seq_stride < (int64_t)A.max_q * A.kv_heads * pages->head_dim))
         return set_error(G4_ERR_INVALID, "kv-read: seq_stride must hold max_q rows and be a multiple of 16 bytes");
-    const dim3 grid((A.tokens + kReadTokens - 1) / kReadTokens, 2);
+    const dim3 grid((A.tokens + kReadTokens - 1) / kReadTokens);
     const int ds = __builtin_ctz(pages->head_dim);
     hipStream_t s = as_stream(stream);
     const bool f16 = pages->kind == G4_KIND_F16, o16 = out_kind == G4_KIND_F16;

@@ -1052,6 +1052,8 @@ static AttnPlan attn_plan(const PagedArgs &A, const g4_kv_pages *pages, int head
     if (P.by_xcd) P.tiles = P.per_seq * (((int64_t)A.seqs + 7) & ~7);
     const int64_t keys = keys_of(rows);
     const int64_t rounds = (keys + P.key_groups * kKeys - 1) / (P.key_groups * kKeys);
+    // the keys are split until every CU has the blocks that it runs at once (32 x 8 tokens on up to 4096 keys and 512
+    // tokens, window 512: 29 and 20 us; with half the splits 34 and 21, with twice as many 39 and 29)
     const int64_t want = (P.rt == 1 ? 2 : 1) * (int64_t)device_cu_count();
     const int64_t blocks = P.tiles * A.kv_heads;
     P.splits = (int)std::max<int64_t>(1, std::min<int64_t>({rounds, (want + blocks - 1) / blocks, 64}));
@@ -1093,6 +1095,8 @@ static int launch_attn(const PagedArgs &A, const AttnArgs &R, const AttnPlan &P,
     return G4_OK;
 }
 
+constexpr int kMaxTiles = 1 << 22;  // times 512 threads, which a grid's x axis holds
+
 static int attn_check(const g4_kv_pages *pages, const g4_chunk *chunk, int heads, int window, PagedArgs *A) {
     if (int st = paged_args("attention-chunk", pages, chunk, A)) return st;
     if (heads <= 0 || heads % A->kv_heads)
@@ -1117,7 +1121,8 @@ size_t g4_attention_chunk_workspace_bytes(const g4_kv_pages *pages, const g4_chu
                                           int window) {
     PagedArgs A;
     if (attn_check(pages, chunk, heads, window, &A)) return 0;
-    return attn_plan(A, pages, heads, window).bytes;
+    const AttnPlan P = attn_plan(A, pages, heads, window);
+    return P.tiles > kMaxTiles ? 0 : P.bytes;
 }
 
 int g4_attention_chunk(const g4_kv_pages *pages, const g4_chunk *chunk, const void *q, int64_t q_stride,
@@ -1138,6 +1143,8 @@ int g4_attention_chunk(const g4_kv_pages *pages, const g4_chunk *chunk, const vo
     if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)workspace) & 15)
         return set_error(G4_ERR_INVALID, "attention-chunk: q, the output and the workspace must be 16-byte aligned");
     const AttnPlan P = attn_plan(A, pages, heads, window);
+    if (P.tiles > kMaxTiles)
+        return set_error(G4_ERR_UNSUPPORTED, "attention-chunk: more than %d blocks of query rows", kMaxTiles);
     if (workspace_bytes < P.bytes)
         return set_error(G4_ERR_INVALID, "attention-chunk: workspace %zu B < %zu B", workspace_bytes, P.bytes);
     float *part_o = static_cast<float *>(workspace);

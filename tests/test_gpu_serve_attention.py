@@ -105,6 +105,18 @@ def test_blocks_of_more_row_tiles(gpu, dim, kind, kv_heads, window):
     check(Batch(lens, kv_heads, dim, 16, kind, seed=window + dim, absent=[(0, 1), (1, 0), (1, 2)]), kv_heads, window)
 
 
+@pytest.mark.parametrize("kind", ["i8", "f16"])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("lens", [
+    [(5 + i % 4, 20 + 37 * i) for i in range(11)],                    # every sequence has two row tiles or room for them
+    [(8 * (i % 3 > 0), 50 + i) for i in range(17)] + [(8, 8)] * 7,
+    [(1, 3 + i) for i in range(100)] + [(90, 200)] + [(2, 9), (0, 5)] * 20,  # one long chunk among many short ones
+    [(1 + i % 2, 2 + 5 * i) for i in range(70)],
+], ids=["eleven", "gaps", "long", "seventy"])
+def test_batches(gpu, lens, dim, kind):
+    check(Batch(lens, 1, dim, 16, kind, seed=len(lens)), 8)
+
+
 @pytest.mark.parametrize("window", [0, 4000])
 def test_int8_blocks_of_two_row_tiles(gpu, window):
     """Many blocks of 4096 keys or more (by the bounds; most sequences are short), one sequence past the window."""

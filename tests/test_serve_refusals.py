@@ -144,6 +144,11 @@ def test_attention_limits(g4, monkeypatch):
     expect(g4, lambda: call(p=gs.KVPages(wide, wide)), 5, "2^31 or more elements apart")
     long = gs.Chunk(Fake((3,), np.int32), Fake((2,), np.int32), Fake((2, (1 << 26) + 1), np.int32), 6, 4, (1 << 30) + 1)
     expect(g4, lambda: call(c=long), 5, "over 2^30 positions")
+    many = 1 << 23
+    crowd = gs.Chunk(Fake((many + 1,), np.int32), Fake((many,), np.int32), Fake((many, 4), np.int32), many, 1, 60)
+    big = Fake((many, 4, 128), np.float16)
+    expect(g4, lambda: gs.attention_chunk(p, crowd, big, big, ws), 5, "blocks of query rows")
+    expect(g4, lambda: gs.attention_chunk_workspace_bytes(p, crowd, 4), 1, "no such call")
     monkeypatch.setattr(gs, "_device", lambda: 1)
     for f in (call, lambda: gs.kv_read(p, chunk(), q, None), lambda: gs.paged_prologue(p, chunk(), q, None, None, q)):
         expect(g4, f, 1, "on another device than the current one")

@@ -9,10 +9,10 @@
 // A drawn token is the one of up to 262144 whose running sum passes a given point: sums that are 1e-7 off
 // would often name its neighbour. So exponents and sums are held in 64 bits and 2^f is good to 1e-12.
 //
-// What bounds it: (1) the 64-bit operations, about 44 a logit with the softcap (264 rows of 262144: 101 us for a
-// read of 54; 160 rows 61; without the softcap 9 rows take 7); (3) reading the drawn rows again (32 sequences, 28 us,
-// two rows each); (2) and (4) a chain of loads, 4-7 and 10-15 us. Parts of 8192 give 4 waves 32 logits a thread,
-// loaded at once; units of 2048 keep the last step one block's work.
+// What bounds it: (1) the 64-bit operations, about 44 a logit with the softcap (264 rows of 262144: 97 us for a
+// read of 54; 160 rows 61; without the softcap 9 rows take 7); (3) reading the drawn rows again (32 sequences, 26 us,
+// two rows each); (2) and (4) a chain of loads, 4-7 and 8-12 us. Parts of 8192 give 4 waves 32 logits a thread,
+// loaded at once; units of 1024 keep the last step one block's work and its code short (2048: 2.4 us more).
 #include "g4_internal.h"
 #include "../../include/g4serve.h"
 #include <cmath>
@@ -20,7 +20,7 @@
 namespace g4 {
 
 constexpr int kPart = 8192, kVerThreads = 256, kPerThread = kPart / kVerThreads;
-constexpr int kUnit = 2048, kUnitPer = kUnit / kVerThreads;
+constexpr int kUnit = 1024, kUnitPer = kUnit / kVerThreads;
 constexpr int kJudgeWaves = 16;
 constexpr int kMaxDrafts = 63;
 
@@ -32,7 +32,7 @@ struct PartStat {
 
 // What the draw of a sequence needs.
 struct Draw {
-    double p_top, p_sum, q_top, q_sum;  // y(max) and sum of exp((y - top) / T) of the two rows; sum 0: no weight
+    double p_top, p_sum, q_top, p_inv, q_inv;  // y(max), sum of exp((y - top) / T) and 1 over it (no weight: 0)
     int taken, refused;                 // drafts taken; whether the next one was refused
 };
 
@@ -322,7 +322,8 @@ __global__ __launch_bounds__(64 * kJudgeWaves) void verify_judge_kernel(VerifyAr
         return;
     }
     const RowStat Q = refused && A.draft_logits ? qs[taken] : RowStat{0.0, 0.0, -1};
-    A.draws[seq] = {S.top, S.sum, Q.top, Q.sum, taken, refused};
+    A.draws[seq] = {S.top, S.sum, Q.top, S.sum > 0.0 ? 1.0 / S.sum : 0.0, Q.sum > 0.0 ? 1.0 / Q.sum : 0.0, taken,
+                    refused};
 }
 
 // The distribution that the next token comes from: max(p - q, 0), with q a row, one token, or nothing.
@@ -339,8 +340,8 @@ __device__ __forceinline__ Source source_of(const VerifyArgs &A, int seq, int st
     S.q = less && A.draft_logits ? A.draft_logits + (int64_t)(start + D.taken) * A.vocab : nullptr;
     S.ps = row_scale(D.p_top, A);
     S.qs = row_scale(D.q_top, A);
-    S.p_inv = D.p_sum > 0.0 ? 1.0 / D.p_sum : 0.0;
-    S.q_inv = D.q_sum > 0.0 ? 1.0 / D.q_sum : 0.0;
+    S.p_inv = D.p_inv;
+    S.q_inv = D.q_inv;
     S.point = less && !A.draft_logits ? A.draft_tokens[start + D.taken] : -1;
     return S;
 }
@@ -454,9 +455,14 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs A) 
     const Draw D = A.draws[seq];
     const double *w = A.weights + (int64_t)seq * A.units;
     const double u = A.u_next[seq];
-    // every wave by itself: the total, then the first unit that takes the running sum past u of it
-    double total = 0.0;
-    for (int c0 = 0; c0 < A.units; c0 += 64) total += c0 + lane < A.units ? w[c0 + lane] : 0.0;
+    // every wave by itself: the total, then the first unit that takes the running sum past u of it; the first 256
+    // units' sums (a vocabulary of 262144) are read once, all at once
+    double total = 0.0, kept[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) kept[i] = 64 * i + lane < A.units ? w[64 * i + lane] : 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) total += kept[i];
+    for (int c0 = 256; c0 < A.units; c0 += 64) total += c0 + lane < A.units ? w[c0 + lane] : 0.0;
     total = wave_sum64(total);
     int64_t token = -1;
     if (total > 0.0) {
@@ -464,7 +470,8 @@ __global__ __launch_bounds__(kVerThreads) void verify_pick_kernel(VerifyArgs A) 
         double before = 0.0, unit_before = 0.0;
         int unit = -1;
         for (int c0 = 0; c0 < A.units; c0 += 64) {
-            const double x = c0 + lane < A.units ? w[c0 + lane] : 0.0;
+            const double x = c0 == 0 ? kept[0] : c0 == 64 ? kept[1] : c0 == 128 ? kept[2] : c0 == 192 ? kept[3]
+                             : c0 + lane < A.units ? w[c0 + lane] : 0.0;
             double run = x;
 #pragma unroll
             for (int s = 1; s < 64; s <<= 1) {

@@ -24,9 +24,9 @@
 // What bounds it. Many rows: of a key tile's 32 products of 32 cycles a wave and its 330 other vector
 // operations of 4, a SIMD's two waves overlap most, but the two streams share the issue; 2048 tokens on 8192
 // keys, 8 heads of 256, int8: 162 us, 743 TFLOP/s, 0.62 of what a large f16 product reaches (8192 tokens on
-// their own: 381 us; f16: 402 us). Few rows: reading the cache (32 single tokens on 16384 keys, f16: 94 us,
-// 5.7 TB/s), and below that a block's way from its arguments to the first keys and from its last to memory,
-// 4 us each: 4 tokens on 4096 keys take 9.8 us and their join 4.4.
+// their own: 381 us; f16: 402 us). Few rows: reading the cache (32 single tokens on 16384 keys, f16: 90 us,
+// 6.0 TB/s), and below that a block's way from its arguments to the first keys and from its last to memory,
+// 4 us each: 4 tokens on 4096 keys take 9.9 us and their join 3.9.
 #include "g4_paged.h"
 #include <algorithm>
 #include <cmath>

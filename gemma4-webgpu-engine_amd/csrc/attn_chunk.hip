@@ -28,6 +28,7 @@
 // 6.0 TB/s), and below that a block's way from its arguments to the first keys and from its last to memory,
 // 4 us each: 4 tokens on 4096 keys take 9.9 us and their join 3.9.
 #include "g4_paged.h"
+#include "g4_key_span.h"
 #include <algorithm>
 #include <cmath>
 
@@ -186,8 +187,9 @@ __device__ __forceinline__ Tile find_tile(const PagedArgs &A, const FastDiv &gro
     T.first = at * per;
     const int p0 = T.S.kv - T.S.rows + group.div(T.first);
     const int p1 = T.S.kv - T.S.rows + group.div(max(min(T.first + per, T.rows) - 1, 0));
-    T.lo = window ? max(0, p0 - window + 1) & ~(kKeys - 1) : 0;
-    T.hi = max(p1 + 1, 0);
+    const KeySpan K = key_span(p0, p1, window, kKeys);
+    T.lo = K.lo;
+    T.hi = K.hi;
     return T;
 }
 
@@ -1099,7 +1101,8 @@ static int launch_attn(const PagedArgs &A, const AttnArgs &R, const AttnPlan &P,
 
 constexpr int kMaxTiles = 1 << 22;  // times 512 threads, which a grid's x axis holds
 
-static int attn_check(const g4_kv_pages *pages, const g4_chunk *chunk, int heads, int window, PagedArgs *A) {
+// `window` on return: 0 where it hides nothing.
+static int attn_check(const g4_kv_pages *pages, const g4_chunk *chunk, int heads, int &window, PagedArgs *A) {
     if (int st = paged_args("attention-chunk", pages, chunk, A)) return st;
     if (heads <= 0 || heads % A->kv_heads)
         return set_error(G4_ERR_INVALID, "attention-chunk: %d query heads do not divide over %d KV heads", heads, A->kv_heads);
@@ -1110,6 +1113,7 @@ static int attn_check(const g4_kv_pages *pages, const g4_chunk *chunk, int heads
         return set_error(G4_ERR_UNSUPPORTED, "attention-chunk: max_kv %d is over 2^30 positions", A->max_kv);
     if (A->page_stride > INT32_MAX || A->slot_stride * pages->page_size > INT32_MAX)
         return set_error(G4_ERR_UNSUPPORTED, "attention-chunk: pages, or a page's slots, 2^31 or more elements apart");
+    window = effective_window(window, A->max_kv);
     return G4_OK;
 }
 

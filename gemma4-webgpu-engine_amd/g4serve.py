@@ -64,13 +64,23 @@ def _packed(x, what, kinds, shape, device):
         raise g4.G4Error(1, f"{what} cannot be {x.dtype}")
     if x.shape != shape:
         raise g4.G4Error(1, f"{what} has shape {list(x.shape)}, expected {list(shape)}")
+    _need_contiguous(x, what)
+    return _address(x, what, device)
+
+
+def _need_contiguous(x, what):
     try:
         packed = x.is_contiguous()
     except AttributeError:  # a DeviceBuffer is
         packed = not hasattr(x, "stride")
     if not packed:
         raise g4.G4Error(1, f"{what} must be contiguous")
-    return _address(x, what, device)
+
+
+def _workspace(x, device):
+    """(address, bytes) of a workspace. One that is not contiguous may hold fewer bytes than it counts."""
+    _need_contiguous(x, "the workspace")
+    return _address(x, "workspace", device), x.nbytes
 
 
 def _rows(x, what, kinds, heads, dim, tokens, device):
@@ -251,7 +261,7 @@ def attention_chunk(pages, chunk, q, out, workspace, scale=1.0, window=0, in_sca
     qp, _, stride = _rows(q, "q", _F16, heads, pages.head_dim, chunk.tokens, device)
     op = _packed(out, "out", _X_KINDS, (chunk.tokens, heads, pages.head_dim), device)
     st = g4.lib().g4_attention_chunk(pages.ref, chunk.ref, qp, stride, heads, scale, window,
-                                     _address(workspace, "workspace", device), workspace.nbytes, op, _kind(out),
+                                     *_workspace(workspace, device), op, _kind(out),
                                      in_scale, stream)
     if st:
         g4._check(st)
@@ -280,7 +290,7 @@ def verify_drafts(logits, draft_logits, draft_tokens, draft_start, u, u_next, to
         _packed(draft_start, "draft_start", _I32, (seqs + 1,), device), seqs, drafts, width - 1, vocab, cap, temperature,
         None if u is None else _packed(u, "u", _F32, (drafts,), device),
         None if u_next is None else _packed(u_next, "u_next", _F32, (seqs,), device),
-        _address(workspace, "workspace", device), workspace.nbytes, _packed(tokens, "tokens", _I32, (seqs, width), device),
+        *_workspace(workspace, device), _packed(tokens, "tokens", _I32, (seqs, width), device),
         _packed(accepted, "accepted", _I32, (seqs,), device),
         None if logprobs is None else _packed(logprobs, "logprobs", _F32, (seqs, width), device), stream)
     if st:

@@ -2,8 +2,9 @@
 with its quantising store, the read-back, attention of the chunk, and draft verification.
 
 Operands are anything with a shape, a dtype and a device address: g4w8a8.DeviceBuffer, or a torch
-tensor on the current device. Types, shapes and layouts are checked here, values and everything else
-by the library, which raises G4Error. Everything computes in the HIP library.
+tensor on the current device (torch imported before the library is loaded, by the first call into it,
+so that both run on one HIP runtime). Types, shapes and layouts are checked here, values and
+everything else by the library, which raises G4Error. Everything computes in the HIP library.
 """
 from __future__ import annotations
 
@@ -36,6 +37,28 @@ def _device() -> int:
     return torch.cuda.current_device() if torch is not None and torch.cuda.is_initialized() else 0
 
 
+_one_runtime = None
+
+
+def _check_runtime():
+    """The library and torch share a HIP runtime only where torch's was loaded first: the library then
+    finds it under its own runtime's name. Else the process has two, and neither's memory and streams
+    are the other's."""
+    global _one_runtime
+    if _one_runtime is None:
+        g4.lib()
+        _one_runtime = len(_mapped("libamdhip64")) == 1
+    if not _one_runtime:
+        raise g4.G4Error(1, "a torch tensor of another HIP runtime than this library's: import torch before the "
+                            "first call into the library")
+
+
+def _mapped(name):
+    """The files of this name that the process has mapped."""
+    with open("/proc/self/maps") as f:
+        return {line.split()[-1] for line in f if name in line}
+
+
 def _address(x, what, device):
     """The device address of a buffer or tensor. A host tensor, or one of another device than the
     current one, is refused: its address means nothing to a kernel launched here."""
@@ -48,6 +71,8 @@ def _address(x, what, device):
     if x.get_device() != device:
         raise g4.G4Error(1, f"{what} is on another device than the current one" if x.is_cuda else
                          f"{what} is not in device memory")
+    if not _one_runtime:
+        _check_runtime()
     return p
 
 

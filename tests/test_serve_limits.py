@@ -1,5 +1,10 @@
 """What the serving operators refuse at the ends of their arguments (no device needed)."""
+import os
+import subprocess
+import sys
+
 import numpy as np
+import pytest
 
 import g4serve as gs
 from test_serve_refusals import Fake, Strided, chunk, expect, pages
@@ -13,3 +18,33 @@ def test_workspaces_that_are_not_contiguous_are_refused(g4):
     expect(g4, lambda: gs.verify_drafts(Fake((3, 100), np.float32), None, Fake((1,), np.int32), Fake((3,), np.int32),
                                         Fake((1,), np.float32), Fake((2,), np.float32), Fake((2, 2), np.int32),
                                         Fake((2,), np.int32), None, expanded), 1, "the workspace must be contiguous")
+
+
+@pytest.mark.parametrize("first", ["torch", "library"])
+def test_tensors_need_the_librarys_runtime(g4, first):
+    """torch brings a HIP runtime of its own. Imported after the library is loaded it stays a second one, and
+    its tensors are refused (a stand-in for one here: there is no device)."""
+    pytest.importorskip("torch")
+    load = ["import torch", "g4.lib()"]
+    code = f"""
+import sys
+sys.path.insert(0, {os.path.dirname(gs.__file__)!r})
+import numpy as np
+import g4w8a8 as g4
+{chr(10).join(load if first == "torch" else load[::-1])}
+import g4serve as gs
+
+class Tensor:
+    shape, dtype, is_cuda = (4, 16, 2, 128), torch.float16, True
+    data_ptr = lambda self: 0x1000
+    get_device = lambda self: 0
+    stride = lambda self: (4096, 256, 128, 1)
+
+try:
+    gs.KVPages(Tensor(), Tensor())
+    print("taken")
+except g4.G4Error as e:
+    print(e)
+"""
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, check=True).stdout
+    assert ("taken" if first == "torch" else "import torch before the first call into the library") in out

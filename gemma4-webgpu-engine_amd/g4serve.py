@@ -5,6 +5,9 @@ Operands are anything with a shape, a dtype and a device address: g4w8a8.DeviceB
 tensor on the current device (torch imported before the library is loaded, by the first call into it,
 so that both run on one HIP runtime). Types, shapes and layouts are checked here, values and
 everything else by the library, which raises G4Error. Everything computes in the HIP library.
+
+stream: a stream's handle (0: the default stream). None: torch's current stream where an operand is a
+tensor, since what makes and reads tensors runs there, else the default stream.
 """
 from __future__ import annotations
 
@@ -74,6 +77,17 @@ def _address(x, what, device):
     if not _one_runtime:
         _check_runtime()
     return p
+
+
+def _stream(stream, device, *operands):
+    """The handle to launch on."""
+    torch = sys.modules.get("torch")
+    if stream is not None or torch is None or not any(hasattr(x, "data_ptr") for x in operands):
+        return stream
+    try:
+        return torch._C._cuda_getCurrentRawStream(device)
+    except AttributeError:  # the same, some microseconds slower
+        return torch.cuda.current_stream(device).cuda_stream
 
 
 def _call_device(pages, chunk) -> int:
@@ -242,7 +256,8 @@ def paged_prologue(pages, chunk, q, k, v, q_out, q_gain=None, k_gain=None, cos=N
     st = g4.lib().g4_paged_prologue(
         pages.ref, chunk.ref, g4.KIND_F32 if kind is None else kind, qa[0], qa[2],
         x_scale if q_scale is None else q_scale, ka[0], ka[2], x_scale if k_scale is None else k_scale, va[0], va[2],
-        x_scale if v_scale is None else v_scale, heads, qg, kg, tab_c, tab_s, positions, eps, qo, stream)
+        x_scale if v_scale is None else v_scale, heads, qg, kg, tab_c, tab_s, positions, eps, qo,
+        _stream(stream, device, *pages.buffers, *chunk.buffers, q, k, v, q_out, q_gain, k_gain, cos, sin))
     if st:
         g4._check(st)
 
@@ -267,7 +282,8 @@ def kv_read(pages, chunk, k_out, v_out, stream=None):
         kinds.append((_kind(x), rows * pages.kv_heads * pages.head_dim))
     if not kinds or kinds[0] != kinds[-1]:
         raise g4.G4Error(1, "kv-read needs k_out and v_out of one type and layout, or one of them")
-    st = g4.lib().g4_kv_read(pages.ref, chunk.ref, at[0], at[1], kinds[0][0], kinds[0][1], stream)
+    st = g4.lib().g4_kv_read(pages.ref, chunk.ref, at[0], at[1], kinds[0][0], kinds[0][1],
+                            _stream(stream, device, *pages.buffers, *chunk.buffers, k_out, v_out))
     if st:
         g4._check(st)
 
@@ -286,8 +302,8 @@ def attention_chunk(pages, chunk, q, out, workspace, scale=1.0, window=0, in_sca
     qp, _, stride = _rows(q, "q", _F16, heads, pages.head_dim, chunk.tokens, device)
     op = _packed(out, "out", _X_KINDS, (chunk.tokens, heads, pages.head_dim), device)
     st = g4.lib().g4_attention_chunk(pages.ref, chunk.ref, qp, stride, heads, scale, window,
-                                     *_workspace(workspace, device), op, _kind(out),
-                                     in_scale, stream)
+                                     *_workspace(workspace, device), op, _kind(out), in_scale,
+                                     _stream(stream, device, *pages.buffers, *chunk.buffers, q, out, workspace))
     if st:
         g4._check(st)
 
@@ -317,6 +333,8 @@ def verify_drafts(logits, draft_logits, draft_tokens, draft_start, u, u_next, to
         None if u_next is None else _packed(u_next, "u_next", _F32, (seqs,), device),
         *_workspace(workspace, device), _packed(tokens, "tokens", _I32, (seqs, width), device),
         _packed(accepted, "accepted", _I32, (seqs,), device),
-        None if logprobs is None else _packed(logprobs, "logprobs", _F32, (seqs, width), device), stream)
+        None if logprobs is None else _packed(logprobs, "logprobs", _F32, (seqs, width), device),
+        _stream(stream, device, logits, draft_logits, draft_tokens, draft_start, u, u_next, tokens, accepted, logprobs,
+                workspace))
     if st:
         g4._check(st)

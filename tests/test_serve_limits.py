@@ -2,6 +2,7 @@
 import os
 import subprocess
 import sys
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
@@ -28,6 +29,7 @@ def test_tensors_need_the_librarys_runtime(g4, first):
     load = ["import torch", "g4.lib()"]
     code = f"""
 import sys
+from types import SimpleNamespace
 sys.path.insert(0, {os.path.dirname(gs.__file__)!r})
 import numpy as np
 import g4w8a8 as g4
@@ -48,3 +50,36 @@ except g4.G4Error as e:
 """
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, check=True).stdout
     assert ("taken" if first == "torch" else "import torch before the first call into the library") in out
+
+
+def test_tensors_are_used_on_torchs_current_stream(g4, monkeypatch):
+    """Without a stream argument, where any operand is a tensor; DeviceBuffers alone go to the default stream."""
+    class Tensor(Fake):
+        is_cuda = True
+        data_ptr = lambda self: self.ptr
+        get_device = lambda self: 0
+        stride = lambda self: tuple(int(np.prod(self.shape[i + 1:])) for i in range(len(self.shape)))
+        is_contiguous = lambda self: True
+
+    seen = []
+    take = staticmethod(lambda *a: seen.append(a[-1]) or 0)
+    library = type("Library", (), dict.fromkeys(("g4_paged_prologue", "g4_kv_read", "g4_attention_chunk", "g4_verify_drafts"), take))
+    cuda = SimpleNamespace(is_initialized=lambda: True, current_device=lambda: 0)
+    monkeypatch.setitem(sys.modules, "torch", SimpleNamespace(cuda=cuda, _C=SimpleNamespace(_cuda_getCurrentRawStream=lambda d: 0x77)))
+    monkeypatch.setattr(gs.g4, "lib", lambda: library)
+    monkeypatch.setattr(gs, "_one_runtime", True, raising=False)
+
+    def calls(kind, **kw):
+        p = gs.KVPages(*[kind((4, 16, 2, 128), np.float16)] * 2)
+        c, f = chunk(), Fake
+        gs.paged_prologue(p, c, None, f((6, 2, 128), np.float16), f((6, 2, 128), np.float16), None, **kw)
+        gs.kv_read(p, c, f((6, 2, 128), np.float16), None, **kw)
+        gs.attention_chunk(p, c, f((6, 4, 128), np.float16), f((6, 4, 128), np.float16), f((99,), np.uint8), **kw)
+        gs.verify_drafts(f((3, 100), np.float32), None, f((1,), np.int32), f((3,), np.int32), f((1,), np.float32),
+                         kind((2,), np.float32), f((2, 2), np.int32), f((2,), np.int32), None, f((99,), np.uint8), **kw)
+
+    calls(Tensor)
+    calls(Fake)
+    calls(Tensor, stream=0)
+    calls(Tensor, stream=5)
+    assert seen == [0x77] * 4 + [None] * 4 + [0] * 4 + [5] * 4

@@ -280,6 +280,8 @@ __global__ __launch_bounds__(256) void kv_read_kernel(PagedArgs A, int d_shift, 
     }
 }
 
+constexpr int64_t kMaxBlocks = (1 << 24) - 1;  // of 256 threads: a grid has less than 2^32 threads
+
 template <int D, int XK>
 static int launch_prologue(const PagedArgs &A, const PrologueArgs &R, int ck, hipStream_t stream) {
     const int64_t rows = (int64_t)A.tokens * (R.heads + (R.k ? 2 * A.kv_heads : 0));
@@ -326,8 +328,8 @@ int g4_paged_prologue(const g4_kv_pages *pages, const g4_chunk *chunk, int x_kin
     const int64_t qw = (int64_t)heads * d, kw = (int64_t)A.kv_heads * d;
     if ((q && q_stride && q_stride < qw) || (k && k_stride && k_stride < kw) || (v && v_stride && v_stride < kw))
         return set_error(G4_ERR_INVALID, "paged-prologue: a row stride is shorter than the row");
-    if ((int64_t)A.tokens * (heads + 2 * (int64_t)A.kv_heads) > ((int64_t)1 << 33))
-        return set_error(G4_ERR_UNSUPPORTED, "paged-prologue: more than 2^33 head rows");
+    if ((int64_t)A.tokens * (heads + (k ? 2 * (int64_t)A.kv_heads : 0)) > 4 * kMaxBlocks)
+        return set_error(G4_ERR_UNSUPPORTED, "paged-prologue: more than %lld head rows", (long long)(4 * kMaxBlocks));
     PrologueArgs R{q, k, v, q_stride ? q_stride : qw, k_stride ? k_stride : kw, v_stride ? v_stride : kw,
                    q_scale, k_scale, v_scale, heads, q_gain, k_gain, cos_tab, sin_tab, eps,
                    static_cast<_Float16 *>(q_out)};
@@ -348,7 +350,9 @@ int g4_kv_read(const g4_kv_pages *pages, const g4_chunk *chunk, void *k_out, voi
     const int64_t unit = out_kind == G4_KIND_F16 ? 8 : 4;
     if (seq_stride && (seq_stride % unit || seq_stride < (int64_t)A.max_q * A.kv_heads * pages->head_dim))
         return set_error(G4_ERR_INVALID, "kv-read: seq_stride must hold max_q rows and be a multiple of 16 bytes");
-    const dim3 grid((A.tokens + kReadTokens - 1) / kReadTokens);
+    if (A.tokens > kReadTokens * kMaxBlocks)
+        return set_error(G4_ERR_UNSUPPORTED, "kv-read: more than %lld rows", (long long)(kReadTokens * kMaxBlocks));
+    const dim3 grid((unsigned)(((int64_t)A.tokens + kReadTokens - 1) / kReadTokens));
     const int ds = __builtin_ctz(pages->head_dim);
     hipStream_t s = as_stream(stream);
     const bool f16 = pages->kind == G4_KIND_F16, o16 = out_kind == G4_KIND_F16;

@@ -80,7 +80,8 @@ typedef struct g4_chunk {
  * An int8 cache row: scale = f32(amax / 127) with amax the largest magnitude of the f32 row, code =
  * RNE(127 * y / amax), exactly rounded; a zero row has scale 0, a row with an infinity or a NaN has
  * scale NaN and codes 0. An f16 row is rounded to nearest even (past the f16 range: infinity).
- * Two rows of a chunk must not share a position of the cache.
+ * Two rows of a chunk must not share a position of the cache. At most 2^26 - 4 head rows (tokens times the heads of
+ * q, k and v that are given).
  */
 int g4_paged_prologue(const g4_kv_pages *pages, const g4_chunk *chunk, int x_kind, const void *q,
                       int64_t q_stride, float q_scale, const void *k, int64_t k_stride, float k_scale,
@@ -94,7 +95,7 @@ int g4_paged_prologue(const g4_kv_pages *pages, const g4_chunk *chunk, int x_kin
  *                   : (q_start[s] + i) * kv_heads * head_dim), f32 or f16 (rounded once). With
  * q_start counting every position of a sequence (its rows = kv_len[s]) the whole sequence is read,
  * for example into a contiguous f32 cache (g4_decode_kv). Rows on absent pages are zeros. k_out or
- * v_out may be NULL; both 16-byte aligned, seq_stride a multiple of 16 bytes.
+ * v_out may be NULL; both 16-byte aligned, seq_stride a multiple of 16 bytes. At most 2^28 - 16 rows.
  */
 int g4_kv_read(const g4_kv_pages *pages, const g4_chunk *chunk, void *k_out, void *v_out, int out_kind,
                int64_t seq_stride, void *stream);

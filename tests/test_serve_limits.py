@@ -83,3 +83,20 @@ def test_tensors_are_used_on_torchs_current_stream(g4, monkeypatch):
     calls(Tensor, stream=0)
     calls(Tensor, stream=5)
     assert seen == [0x77] * 4 + [None] * 4 + [0] * 4 + [5] * 4
+
+
+def test_grids_of_2_to_the_32_threads_are_refused(g4):
+    """The store has a wave per head row, the read-back a block per 16 rows."""
+    L, p = g4.lib(), pages(shape=(4, 16, 2, 64))
+
+    def store(tokens, heads, k):
+        c = chunk(tokens=tokens)
+        g4._check(L.g4_paged_prologue(p.ref, c.ref, 0, 0x1000 if heads else None, 0, 1.0, k, 0, 1.0, k, 0, 1.0, heads, None, None,
+                                      None, None, 0, 1e-6, 0x1000 if heads else None, None))
+    expect(g4, lambda: store(1 << 20, 61, 0x1000), 5, "more than 67108860 head rows")
+    expect(g4, lambda: store((1 << 26) - 3, 1, None), 5, "more than 67108860 head rows")
+    expect(g4, lambda: store((1 << 24), 0, 0x1000), 5, "more than 67108860 head rows")
+    expect(g4, lambda: g4._check(L.g4_kv_read(p.ref, chunk(tokens=(1 << 28) - 15).ref, 0x1000, None, 0, 0, None)), 5,
+           "more than 268435440 rows")
+    expect(g4, lambda: g4._check(L.g4_kv_read(p.ref, chunk(tokens=(1 << 31) - 1).ref, 0x1000, None, 0, 0, None)), 5,
+           "more than 268435440 rows")

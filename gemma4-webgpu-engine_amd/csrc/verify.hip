@@ -53,22 +53,14 @@ struct VerifyArgs {
     float *logprobs;
 };
 
-__device__ __forceinline__ double softcap64(double x, double cap) {
-    if (cap == 0.0) return x;
-    const double a = fabs(x) / cap;
-    return copysign(cap * (1.0 - 2.0 / (exp(2.0 * a) + 1.0)), x);
-}
-
-// exp((y - top) / T), 1 at the maximum itself (both infinite included).
-__device__ __forceinline__ double weight(float x, double top, const VerifyArgs &A) {
-    const double y = softcap64(x, A.cap);
-    return y == top ? 1.0 : exp((y - top) * A.inv_t);
-}
-
-// weight() for the bulk of a row. 2^z: z = n + f, |f| <= 1/2, a polynomial in f (fitted on Chebyshev nodes,
-// relative error 1.1e-12) and n into the exponent: 14 operations of the 64-bit unit a logit, about what its 4
-// bytes cost to read. The softcap of |x| <= cap / 2 as x + x t P(t), t = (x / cap)^2 (fitted likewise, 8e-14
-// t x off): 11 more; past that the definition.
+// The softcap, tanh(x / cap) cap: |x| <= cap / 2 as x + x t P(t), t = (x / cap)^2 (a polynomial fitted on Chebyshev
+// nodes, 8e-14 t x off, 11 operations), past that 1 - 2 / (e^2a + 1), which would lose digits where a is small. A
+// row's maximum, the bulk of its sums and the judged logits all go through the same two, so that the maximum's
+// exponent is 0 and no other's is above: at a temperature of 1e-12 a difference of 1e-13 would count. (Neither falls
+// as x grows: below half the cap the values of neighbouring f32 logits are 2^-25 of them apart and 2^-44 off.)
+//
+// The weight of the bulk of a row, 2^z: z = n + f, |f| <= 1/2, a polynomial in f (fitted likewise, relative error
+// 1.1e-12) and n into the exponent: 14 operations of the 64-bit unit a logit, about what its 4 bytes cost to read.
 struct RowScale {
     double top, slope;  // 2^((y - top) slope)
 };
@@ -93,6 +85,19 @@ __device__ __forceinline__ double near_cap(double x, const VerifyArgs &A) {
     c = fma_k(c, t, -0.3333333333332598);
     return __builtin_fma(x, t * c, x);
 }
+__device__ __forceinline__ double far_cap(double x, double cap) {
+    const double a = fabs(x) / cap;
+    return copysign(cap * (1.0 - 2.0 / (exp(2.0 * a) + 1.0)), x);
+}
+__device__ __forceinline__ double softcap64(float x, const VerifyArgs &A) {
+    if (A.cap == 0.0) return x;
+    return fabsf(x) > A.half_cap ? far_cap(x, A.cap) : near_cap(x, A);
+}
+// exp((y - top) / T), 1 at the maximum itself (both infinite included).
+__device__ __forceinline__ double weight(float x, double top, const VerifyArgs &A) {
+    const double y = softcap64(x, A);
+    return y == top ? 1.0 : exp((y - top) * A.inv_t);
+}
 // 2^z; below 2^-1000 that (too small to count, and the exponent stays normal), and for a NaN.
 __device__ __forceinline__ double pow2(double z) {
     z = z > -1000.0 ? z : -1000.0;
@@ -116,7 +121,7 @@ __device__ __forceinline__ double bulk_weight(float x, const RowScale &S, const 
     double y = x;
     if (CAP) {
         y = near_cap(y, A);
-        if (is_far(x, A)) y = softcap64(x, A.cap);
+        if (is_far(x, A)) y = far_cap(x, A.cap);
     }
     const double z = (y - S.top) * S.slope;
     const double e = z > -1000.0 ? pow2(z) : 0.0;  // under 2^-1000 of the largest: none
@@ -201,7 +206,7 @@ __global__ __launch_bounds__(kVerThreads) void verify_stats_kernel(VerifyArgs A)
 #pragma unroll
             for (int j = 0; j < kPerThread; ++j) sum += v[j] == m ? 1.0 : 0.0;
         } else {
-            const RowScale S = row_scale(softcap64(m, A.cap), A);
+            const RowScale S = row_scale(softcap64(m, A), A);
             uint32_t far = 0;  // elements left out here
 #pragma unroll
             for (int j = 0; j < kPerThread; ++j) {
@@ -243,7 +248,7 @@ __device__ __forceinline__ RowStat row_stat(const VerifyArgs &A, int row) {
 #pragma unroll
     for (int s = 32; s; s >>= 1) first_max(m, at, __shfl_xor(m, s), __shfl_xor(at, s));
     if (!(m > -INFINITY)) return {0.0, 0.0, -1};
-    const double top = softcap64(m, A.cap);
+    const double top = softcap64(m, A);
     double sum = 0.0;
     for (int c = lane; c < A.parts; c += 64) {
         const PartStat s = c == lane ? mine : p[c];
@@ -261,7 +266,7 @@ __device__ __forceinline__ void draft_span(const VerifyArgs &A, int seq, int *st
 
 // log p of a token of target row `row`.
 __device__ __forceinline__ float log_p(const VerifyArgs &A, int row, int token, const RowStat &P) {
-    const double y = softcap64(A.logits[row * A.vocab + token], A.cap);
+    const double y = softcap64(A.logits[row * A.vocab + token], A);
     return (float)((y == P.top ? 0.0 : (y - P.top) * A.inv_t) - log(P.sum));
 }
 

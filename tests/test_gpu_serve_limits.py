@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 import g4serve as gs
+import test_gpu_serve_verify as verifycase
 from servecases import Batch, attention, dev, to_kind
 
 pytestmark = pytest.mark.gpu
@@ -30,3 +31,31 @@ def test_windows_of_any_size_and_rows_without_positions(gpu, kind, window):
     assert (np.abs(got - want) <= to_kind(want, bound, np.float32)).all()
     assert (got[:11] == 0).all()
     assert np.array_equal(got.view(np.uint32), run(b, q, 0).view(np.uint32))
+
+
+def on_a_grid(c, step, most):
+    """The case's logits on multiples of `step`, under `most` in magnitude: two that differ do so by far more than the
+    smallest temperatures, ties are exact."""
+    snap = lambda x: (np.clip(np.rint(x / step), -most // step, most // step) * step).astype(np.float32)
+    return (snap(c[0]), snap(c[1]), *c[2:])
+
+
+@pytest.mark.parametrize("t", [1e-3, 1e-6, 1e-9, 1e-12, 1e-13, 1e-16, 1e-30, 1e-40])
+@pytest.mark.parametrize("cap,most", [(30.0, 12), (30.0, 60), (2.0, 0.75), (2.0, 5), (0.0, 60)])
+def test_small_temperatures(gpu, cap, most, t):
+    """All weight on the row's maximum, shared evenly where several logits have it, below half the cap and past it."""
+    for seed in (1, 2):
+        c = on_a_grid(verifycase.case([4, 1, 0, 7, 2], 3001, seed, spread=most / 3), most / 64, most)
+        verifycase.check(c, 7, cap, t)
+
+
+@pytest.mark.parametrize("shift", [0.0, 2000.0])
+@pytest.mark.parametrize("cap", [1e-30, 1e-3, 100.0, 1e4, 1e9, 1e16, 1e30, 3e38])
+def test_caps_of_every_size(gpu, cap, shift):
+    """A cap far above the logits changes nothing, one far below them leaves them nearly alike."""
+    c = verifycase.case([4, 1, 0, 7, 2], 9001, 3)
+    c = (*(x + np.float32(shift) for x in c[:2]), *c[2:])
+    got = verifycase.check(c, 7, cap, 0.9)
+    if cap >= 1e16:
+        plain = verifycase.check(c, 7, 0.0, 0.9)
+        assert np.array_equal(got[0], plain[0]) and np.array_equal(got[1], plain[1])

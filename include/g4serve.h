@@ -134,7 +134,8 @@ size_t g4_attention_chunk_workspace_bytes(const g4_kv_pages *pages, const g4_chu
  *   sum of weights, in token order, exceeds u_next[s] * their sum.
  * draft_logits NULL: a drafter without probabilities, q_i = 1 at t_i. temperature 0: greedy, draft i is
  * taken while it is the first maximum of row i (u, u_next and draft_logits are not read), as g4_softcap_argmax.
- * A NaN logit has no weight; a drafted id outside the vocabulary is refused; a row without any weight
+ * A logit that is NaN or -infinity (a token masked out) has no weight, under a cap too (tanh alone would leave a
+ * masked token e^(-cap / temperature)); a drafted id outside the vocabulary is refused; a row without any weight
  * gives token -1 and log probability 0.
  * Out: tokens [seqs][max_drafts + 1]: the drafts taken, the drawn token, then -1; accepted [seqs]; logprobs
  * (optional) [seqs][max_drafts + 1]: log p of each token under the target at the temperature (1 when

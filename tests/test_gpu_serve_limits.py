@@ -59,3 +59,24 @@ def test_caps_of_every_size(gpu, cap, shift):
     if cap >= 1e16:
         plain = verifycase.check(c, 7, 0.0, 0.9)
         assert np.array_equal(got[0], plain[0]) and np.array_equal(got[1], plain[1])
+
+
+@pytest.mark.parametrize("drafter", [True, False])
+@pytest.mark.parametrize("t", [0.0, 0.9])
+@pytest.mark.parametrize("cap", [0.0, 2.0, 30.0])
+def test_masked_tokens_have_no_weight(gpu, cap, t, drafter):
+    """-infinity is out of the draw whatever the cap, as NaN is; a drafted one is refused, a row of them is empty."""
+    logits, dl, drafts, start, u, un = verifycase.case([4, 1, 0, 7, 2], 3001, 4, spread=0.3)
+    logits[:, 7::2] = dl[:, 7::2] = np.nan
+    logits[5, :2000] = np.nan
+    drafts[0], drafts[5] = 8, 9  # sequence 3 drafted a token that is out
+    dl[4] = np.nan
+    logits[7] = np.nan  # sequence 2
+    with np.errstate(invalid="ignore"):
+        want = verifycase.verify(logits, dl if drafter else None, drafts, start, u, un, 7, cap, t)
+    assert t == 0 or want[3] > 2.0 ** -32
+    masked = lambda x: np.where(np.isnan(x), np.float32(-np.inf), x)
+    got = verifycase.run(masked(logits), masked(dl) if drafter else None, drafts, start, u, un, 7, cap, t)
+    assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+    assert (np.abs(got[2] - want[2]) <= np.abs(want[2]) * 2.0 ** -24 * 1.01 + 2.0 ** -36).all()
+    assert got[1][3] == 0 and got[0][2, 0] == -1

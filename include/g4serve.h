@@ -133,7 +133,9 @@ size_t g4_attention_chunk_workspace_bytes(const g4_kv_pages *pages, const g4_chu
  *   everywhere), and when all are taken one more token is drawn from p_n: the first token whose running
  *   sum of weights, in token order, exceeds u_next[s] * their sum.
  * draft_logits NULL: a drafter without probabilities, q_i = 1 at t_i. temperature 0: greedy, draft i is
- * taken while it is the first maximum of row i (u, u_next and draft_logits are not read), as g4_softcap_argmax.
+ * taken while it is the first maximum of row i (u, u_next and draft_logits are not read). That is the maximum of the
+ * logits as given, whose order the cap keeps. g4_softcap_argmax compares capped f32 values: where it finds another
+ * token, that one is earlier and its logit so near the maximum, or both so far past the cap, that they are capped alike.
  * A logit that is NaN or -infinity (a token masked out) has no weight, under a cap too (tanh alone would leave a
  * masked token e^(-cap / temperature)); a drafted id outside the vocabulary is refused; a row without any weight
  * gives token -1 and log probability 0.

@@ -80,3 +80,33 @@ def test_masked_tokens_have_no_weight(gpu, cap, t, drafter):
     assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
     assert (np.abs(got[2] - want[2]) <= np.abs(want[2]) * 2.0 ** -24 * 1.01 + 2.0 ** -36).all()
     assert got[1][3] == 0 and got[0][2, 0] == -1
+
+
+def softcap_argmax(g4, logits, cap):
+    rows, vocab = logits.shape
+    ws = g4.DeviceBuffer(g4.lib().g4_argmax_workspace_bytes(rows, vocab))
+    tok, capped = dev(np.zeros(rows, np.int32)), dev(np.zeros_like(logits))
+    g4._check(g4.lib().g4_softcap_argmax(dev(logits).ptr, rows, vocab, cap, capped.ptr, ws.ptr, ws.nbytes, tok.ptr, None))
+    return tok.download(), capped.download()
+
+
+@pytest.mark.parametrize("cap", [2.0, 30.0])
+def test_greedy_takes_the_first_maximum_of_the_logits(gpu, cap):
+    """Under a cap too, and g4_softcap_argmax's token but where capping makes an earlier logit equal to it."""
+    r = np.random.default_rng(int(cap))
+    rows, vocab = 12, 9001
+    logits = r.standard_normal((rows, vocab)).astype(np.float32)
+    at, before = r.integers(4500, vocab, rows), r.integers(0, 4500, rows)
+    n = np.arange(rows)
+    logits[n, at] = 6
+    for i in range(rows):  # one step, some steps, far past the cap, equal
+        logits[i, before[i]] = [np.nextafter(np.float32(6), np.float32(0)), 6 - 2.0 ** -6, 20 * cap, 6][i % 4]
+        logits[i, at[i]] = [6, 6, 30 * cap, 6][i % 4]
+    z = np.zeros(0, np.int32)
+    got = verifycase.run(logits, None, z, np.zeros(rows + 1, np.int32), z, z, 0, cap, 0.0)[0][:, 0]
+    assert np.array_equal(got, logits.argmax(1))
+    tokens, capped = softcap_argmax(gpu, logits, cap)
+    same = got == tokens
+    assert same[1::4].all() and same[3::4].all()
+    assert not same[2::4].any()
+    assert (capped[n, got] == capped[n, tokens])[~same].all() and (tokens < got)[~same].all()

@@ -482,9 +482,15 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
 #pragma unroll
             for (int g = 0; g < KG; ++g) top = max(top, __float_as_uint(ml[(g * RT + rt) * kRows + c].x));
             const float amax = (float)bits_h2(top)[0];
-            const float inv = top ? (R.q_sign ? -32512.0f : 32512.0f) / amax : 0.0f;
-            sc = fmaxf(R.scale2 * (amax / 32512.0f), 0x1p-126f);
-            if (top >= 0x7c00u) sc = __builtin_nanf("");  // a NaN or an infinity in Q
+            // With a NaN or an infinity in Q the digits are zeros and the scale is infinite: a score of a key that
+            // the row sees is NaN, a masked one still minus infinity.
+            const bool odd = top >= 0x7c00u;
+            const float inv = top && !odd ? (R.q_sign ? -32512.0f : 32512.0f) / amax : 0.0f;
+            sc = odd ? INFINITY : fmaxf(R.scale2 * (amax / 32512.0f), 0x1p-126f);
+#pragma unroll
+            for (int s = 0; s < 2 * QN; ++s)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) x[s][n] = odd ? 0 : x[s][n];
             auto stage = [&](int at) {  // of the row tile's KS operands
                 const int e = rt * KS + at;
                 return lds + ring(NS - 1, 1) + (e / (KS / 2) - kg) * (NS * 2 * P::HALF) + e % (KS / 2) * 1024 + lane * 16;

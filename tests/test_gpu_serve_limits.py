@@ -110,3 +110,39 @@ def test_greedy_takes_the_first_maximum_of_the_logits(gpu, cap):
     assert same[1::4].all() and same[3::4].all()
     assert not same[2::4].any()
     assert (capped[n, got] == capped[n, tokens])[~same].all() and (tokens < got)[~same].all()
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("kind", ["i8", "f16"])
+@pytest.mark.parametrize("lens,absent,window", [
+    ([(4, 40), (3, 1), (2, 33)], [(0, 0), (0, 1), (0, 2), (2, 1)], 0),  # none left; two rows without a position; some left
+    ([(70, 100), (5, 300)], [(0, 5), (0, 6), (1, 18)], 5),  # rows of a tile whose window's pages are gone
+], ids=["tokens", "chunk"])
+def test_queries_that_are_not_finite(gpu, lens, absent, window, kind, bad):
+    """A row whose query has a NaN or an infinity is not finite where it sees a key, and zeros where it sees none; the
+    rows beside it are as without it."""
+    b = Batch(lens, 1, 128, 16, kind, seed=len(lens), absent=absent).upload()
+    q = queries(b, 4)
+    want, bound = attention(b, q, float(np.float32(0.1)), window)
+    odd = q.copy()
+    odd[::2, 1::2, 5] = bad
+    odd[::2, 3, 6] = -bad
+    got = run(b, odd, window)
+    hit = np.zeros((b.tokens, 4), bool)
+    hit[::2, 1::2] = True
+    seen, none_finite = np.zeros(b.tokens, bool), np.zeros((b.tokens, 4), bool)
+    for s, (m, kv) in enumerate(lens):
+        k, there = b.held(b.k, b.ks, s)
+        for i in range(m):
+            t, pos = b.start[s] + i, kv - m + i
+            j = np.arange(kv)
+            see = there & (j <= pos) & (j > (pos - window if window else -1))
+            seen[t] = see.any()
+            with np.errstate(invalid="ignore"):
+                score = odd[t].astype(np.float64) @ k[see, 0].T
+            # int8 keys: any; f16: a score that is NaN or +infinity (one of -infinity has no weight)
+            none_finite[t] = hit[t] & seen[t] if kind == "i8" else (np.isnan(score) | (score == np.inf)).any(1)
+    assert 0 < seen.sum() < b.tokens and none_finite.any()
+    assert (got[~seen] == 0).all()
+    assert not np.isfinite(got[none_finite]).any()
+    assert (np.abs(got - want) <= to_kind(want, bound, np.float32))[~hit].all()

@@ -146,3 +146,26 @@ def test_queries_that_are_not_finite(gpu, lens, absent, window, kind, bad):
     assert (got[~seen] == 0).all()
     assert not np.isfinite(got[none_finite]).any()
     assert (np.abs(got - want) <= to_kind(want, bound, np.float32))[~hit].all()
+
+
+@pytest.mark.parametrize("dim,heads,kv", [(64, 8, 300001), (256, 2, 150001)])
+def test_long_sums_of_int8_rows(gpu, dim, heads, kv):
+    """Equal weights and V scales of 1 to 1/8: sums of codes times powers of two, which f32 holds exactly as long as no
+    partial sum passes 2^24 eighths. So a row is off by the last division and product alone, however many keys it has
+    (enough rows that the keys of one are not split over blocks)."""
+    m, page = 16384 // heads, 4096
+    r = np.random.default_rng(dim)
+    pages = -(-kv // page)
+    k, v = (r.integers(-127, 128, (pages, page, 1, dim)).astype(np.int8) for _ in range(2))
+    vs = (2.0 ** -r.integers(0, 4, (pages, 1, page))).astype(np.float32)
+    ks = np.full((pages, 1, page), 0.01, np.float32)
+    p = gs.KVPages(dev(k), dev(v), dev(ks), dev(vs))
+    c = gs.Chunk(dev(np.array([0, m], np.int32)), dev(np.array([kv], np.int32)), dev(np.arange(pages, dtype=np.int32)[None]), m, m, kv)
+    q = r.standard_normal((m, heads, dim)).astype(np.float16)
+    o = dev(np.zeros(q.shape, np.float32))
+    ws = gpu.DeviceBuffer(gs.attention_chunk_workspace_bytes(p, c, heads))
+    gs.attention_chunk(p, c, dev(q), o, ws, scale=0.0)
+    sums = np.cumsum((v.astype(np.float64) * vs.transpose(0, 2, 1)[..., None]).reshape(-1, dim)[:kv], 0)[kv - m:]
+    assert np.abs(sums).max() * 8 < 2 ** 24
+    want = (sums / np.arange(kv - m + 1, kv + 1)[:, None])[:, None]
+    assert (np.abs(o.download() - want) <= 4 * 2.0 ** -24 * np.abs(want)).all()

@@ -17,9 +17,12 @@
 // int8 rows: the scores are integer products of K's codes with Q as 16-bit fixed point of the row's largest
 // magnitude, in two 8-bit digits (v_mfma_i32_32x32x32_i8 twice: the matrix time of one f16 product, K read
 // once and not converted, which took 96 vector operations a tile). An element of Q is off by 2^-16 of the
-// row's largest at most, K's codes not at all. K's scale multiplies the score, V's the weight, taken relative
-// to a power of two above the largest scale that the row has seen, which scales the row's output and sum (f16
-// would not hold scales of every size) and enters the weights by their exponent. V's codes are f16 subnormals.
+// row's largest at most, K's codes not at all. K's scale multiplies the score, V's the weight. f16 would
+// not hold scales of every size: weights are taken relative to a power of two at or up to 4 times the row's largest
+// weight times scale, which scales the row's output and sum and enters the weights by their exponent. It moves only
+// where the maximum does or a scale is 2^6 times as large, so a weight reaches 2^14 at most. (A power above the
+// largest scale alone would lose a key of small scale beside one of large scale that weighs nothing.) V's codes are
+// f16 subnormals.
 //
 // What bounds it. Many rows: of a key tile's 32 products of 32 cycles a wave and its 330 other vector
 // operations of 4, a SIMD's two waves overlap most, but the two streams share the issue; 2048 tokens on 8192
@@ -88,10 +91,11 @@ __device__ __forceinline__ float other_half_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// The next power of two above a scale (2^99 and more: 2^100), and a power of two's exponent.
+// The next power of two above a scale (2^99 and more: 2^100), the same from 2^-100 on, and a power of two's exponent.
 __device__ __forceinline__ float pow2_above(float v) {
     return __uint_as_float((__float_as_uint(fminf(v, 0x1p99f)) & 0x7f800000u) + 0x00800000u);
 }
+__device__ __forceinline__ float v_unit(float v) { return pow2_above(fmaxf(v, 0x1p-101f)); }
 __device__ __forceinline__ float pow2_log(float v) { return (float)((int)(__float_as_uint(v) >> 23) - 127); }
 
 // The maximum over lanes 0..31, with lanes 32..63 holding the same values.
@@ -252,7 +256,8 @@ struct Shape {
     static constexpr int QL = D == 256 && (CK == G4_KIND_I8 || RT == 4) ? 3 : 0;
     static constexpr bool TIGHT = D == 256 && CK == G4_KIND_F16 && RT == 4;  // no registers for V's reads ahead
     static constexpr int LDS = (RING > JOIN ? RING : JOIN) + SCALES + WAVES * (kRows * 8 + QL * 1024);
-    static constexpr int MIN_WAVES = WAVES == 4 && LDS > 80 * 1024 ? 1 : 2;  // per SIMD: one block a CU, or two
+    // per SIMD: one block a CU, or two; int8 of 64 is a register over what four blocks may have
+    static constexpr int MIN_WAVES = WAVES == 4 && LDS > 80 * 1024 ? 1 : (D == 64 && CK == G4_KIND_I8 ? 4 : 2);
 };
 
 // Byte of chunk x (16 bytes) of K row c of a tile: the chunk index is XORed so that a b128 read of one
@@ -538,11 +543,12 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
     f16x o[DPL];
 #pragma unroll
     for (int j = 0; j < DPL; ++j) o[j] = f16x{};
-    // vref: the power of two of the row's V scales; w_sum: the sum of the rounded weights (int8)
-    // off: the exponents' offset, -m scale2 - log2(vref); l is in units of vref too
-    // v_low: the least vref of the wave's rows (a lane without a row keeps out of it)
-    float m = -INFINITY, l = 0.0f, w_sum = 0.0f, off = I8 ? 100.0f : 0.0f;
-    float vref = real ? 0x1p-100f : 0x1p100f, v_low = 0x1p-100f;
+    // int8: v_need: the largest weight times V's scale that the row has seen, up to a factor of 2, as of its last
+    // rescaling; v_unit(v_need) is what the weights, off (the exponents' offset, -m scale2 - log2 of it) and l are
+    // relative to. v_low: V scales up to it need no rescaling. w_sum: the sum of the rounded weights.
+    float m = -INFINITY, l = 0.0f, w_sum = 0.0f, off = I8 ? -100.0f : 0.0f;
+    float v_low = 0x1p106f;
+    if (I8) ml[wave * kRows + c].y = 0x1p99f;  // v_need: rarely used, and the registers are full
 
     const int lane_ = lane;
     constexpr int KC = NK < 4 ? NK : 4, AHEAD = D == 256 && I8 && RT == 1 ? 1 : 2;
@@ -707,36 +713,42 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
 #pragma unroll
             for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
             top = other_half_max(top);
-            // V's scales, lane c key c's: those above the least vref of the wave lead to the closer look below
-            uint32_t v_scales = sc_slot * 256 + 32 + 16 * h;
-            float v_mine = 0.0f;
+            const uint32_t v_scales = sc_slot * 256 + 32 + 16 * h;
+            float v_mine = 0.0f;  // of V's scales, lane c key c's
             if (I8) v_mine = fabsf(*reinterpret_cast<const float *>(scales + sc_slot * 256 + (c >> 3) * 64 + 32 + c % 8 * 4));
-            float vto = vref;
-            if (I8 && __any(v_mine > v_low)) {
-                float vtop = 0.0f;  // the largest scale that the row sees
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f4 y = *reinterpret_cast<const f4 *>(scales + v_scales + 64 * g);
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) vtop = fmaxf(vtop, seen >> (8 * g + n) & 1 ? fabsf(y[n]) : 0.0f);
-                }
-                vtop = other_half_max(vtop);
-                if (vtop > vref) vto = pow2_above(vtop);
-                v_low = -half_max(-vto);
-            }
-            if (__any((top - m) * sc > kLazy || (I8 && vto > vref))) {
+            if (__any((top - m) * sc > kLazy || (I8 && v_mine > v_low))) {
                 const float mn = fmaxf(m, top);
-                float f = mn == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * sc);
+                off = mn == -INFINITY ? 0.0f : -mn * sc;
+                float f;
                 if (I8) {
-                    f *= vref / vto;
+                    float need = 0.0f;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const f4 y = *reinterpret_cast<const f4 *>(scales + v_scales + 64 * g);
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            // a masked key's exponent is -1000: nothing, whatever its scale is
+                            const float e = __builtin_amdgcn_fmed3f(__builtin_fmaf(x[4 * g + n], sc, off), -1000.0f, 0.0f);
+                            need = fmaxf(need, __builtin_amdgcn_ldexpf(fminf(fabsf(y[n]), 0x1p100f), (int)e));
+                        }
+                    }
+                    f = m == mn ? 0.0f : (m - mn) * sc;
+                    float *const v_need = &ml[wave * kRows + c].y;
+                    const float had = *v_need, unit = pow2_log(v_unit(had));
+                    need = fmaxf(other_half_max(need), had * __builtin_amdgcn_exp2f(f));
+                    *v_need = need;
+                    const float vref = v_unit(need), log = pow2_log(vref);
+                    f = __builtin_amdgcn_exp2f(f + (unit - log));
                     w_sum *= f;
-                    vref = vto;
+                    off -= log;
+                    v_low = -half_max(-vref) * 64.0f;
+                } else {
+                    f = m == mn ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * sc);
                 }
                 l *= f;
 #pragma unroll
                 for (int j = 0; j < DPL; ++j) o[j] *= f;
                 m = mn;
-                off = (m == -INFINITY ? 0.0f : -m * sc) - (I8 ? pow2_log(vref) : 0.0f);
             }
             if (I8 && __builtin_expect(i % kBiasTiles == kBiasTiles - 1, 0)) {  // the bias comes off
                 const float b = other_half_sum(w_sum) * 0x1p-17f;  // 128 2^-24 of the weights' sum
@@ -861,6 +873,7 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
     else run(std::integral_constant<bool, false>{});
     if (RT > 1 && P::WAVES > 4 && wave < 4 && rounds) barrier();
     l = other_half_sum(l);
+    const float vref = I8 ? v_unit(ml[wave * kRows + c].y) : 1.0f;
     if (I8) {
         w_sum = other_half_sum(w_sum);
         l *= vref;

@@ -111,9 +111,10 @@ int g4_kv_read(const g4_kv_pages *pages, const g4_chunk *chunk, void *k_out, voi
  * f16 rows: products of f16 values, added up in f32; a weight is rounded to f16 (relative to a maximum
  * within 2^8 of the row's), and the softmax's sum adds the rounded ones. int8 rows: q enters the scores as
  * 16-bit fixed point of the row's largest magnitude (off by 2^-16 of that at most) and the codes exactly;
- * a weight is rounded to f16 with V's scale in it (scales up to 2^99 in magnitude). A masked position's
- * contents, NaN included, change nothing. Of what a row sees: a NaN or an infinity in V, and a score that is NaN or
- * +infinity, make its outputs non-finite; a score of -infinity has no weight.
+ * a weight is rounded to f16 with V's scale in it (scales up to 2^99 in magnitude, K's to 2^96), relative to a power of
+ * two of at most 4 times the row's largest such product. A masked position's contents, NaN included, change nothing.
+ * Of what a row sees: a NaN or an infinity in V, and a score that is NaN or +infinity, make its outputs non-finite; a
+ * score of -infinity has no weight. A NaN or an infinity in q makes an int8 row's outputs non-finite where it sees a key.
  * page_stride and page_size * slot_stride below 2^31 elements; |scale| below 2^127.
  * workspace: g4_attention_chunk_workspace_bytes(...) bytes, 16-byte aligned.
  */

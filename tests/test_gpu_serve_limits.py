@@ -169,3 +169,88 @@ def test_long_sums_of_int8_rows(gpu, dim, heads, kv):
     assert np.abs(sums).max() * 8 < 2 ** 24
     want = (sums / np.arange(kv - m + 1, kv + 1)[:, None])[:, None]
     assert (np.abs(o.download() - want) <= 4 * 2.0 ** -24 * np.abs(want)).all()
+
+
+def scaled_attention(b, q, scale, window, rows=slice(None)):
+    """attention() of servecases with a bound for V scales of very different sizes, over what a row sees alone. A weight
+    is rounded to f16 with V's scale in it, relative to a power of two of at most 4 times the largest product of the
+    two that the row sees: by 2^-11 of itself, or below 2^-14 of that power by up to 2^-25 of it; times a code of at most 127."""
+    want, bound = np.zeros(q.shape), np.zeros(q.shape)
+    for s, (m, kv) in enumerate(b.lens):
+        k, there = b.held(b.k, b.ks, s)
+        v, _ = b.held(b.v, b.vs, s)
+        j = np.arange(kv)
+        page = np.where(there, b.table[s, j // b.page], 0)
+        for i in range(m):
+            pos, t = kv - m + i, b.start[s] + i
+            see = there & (j <= pos) & (j > (pos - window if window else -1))
+            if not see.any():
+                continue
+            for h in range(q.shape[1]):
+                g = h // (q.shape[1] // b.kv_heads)
+                kk, vv, qq = k[see, g], v[see, g], q[t, h].astype(np.float64)
+                vs = np.abs(b.vs[page[see], g, j[see] % b.page].astype(np.float64))
+                sc = kk @ qq * scale
+                p = np.exp(sc - sc.max())
+                p /= p.sum()
+                n = see.sum()
+                ds = ((np.abs(kk) @ np.abs(qq)).max() * abs(scale) * (b.dim + 4) + 16) * 2.0 ** -24 + \
+                    np.abs(qq).max() / 65024 * np.abs(kk).sum(1).max() * abs(scale)
+                want[t, h] = p @ vv
+                bound[t, h] = p @ np.abs(vv) * (4 * ds + 2.0 ** -11 + 2 * (n + 8) * 2.0 ** -24) + \
+                    n * 2.0 ** -25 * 4 * 127 * (p * vs).max()
+    return want, bound
+
+
+def scales_of_all_sizes(b, seed):
+    r = np.random.default_rng(seed)
+    b.vs *= np.float32(10) ** r.integers(-14, 10, b.vs.shape).astype(np.float32)
+    b.vs[r.random(b.vs.shape) < 0.1] = 0
+    return b
+
+
+@pytest.mark.parametrize("lens,heads,kv_heads,dim,window,max_kv", [
+    ([(3, 150), (1, 400), (2, 33)], 4, 1, 128, 0, None),
+    ([(70, 150)], 4, 1, 256, 0, None),
+    ([(70, 150), (5, 90)], 4, 1, 64, 40, None),
+    ([(70, 150)], 128, 128, 256, 0, 4100),  # blocks of two row tiles
+])
+def test_int8_scales_of_all_sizes(gpu, lens, heads, kv_heads, dim, window, max_kv):
+    """Each row to its own precision: scales that it does not see change nothing, and those of keys that weigh nothing
+    do not take it from the ones that do. Scores over +-20 make most keys weigh nothing."""
+    for seed in (1, 2, 3):
+        b = scales_of_all_sizes(Batch(lens, kv_heads, dim, 16, "i8", seed=seed, max_kv=max_kv), seed)
+        # the last positions' scales are out of the range of f16 a million times: only the last rows see them
+        for s, (m, kv) in enumerate(lens):
+            for p in range(kv - min(m, 3) + 1, kv):
+                b.vs[b.table[s, p // 16], :, p % 16] = 1e25
+        b.upload()
+        q = queries(b, heads)
+        want, bound = scaled_attention(b, q, float(np.float32(0.6)), window)
+        got = run(b, q, window, 0.6)
+        assert (np.abs(got - want) <= to_kind(want, bound, np.float32)).all()
+
+
+@pytest.mark.parametrize("first,big,later", [(100, 101, None), (100, 20, None), (20, 100, None), (90, 10, 170)])
+def test_a_large_scale_that_weighs_nothing(gpu, first, big, later):
+    """The key that takes all the weight has a V scale of about 1e-5, a key of weight e^-32 one of 1e5, in its key tile,
+    before it or behind it; or the large one led until a later key outweighs it."""
+    b = Batch([(2, 200)], 1, 64, 16, "i8", seed=9)
+    k = np.zeros((200, 64), np.float32)
+    k[:, 0], k[:, 1] = -2, 4
+    k[first, 0] = 2
+    if later is not None:
+        k[big, 0], k[later, 0] = 0, 4
+    for p in range(200):
+        page, slot = b.table[0, p // 16], p % 16
+        amax = np.abs(k[p]).max()
+        b.k[page, slot, 0] = np.rint(127 * k[p] / amax)
+        b.ks[page, 0, slot] = amax / 127
+        b.vs[page, 0, slot] = 1e5 if p == big else 1e-5
+    b.upload()
+    q = np.zeros((2, 1, 64), np.float16)
+    q[..., 0] = 8
+    want, bound = scaled_attention(b, q, 1.0, 0)
+    got = run(b, q, 0, 1.0)
+    assert (np.abs(got - want) <= to_kind(want, bound, np.float32)).all()
+    assert np.abs(want).max() > 20 * bound.max()

@@ -92,7 +92,7 @@ int g4_paged_prologue(const g4_kv_pages *pages, const g4_chunk *chunk, int x_kin
 /*
  * The chunk's rows read back from the cache: row i of sequence s to
  * out + (seq_stride ? s * seq_stride + i * kv_heads * head_dim
- *                   : (q_start[s] + i) * kv_heads * head_dim), f32 or f16 (rounded once). With
+ *                   : (q_start[s] + i) * kv_heads * head_dim), f32 (code * scale rounded once) or that as f16. With
  * q_start counting every position of a sequence (its rows = kv_len[s]) the whole sequence is read,
  * for example into a contiguous f32 cache (g4_decode_kv). Rows on absent pages are zeros. k_out or
  * v_out may be NULL; both 16-byte aligned, seq_stride a multiple of 16 bytes. At most 2^28 - 16 rows.

@@ -103,7 +103,8 @@ __device__ __forceinline__ int quant_code(float y, float amax, float r) {
 }
 
 // Bound by each wave's way, q_start -> kv_len and page -> row (2048 tokens, 10 rows of 256 each, codes in: 13.4 us,
-// 16 MB; one token 4 us): a wave per row has all of them on their way at once.
+// 16 MB; one token 4 us): a wave per row has all of them on their way at once, but looks its sequence and page up by
+// itself.
 // One wave per head row: lane l holds elements E l .. E l + E - 1 (E = D / 64), so the RoPE pair
 // (i, i + D / 2) is lanes l and l + 32 of the same register. Row 0 .. heads - 1 of a token are its
 // queries, then kv_heads of K, then of V.
@@ -188,8 +189,9 @@ __global__ __launch_bounds__(256) void paged_prologue_kernel(PagedArgs A, Prolog
 
 // ---- the read-back ------------------------------------------------------------------------------------
 
-// Bound by HBM: 67000 tokens of 4 heads of 128, codes to f16, 209 MB in 32.2 us; 45 with K and V in blocks of their
-// own and a search per row. Batches of 2 and blocks of 8 or 32 tokens: 33.6-34.2.
+// Bound by HBM: 67000 tokens of 4 heads of 128, codes to f16, 209 MB, on other pages in each call 46.5 us (4.5 TB/s);
+// 65 with K and V in blocks of their own and a search per row; batches of 2 and 8 47.6 and 45.6, blocks of 8 and 32
+// tokens 45.7 and 46.7. On the same pages call after call, of which the 256 MB cache holds part: 32.7; 34.0, 33.3, 33.1, 34.2.
 // A block takes kReadTokens rows: a wave looks them up at once (the first one's sequence by ballots over the
 // ends, the others' from there on), then threads move units of 8 elements, K's and V's of kReadBatch at a time.
 constexpr int kReadTokens = 16, kReadBatch = 4;

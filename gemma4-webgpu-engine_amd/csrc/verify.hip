@@ -9,9 +9,10 @@
 // A drawn token is the one of up to 262144 whose running sum passes a given point: sums that are 1e-7 off
 // would often name its neighbour. So exponents and sums are held in 64 bits and 2^f is good to 1e-12.
 //
-// What bounds it: (1) the 64-bit operations, about 44 a logit with the softcap (264 rows of 262144: 97 us for a
-// read of 54; 160 rows 61; without the softcap 9 rows take 7); (3) reading the drawn rows again (32 sequences, 26 us,
-// two rows each); (2) and (4) a chain of loads, 4-7 and 8-12 us. Parts of 8192 give 4 waves 32 logits a thread,
+// What bounds it: (1) issue, about 55 vector operations a logit with the softcap, 29 of them 64-bit, and 37 and 18
+// without (264 rows of 262144, with: 98 us, what 55 take at 16 lanes a cycle and SIMD, for a read of 43; 160 rows 60;
+// without, 9 rows 7, latency); (3) reading the drawn rows again (32 sequences, 26 us,
+// two rows each); (2) and (4) a chain of loads, 4-8 and 8-13 us. Parts of 8192 give 4 waves 32 logits a thread,
 // loaded at once; units of 1024 keep the last step one block's work and its code short (2048: 2.4 us more).
 #include "g4_internal.h"
 #include "../../include/g4serve.h"
@@ -60,7 +61,7 @@ struct VerifyArgs {
 // as x grows: below half the cap the values of neighbouring f32 logits are 2^-25 of them apart and 2^-44 off.)
 //
 // The weight of the bulk of a row, 2^z: z = n + f, |f| <= 1/2, a polynomial in f (fitted likewise, relative error
-// 1.1e-12) and n into the exponent: 14 operations of the 64-bit unit a logit, about what its 4 bytes cost to read.
+// 1.1e-12) and n into the exponent: 16 64-bit operations a logit.
 struct RowScale {
     double top, slope;  // 2^((y - top) slope)
 };

@@ -12,6 +12,7 @@ tensor, since what makes and reads tensors runs there, else the default stream.
 from __future__ import annotations
 
 import ctypes
+import os
 import sys
 
 import g4w8a8 as g4
@@ -49,17 +50,16 @@ def _check_runtime():
     are the other's."""
     global _one_runtime
     if _one_runtime is None:
-        g4.lib()
-        _one_runtime = len(_mapped("libamdhip64")) == 1
+        torch_lib = os.path.join(os.path.dirname(sys.modules["torch"].__file__), "lib", "libc10_hip.so")
+        try:  # what each of the two calls
+            ours, torchs = (ctypes.cast(x.hipGetDevice, _vp).value for x in (g4.lib(), ctypes.CDLL(torch_lib)))
+            _one_runtime = ours == torchs
+        except OSError:  # a torch of another layout: as many runtimes as files
+            with open("/proc/self/maps") as f:
+                _one_runtime = len({line.split()[-1] for line in f if "libamdhip64" in line}) == 1
     if not _one_runtime:
         raise g4.G4Error(1, "a torch tensor of another HIP runtime than this library's: import torch before the "
                             "first call into the library")
-
-
-def _mapped(name):
-    """The files of this name that the process has mapped."""
-    with open("/proc/self/maps") as f:
-        return {line.split()[-1] for line in f if name in line}
 
 
 def _address(x, what, device):

@@ -8,8 +8,8 @@
 // they stand. The order of the k index of a product is free as long as both operands agree on it; the
 // layouts below use that twice:
 //  - P: lane half h holds, for k-step t of 16 keys, keys 16 t + 4 h + 0..3 and 16 t + 8 + 4 h + 0..3;
-//  - V: a lane reads UD consecutive dims of each of these eight keys and byte-permutes them into UD operands
-//    of eight keys each. No LDS transposes anything.
+//  - V: a lane reads UD consecutive dims of each of these eight keys and permutes (f16) or converts (int8) them
+//    into UD operands of eight keys each. No LDS transposes anything.
 // The softmax keeps a running maximum (base 2) and sum in f32; the maximum moves, and the output is
 // rescaled, only when a score passes it by more than 2^8, so weights reach 2^8 at most and are rounded to
 // f16 (11 bits; an f16 cache's sum adds the rounded ones, an int8 cache's the exact ones, whose weights
@@ -21,8 +21,7 @@
 // not hold scales of every size: weights are taken relative to a power of two at or up to 4 times the row's largest
 // weight times scale, which scales the row's output and sum and enters the weights by their exponent. It moves only
 // where the maximum does or a scale is 2^6 times as large, so a weight reaches 2^14 at most. (A power above the
-// largest scale alone would lose a key of small scale beside one of large scale that weighs nothing.) V's codes are
-// f16 subnormals.
+// largest scale alone would lose a key of small scale beside one of large scale that weighs nothing.)
 //
 // What bounds it. Many rows: a key tile is 32 products of 32 cycles a wave and 330 other vector operations of 4, and a
 // SIMD has two waves to overlap them. 2048 tokens on 8192 keys, 8 heads of 256, int8: 159 us, 756 TFLOP/s, 0.63 of
@@ -81,7 +80,6 @@ struct AttnArgs {
 
 constexpr int kRows = 32, kKeys = 32;
 constexpr float kLazy = 8.0f;
-constexpr int kBiasTiles = 64;  // see code_pair
 
 __device__ __forceinline__ float other_half_max(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -116,16 +114,24 @@ __device__ __forceinline__ h8 words_h8(uint32_t a, uint32_t b, uint32_t c, uint3
     return __builtin_bit_cast(h8, w);
 }
 
-// A V code as f16 without arithmetic: the byte code + 128 zero-extended is the subnormal (code + 128) 2^-24,
-// exact, and the matrix products keep subnormals. The 128s come off the output by the sum of the rounded weights,
-// every kBiasTiles key tiles and at the end: sums of biased codes grow with the keys where those of the codes do not
-// (weights that are alike), and f32 would lose the difference. (Taken off at the end only, 131072 keys in one run
-// were 6e-4 off and 524288 4e-3; now 2e-4, the rounding of the weights. 2048 tokens on 4096 keys of
-// 128, 32 heads on 8, 213 us for 210; head_dim 256 as before.)
-// Element j of words a and b as a pair; the codes' signs are flipped already.
+// Byte J of each of eight words of V codes, as the f16 operand: converted byte by byte, into the low half of a word
+// and then into the high one. (A partial write is read a wait state later at the earliest.) Codes + 128 put together by
+// byte permutes as f16 subnormals, the 128s taken off the output by the sum of the weights, are 2 operations a pair
+// fewer; but beside a weight near 1 the f32 sums of such products lose what small weights add (an output of 3e-5 in a
+// row of 2 was 17% off), and long runs of alike weights lost more (6e-4 over 131072 keys). 2048 tokens on 8192 keys 161 us for 157,
+// 8192 on their own 398 for 379, 32 single tokens as before.
 template <int J>
-__device__ __forceinline__ uint32_t code_pair(uint32_t a, uint32_t b) {
-    return __builtin_amdgcn_perm(b, a, 0x0c000c00u | ((4 + J) << 16) | J);
+__device__ __forceinline__ h8 code_operand(const uint32_t (&v)[8][1]) {
+    u32x4 r;
+#define G4_CVT(to, from, half, keep) \
+    "v_cvt_f16_i16_sdwa " to ", sext(" from ") dst_sel:WORD_" half " dst_unused:UNUSED_" keep " src0_sel:BYTE_%12\n\t"
+    asm(G4_CVT("%0", "%4", "0", "PAD") G4_CVT("%1", "%6", "0", "PAD") G4_CVT("%2", "%8", "0", "PAD") G4_CVT("%3", "%10", "0", "PAD")
+        G4_CVT("%0", "%5", "1", "PRESERVE") G4_CVT("%1", "%7", "1", "PRESERVE") G4_CVT("%2", "%9", "1", "PRESERVE")
+        G4_CVT("%3", "%11", "1", "PRESERVE") "s_nop 0"
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+        : "v"(v[0][0]), "v"(v[1][0]), "v"(v[2][0]), "v"(v[3][0]), "v"(v[4][0]), "v"(v[5][0]), "v"(v[6][0]), "v"(v[7][0]), "n"(J));
+#undef G4_CVT
+    return __builtin_bit_cast(h8, r);
 }
 template <int J, int N>
 __device__ __forceinline__ uint32_t half_pair(const uint32_t (&a)[N], const uint32_t (&b)[N]) {
@@ -546,8 +552,8 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
     for (int j = 0; j < DPL; ++j) o[j] = f16x{};
     // int8: v_need: the largest weight times V's scale that the row has seen, up to a factor of 2, as of its last
     // rescaling; v_unit(v_need) is what the weights, off (the exponents' offset, -m scale2 - log2 of it) and l are
-    // relative to. v_low: V scales up to it need no rescaling. w_sum: the sum of the rounded weights.
-    float m = -INFINITY, l = 0.0f, w_sum = 0.0f, off = I8 ? -100.0f : 0.0f;
+    // relative to. v_low: V scales up to it need no rescaling.
+    float m = -INFINITY, l = 0.0f, off = I8 ? -100.0f : 0.0f;
     float v_low = 0x1p106f;
     if (I8) ml[wave * kRows + c].y = 0x1p99f;  // v_need: rarely used, and the registers are full
 
@@ -723,9 +729,11 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
                 float f;
                 if (I8) {
                     float need = 0.0f;
+                    uint32_t at = v_scales;
+                    asm volatile("" : "+v"(at));  // loads of its own: those below would be kept from here on
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
-                        const f4 y = *reinterpret_cast<const f4 *>(scales + v_scales + 64 * g);
+                        const f4 y = *reinterpret_cast<const f4 *>(scales + at + 64 * g);
 #pragma unroll
                         for (int n = 0; n < 4; ++n) {
                             // a masked key's exponent is -1000: nothing, whatever its scale is
@@ -740,7 +748,6 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
                     *v_need = need;
                     const float vref = v_unit(need), log = pow2_log(vref);
                     f = __builtin_amdgcn_exp2f(f + (unit - log));
-                    w_sum *= f;
                     off -= log;
                     v_low = -half_max(-vref) * 64.0f;
                 } else {
@@ -750,12 +757,6 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
 #pragma unroll
                 for (int j = 0; j < DPL; ++j) o[j] *= f;
                 m = mn;
-            }
-            if (I8 && __builtin_expect(i % kBiasTiles == kBiasTiles - 1, 0)) {  // the bias comes off
-                const float b = other_half_sum(w_sum) * 0x1p-17f;  // 128 2^-24 of the weights' sum
-#pragma unroll
-                for (int j = 0; j < DPL; ++j) o[j] -= b;
-                w_sum = 0.0f;
             }
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -778,12 +779,15 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
                     p[k / 4] = __builtin_bit_cast(h8, w);
                 }
             }
-            // the sum of the rounded weights: the row's sum (f16), or what takes the codes' bias off (int8)
-            const h2 one = {(_Float16)1.0f, (_Float16)1.0f};
-            float &sum = I8 ? w_sum : l;
+            if (!I8) {  // the sum of the rounded weights
+                const h2 one = {(_Float16)1.0f, (_Float16)1.0f};
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
-                sum = __builtin_amdgcn_fdot2(h2{p[r / 4][2 * (r % 4)], p[r / 4][2 * (r % 4) + 1]}, one, sum, false);
+                for (int r = 0; r < 8; ++r)
+                    l = __builtin_amdgcn_fdot2(h2{p[r / 4][2 * (r % 4)], p[r / 4][2 * (r % 4) + 1]}, one, l, false);
+            }
+            if (I8)  // made here: the registers are full below
+#pragma unroll
+                for (int k = 0; k < 2; ++k) asm volatile("" : "+v"(p[k]));
             wait_v();
             softmax_done();
             bool odd = false;
@@ -804,8 +808,7 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
             auto v_operand = [&](auto W, const uint32_t (&v)[8][(VB + 3) / 4]) {
                 constexpr int w = decltype(W)::value;
                 if constexpr (I8)
-                    return words_h8(code_pair<w>(v[0][0], v[1][0]), code_pair<w>(v[2][0], v[3][0]),
-                                    code_pair<w>(v[4][0], v[5][0]), code_pair<w>(v[6][0], v[7][0]));
+                    return code_operand<w>(v);
                 else
                     return words_h8(half_pair<w>(v[0], v[1]), half_pair<w>(v[2], v[3]), half_pair<w>(v[4], v[5]),
                                     half_pair<w>(v[6], v[7]));
@@ -837,9 +840,6 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
                 constexpr int next = P::TIGHT ? step : step + 1;
                 if (next < 2 * U) v_words(next / U, next % U, v[next]);
                 __builtin_amdgcn_sched_barrier(0);
-                if (I8)
-#pragma unroll
-                    for (int n = 0; n < 8; ++n) v[step][n][0] ^= 0x80808080u;
                 if (odd)
 #pragma unroll
                     for (int n = 0; n < 8; ++n)
@@ -875,10 +875,7 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
     if (RT > 1 && P::WAVES > 4 && wave < 4 && rounds) barrier();
     l = other_half_sum(l);
     const float vref = I8 ? v_unit(ml[wave * kRows + c].y) : 1.0f;
-    if (I8) {
-        w_sum = other_half_sum(w_sum);
-        l *= vref;
-    }
+    if (I8) l *= vref;
     m *= sc;  // from here on in exponents
 
     // The key groups' parts of a row, relative to their common maximum, summed in LDS PH quarters of the
@@ -892,9 +889,8 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
 #pragma unroll
         for (int g = 0; g < KG; ++g) top = fmaxf(top, ml[(g * RT + rt) * kRows + c].x);
         f = __builtin_amdgcn_exp2f(m - (top == -INFINITY ? 0.0f : top));
-        if (I8) f *= vref * 0x1p24f;
+        if (I8) f *= vref;
     }
-    const float bias = I8 ? -(w_sum * 0x1p-17f) * f : 0.0f;
     constexpr int PH = P::PH;
     // chunk e of half h of row c in block u and quarter ph; the XOR spreads a row's chunks over the banks
     auto chunk = [&](int wave, int ph, int u, int e, int h, int c) {
@@ -945,7 +941,7 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
                     f4 y;
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        y[k] = __builtin_fmaf(o[u * UD + (4 * e + k) % UD][4 * (ph0 + ph) + (4 * e + k) / UD], f, bias);
+                        y[k] = o[u * UD + (4 * e + k) % UD][4 * (ph0 + ph) + (4 * e + k) / UD] * f;
                     *reinterpret_cast<f4 *>(chunk(wave, ph, u, e, h, c)) = y;
                 }
         __syncthreads();

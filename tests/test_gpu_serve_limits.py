@@ -254,3 +254,16 @@ def test_a_large_scale_that_weighs_nothing(gpu, first, big, later):
     got = run(b, q, 0, 1.0)
     assert (np.abs(got - want) <= to_kind(want, bound, np.float32)).all()
     assert np.abs(want).max() > 20 * bound.max()
+
+
+@pytest.mark.parametrize("kind", ["i8", "f16"])
+@pytest.mark.parametrize("lens,window,dim", [([(115, 33), (31, 36), (1, 90)], 33, 128), ([(70, 200)], 0, 256), ([(5, 40), (33, 60)], 0, 64)])
+def test_small_outputs_beside_a_large_weight(gpu, lens, window, dim, kind):
+    """Sharp rows: where the key that takes nearly all the weight has a small element of V, that element of the output is
+    made by keys of weight 1e-4 and less, and is right to its own size."""
+    for seed in (1, 2):
+        b = Batch(lens, 3, dim, 64, kind, seed=seed, absent=[(1, 0)] if len(lens) > 2 else ()).upload()
+        q = queries(b, 24)
+        got = run(b, q, window, 0.5)
+        want, bound = attention(b, q, 0.5, window)
+        assert (np.abs(got - want) <= to_kind(want, bound, np.float32)).all()

@@ -23,13 +23,13 @@
 // where the maximum does or a scale is 2^6 times as large, so a weight reaches 2^14 at most. (A power above the
 // largest scale alone would lose a key of small scale beside one of large scale that weighs nothing.)
 //
-// What bounds it. Many rows: a key tile is 32 products of 32 cycles a wave and 330 other vector operations of 4, and a
-// SIMD has two waves to overlap them. 2048 tokens on 8192 keys, 8 heads of 256, int8: 159 us, 756 TFLOP/s, 0.63 of
-// what a large f16 product reaches. Of its 379 thousand cycles a SIMD's matrix unit is busy 116 and its vector
-// unit 149; a wave waits 38% of its time, for loads, LDS and barriers. Neither unit is full: two waves do not hide
-// all of each other's waits, and a third has no registers (8192 tokens on their own: 386 us; f16: 405 us). Few rows: reading
-// the cache (32 single tokens on 16384 keys, f16: 89 us, 6.0 TB/s), and below that a block's way from its arguments to
-// the first keys and from its last to memory, 4 us each: 4 tokens on 4096 keys take 9.9 us and their join 4.2.
+// What bounds it. Many rows: a key tile is 32 products of 32 cycles a wave and 354 other vector operations of 4, and a
+// SIMD has two waves to overlap them. 2048 tokens on 8192 keys, 8 heads of 256, int8: 160 us, 752 TFLOP/s, 0.62 of
+// what a large f16 product reaches. Of its 400 thousand cycles a SIMD's matrix unit is busy 116 and its vector
+// unit 160; a wave waits 38% of its time, for loads, LDS and barriers. Neither unit is full: two waves do not hide
+// all of each other's waits, and a third has no registers (8192 tokens on their own: 397 us; f16: 396-405 us). Few rows: reading
+// the cache (32 single tokens on 16384 keys, f16: 89-94 us, 5.7-6.0 TB/s), and below that a block's way from its arguments to
+// the first keys and from its last to memory, 4 us each: 4 tokens on 4096 keys take 9.8 us and their join 4.2-4.5.
 #include "g4_paged.h"
 #include "g4_key_span.h"
 #include <algorithm>

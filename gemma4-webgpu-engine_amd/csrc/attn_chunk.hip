@@ -244,7 +244,8 @@ __device__ __forceinline__ void attn_put(void *out, int kind, float in_scale, co
 //  RT 2, 4: two block barriers a key tile, one before the softmax and one after it, and waves 4..7 one barrier
 //        behind waves 0..3: of the two waves that share a SIMD, one has the matrix unit (a tile's output and
 //        the next tile's scores) while the other has the vector unit. K comes two tiles ahead and V one. In
-//        step, 8192 tokens took 447 us for 381 (int8, RT 2) and 436 for 402 (f16, RT 4), head_dim 128 221 for 181.
+//        step, 8192 tokens took 447 us for 381 (int8, RT 2, V's codes by permutes) and 436 for 402 (f16, RT 4),
+//        head_dim 128 221 for 181.
 template <int D, int CK, int RT>
 struct Shape {
     static constexpr int EB = CK == G4_KIND_I8 ? 1 : 2;  // bytes of an element
@@ -1034,12 +1035,13 @@ struct AttnPlan {
 };
 
 // Row tiles of a block (kRows rows of a sequence or fewer: 1). Blocks of one need no barrier and run two to a
-// CU where LDS holds two; blocks of more share each key tile's loads. Measured with 1, 2 and 4 (us):
+// CU where LDS holds two; blocks of more share each key tile's loads. Measured with 1, 2 and 4 (us; int8 of 256 with
+// 1 and 2):
 //   int8, head_dim 64 and 128: 1. 2048 tokens, 32 heads on 8, on 4096 keys: 140, 171, 152 and 214, 261, 254.
 //   int8, head_dim 256, 8 heads on 1: 2 where a block then has 4096 keys or more of its own, else 1. 8192 tokens on
-//     their own 398, 381, 415; 2048 on 8192 keys 181, 164, 170 (four split the keys in two); 4096 on their own 122,
-//     123; 300 on 8300 keys 46, 60; 64 x 64 tokens on up to 2064 keys 62, 80; 32 x 8 on up to 4096 28, 28;
-//     1000 tokens, window 512, 30, 37, 47; 100 on 1100 keys 18, 20, 28.
+//     their own 407, 402; 2048 on 8192 keys 173, 163; 16 x 512 on up to 4600 389, 374; 4096 on their own 124, 126;
+//     2048 45, 47; 300 on 8300 keys 47, 60; 64 x 64 on up to 2064 62, 80; 32 x 8 on up to 4096 26, 28;
+//     1000 tokens, window 512, 30, 37; 100 on 1100 keys 18, 20.
 //   f16: 4 where that gives every second CU a block, so that the keys are split in two at most, for the parts'
 //     way through memory costs more from there on. head_dim 256, 8 heads on 1: 8192 tokens 555, 580, 402; 2048 on
 //     8192 keys 226, 245, 168; head_dim 128, 2048 tokens, 32 heads on 8, 197, 196, 181; head_dim 64 111, 116, 103.

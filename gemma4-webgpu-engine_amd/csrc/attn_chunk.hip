@@ -27,9 +27,10 @@
 // SIMD has two waves to overlap them. 2048 tokens on 8192 keys, 8 heads of 256, int8: 160 us, 752 TFLOP/s, 0.62 of
 // what a large f16 product reaches. Of its 400 thousand cycles a SIMD's matrix unit is busy 116 and its vector
 // unit 160; a wave waits 38% of its time, for loads, LDS and barriers. Neither unit is full: two waves do not hide
-// all of each other's waits, and a third has no registers (8192 tokens on their own: 397 us; f16: 396-405 us). Few rows: reading
-// the cache (32 single tokens on 16384 keys, f16: 89-94 us, 5.7-6.0 TB/s), and below that a block's way from its arguments to
-// the first keys and from its last to memory, 4 us each: 4 tokens on 4096 keys take 9.8 us and their join 4.2-4.5.
+// all of each other's waits, and a third has no registers (8192 tokens on their own: 397 us; f16: 396-405 us).
+// Few rows: reading the cache (32 single tokens on 16384 keys, f16: 89-94 us, 5.7-6.0 TB/s), and below that a block's
+// way from its arguments to the first keys and from its last to memory, 4 us each: 4 tokens on 4096 keys take 9.8 us
+// and their join 4.2-4.5.
 #include "g4_paged.h"
 #include "g4_key_span.h"
 #include <algorithm>
@@ -118,8 +119,8 @@ __device__ __forceinline__ h8 words_h8(uint32_t a, uint32_t b, uint32_t c, uint3
 // and then into the high one. (A partial write is read a wait state later at the earliest.) Codes + 128 put together by
 // byte permutes as f16 subnormals, the 128s taken off the output by the sum of the weights, are 2 operations a pair
 // fewer; but beside a weight near 1 the f32 sums of such products lose what small weights add (an output of 3e-5 in a
-// row of 2 was 17% off), and long runs of alike weights lost more (6e-4 over 131072 keys). 2048 tokens on 8192 keys 161 us for 157,
-// 8192 on their own 398 for 379, 32 single tokens as before.
+// row of 2 was 17% off), and long runs of alike weights lost more (6e-4 over 131072 keys). 2048 tokens on 8192
+// keys 161 us for 157, 8192 on their own 398 for 379, 32 single tokens as before.
 template <int J>
 __device__ __forceinline__ h8 code_operand(const uint32_t (&v)[8][1]) {
     u32x4 r;
@@ -786,9 +787,6 @@ void attn_kernel(PagedArgs A, AttnArgs R) {
                 for (int r = 0; r < 8; ++r)
                     l = __builtin_amdgcn_fdot2(h2{p[r / 4][2 * (r % 4)], p[r / 4][2 * (r % 4) + 1]}, one, l, false);
             }
-            if (I8)  // made here: the registers are full below
-#pragma unroll
-                for (int k = 0; k < 2; ++k) asm volatile("" : "+v"(p[k]));
             wait_v();
             softmax_done();
             bool odd = false;

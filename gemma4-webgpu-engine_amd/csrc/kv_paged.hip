@@ -191,7 +191,8 @@ __global__ __launch_bounds__(256) void paged_prologue_kernel(PagedArgs A, Prolog
 
 // Bound by HBM: 67000 tokens of 4 heads of 128, codes to f16, 209 MB, on other pages in each call 46.5 us (4.5 TB/s);
 // 65 with K and V in blocks of their own and a search per row; batches of 2 and 8 47.6 and 45.6, blocks of 8 and 32
-// tokens 45.7 and 46.7. On the same pages call after call, of which the 256 MB cache holds part: 32.7; 34.0, 33.3, 33.1, 34.2.
+// tokens 45.7 and 46.7. On the same pages call after call, of which the 256 MB cache holds part: 32.7; 34.0, 33.3,
+// 33.1 and 34.2.
 // A block takes kReadTokens rows: a wave looks them up at once (the first one's sequence by ballots over the
 // ends, the others' from there on), then threads move units of 8 elements, K's and V's of kReadBatch at a time.
 constexpr int kReadTokens = 16, kReadBatch = 4;

@@ -10,10 +10,10 @@
 // would often name its neighbour. So exponents and sums are held in 64 bits and 2^f is good to 1e-12.
 //
 // What bounds it: (1) issue, about 55 vector operations a logit with the softcap, 29 of them 64-bit, and 37 and 18
-// without (264 rows of 262144, with: 98 us, what 55 take at 16 lanes a cycle and SIMD, for a read of 43; 160 rows 60;
-// without, 9 rows 7, latency); (3) reading the drawn rows again (32 sequences, 26 us,
-// two rows each); (2) and (4) a chain of loads, 4-8 and 8-13 us. Parts of 8192 give 4 waves 32 logits a thread,
-// loaded at once; units of 1024 keep the last step one block's work and its code short (2048: 2.4 us more).
+// without (264 rows of 262144, with: 98 us, what 55 take at 16 lanes a cycle and SIMD, for a read of 43; 160 rows
+// 60; without, 9 rows 7, latency); (3) reading the drawn rows again (32 sequences, 26 us, two rows each); (2) and
+// (4) a chain of loads, 4-8 and 8-13 us. Parts of 8192 give 4 waves 32 logits a thread, loaded at once; units of
+// 1024 keep the last step one block's work and its code short (2048: 2.4 us more).
 #include "g4_internal.h"
 #include "../../include/g4serve.h"
 #include <cmath>

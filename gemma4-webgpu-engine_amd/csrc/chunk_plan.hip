@@ -1,0 +1,268 @@
+// The plan of a chunk and the release of pages (include/g4serve.h): prefix sums over the requests' rows
+// and pages, then one item per chunk row and per page.
+//
+// No block waits for another: each computes the prefix sums of all sequences (at most 4096, a few loads a
+// thread) into LDS and finds its items' sequences there by binary search. That is why a call's counts are
+// read from other arrays than it writes.
+#include "g4_internal.h"
+#include "../../include/g4serve.h"
+
+namespace g4 {
+
+constexpr int kPlanSeqs = 4096, kPlanThreads = 256, kPlanItems = 1024;  // items a block
+constexpr int kPlanBlocks = 1024;
+
+struct PlanArgs {
+    int32_t *free_pages;
+    const int32_t *count, *cached, *rows, *held, *seq_adapter;
+    int32_t *table;
+    int64_t table_stride;
+    int32_t *q_start, *kv_len, *held_out, *free_left, *served, *row_pos, *row_slot, *row_adapter, *last_row;
+    int capacity, num_pages, page_shift, seqs, tokens, max_q, max_kv, table_pages;
+};
+
+// What sequence s asks for, before it is known whether it is served.
+struct Wish {
+    int cached, rows, held, need;
+};
+
+__device__ __forceinline__ Wish wish_of(const PlanArgs &A, int s) {
+    Wish w;
+    w.cached = min(max(A.cached[s], 0), A.max_kv);
+    w.rows = min(max(A.rows[s], 0), min(A.max_q, A.max_kv - w.cached));
+    const int last = (1 << A.page_shift) - 1;
+    // positions are below table_pages pages, which fit in 32 bits with a page to spare
+    const int now = (int)(((int64_t)w.cached + last) >> A.page_shift);
+    const int then = (int)(((int64_t)w.cached + w.rows + last) >> A.page_shift);
+    w.held = A.held ? min(max(A.held[s], 0), A.table_pages) : now;
+    w.need = w.rows > 0 ? max(then - w.held, 0) : 0;
+    return w;
+}
+
+// Exclusive sum over the block's threads of v; *total: of all.
+__device__ __forceinline__ int64_t block_before(int64_t v, int64_t *lds, int64_t *total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t run = v;
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        const int64_t o = __shfl_up((long long)run, s);
+        if (lane >= s) run += o;
+    }
+    __syncthreads();
+    if (lane == 63) lds[wave] = run;
+    __syncthreads();
+    int64_t before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kPlanThreads / 64; ++w) {
+        if (w < wave) before += lds[w];
+        all += lds[w];
+    }
+    *total = all;
+    return before + run - v;
+}
+
+// The last s with start[s] <= i of an ascending start[0 .. n], for i < start[n].
+__device__ __forceinline__ int owner(const int32_t *start, int n, int i) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        (start[mid] <= i ? lo : hi) = mid;
+    }
+    return lo;
+}
+
+// Bound by its chain of dependent steps: count and lengths, two block sums, a search in LDS, a page, the stores.
+__global__ __launch_bounds__(kPlanThreads) void plan_chunk_kernel(PlanArgs A) {
+    extern __shared__ int32_t plan_lds[];
+    __shared__ int64_t sums[kPlanThreads / 64];
+    __shared__ int fit;
+    int32_t *start = plan_lds, *pages = plan_lds + A.seqs + 1;
+    const int t = threadIdx.x, per = (A.seqs + kPlanThreads - 1) / kPlanThreads;
+    const int s0 = min(t * per, A.seqs), s1 = min(s0 + per, A.seqs);
+    const int count = min(max(*A.count, 0), A.capacity);
+    if (t == 0) fit = 0;
+    int64_t rows = 0, need = 0;
+    for (int s = s0; s < s1; ++s) {
+        const Wish w = wish_of(A, s);
+        rows += w.rows;
+        need += w.need;
+    }
+    int64_t all;
+    int64_t r = block_before(rows, sums, &all), n = block_before(need, sums, &all);
+    int mine = 0;
+    for (int s = s0; s < s1; ++s) {
+        const Wish w = wish_of(A, s);
+        // of a sequence that is not served nothing is read but whether it is
+        start[s] = (int)min(r, (int64_t)A.tokens);
+        pages[s] = (int)min(n, (int64_t)count);
+        r += w.rows;
+        n += w.need;
+        if (r <= A.tokens && n <= count) {
+            ++mine;
+            start[s + 1] = (int)r;  // the next thread writes the same, or is not served
+            pages[s + 1] = (int)n;
+        }
+    }
+    if (mine) atomicAdd(&fit, mine);
+    __syncthreads();
+    const int served = fit;
+    const int total_rows = start[served], total_pages = pages[served], left = count - total_pages;
+    const int64_t stride = (int64_t)gridDim.x * kPlanThreads, first = (int64_t)blockIdx.x * kPlanThreads + t;
+    for (int64_t i = first; i < total_pages; i += stride) {
+        const int s = owner(pages, served, (int)i);
+        const Wish w = wish_of(A, s);
+        A.table[s * A.table_stride + w.held + ((int)i - pages[s])] = A.free_pages[left + i];
+    }
+    if (A.row_pos || A.row_slot || A.row_adapter)
+        for (int64_t i = first; i < A.tokens; i += stride) {
+            int pos = -1, slot = -1, adapter = -2;
+            if (i < total_rows) {
+                const int s = owner(start, served, (int)i);
+                const Wish w = wish_of(A, s);
+                pos = w.cached + ((int)i - start[s]);
+                adapter = A.seq_adapter ? A.seq_adapter[s] : -1;
+                if (A.row_slot) {
+                    const int p = pos >> A.page_shift;
+                    const int page = p < w.held || p >= w.held + w.need ? A.table[s * A.table_stride + p]
+                                                                        : A.free_pages[left + pages[s] + (p - w.held)];
+                    if ((unsigned)page < (unsigned)A.num_pages)
+                        slot = (page << A.page_shift) + (pos & ((1 << A.page_shift) - 1));
+                }
+            }
+            if (A.row_pos) A.row_pos[i] = pos;
+            if (A.row_slot) A.row_slot[i] = slot;
+            if (A.row_adapter) A.row_adapter[i] = adapter;
+        }
+    for (int64_t i = first; i < A.seqs; i += stride) {
+        const int s = (int)i;
+        const Wish w = wish_of(A, s);
+        const bool in = s < served;
+        A.q_start[s + 1] = in ? start[s + 1] : total_rows;
+        A.kv_len[s] = w.cached + (in ? w.rows : 0);
+        if (A.held_out) A.held_out[s] = w.held + (in ? w.need : 0);
+        if (A.last_row) A.last_row[s] = in && w.rows ? start[s + 1] - 1 : -1;
+    }
+    if (first == 0) {
+        A.q_start[0] = 0;
+        *A.free_left = left;
+        *A.served = served;
+    }
+}
+
+struct ReleaseArgs {
+    int32_t *free_pages;
+    const int32_t *count, *table, *first, *last;
+    int64_t table_stride;
+    int32_t *count_out;
+    int capacity, seqs, table_pages;
+};
+
+__device__ __forceinline__ int2 range_of(const ReleaseArgs &A, int s) {
+    const int a = min(max(A.first[s], 0), A.table_pages);
+    return make_int2(a, max(min(A.last[s], A.table_pages), a));
+}
+
+__global__ __launch_bounds__(kPlanThreads) void release_pages_kernel(ReleaseArgs A) {
+    extern __shared__ int32_t plan_lds[];
+    __shared__ int64_t sums[kPlanThreads / 64];
+    int32_t *start = plan_lds;
+    const int t = threadIdx.x, per = (A.seqs + kPlanThreads - 1) / kPlanThreads;
+    const int s0 = min(t * per, A.seqs), s1 = min(s0 + per, A.seqs);
+    const int count = min(max(*A.count, 0), A.capacity), room = A.capacity - count;
+    int64_t n = 0, all;
+    for (int s = s0; s < s1; ++s) {
+        const int2 r = range_of(A, s);
+        n += r.y - r.x;
+    }
+    int64_t before = block_before(n, sums, &all);
+    for (int s = s0; s < s1; ++s) {
+        const int2 r = range_of(A, s);
+        start[s] = (int)min(before, (int64_t)room);
+        before += r.y - r.x;
+    }
+    const int total = (int)min(all, (int64_t)room);
+    if (t == 0) start[A.seqs] = total;
+    __syncthreads();
+    const int64_t stride = (int64_t)gridDim.x * kPlanThreads, first = (int64_t)blockIdx.x * kPlanThreads + t;
+    for (int64_t i = first; i < total; i += stride) {
+        const int s = owner(start, A.seqs, (int)i);
+        A.free_pages[count + i] = A.table[s * A.table_stride + range_of(A, s).x + ((int)i - start[s])];
+    }
+    if (first == 0) *A.count_out = count + total;
+}
+
+static int check_list(const char *who, const g4_free_pages *L) {
+    if (!L || !L->pages || !L->count) return set_error(G4_ERR_INVALID, "%s needs the free pages and their count", who);
+    if (L->capacity <= 0 || L->num_pages <= 0)
+        return set_error(G4_ERR_INVALID, "%s: a free list of %d of %d pages", who, L->capacity, L->num_pages);
+    if (L->page_size < 8 || L->page_size > 4096 || (L->page_size & (L->page_size - 1)))
+        return set_error(G4_ERR_INVALID, "%s: page_size %d is not a power of two from 8 to 4096", who, L->page_size);
+    if ((int64_t)L->num_pages * L->page_size > INT32_MAX)
+        return set_error(G4_ERR_UNSUPPORTED, "%s: %d pages of %d slots (slots are 32-bit)", who, L->num_pages, L->page_size);
+    return G4_OK;
+}
+
+static int check_table(const char *who, const void *table, int table_pages, int64_t table_stride, int seqs) {
+    if (!table || seqs <= 0 || table_pages <= 0)
+        return set_error(G4_ERR_INVALID, "%s: %d sequences, %d table pages", who, seqs, table_pages);
+    if (seqs > kPlanSeqs)
+        return set_error(G4_ERR_UNSUPPORTED, "%s: %d sequences in one call (at most %d)", who, seqs, kPlanSeqs);
+    if (table_stride && table_stride < table_pages)
+        return set_error(G4_ERR_INVALID, "%s: table_stride %lld < %d table pages", who, (long long)table_stride, table_pages);
+    return G4_OK;
+}
+
+static unsigned plan_blocks(int64_t items) {
+    const int64_t n = (items + kPlanItems - 1) / kPlanItems;
+    return (unsigned)(n < 1 ? 1 : n > kPlanBlocks ? kPlanBlocks : n);
+}
+
+}  // namespace g4
+
+using namespace g4;
+
+extern "C" {
+
+int g4_plan_chunk(const g4_free_pages *list, const int32_t *cached, const int32_t *rows, const int32_t *held,
+                  const int32_t *seq_adapter, int seqs, int tokens, int max_q, int max_kv, int32_t *page_table,
+                  int table_pages, int64_t table_stride, int32_t *q_start, int32_t *kv_len, int32_t *held_out,
+                  int32_t *free_left, int32_t *served, int32_t *row_pos, int32_t *row_slot, int32_t *row_adapter,
+                  int32_t *last_row, void *stream) {
+    if (int st = check_list("plan-chunk", list)) return st;
+    if (int st = check_table("plan-chunk", page_table, table_pages, table_stride, seqs)) return st;
+    if (!cached || !rows || !q_start || !kv_len || !free_left || !served)
+        return set_error(G4_ERR_INVALID, "plan-chunk needs cached, rows, q_start, kv_len, free_left and served");
+    if (tokens <= 0 || max_q <= 0 || max_kv <= 0)
+        return set_error(G4_ERR_INVALID, "plan-chunk: %d tokens, max_q %d, max_kv %d", tokens, max_q, max_kv);
+    if ((int64_t)table_pages * list->page_size < max_kv)
+        return set_error(G4_ERR_INVALID, "plan-chunk: %d table pages of %d slots do not hold max_kv %d positions", table_pages,
+                         list->page_size, max_kv);
+    if (free_left == list->count || kv_len == cached || (held && held_out == held))
+        return set_error(G4_ERR_INVALID, "plan-chunk: free_left, kv_len and held_out cannot be the arrays they are made from");
+    PlanArgs A{list->pages, list->count, cached, rows, held, seq_adapter, page_table,
+               table_stride ? table_stride : table_pages, q_start, kv_len, held_out, free_left, served, row_pos, row_slot,
+               row_adapter, last_row, list->capacity, list->num_pages, __builtin_ctz(list->page_size), seqs, tokens, max_q,
+               max_kv, table_pages};
+    const size_t lds = 2 * ((size_t)seqs + 1) * sizeof(int32_t);
+    hipLaunchKernelGGL(plan_chunk_kernel, dim3(plan_blocks(tokens)), dim3(kPlanThreads), lds, as_stream(stream), A);
+    G4_LAUNCHED("plan_chunk_kernel");
+    return G4_OK;
+}
+
+int g4_release_pages(const g4_free_pages *list, const int32_t *page_table, int table_pages, int64_t table_stride,
+                     const int32_t *first, const int32_t *last, int seqs, int32_t *count_out, void *stream) {
+    if (int st = check_list("release-pages", list)) return st;
+    if (int st = check_table("release-pages", page_table, table_pages, table_stride, seqs)) return st;
+    if (!first || !last || !count_out) return set_error(G4_ERR_INVALID, "release-pages needs first, last and count_out");
+    if (count_out == list->count)
+        return set_error(G4_ERR_INVALID, "release-pages: count_out cannot be the list's count");
+    ReleaseArgs A{list->pages, list->count, page_table, first, last, table_stride ? table_stride : table_pages, count_out,
+                  list->capacity, seqs, table_pages};
+    const int64_t most = (int64_t)seqs * table_pages;
+    hipLaunchKernelGGL(release_pages_kernel, dim3(plan_blocks(most < list->capacity ? most : list->capacity)),
+                       dim3(kPlanThreads), ((size_t)seqs + 1) * sizeof(int32_t), as_stream(stream), A);
+    G4_LAUNCHED("release_pages_kernel");
+    return G4_OK;
+}
+
+}  // extern "C"

@@ -14,7 +14,7 @@
 // 60; without, 9 rows 7, latency); (3) reading the drawn rows again (32 sequences, 26 us, two rows each); (2) and
 // (4) a chain of loads, 4-8 and 8-13 us. Parts of 8192 give 4 waves 32 logits a thread, loaded at once; units of
 // 1024 keep the last step one block's work and its code short (2048: 2.4 us more).
-#include "g4_internal.h"
+#include "g4_logits.h"
 #include "../../include/g4serve.h"
 #include <cmath>
 
@@ -54,69 +54,18 @@ struct VerifyArgs {
     float *logprobs;
 };
 
-// The softcap, tanh(x / cap) cap: |x| <= cap / 2 as x + x t P(t), t = (x / cap)^2 (a polynomial fitted on Chebyshev
-// nodes, 8e-14 t x off, 11 operations), past that 1 - 2 / (e^2a + 1), which would lose digits where a is small. A
-// row's maximum, the bulk of its sums and the judged logits all go through the same two, so that the maximum's
-// exponent is 0 and no other's is above: at a temperature of 1e-12 a difference of 1e-13 would count. (Neither falls
-// as x grows: below half the cap the values of neighbouring f32 logits are 2^-25 of them apart and 2^-44 off.)
-//
-// The weight of the bulk of a row, 2^z: z = n + f, |f| <= 1/2, a polynomial in f (fitted likewise, relative error
-// 1.1e-12) and n into the exponent: 16 64-bit operations a logit.
+// The weight of the bulk of a row, 2^((y - top) slope): 16 64-bit operations a logit.
 struct RowScale {
     double top, slope;  // 2^((y - top) slope)
 };
 __device__ __forceinline__ RowScale row_scale(double top, const VerifyArgs &A) {
     return {top, A.inv_t * 1.4426950408889634074};
 }
-// a b + k with k in scalar registers (the compiler would copy it to vector ones first, two moves a step).
-__device__ __forceinline__ double fma_k(double a, double b, double k) {
-    double r;
-    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(k));
-    return r;
-}
-__device__ __forceinline__ double near_cap(double x, const VerifyArgs &A) {
-    const double t = x * x * A.inv_cap2;
-    double c = 0.00039943422382545215;
-    c = fma_k(c, t, -0.0013843999024647944);
-    c = fma_k(c, t, 0.0035776163994480498);
-    c = fma_k(c, t, -0.008861575554686911);
-    c = fma_k(c, t, 0.021869384578835853);
-    c = fma_k(c, t, -0.053968250756296965);
-    c = fma_k(c, t, 0.1333333332954187);
-    c = fma_k(c, t, -0.3333333333332598);
-    return __builtin_fma(x, t * c, x);
-}
-__device__ __forceinline__ double far_cap(double x, double cap) {
-    const double a = fabs(x) / cap;
-    return copysign(cap * (1.0 - 2.0 / (exp(2.0 * a) + 1.0)), x);
-}
-__device__ __forceinline__ double softcap64(float x, const VerifyArgs &A) {
-    if (A.cap == 0.0) return x;
-    return fabsf(x) > A.half_cap ? far_cap(x, A.cap) : near_cap(x, A);
-}
 // exp((y - top) / T), 1 at the maximum itself (both infinite included).
 __device__ __forceinline__ double weight(float x, double top, const VerifyArgs &A) {
     const double y = softcap64(x, A);
     return y == top ? 1.0 : exp((y - top) * A.inv_t);
 }
-// 2^z; below 2^-1000 that (too small to count, and the exponent stays normal), and for a NaN.
-__device__ __forceinline__ double pow2(double z) {
-    z = z > -1000.0 ? z : -1000.0;
-    const double r = z + 0x1.8p52;  // n in the low word
-    const double f = z - (r - 0x1.8p52);
-    double e = 1.3259689002093833e-06;
-    e = fma_k(e, f, 1.531008106933654e-05);
-    e = fma_k(e, f, 0.00015403433582607232);
-    e = fma_k(e, f, 0.0013333450560096254);
-    e = fma_k(e, f, 0.009618129194093111);
-    e = fma_k(e, f, 0.05550410941217064);
-    e = fma_k(e, f, 0.24022650695640319);
-    e = fma_k(e, f, 0.6931471805459295);
-    e = fma_k(e, f, 1.0000000000000135);
-    return __hiloint2double(__double2hiint(e) + (int)((uint32_t)__double2loint(r) << 20), __double2loint(e));
-}
-// |x| past what near_cap is good for, -infinity (no weight) not included
-__device__ __forceinline__ bool is_far(float x, const VerifyArgs &A) { return fabsf(x) > A.half_cap && x > -INFINITY; }
 template <bool CAP>
 __device__ __forceinline__ double bulk_weight(float x, const RowScale &S, const VerifyArgs &A) {
     double y = x;
@@ -128,8 +77,6 @@ __device__ __forceinline__ double bulk_weight(float x, const RowScale &S, const 
     const double e = z > -1000.0 ? pow2(z) : 0.0;  // under 2^-1000 of the largest: none
     return !CAP && x == INFINITY ? 1.0 : e;
 }
-
-__device__ __forceinline__ float clean(float x) { return x == x ? x : -INFINITY; }
 
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll

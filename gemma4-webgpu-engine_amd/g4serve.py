@@ -1,5 +1,6 @@
-"""Serving operators on a paged KV cache (include/g4serve.h): the prologue of a chunk of new tokens
-with its quantising store, the read-back, attention of the chunk, and draft verification.
+"""Serving operators on a paged KV cache (include/g4serve.h): the plan of a chunk of new tokens, its
+prologue with the quantising store, the read-back, attention of the chunk, low-rank adapters beside the
+linears, draft verification, and sampling.
 
 Operands are anything with a shape, a dtype and a device address: g4w8a8.DeviceBuffer, or a torch
 tensor on the current device (torch imported before the library is loaded, by the first call into it,
@@ -198,24 +199,13 @@ class Chunk:
     max_q, max_kv: the most rows and positions that a sequence has. Keeps its buffers alive."""
 
     def __init__(self, q_start, kv_len, page_table, tokens, max_q, max_kv):
-        if len(page_table.shape) != 2:
-            raise g4.G4Error(1, f"page_table has shape {list(page_table.shape)}, expected [seqs][pages]")
-        seqs, width = (int(n) for n in page_table.shape)
-        stride = width
-        if hasattr(page_table, "stride"):
-            st = page_table.stride()
-            if (width > 1 and st[1] != 1) or (seqs > 1 and st[0] < width):
-                raise g4.G4Error(1, "page_table rows must be packed")
-            stride = st[0] if seqs > 1 else width
-        if _kind(page_table) != g4.KIND_I32:
-            raise g4.G4Error(1, f"page_table cannot be {page_table.dtype}")
         device = self.device = _device()
+        at, seqs, width, stride = _table(page_table, device)
         self.buffers = (q_start, kv_len, page_table)
         self.seqs, self.tokens, self.max_q, self.max_kv = seqs, int(tokens), int(max_q), int(max_kv)
         self.c = ChunkStruct(seqs, self.tokens, self.max_q, self.max_kv,
                              _packed(q_start, "q_start", _I32, (seqs + 1,), device),
-                             _packed(kv_len, "kv_len", _I32, (seqs,), device),
-                             _address(page_table, "page_table", device), width, stride)
+                             _packed(kv_len, "kv_len", _I32, (seqs,), device), at, width, stride)
         self.ref = ctypes.byref(self.c)
 
 
@@ -336,5 +326,213 @@ def verify_drafts(logits, draft_logits, draft_tokens, draft_start, u, u_next, to
         None if logprobs is None else _packed(logprobs, "logprobs", _F32, (seqs, width), device),
         _stream(stream, device, logits, draft_logits, draft_tokens, draft_start, u, u_next, tokens, accepted, logprobs,
                 workspace))
+    if st:
+        g4._check(st)
+
+
+class FreePagesStruct(ctypes.Structure):
+    """include/g4serve.h g4_free_pages."""
+    _fields_ = [("pages", _vp), ("count", _vp), ("capacity", ctypes.c_int), ("num_pages", ctypes.c_int),
+                ("page_size", ctypes.c_int)]
+
+
+class AdaptersStruct(ctypes.Structure):
+    """include/g4serve.h g4_adapters."""
+    _fields_ = [("a", _vp), ("b", _vp), ("scales", _vp), ("ranks", _vp), ("count", ctypes.c_int),
+                ("max_rank", ctypes.c_int), ("k", ctypes.c_int), ("n", ctypes.c_int), ("a_stride", ctypes.c_int64),
+                ("b_stride", ctypes.c_int64)]
+
+
+def _need_device(x, device, what):
+    if x.device != device:
+        raise g4.G4Error(1, f"{what} are on another device than the current one")
+
+
+def _optional(x, what, kinds, shape, device):
+    return None if x is None else _packed(x, what, kinds, shape, device)
+
+
+def _table(page_table, device):
+    """(address, sequences, pages, elements between rows) of a page table."""
+    if len(page_table.shape) != 2:
+        raise g4.G4Error(1, f"page_table has shape {list(page_table.shape)}, expected [seqs][pages]")
+    seqs, width = (int(n) for n in page_table.shape)
+    stride = width
+    if hasattr(page_table, "stride"):
+        st = page_table.stride()
+        if (width > 1 and st[1] != 1) or (seqs > 1 and st[0] < width):
+            raise g4.G4Error(1, "page_table rows must be packed")
+        stride = st[0] if seqs > 1 else width
+    if _kind(page_table) != g4.KIND_I32:
+        raise g4.G4Error(1, f"page_table cannot be {page_table.dtype}")
+    return _address(page_table, "page_table", device), seqs, width, stride
+
+
+class FreePages:
+    """The pages that no sequence holds: pages int32 [capacity], of which the first count (int32 [1]) are
+    free. A plan or a release reads them and writes the count it leaves elsewhere: make one FreePages for each of
+    two count buffers, on the same pages, and take them in turn. Keeps its buffers alive."""
+
+    def __init__(self, pages, count, num_pages, page_size):
+        device = self.device = _device()
+        self.buffers = (pages, count)
+        capacity = int(pages.shape[0])
+        self.c = FreePagesStruct(_packed(pages, "free pages", _I32, (capacity,), device),
+                                 _packed(count, "count", _I32, (1,), device), capacity, int(num_pages), int(page_size))
+        self.ref = ctypes.byref(self.c)
+
+
+def plan_chunk(free, cached, rows, page_table, q_start, kv_len, free_left, served, tokens, max_q, max_kv, held=None,
+               held_out=None, seq_adapter=None, row_pos=None, row_slot=None, row_adapter=None, last_row=None,
+               stream=None):
+    """g4_plan_chunk: the arrays of a Chunk (q_start [seqs + 1], kv_len [seqs], new entries of page_table) from
+    each request's cached positions and rows (int32 [seqs]), the free list's new count (free_left [1]), the number of
+    sequences served ([1]), and optionally held_out and last_row [seqs], row_pos, row_slot and row_adapter [tokens];
+    all int32."""
+    device = _device()
+    _need_device(free, device, "the free pages")
+    at, seqs, width, stride = _table(page_table, device)
+    per_seq = [_optional(x, what, _I32, (seqs,), device) for x, what in (
+        (cached, "cached"), (rows, "rows"), (held, "held"), (seq_adapter, "seq_adapter"))]
+    per_row = [_optional(x, what, _I32, (tokens,), device) for x, what in (
+        (row_pos, "row_pos"), (row_slot, "row_slot"), (row_adapter, "row_adapter"))]
+    st = g4.lib().g4_plan_chunk(
+        free.ref, *per_seq, seqs, tokens, max_q, max_kv, at, width, stride, _packed(q_start, "q_start", _I32, (seqs + 1,), device),
+        _packed(kv_len, "kv_len", _I32, (seqs,), device), _optional(held_out, "held_out", _I32, (seqs,), device),
+        _packed(free_left, "free_left", _I32, (1,), device), _packed(served, "served", _I32, (1,), device), *per_row,
+        _optional(last_row, "last_row", _I32, (seqs,), device),
+        _stream(stream, device, *free.buffers, cached, rows, held, seq_adapter, page_table, q_start, kv_len, held_out, free_left,
+                served, row_pos, row_slot, row_adapter, last_row))
+    if st:
+        g4._check(st)
+
+
+def release_pages(free, page_table, first, last, count_out, stream=None):
+    """g4_release_pages: entries first[s] .. last[s] - 1 (int32 [seqs]) of every sequence's row of page_table back to the
+    free pages; count_out int32 [1] is the new count."""
+    device = _device()
+    _need_device(free, device, "the free pages")
+    at, seqs, width, stride = _table(page_table, device)
+    st = g4.lib().g4_release_pages(
+        free.ref, at, width, stride, _packed(first, "first", _I32, (seqs,), device), _packed(last, "last", _I32, (seqs,), device),
+        seqs, _packed(count_out, "count_out", _I32, (1,), device),
+        _stream(stream, device, *free.buffers, page_table, first, last, count_out))
+    if st:
+        g4._check(st)
+
+
+class Adapters:
+    """Low-rank adapters of one linear: a f16 [count][max_rank][k] and b f16 [count][n][max_rank] (adapters may lie
+    apart, each packed), scales f32 [count] (1 where not given), ranks int32 [count] (max_rank). Keeps its buffers alive."""
+
+    def __init__(self, a, b, scales=None, ranks=None):
+        if len(a.shape) != 3 or len(b.shape) != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+            raise g4.G4Error(1, f"adapters need a [count][max_rank][k] and b [count][n][max_rank], got {list(a.shape)} and "
+                                f"{list(b.shape)}")
+        device = self.device = _device()
+        count, rank, k = (int(n) for n in a.shape)
+        n = int(b.shape[1])
+        self.buffers, self.count, self.k, self.n = (a, b, scales, ranks), count, k, n
+        at = []
+        for x, what, rows, width in ((a, "a", rank, k), (b, "b", n, rank)):
+            if _kind(x) != g4.KIND_F16:
+                raise g4.G4Error(1, f"{what} cannot be {x.dtype}")
+            stride = rows * width
+            if hasattr(x, "stride"):
+                st = x.stride()
+                if (width > 1 and st[2] != 1) or (rows > 1 and st[1] != width) or (count > 1 and st[0] < stride):
+                    raise g4.G4Error(1, f"{what}: an adapter must be packed, and adapters apart")
+                stride = st[0] if count > 1 else stride
+            at.append((_address(x, what, device), stride))
+        self.c = AdaptersStruct(at[0][0], at[1][0], _optional(scales, "scales", _F32, (count,), device),
+                                _optional(ranks, "ranks", _I32, (count,), device), count, rank, k, n, at[0][1], at[1][1])
+        self.ref = ctypes.byref(self.c)
+
+
+def adapter_groups_bytes(tokens, adapters) -> int:
+    n = g4.lib().g4_adapter_groups_bytes(tokens, adapters)
+    if not n:
+        raise g4.G4Error(1, f"adapter-groups: no such call ({tokens} tokens, {adapters} adapters)")
+    return n
+
+
+def adapter_groups(row_adapter, groups, adapters, stream=None):
+    """g4_adapter_groups: the rows of a batch by adapter, for every adapter_linear of a step. row_adapter int32
+    [tokens] (-1: none, -2: no row), groups adapter_groups_bytes(tokens, adapters) bytes."""
+    device = _device()
+    tokens = int(row_adapter.shape[0])
+    st = g4.lib().g4_adapter_groups(_packed(row_adapter, "row_adapter", _I32, (tokens,), device), tokens, adapters,
+                                    *_workspace(groups, device), _stream(stream, device, row_adapter, groups))
+    if st:
+        g4._check(st)
+
+
+def adapter_workspace_bytes(adapters, tokens) -> int:
+    n = g4.lib().g4_adapter_workspace_bytes(adapters.ref, tokens)
+    if not n:
+        raise g4.G4Error(1, f"adapter-linear: no such call ({tokens} tokens, adapters {list(adapters.buffers[0].shape)} and "
+                            f"{list(adapters.buffers[1].shape)})")
+    return n
+
+
+def _matrix(x, what, tokens, width, device):
+    """(address, kind, elements between rows) of [tokens][width], whose rows may lie apart."""
+    kind = _kind(x)
+    if kind not in _X_KINDS:
+        raise g4.G4Error(1, f"{what} cannot be {x.dtype}")
+    if x.shape != (tokens, width):
+        raise g4.G4Error(1, f"{what} has shape {list(x.shape)}, expected {[tokens, width]}")
+    stride = width
+    if hasattr(x, "stride"):
+        st = x.stride()
+        if (width > 1 and st[1] != 1) or (tokens > 1 and st[0] < width):
+            raise g4.G4Error(1, f"{what}: rows must be packed, and apart")
+        stride = st[0] if tokens > 1 else width
+    return _address(x, what, device), kind, stride
+
+
+def adapter_linear(adapters, groups, x, base, out, workspace, x_scale=1.0, base_scale=1.0, out_scale=0.0, stream=None):
+    """g4_adapter_linear: out = base + scale * (x A^T) B^T with each row's adapter. x [tokens][k] and base (or None)
+    [tokens][n]: f32, f16 or int8 codes on x_scale / base_scale; out f32, f16, or int8 codes on out_scale; out may be
+    base. groups: of adapter_groups, for as many tokens."""
+    device = _device()
+    _need_device(adapters, device, "the adapters")
+    tokens = int(x.shape[0])
+    xa = _matrix(x, "x", tokens, adapters.k, device)
+    ba = (None, g4.KIND_F32, 0) if base is None else _matrix(base, "base", tokens, adapters.n, device)
+    oa = _matrix(out, "out", tokens, adapters.n, device)
+    st = g4.lib().g4_adapter_linear(adapters.ref, *_workspace(groups, device), tokens, *xa, x_scale, *ba, base_scale, *oa,
+                                    out_scale, *_workspace(workspace, device),
+                                    _stream(stream, device, *adapters.buffers, groups, x, base, out, workspace))
+    if st:
+        g4._check(st)
+
+
+def sample_workspace_bytes(rows, vocab) -> int:
+    n = g4.lib().g4_sample_workspace_bytes(rows, vocab)
+    if not n:
+        raise g4.G4Error(1, f"sample-tokens: no such call ({rows} rows, vocabulary {vocab})")
+    return n
+
+
+def sample_tokens(logits, u, tokens, logprobs, workspace, row_index=None, temperature=None, top_k=None, top_p=None,
+                  min_p=None, cap=0.0, stream=None):
+    """g4_sample_tokens. logits f32 [rows of logits][vocab] (rows may lie apart), u f32 [rows] in [0, 1), tokens int32 and
+    logprobs f32 (or None) [rows] out; optional: row_index and top_k int32, temperature, top_p and min_p f32 [rows]."""
+    device = _device()
+    if len(logits.shape) != 2:
+        raise g4.G4Error(1, f"logits has shape {list(logits.shape)}, expected [rows][vocab]")
+    logit_rows, vocab, rows = int(logits.shape[0]), int(logits.shape[1]), int(u.shape[0])
+    at, kind, stride = _matrix(logits, "logits", logit_rows, vocab, device)
+    if kind != g4.KIND_F32:
+        raise g4.G4Error(1, f"logits cannot be {logits.dtype}")
+    given = [_optional(x, what, kinds, (rows,), device) for x, what, kinds in (
+        (row_index, "row_index", _I32), (temperature, "temperature", _F32), (top_k, "top_k", _I32), (top_p, "top_p", _F32),
+        (min_p, "min_p", _F32))]
+    st = g4.lib().g4_sample_tokens(
+        at, logit_rows, stride, given[0], rows, vocab, cap, *given[1:], _packed(u, "u", _F32, (rows,), device),
+        *_workspace(workspace, device), _packed(tokens, "tokens", _I32, (rows,), device),
+        _optional(logprobs, "logprobs", _F32, (rows,), device),
+        _stream(stream, device, logits, u, tokens, logprobs, workspace, row_index, temperature, top_k, top_p, min_p))
     if st:
         g4._check(st)

@@ -248,6 +248,17 @@ SIGNATURES = {
     "g4_verify_drafts": (_c_int, [_vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _i64, _c_float,
                                   _c_float, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _vp]),
     "g4_verify_workspace_bytes": (_sz, [_c_int, _c_int, _i64]),
+    "g4_plan_chunk": (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _vp, _c_int, _i64,
+                               _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "g4_release_pages": (_c_int, [_vp, _vp, _c_int, _i64, _vp, _vp, _c_int, _vp, _vp]),
+    "g4_adapter_groups": (_c_int, [_vp, _c_int, _c_int, _vp, _sz, _vp]),
+    "g4_adapter_groups_bytes": (_sz, [_c_int, _c_int]),
+    "g4_adapter_linear": (_c_int, [_vp, _vp, _sz, _c_int, _vp, _c_int, _i64, _c_float, _vp, _c_int, _i64, _c_float,
+                                   _vp, _c_int, _i64, _c_float, _vp, _sz, _vp]),
+    "g4_adapter_workspace_bytes": (_sz, [_vp, _c_int]),
+    "g4_sample_tokens": (_c_int, [_vp, _c_int, _i64, _vp, _c_int, _i64, _c_float, _vp, _vp, _vp, _vp, _vp, _vp,
+                                  _sz, _vp, _vp, _vp]),
+    "g4_sample_workspace_bytes": (_sz, [_c_int, _i64]),
     # include/g4ckpt.h
     "g4_st_parse": (_c_int, [_vp, _sz, _c_int, ctypes.POINTER(_vp)]),
     "g4_st_open": (_c_int, [ctypes.c_char_p, ctypes.POINTER(_vp)]),

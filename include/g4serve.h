@@ -1,7 +1,8 @@
 /*
- * g4serve.h - serving operators on a paged KV cache: the prologue of a chunk of new tokens with its
- * quantising store, the read-back, attention of the chunk over the cache, and the verification of
- * drafted tokens. No counterpart in the reference, whose cache is one contiguous f32 buffer per
+ * g4serve.h - serving operators on a paged KV cache: the plan of a chunk of new tokens (pages, block
+ * tables, slot maps), its prologue with the quantising store, the read-back, attention of the chunk over
+ * the cache, per-request low-rank adapters beside the linears, the verification of drafted tokens, and
+ * sampling. No counterpart in the reference, whose cache is one contiguous f32 buffer per
  * sequence and whose chunks are two tokens: these run the same layer (linears of g4w8a8.h, norms and
  * head of g4decode.h) for a batch of sequences of different lengths.
  *
@@ -153,6 +154,118 @@ int g4_verify_drafts(const float *logits, const float *draft_logits, const int32
                      void *workspace, size_t workspace_bytes, int32_t *tokens, int32_t *accepted,
                      float *logprobs, void *stream);
 size_t g4_verify_workspace_bytes(int seqs, int drafts, int64_t vocab);
+
+/*
+ * Pages that no sequence holds: the first *count of `pages` (a count outside [0, capacity] is clamped).
+ * A step reads the count and writes the new one elsewhere, so that the step after it can be enqueued
+ * before this one has run: two count words (and two `held` arrays, below) in turn.
+ */
+typedef struct g4_free_pages {
+    int32_t *pages;       /* [capacity] ids */
+    const int32_t *count; /* [1] */
+    int capacity;
+    int num_pages; /* of the pools */
+    int page_size; /* a power of two from 8 to 4096 */
+} g4_free_pages;
+
+/*
+ * The plan of a chunk from the requests' lengths: the arrays of g4_chunk, the pages of the new positions, and where
+ * each row goes. Sequence s has c = cached[s] positions (clamped to [0, max_kv]) and asks for n = rows[s] new ones
+ * (clamped to [0, min(max_q, max_kv - c)]). It holds held[s] pages, the first entries of its row of page_table (held
+ * NULL: those that c positions need), and needs max(0, ceil((c + n) / page_size) - held[s]) more where n > 0.
+ * Sequences are served in order, while their rows fit into `tokens` and their pages into the free ones: from the first
+ * that does not fit on, all get no rows and no pages in this chunk. served: how many fit.
+ * The pages given are the last ones of the free list, in the list's order: by sequence, then by position.
+ * Out: q_start [seqs + 1], kv_len [seqs] (c + the rows given), free_left [1] and served [1], the new entries of
+ * page_table (no other entry is touched); optional (NULL): held_out [seqs], last_row [seqs] (q_start[s + 1] - 1, -1
+ * without rows: the row of g4_sample_tokens), and of each of the `tokens` rows its position row_pos, its cache slot
+ * row_slot (page * page_size + position % page_size, -1 on an absent page) and its adapter row_adapter
+ * (seq_adapter[s], -1 where that is NULL). Rows behind the last sequence: -1, -1 and -2.
+ * free_left must not be the free list's count, kv_len not cached and held_out not held: those are read throughout.
+ * At most 4096 sequences, and num_pages * page_size below 2^31.
+ */
+int g4_plan_chunk(const g4_free_pages *list, const int32_t *cached, const int32_t *rows, const int32_t *held,
+                  const int32_t *seq_adapter, int seqs, int tokens, int max_q, int max_kv, int32_t *page_table,
+                  int table_pages, int64_t table_stride, int32_t *q_start, int32_t *kv_len, int32_t *held_out,
+                  int32_t *free_left, int32_t *served, int32_t *row_pos, int32_t *row_slot, int32_t *row_adapter,
+                  int32_t *last_row, void *stream);
+
+/*
+ * Pages back to the free list: entries first[s] .. last[s] - 1 of every sequence's row of page_table (clamped to
+ * [0, table_pages]; a finished request's all, or those that a window has left behind) are appended to the free pages, by
+ * sequence, then by position; count_out is the new count. Entries that would pass the list's capacity are dropped.
+ * page_table stays as it is: its user no longer counts these pages as held. An entry must not be released
+ * twice, nor one that two sequences share. count_out must not be the list's count. At most 4096 sequences.
+ */
+int g4_release_pages(const g4_free_pages *list, const int32_t *page_table, int table_pages, int64_t table_stride,
+                     const int32_t *first, const int32_t *last, int seqs, int32_t *count_out, void *stream);
+
+/*
+ * Low-rank adapters of one linear, f16: adapter i adds scales[i] * (x A_i^T) B_i^T to its rows.
+ * A_i = a + i * a_stride, [max_rank][k]; B_i = b + i * b_stride, [n][max_rank] (strides in elements, 0: packed). ranks
+ * (NULL: max_rank for all): adapter i has ranks[i] (clamped to [0, max_rank]) rows of A_i and columns of B_i; what lies
+ * behind them is not used, whatever it holds. k and max_rank multiples of 8, max_rank up to 128, at most 4096 adapters; a and
+ * b 16-byte aligned, the strides multiples of 8.
+ */
+typedef struct g4_adapters {
+    const void *a, *b;
+    const float *scales;  /* [count], NULL: 1 */
+    const int32_t *ranks; /* [count] or NULL */
+    int count, max_rank, k, n;
+    int64_t a_stride, b_stride;
+} g4_adapters;
+
+/*
+ * The rows of a batch grouped by their adapter, once for every linear of a step: row_adapter [tokens] (of g4_plan_chunk,
+ * for example) into `groups`, g4_adapter_groups_bytes(...) bytes, 16-byte aligned. An id in [0, adapters) is that
+ * adapter, -2 no row (its outputs are left as they were), any other one no adapter. At most 2^19 tokens.
+ */
+int g4_adapter_groups(const int32_t *row_adapter, int tokens, int adapters, void *groups, size_t groups_bytes,
+                      void *stream);
+size_t g4_adapter_groups_bytes(int tokens, int adapters);
+
+/*
+ * A linear's output with its rows' adapters added:
+ *   out[t] = base[t] + scales[i] * ((x[t] A_i^T) B_i^T), i the row's adapter, and base[t] for a row without one.
+ * x [tokens][k] is the linear's input: f32, f16, or int8 codes times x_scale; base [tokens][n] what the shared
+ * linear gave: f32, f16, or int8 codes times base_scale, or NULL (zeros). out: f32, f16, or int8 codes on out_scale;
+ * out_scale != 0 snaps f32 and f16 outputs to that grid too, as g4_linear does (a f32 output code * out_scale; the
+ * quotient's clamp takes a NaN to -128). Rows start x_stride, base_stride and out_stride elements apart (0: packed); x 16-byte
+ * aligned, x_stride a multiple of 16 bytes (codes: of 8). out may be base, of the same type and stride. groups: of
+ * g4_adapter_groups, for the same tokens and number of adapters.
+ * Products are exact (f16 and f32 values in f32), added up in f32, as is x A^T, which is not rounded in between.
+ * workspace: g4_adapter_workspace_bytes(...) bytes, 16-byte aligned.
+ */
+int g4_adapter_linear(const g4_adapters *adapters, const void *groups, size_t groups_bytes, int tokens, const void *x,
+                      int x_kind, int64_t x_stride, float x_scale, const void *base, int base_kind, int64_t base_stride,
+                      float base_scale, void *out, int out_kind, int64_t out_stride, float out_scale, void *workspace,
+                      size_t workspace_bytes, void *stream);
+size_t g4_adapter_workspace_bytes(const g4_adapters *adapters, int tokens);
+
+/*
+ * Sampling: one token for each of `rows` requests, from given random numbers. Request i reads row row_index[i] of
+ * logits (NULL: row i; several may read one row), logit_rows rows of vocab f32 that start logit_stride elements apart
+ * (0: packed). With y = tanh(x / cap) * cap (cap 0: y = x) and w = exp((y - max y) / temperature[i]), the row's tokens are
+ * ordered by their logits, the lower id first among equal ones, and each filter keeps a part of what the one before it left:
+ *   top_k[i]: the first top_k (0 or less, or vocab or more: all);
+ *   top_p[i]: those before which the sum of weights is under top_p * the sum of all that top_k left, and the
+ *             first one always (1 or more: all);
+ *   min_p[i]: those with w >= min_p (0 or less: all; more than 1 counts as 1).
+ * The token drawn is the first, in token order, where the running sum of the kept weights exceeds u[i] * their sum.
+ * A temperature that is not above 0 (NaN too) is greedy: the first maximum. A NULL array: temperature 1, the filter off; a NaN
+ * in one turns the filter off. A logit that is NaN or -infinity has no weight. A row without any, or a row_index outside
+ * [0, logit_rows), gives token -1 and log probability 0. u in [0, 1) (clamped to it, NaN: 0).
+ * logprobs (optional): (y - max y) / temperature - log(the sum of all weights), before the filters (greedy: at 1).
+ * Weights are counted in whole steps of 2^-min(51, 62 - ceil(log2 vocab)) of the row's largest (2^-44 for
+ * 262144 tokens) and added up exactly, so that a result does not depend on the order of the additions; what rounds to
+ * no step is not drawn. vocab up to 2^22, at most 65535 rows.
+ * workspace: g4_sample_workspace_bytes(...) bytes, 16-byte aligned.
+ */
+int g4_sample_tokens(const float *logits, int logit_rows, int64_t logit_stride, const int32_t *row_index, int rows,
+                     int64_t vocab, float cap, const float *temperature, const int32_t *top_k, const float *top_p,
+                     const float *min_p, const float *u, void *workspace, size_t workspace_bytes, int32_t *tokens,
+                     float *logprobs, void *stream);
+size_t g4_sample_workspace_bytes(int rows, int64_t vocab);
 
 #ifdef __cplusplus
 }

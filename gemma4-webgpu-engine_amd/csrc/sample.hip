@@ -1,11 +1,12 @@
 // Sampling with temperature, top-k, top-p and min-p from given random numbers (include/g4serve.h).
 //
 // All filters keep a prefix of the row ordered by (logit down, id up), so a row's kept set is one cut in that
-// order, and min-p a bound on the logit beside it. The order is never made: (1) every part's maximum and minimum; (2)
-// weights, and for a row with top-k or top-p a histogram of them over bins of the capped logit; (3) the bins where the
-// cuts lie, from the histogram, the weights of what lies above them by units of 1024 tokens, and a list of what
-// lies in them; (4) a block per row refines the cuts within its list, finds the unit and then the token where the
-// running sum passes u of the total. A row without top-k and top-p has its units' weights from (2).
+// order, and min-p a bound on the logit beside it. The order is never made: (1) the maximum of every unit of 1024 tokens
+// and part of the row; (2) weights, and for a row with top-k or top-p a histogram of them over bins of the capped
+// logit; (3) the bins where the cuts lie, from the histogram, the units' weights above them, and a list of what lies in
+// them, for which only units that reach up to them are read again; (4) a block per row finds the cuts within its list,
+// the unit and then the token where the running sum passes u of the total. A row without top-k and top-p has its
+// units' weights from (2).
 //
 // Weights are integers, steps of 2^-shift of the row's largest: sums are exact, and additions in any order, atomic ones
 // too, give the same. A bin never falls as a logit falls, so that bins and logits have one order.
@@ -20,11 +21,12 @@ typedef unsigned long long u64;
 constexpr int kSampleThreads = 256, kSampleWaves = kSampleThreads / 64;
 constexpr int kSampleUnit = 1024, kSamplePer = kSampleUnit / 64;  // a wave's range, and a lane's part of it
 constexpr int kSamplePart = kSampleWaves * kSampleUnit;
-constexpr int kBins = 1024, kBinsPer = kBins / kSampleThreads;
+constexpr int kWideThreads = 512, kWideWaves = kWideThreads / 64;  // of (2) and (3): a unit a wave
+constexpr int kBins = 1024, kBinsPer = kBins / kWideThreads;
 constexpr int kList = 4096;  // entries; a row with more is read again
-constexpr int kPickThreads = 1024, kListPer = kList / kPickThreads;
-constexpr int kSub = 1024;  // ranges of one refinement step, one a thread
-static_assert(kSub == kPickThreads && kSampleUnit == kPickThreads, "the last kernel has one thread each");
+constexpr int kFew = 64;     // entries that a wave orders by itself
+constexpr int kSub = 1024, kSubPer = kSub / kSampleThreads;  // ranges of one refinement step
+constexpr int kUnitPer = kSampleUnit / kSampleThreads;
 constexpr int kMaxVocab = 1 << 22;
 
 struct PartMax {
@@ -37,6 +39,15 @@ struct PartMax {
 struct Cuts {
     int k_bin, p_low, p_high, k_rest;  // the k-th token is the k_rest-th of k_bin
     u64 k_before, p_before;            // weight of the bins above k_bin and above p_low
+    float least, pad;                  // no logit below this is in one of these bins, or above
+};
+
+// What a row's weights are made with.
+struct Row {
+    double top, slope, d_min, bins;  // weight 2^((y - top) slope), kept from d_min on, bin (top - y) bins
+    double inv_t, p;
+    int index, k;                // the first maximum (-1: no logit)
+    int greedy, filtered, inf, pad;  // inf: the maximum is +infinity, whose like share all weight
 };
 
 struct SampleArgs {
@@ -48,13 +59,16 @@ struct SampleArgs {
     const float *top_p, *min_p, *u;
     CapArgs cap;
     int logit_rows, vocab, parts, units, shift, vec, cuts;  // cuts: top-k or top-p given
+    int spans;                   // blocks a row of (2) and (3)
     PartMax *stats;              // [rows][parts]
-    u64 *part_sums, *unit_sums;  // [rows][parts], [rows][units]
+    Row *row;                    // [rows]
+    Cuts *cut;                   // [rows]
+    u64 *span_sums, *unit_sums;  // [rows][spans], [rows][units]
     u64 *bin_mass;               // [rows][kBins]
     u64 *list;                   // [rows][kList]
-    Cuts *cut;                   // [rows]
     uint32_t *bin_count;         // [rows][kBins]
     uint32_t *listed;            // [rows]
+    float *unit_max;             // [rows][units]
     int32_t *tokens;
     float *logprobs;
 };
@@ -134,6 +148,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_max_kernel(SampleArgs A
     m = wave_join(m);
     if (lane == 0) ms[wave] = m;
     if (A.cuts) {
+        if (lane == 0 && base < A.vocab) A.unit_max[(int64_t)row * A.units + part * kSampleWaves + wave] = m.max;
         for (int i = part * kSampleThreads + t; i < kBins; i += A.parts * kSampleThreads) {
             A.bin_mass[(int64_t)row * kBins + i] = 0;
             A.bin_count[(int64_t)row * kBins + i] = 0;
@@ -146,14 +161,6 @@ __global__ __launch_bounds__(kSampleThreads) void sample_max_kernel(SampleArgs A
     for (int w = 1; w < kSampleWaves; ++w) join_max(m, ms[w].max, ms[w].min, ms[w].index);
     A.stats[(int64_t)row * A.parts + part] = m;
 }
-
-// What a row's weights are made with.
-struct Row {
-    double top, slope, d_min, bins;  // weight 2^((y - top) slope), kept from d_min on, bin (top - y) bins
-    double inv_t, p;
-    int index, k;                // the first maximum (-1: no logit)
-    bool greedy, filtered, inf;  // inf: the maximum is +infinity, whose like share all weight
-};
 
 // By one wave, the same in every lane.
 __device__ __forceinline__ Row row_params(const SampleArgs &A, int row) {
@@ -175,21 +182,43 @@ __device__ __forceinline__ Row row_params(const SampleArgs &A, int row) {
     R.slope = R.inv_t * 1.4426950408889634074;
     R.inf = A.cap.cap == 0.0 && m.max == INFINITY;
     R.top = R.inf || m.index < 0 ? 0.0 : softcap64(m.max, A.cap);
-    R.d_min = mf > 0.0f ? (mf >= 1.0f ? 0.0 : log((double)mf) * t) : -INFINITY;
+    R.d_min = -INFINITY;
+    if (mf > 0.0f) R.d_min = mf >= 1.0f ? 0.0 : log((double)mf) * t;
     R.k = k < A.vocab ? k : 0;
     R.p = pf < 1.0f ? (double)pf : 1.0;  // NaN: off
     R.filtered = !R.greedy && m.index >= 0 && (R.k > 0 || R.p < 1.0);
-    // the bins reach from the top to the lowest logit, or to where weights round to no step
-    double range = R.inf || m.index < 0 ? 0.0 : R.top - softcap64(m.min, A.cap);
-    range = fmin(range, (A.shift + 1) / R.slope);
-    R.bins = range > 0.0 ? fmin((kBins - 1) / range, 1e300) : 0.0;
+    R.bins = 0.0;
+    if (R.filtered && !R.inf) {
+        // the bins reach from the top to the lowest logit, or to where weights round to no step
+        const double range = fmin(R.top - softcap64(m.min, A.cap), (A.shift + 1) * 0.69314718055994530942 * t);
+        if (range > 0.0) R.bins = fmin((kBins - 1) * __builtin_amdgcn_rcp(range), 1e300);
+    }
+    R.pad = 0;
     return R;
+}
+
+// The same value in scalar registers: it is the block's.
+template <class T>
+__device__ __forceinline__ T uniform(const T &v) {
+    static_assert(sizeof(T) % 4 == 0, "words");
+    struct Words {
+        int w[sizeof(T) / 4];
+    };
+    Words a = __builtin_bit_cast(Words, v);
+#pragma unroll
+    for (size_t i = 0; i < sizeof(T) / 4; ++i) a.w[i] = __builtin_amdgcn_readfirstlane(a.w[i]);
+    return __builtin_bit_cast(T, a);
 }
 
 // Under an infinite maximum a logit is as good as it, or nothing.
 __device__ __forceinline__ float seen(float x, const Row &R) { return R.inf ? (x == INFINITY ? 0.0f : -INFINITY) : x; }
 
-// y - top; for a -infinity that, or NaN.
+// y - top of a logit that is not past half the cap; for a -infinity that, or NaN.
+template <bool CAP>
+__device__ __forceinline__ double near_distance(float x, const Row &R, const SampleArgs &A) {
+    return (CAP ? near_cap((double)x, A.cap) : (double)x) - R.top;
+}
+// And of any.
 template <bool CAP>
 __device__ __forceinline__ double distance(float x, const Row &R, const SampleArgs &A) {
     double y = x;
@@ -219,7 +248,7 @@ __device__ __forceinline__ u64 wave_sum(u64 v) {
 }
 
 // Inclusive sum over the block's threads; *total: of all.
-template <int THREADS>
+template <int THREADS = kSampleThreads>
 __device__ __forceinline__ u64 block_run(u64 v, u64 *lds, u64 *total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -241,36 +270,37 @@ __device__ __forceinline__ u64 block_run(u64 v, u64 *lds, u64 *total) {
     return before + v;
 }
 
-// Grid (parts, rows).
+// Grid (spans, rows).
 template <bool CAP>
-__global__ __launch_bounds__(kSampleThreads) void sample_weights_kernel(SampleArgs A) {
+__global__ __launch_bounds__(kWideThreads) void sample_weights_kernel(SampleArgs A) {
     __shared__ u64 mass[kBins];
     __shared__ uint32_t count[kBins];
-    __shared__ u64 ss[kSampleWaves];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, part = blockIdx.x, row = blockIdx.y;
+    __shared__ u64 ss[kWideWaves];
+    __shared__ Row shared_row;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, row = blockIdx.y;
     const float *x = row_of(A, row);
-    const int unit = part * kSampleWaves + wave, base = unit * kSampleUnit;
+    const int unit = blockIdx.x * kWideWaves + wave, base = unit * kSampleUnit;
     float v[kSamplePer];
-    if (x && base < A.vocab) {
-        load_unit(x + base, A.vocab - base, lane, A.vec, v);
-    } else {
-#pragma unroll
-        for (int j = 0; j < kSamplePer; ++j) v[j] = -INFINITY;
+    load_unit(x + base, x ? A.vocab - base : 0, lane, A.vec, v);
+    if (wave == 0) {  // once a block: as many operations as the weights of a unit
+        const Row R = row_params(A, row);
+        if (lane == 0) {
+            shared_row = R;
+            if (blockIdx.x == 0) A.row[row] = R;
+        }
     }
-    const Row R = row_params(A, row);
-    if (R.index < 0) return;
-    if (R.filtered) {
+    if (A.cuts) {
 #pragma unroll
         for (int i = 0; i < kBinsPer; ++i) {
-            mass[i * kSampleThreads + t] = 0;
-            count[i * kSampleThreads + t] = 0;
+            mass[i * kWideThreads + t] = 0;
+            count[i * kWideThreads + t] = 0;
         }
-        __syncthreads();
     }
+    __syncthreads();
+    const Row R = uniform(shared_row);
+    if (R.index < 0) return;
     u64 all = 0, kept = 0;
-#pragma unroll
-    for (int j = 0; j < kSamplePer; ++j) {
-        const double d = distance<CAP>(seen(v[j], R), R, A);
+    auto add = [&](double d) {
         const u64 w = steps(d, R, A);
         all += w;
         if (!R.filtered) {
@@ -280,7 +310,17 @@ __global__ __launch_bounds__(kSampleThreads) void sample_weights_kernel(SampleAr
             atomicAdd(&mass[b], w);
             atomicAdd(&count[b], 1u);
         }
+    };
+    uint32_t far = 0;  // few: past half the cap, one at a time
+#pragma unroll
+    for (int j = 0; j < kSamplePer; ++j) {
+        const float xs = seen(v[j], R);
+        const bool f = CAP && is_far(xs, A.cap);
+        far |= f ? 1u << j : 0u;
+        add(f ? -INFINITY : near_distance<CAP>(xs, R, A));
     }
+    if (CAP)
+        for (; far; far &= far - 1) add(distance<CAP>(x[base + unit_place(__ffs(far) - 1, lane, A.vec)], R, A));
     all = wave_sum(all);
     if (lane == 0) ss[wave] = all;
     if (!R.filtered) {
@@ -288,11 +328,15 @@ __global__ __launch_bounds__(kSampleThreads) void sample_weights_kernel(SampleAr
         if (lane == 0 && unit < A.units) A.unit_sums[(int64_t)row * A.units + unit] = kept;
     }
     __syncthreads();
-    if (t == 0) A.part_sums[(int64_t)row * A.parts + part] = (ss[0] + ss[1]) + (ss[2] + ss[3]);
+    if (t == 0) {
+#pragma unroll
+        for (int w = 1; w < kWideWaves; ++w) all += ss[w];
+        A.span_sums[(int64_t)row * A.spans + blockIdx.x] = all;
+    }
     if (!R.filtered) return;
 #pragma unroll
     for (int i = 0; i < kBinsPer; ++i) {
-        const int b = i * kSampleThreads + t;
+        const int b = i * kWideThreads + t;
         if (!count[b]) continue;
         atomicAdd(&A.bin_mass[(int64_t)row * kBins + b], mass[b]);
         atomicAdd(&A.bin_count[(int64_t)row * kBins + b], count[b]);
@@ -305,22 +349,28 @@ __device__ __forceinline__ u64 mass_target(double p, u64 total) {
     return m >= 1.0 ? (u64)m : 1;
 }
 
-// Grid (parts, rows): every block finds the bins of its row's cuts, then weighs its tokens above them.
+// A logit below which all lie in bins behind `bin`, a little lower than the least such one, so that f32 will do.
+__device__ __forceinline__ float least_of(const SampleArgs &A, const Row &R, int bin) {
+    if (R.inf || !(R.bins > 0.0) || bin >= kBins - 1) return -INFINITY;
+    const float y = (float)(R.top - (bin + 1.5) * __builtin_amdgcn_rcp(R.bins));
+    if (A.cap.cap == 0.0) return y - 1e-6f * fabsf(y);
+    const float cap = (float)A.cap.cap, r = fminf(y / cap, 0.9999f);
+    if (!(r > -0.9999f)) return -INFINITY;
+    const float z = 0.5f * cap * __logf((1.0f + r) / (1.0f - r));
+    return z - 1e-3f * (fabsf(z) + cap);
+}
+
+// Grid (spans, rows): every block finds the bins of its row's cuts, then weighs its tokens above them.
 template <bool CAP>
-__global__ __launch_bounds__(kSampleThreads) void sample_cut_kernel(SampleArgs A) {
-    __shared__ u64 sums[kSampleWaves];
+__global__ __launch_bounds__(kWideThreads) void sample_cut_kernel(SampleArgs A) {
+    __shared__ u64 sums[kWideWaves];
     __shared__ Cuts C;
     __shared__ u64 k_after;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, part = blockIdx.x, row = blockIdx.y;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, row = blockIdx.y;
+    const Row R = uniform(A.row[row]);
+    if (!R.filtered) return;  // (a row without a logit, too)
     const float *x = row_of(A, row);
-    const int unit = part * kSampleWaves + wave, base = unit * kSampleUnit;
-    float v[kSamplePer];
-    if (x && base < A.vocab) {
-        load_unit(x + base, A.vocab - base, lane, A.vec, v);
-    } else {
-#pragma unroll
-        for (int j = 0; j < kSamplePer; ++j) v[j] = -INFINITY;
-    }
+    const int unit = blockIdx.x * kWideWaves + wave, base = unit * kSampleUnit;
     u64 m[kBinsPer], n[kBinsPer], m_sum = 0, n_sum = 0;
 #pragma unroll
     for (int i = 0; i < kBinsPer; ++i) {
@@ -329,15 +379,13 @@ __global__ __launch_bounds__(kSampleThreads) void sample_cut_kernel(SampleArgs A
         m_sum += m[i];
         n_sum += n[i];
     }
-    const Row R = row_params(A, row);
-    if (!R.filtered) return;
     if (t == 0) {
-        C = {kBins, kBins, kBins, 0, 0, 0};
+        C = {kBins, kBins, kBins, 0, 0, 0, 0.0f, 0.0f};
         k_after = 0;
     }
     u64 m_all, n_all;
-    const u64 m_first = block_run<kSampleThreads>(m_sum, sums, &m_all) - m_sum;
-    const u64 n_first = block_run<kSampleThreads>(n_sum, sums, &n_all) - n_sum;
+    const u64 m_first = block_run<kWideThreads>(m_sum, sums, &m_all) - m_sum;
+    const u64 n_first = block_run<kWideThreads>(n_sum, sums, &n_all) - n_sum;
     const bool by_k = R.k > 0 && (u64)R.k < n_all;
     if (by_k) {
         u64 mb = m_first, nb = n_first;
@@ -371,30 +419,48 @@ __global__ __launch_bounds__(kSampleThreads) void sample_cut_kernel(SampleArgs A
         C.p_low = C.p_high = C.k_bin;
     }
     __syncthreads();
-    const Cuts c = C;
-    if (part == 0 && t == 0) A.cut[row] = c;
-    const int last = max(c.p_high, c.k_bin < kBins ? c.k_bin : 0);
+    Cuts c = uniform(C);
+    const int behind = max(c.p_high, c.k_bin < kBins ? c.k_bin : 0);
+    c.least = uniform(least_of(A, R, behind));
+    if (blockIdx.x == 0 && t == 0) A.cut[row] = c;
+    if (unit >= A.units) return;
     u64 sure = 0;
+    if (A.unit_max[(int64_t)row * A.units + unit] >= c.least) {
+        float v[kSamplePer];
+        load_unit(x + base, A.vocab - base, lane, A.vec, v);
+        uint32_t look = 0, in = 0;  // elements that may be in these bins, and those for the list
 #pragma unroll
-    for (int j = 0; j < kSamplePer; ++j) {
-        const float xs = seen(v[j], R);
-        const double d = distance<CAP>(xs, R, A);
-        const bool near = d >= -INFINITY && xs > -INFINITY && bin_of(d, R) <= last;
-        if (!__any(near)) continue;
-        const int b = bin_of(d, R);
-        const u64 w = near ? steps(d, R, A) : 0;
-        if (w && b < c.p_low && d >= R.d_min) sure += w;
-        const bool in = w && ((b >= c.p_low && b <= c.p_high) || b == c.k_bin);
-        const u64 who = __ballot(in);
-        if (!who) continue;
-        uint32_t at = 0;
-        if (lane == __ffsll((long long)who) - 1) at = atomicAdd(&A.listed[row], (uint32_t)__popcll(who));
-        at = __shfl(at, __ffsll((long long)who) - 1) + __popcll(who & ((1ull << lane) - 1));
-        if (in && at < (uint32_t)kList)
-            A.list[(int64_t)row * kList + at] = order_key(xs, base + unit_place(j, lane, A.vec));
+        for (int j = 0; j < kSamplePer; ++j) look |= v[j] >= c.least ? 1u << j : 0u;
+        int many = 0;
+#pragma unroll
+        for (int j = 0; j < kSamplePer; ++j) {
+            if (!__any(look >> j & 1)) continue;
+            const float xs = seen(v[j], R);
+            const double d = distance<CAP>(xs, R, A);
+            const u64 w = xs > -INFINITY ? steps(d, R, A) : 0;
+            const int b = bin_of(d, R);
+            if (b < c.p_low && d >= R.d_min) sure += w;
+            const bool mine = w && ((b >= c.p_low && b <= c.p_high) || b == c.k_bin);
+            in |= mine ? 1u << j : 0u;
+            many += __popcll(__ballot(mine));
+        }
+        if (many) {
+            uint32_t at = 0;
+            if (lane == 0) at = atomicAdd(&A.listed[row], (uint32_t)many);
+            at = __shfl(at, 0);
+#pragma unroll
+            for (int j = 0; j < kSamplePer; ++j) {
+                const bool mine = in >> j & 1;
+                const u64 who = __ballot(mine);
+                const uint32_t place = at + __popcll(who & ((1ull << lane) - 1));
+                if (mine && place < (uint32_t)kList)
+                    A.list[(int64_t)row * kList + place] = order_key(seen(v[j], R), base + unit_place(j, lane, A.vec));
+                at += __popcll(who);
+            }
+        }
+        sure = wave_sum(sure);
     }
-    sure = wave_sum(sure);
-    if (lane == 0 && unit < A.units) A.unit_sums[(int64_t)row * A.units + unit] = sure;
+    if (lane == 0) A.unit_sums[(int64_t)row * A.units + unit] = sure;
 }
 
 __device__ __forceinline__ float logit_of(u64 key) {
@@ -405,37 +471,55 @@ __device__ __forceinline__ float logit_of(u64 key) {
 // A token that a cut is looked for among: in top-k's bin, in top-p's bins, or in neither (then it is none).
 struct Near {
     u64 key, w;
-    double d;
-    bool k, p;
+    bool k, p, kept;  // kept: by min-p
 };
 template <bool CAP>
 __device__ __forceinline__ Near near_of(const SampleArgs &A, const Row &R, const Cuts &C, u64 key) {
-    Near e{key, 0, 0.0, false, false};
+    Near e{key, 0, false, false, false};
     if (!key) return e;
-    e.d = distance<CAP>(logit_of(key), R, A);
-    e.w = steps(e.d, R, A);
-    const int b = bin_of(e.d, R);
+    const double d = distance<CAP>(logit_of(key), R, A);
+    e.w = steps(d, R, A);
+    const int b = bin_of(d, R);
     e.k = e.w && b == C.k_bin;
     e.p = e.w && b >= C.p_low && b <= C.p_high;
+    e.kept = d >= R.d_min;
     return e;
 }
-// The same of token `id`, from the row: for lists that overflowed.
-template <bool CAP>
-__device__ __noinline__ Near near_at(const SampleArgs &A, const Row &R, const Cuts &C, const float *x, int id) {
-    const float v = seen(clean(x[id]), R);
-    return near_of<CAP>(A, R, C, v > -INFINITY ? order_key(v, id) : 0);
+
+__device__ __forceinline__ u64 lane64(u64 v, int lane) {
+    return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+
+// Among a wave's tokens, one a lane where `is`, in falling order of their keys: the one where the running weight
+// (by_p) or count first reaches `target`. Returns its key, and in *mass the weight up to it; the same in every lane.
+__device__ __forceinline__ u64 wave_cut(u64 key, u64 w, bool is, bool by_p, u64 target, u64 *mass) {
+    u64 m = 0, n = 0;
+    for (u64 left = __ballot(is); left; left &= left - 1) {
+        const int j = __ffsll((long long)left) - 1;
+        const u64 k = lane64(key, j), o = lane64(w, j);
+        m += k > key ? o : 0;
+        n += k > key ? 1 : 0;
+    }
+    const u64 run = by_p ? m : n, one = by_p ? w : 1;
+    const u64 at = __ballot(is && run < target && target <= run + one);
+    if (!at) return 0;  // nothing reaches it: all are kept
+    const int j = __ffsll((long long)at) - 1;
+    *mass = lane64(m + w, j);
+    return lane64(key, j);
 }
 
 struct PickShared {
-    u64 extra[kMaxVocab / kSampleUnit];  // of the units, from the list
+    u64 extra[kMaxVocab / kSampleUnit];  // of the units, from a list of more than kFew
     u64 mass[kSub];
     uint32_t count[kSub];
-    u64 sums[kPickThreads / 64];
-    u64 high, low, before, mass_before, mass_at, cut;
-    uint32_t at, count_at;
+    u64 sums[kSampleWaves];
+    u64 few_key[kFew], few_w[kFew];
+    u64 high, low, before, mass_before;
+    uint32_t at, count_at, few;
 };
 
-// What the last kernel's block looks its row's cuts up in: the list, a few elements a thread, or the row again.
+// What a block looks its row's cuts up in where a wave cannot: the list, or where that overflowed the row.
 template <bool CAP>
 struct Search {
     const SampleArgs &A;
@@ -443,37 +527,31 @@ struct Search {
     const Cuts &C;
     const float *x;
     PickShared &S;
-    Near near[kListPer];
-    bool whole;
+    const u64 *list;
+    int n;
 
-    __device__ __forceinline__ void load(int row) {
-        const uint32_t n = A.listed[row];
-        whole = n > (uint32_t)kList;
-#pragma unroll
-        for (int i = 0; i < kListPer; ++i) {
-            const uint32_t at = i * kPickThreads + threadIdx.x;
-            near[i] = near_of<CAP>(A, R, C, !whole && at < n ? A.list[(int64_t)row * kList + at] : 0);
-        }
-    }
+    // All of them with f. Both loops take one element a thread at a time: lists of more than kFew are rare.
     template <class F>
     __device__ __forceinline__ void each(F f) {
-        if (!whole) {
-#pragma unroll
-            for (int i = 0; i < kListPer; ++i)
-                if (near[i].k || near[i].p) f(near[i]);
-        } else {
-            for (int i = threadIdx.x; i < A.vocab; i += kPickThreads) {
-                const Near e = near_at<CAP>(A, R, C, x, i);
-                if (e.k || e.p) f(e);
+        const bool whole = n > kList;
+        const int end = whole ? A.vocab : n;
+        for (int i = threadIdx.x; i < end; i += kSampleThreads) {
+            u64 key;
+            if (whole) {
+                const float v = seen(clean(x[i]), R);
+                key = v > -INFINITY && v >= C.least ? order_key(v, i) : 0;
+            } else {
+                key = list[i];
             }
+            const Near e = near_of<CAP>(A, R, C, key);
+            if (e.k || e.p) f(e);
         }
     }
 
-    // Among top-p's (by_p) or top-k's tokens with a key of at least `least`, in falling order: the one where the
-    // running weight (by_p) or count first reaches `target`. Returns its key, and in *mass the weight up to
-    // it. Each step splits the range of keys in 1024.
-    __device__ __forceinline__ u64 refine(bool by_p, u64 least, u64 target, u64 *mass) {
-        const int t = threadIdx.x;
+    // As wave_cut, among top-p's (by_p) or top-k's tokens with a key of at least `least`. Each step splits the range of
+    // keys in 1024, until a wave can order what is left.
+    __device__ u64 refine(bool by_p, u64 least, u64 target, u64 *mass) {
+        const int t = threadIdx.x, lane = t & 63;
         __syncthreads();
         if (t == 0) {
             S.high = 0;
@@ -496,56 +574,76 @@ struct Search {
         u64 mass_sum = 0;
         while (true) {
             const int bits = 64 - __clzll((long long)((hi - lo) | 1)), sh = bits > 10 ? bits - 10 : 0;
-            S.mass[t] = 0;
-            S.count[t] = 0;
-            if (t == 0) S.at = kSub;
+#pragma unroll
+            for (int i = 0; i < kSubPer; ++i) S.mass[t * kSubPer + i] = S.count[t * kSubPer + i] = 0;
+            if (t == 0) {
+                S.at = kSub;
+                S.few = 0;
+            }
             __syncthreads();
             each([&](const Near &e) {
                 if (!(by_p ? e.p : e.k) || e.key < lo || e.key > hi) return;
                 atomicAdd(&S.mass[(hi - e.key) >> sh], e.w);
                 atomicAdd(&S.count[(hi - e.key) >> sh], 1u);
-                S.cut = e.key;  // the key, where it is the only one
             });
             __syncthreads();
-            u64 all, m_all;
-            const u64 m = S.mass[t], n = S.count[t];
-            const u64 n_run = block_run<kPickThreads>(n, S.sums, &all);
-            const u64 m_run = block_run<kPickThreads>(m, S.sums, &m_all);
-            const u64 run = by_p ? m_run : n_run, one = by_p ? m : n;
-            if (run - one < target && target <= run) {  // one thread, or none where nothing reaches it
-                S.at = t;
-                S.before = run - one;
-                S.mass_before = m_run - m;
-                S.mass_at = m;
-                S.count_at = (uint32_t)n;
+            u64 m[kSubPer], c[kSubPer], m_sum = 0, c_sum = 0, m_all, c_all;
+#pragma unroll
+            for (int i = 0; i < kSubPer; ++i) {
+                m[i] = S.mass[t * kSubPer + i];
+                c[i] = S.count[t * kSubPer + i];
+                m_sum += m[i];
+                c_sum += c[i];
+            }
+            u64 m_run = block_run(m_sum, S.sums, &m_all) - m_sum, c_run = block_run(c_sum, S.sums, &c_all) - c_sum;
+#pragma unroll
+            for (int i = 0; i < kSubPer; ++i) {
+                const u64 run = by_p ? m_run : c_run, one = by_p ? m[i] : c[i];
+                if (run < target && target <= run + one) {  // one thread, or none where nothing reaches it
+                    S.at = t * kSubPer + i;
+                    S.before = run;
+                    S.mass_before = m_run;
+                    S.count_at = (uint32_t)c[i];
+                }
+                m_run += m[i];
+                c_run += c[i];
             }
             __syncthreads();
-            const uint32_t at = S.at;
-            if (at == kSub || all == 1) {
+            const uint32_t at = S.at, left = S.count_at;
+            if (at == kSub) {
                 *mass = mass_sum + m_all;
-                return all == 1 ? S.cut : lo;
+                return lo;
             }
             target -= S.before;
             mass_sum += S.mass_before;
             hi -= (u64)at << sh;
             const u64 width = (1ull << sh) - 1;
             lo = hi - lo > width ? hi - width : lo;
-            if (sh == 0) {  // a range is one key
-                *mass = mass_sum + S.mass_at;
-                return hi;
-            }
             __syncthreads();
+            if (left > kFew) continue;  // (a range of one key holds one token)
+            each([&](const Near &e) {
+                if (!(by_p ? e.p : e.k) || e.key < lo || e.key > hi) return;
+                const uint32_t place = atomicAdd(&S.few, 1u);
+                S.few_key[place] = e.key;
+                S.few_w[place] = e.w;
+            });
+            __syncthreads();
+            const bool is = lane < (int)left;
+            u64 rest = 0;
+            const u64 cut = wave_cut(is ? S.few_key[lane] : 0, is ? S.few_w[lane] : 0, is, by_p, target, &rest);
+            *mass = mass_sum + rest;
+            return cut;
         }
     }
 };
 
 // One block per row.
 template <bool CAP>
-__global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs A) {
+__global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(SampleArgs A) {
     __shared__ PickShared S;
-    const int t = threadIdx.x, row = blockIdx.x;
+    const int t = threadIdx.x, lane = t & 63, row = blockIdx.x;
     const float *x = row_of(A, row);
-    const Row R = row_params(A, row);
+    const Row R = uniform(A.row[row]);
     if (R.index < 0) {
         if (t == 0) {
             A.tokens[row] = -1;
@@ -553,90 +651,129 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs A)
         }
         return;
     }
-    u64 sum = 0, all;
-    for (int c = t; c < A.parts; c += kPickThreads) sum += A.part_sums[(int64_t)row * A.parts + c];
-    block_run<kPickThreads>(sum, S.sums, &all);
-    // log of the sum of all weights: steps back to weights
-    const double log_all = log((double)all) - A.shift * 0.69314718055994530942;
+    // every wave by itself: the sum of all weights
+    u64 all = 0;
+    for (int c = lane; c < A.spans; c += 64) all += A.span_sums[(int64_t)row * A.spans + c];
+    const u64 *units = A.unit_sums + (int64_t)row * A.units;
+    const int per = (A.units + kSampleThreads - 1) / kSampleThreads, u0 = min(t * per, A.units), u1 = min(u0 + per, A.units);
+    u64 mine = 0;
+    if (!R.greedy)
+        for (int i = u0; i < u1; ++i) mine += units[i];
+    all = wave_sum(all);
     if (R.greedy) {
         if (t == 0) {
             A.tokens[row] = R.index;
-            if (A.logprobs) A.logprobs[row] = (float)-log_all;
+            if (A.logprobs) A.logprobs[row] = (float)(A.shift * 0.69314718055994530942 - log((double)all));
         }
         return;
     }
-    for (int i = t; i < A.units; i += kPickThreads) S.extra[i] = 0;
+    u64 cut = 0;  // the last kept key
+    bool spread = false;  // the list's weights are in S.extra
+    Near e{0, 0, false, false, false};
+    u64 few = 0;  // lanes with an element that is kept
+    if (R.filtered) {
+        const Cuts C = uniform(A.cut[row]);
+        if (C.p_low < kBins) {
+            const uint32_t n = A.listed[row];
+            const u64 *list = A.list + (int64_t)row * kList;
+            u64 mass = all;
+            if (n <= kFew) {
+                e = near_of<CAP>(A, R, C, lane < (int)n ? list[lane] : 0);
+                if (C.k_bin < kBins) {
+                    cut = wave_cut(e.key, e.w, e.k, false, C.k_rest, &mass);
+                    mass += C.k_before;
+                }
+                if (R.p < 1.0)
+                    cut = wave_cut(e.key, e.w, e.p && e.key >= cut, true, mass_target(R.p, mass) - C.p_before, &mass);
+                few = __ballot((e.k || e.p) && e.key >= cut && e.kept);
+                for (u64 left = few; left; left &= left - 1) {
+                    const int j = __ffsll((long long)left) - 1;
+                    const int unit = (int)(~(uint32_t)__builtin_amdgcn_readlane((int)e.key, j) / kSampleUnit);
+                    const u64 w = lane64(e.w, j);
+                    mine += unit >= u0 && unit < u1 ? w : 0;
+                }
+            } else {
+                Search<CAP> L{A, R, C, x, S, list, (int)min(n, (uint32_t)kList + 1)};
+                if (C.k_bin < kBins) {
+                    cut = L.refine(false, 0, C.k_rest, &mass);
+                    mass += C.k_before;
+                }
+                if (R.p < 1.0) cut = L.refine(true, cut, mass_target(R.p, mass) - C.p_before, &mass);
+                for (int i = t; i < A.units; i += kSampleThreads) S.extra[i] = 0;
+                __syncthreads();
+                L.each([&](const Near &o) {
+                    if (o.key >= cut && o.kept) atomicAdd(&S.extra[~(uint32_t)o.key / kSampleUnit], o.w);
+                });
+                __syncthreads();
+                spread = true;
+                for (int i = u0; i < u1; ++i) mine += S.extra[i];
+            }
+        }
+    }
+    // the unit, then the token, where the running sum passes u of the total
+    u64 total;
     if (t == 0) {
         S.at = 0;
         S.before = 0;
     }
-    __syncthreads();
-    u64 cut = 0;  // the last kept key
-    if (R.filtered) {
-        const Cuts C = A.cut[row];
-        if (C.p_low < kBins) {
-            Search<CAP> L{A, R, C, x, S};
-            L.load(row);
-            u64 mass = all;
-            if (C.k_bin < kBins) {
-                cut = L.refine(false, 0, C.k_rest, &mass);
-                mass += C.k_before;
-            }
-            if (R.p < 1.0) cut = L.refine(true, cut, mass_target(R.p, mass) - C.p_before, &mass);
-            L.each([&](const Near &e) {
-                if (e.key >= cut && e.d >= R.d_min) atomicAdd(&S.extra[~(uint32_t)e.key / kSampleUnit], e.w);
-            });
-            __syncthreads();
-        }
-    }
-    // the unit, then the token, where the running sum passes u of the total
-    const u64 *units = A.unit_sums + (int64_t)row * A.units;
-    const int per = (A.units + kPickThreads - 1) / kPickThreads, u0 = min(t * per, A.units), u1 = min(u0 + per, A.units);
-    u64 mine = 0, total;
-    for (int i = u0; i < u1; ++i) mine += units[i] + S.extra[i];
-    u64 run = block_run<kPickThreads>(mine, S.sums, &total) - mine;
+    u64 run = block_run(mine, S.sums, &total) - mine;
     const float uf = fminf(fmaxf(A.u[row], 0.0f), 0x1.fffffep-1f);  // NaN: 0
     u64 target = (u64)((double)uf * (double)total);
-    if (run <= target && target < run + mine) {
+    const bool here = run <= target && target < run + mine;  // one thread
+    if (__any(here)) {
         for (int i = u0; i < u1; ++i) {
-            const u64 w = units[i] + S.extra[i];
-            if (target < run + w) {
+            u64 w = units[i] + (spread ? S.extra[i] : 0);
+            for (u64 left = few; left; left &= left - 1) {
+                const int j = __ffsll((long long)left) - 1;
+                if ((int)(~(uint32_t)__builtin_amdgcn_readlane((int)e.key, j) / kSampleUnit) == i) w += lane64(e.w, j);
+            }
+            if (here && run <= target && target < run + w) {
                 S.at = i;
                 S.before = run;
-                break;
             }
             run += w;
         }
     }
     __syncthreads();
-    const int id = (int)S.at * kSampleUnit + t;
+    const int base = (int)S.at * kSampleUnit + t * kUnitPer;
     target -= S.before;
-    u64 w = 0;
-    double d = 0.0;
-    if (id < A.vocab) {
-        const float v = seen(clean(x[id]), R);
-        d = distance<CAP>(v, R, A);
-        if (v > -INFINITY && d >= R.d_min && order_key(v, id) >= cut) w = steps(d, R, A);
+    u64 w[kUnitPer];
+    double d[kUnitPer];
+    mine = 0;
+#pragma unroll
+    for (int i = 0; i < kUnitPer; ++i) {
+        const int id = base + i;
+        const float v = id < A.vocab ? seen(clean(x[id]), R) : -INFINITY;
+        d[i] = distance<CAP>(v, R, A);
+        w[i] = v > -INFINITY && d[i] >= R.d_min && order_key(v, id) >= cut ? steps(d[i], R, A) : 0;
+        mine += w[i];
     }
-    run = block_run<kPickThreads>(w, S.sums, &total) - w;
-    if (run <= target && target < run + w) {
-        A.tokens[row] = id;
-        if (A.logprobs) A.logprobs[row] = (float)(d * R.inv_t - log_all);
+    run = block_run(mine, S.sums, &total) - mine;
+    if (run <= target && target < run + mine) {
+#pragma unroll
+        for (int i = 0; i < kUnitPer; ++i) {
+            if (run <= target && target < run + w[i]) {
+                A.tokens[row] = base + i;
+                if (A.logprobs)  // less the log of the sum of all weights, from steps
+                    A.logprobs[row] = (float)(d[i] * R.inv_t + A.shift * 0.69314718055994530942 - log((double)all));
+            }
+            run += w[i];
+        }
     }
 }
 
 template <bool CAP>
 static int launch_sample(const SampleArgs &A, int rows, hipStream_t s) {
-    const dim3 grid(A.parts, rows);
-    hipLaunchKernelGGL(sample_max_kernel, grid, dim3(kSampleThreads), 0, s, A);
+    hipLaunchKernelGGL(sample_max_kernel, dim3(A.parts, rows), dim3(kSampleThreads), 0, s, A);
     G4_LAUNCHED("sample_max_kernel");
-    hipLaunchKernelGGL(sample_weights_kernel<CAP>, grid, dim3(kSampleThreads), 0, s, A);
+    const dim3 grid(A.spans, rows);
+    hipLaunchKernelGGL(sample_weights_kernel<CAP>, grid, dim3(kWideThreads), 0, s, A);
     G4_LAUNCHED("sample_weights_kernel");
     if (A.cuts) {
-        hipLaunchKernelGGL(sample_cut_kernel<CAP>, grid, dim3(kSampleThreads), 0, s, A);
+        hipLaunchKernelGGL(sample_cut_kernel<CAP>, grid, dim3(kWideThreads), 0, s, A);
         G4_LAUNCHED("sample_cut_kernel");
     }
-    hipLaunchKernelGGL(sample_pick_kernel<CAP>, dim3(rows), dim3(kPickThreads), 0, s, A);
+    hipLaunchKernelGGL(sample_pick_kernel<CAP>, dim3(rows), dim3(kSampleThreads), 0, s, A);
     G4_LAUNCHED("sample_pick_kernel");
     return G4_OK;
 }
@@ -652,8 +789,9 @@ extern "C" {
 
 size_t g4_sample_workspace_bytes(int rows, int64_t vocab) {
     if (rows <= 0 || rows > 65535 || vocab <= 0 || vocab > kMaxVocab) return 0;
-    const size_t row = (size_t)sample_parts(vocab) * (sizeof(PartMax) + sizeof(u64)) + (size_t)sample_units(vocab) * sizeof(u64) +
-                       kBins * (sizeof(u64) + sizeof(uint32_t)) + kList * sizeof(u64) + sizeof(Cuts) + sizeof(uint32_t);
+    const size_t row = (size_t)sample_parts(vocab) * (sizeof(PartMax) + sizeof(u64)) +
+                       (size_t)sample_units(vocab) * (sizeof(u64) + sizeof(float)) + kBins * (sizeof(u64) + sizeof(uint32_t)) +
+                       kList * sizeof(u64) + sizeof(Row) + sizeof(Cuts) + sizeof(uint32_t);
     return rows * row;
 }
 
@@ -696,14 +834,17 @@ int g4_sample_tokens(const float *logits, int logit_rows, int64_t logit_stride, 
     A.shift = 62 - bits < 51 ? 62 - bits : 51;
     A.vec = A.stride % 4 == 0 && ((uintptr_t)logits & 15) == 0;
     A.cuts = top_k || top_p;
+    A.spans = (A.units + kWideWaves - 1) / kWideWaves;  // at most parts
     A.stats = static_cast<PartMax *>(workspace);
-    A.part_sums = reinterpret_cast<u64 *>(A.stats + (int64_t)rows * A.parts);
-    A.unit_sums = A.part_sums + (int64_t)rows * A.parts;
+    A.row = reinterpret_cast<Row *>(A.stats + (int64_t)rows * A.parts);
+    A.cut = reinterpret_cast<Cuts *>(A.row + rows);
+    A.span_sums = reinterpret_cast<u64 *>(A.cut + rows);
+    A.unit_sums = A.span_sums + (int64_t)rows * A.parts;
     A.bin_mass = A.unit_sums + (int64_t)rows * A.units;
     A.list = A.bin_mass + (int64_t)rows * kBins;
-    A.cut = reinterpret_cast<Cuts *>(A.list + (int64_t)rows * kList);
-    A.bin_count = reinterpret_cast<uint32_t *>(A.cut + rows);
+    A.bin_count = reinterpret_cast<uint32_t *>(A.list + (int64_t)rows * kList);
     A.listed = A.bin_count + (int64_t)rows * kBins;
+    A.unit_max = reinterpret_cast<float *>(A.listed + rows);
     A.tokens = tokens;
     A.logprobs = logprobs;
     hipStream_t s = as_stream(stream);

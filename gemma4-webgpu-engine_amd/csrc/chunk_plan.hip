@@ -9,8 +9,8 @@
 
 namespace g4 {
 
-constexpr int kPlanSeqs = 4096, kPlanThreads = 256, kPlanItems = 1024;  // items a block
-constexpr int kPlanBlocks = 1024;
+constexpr int kPlanSeqs = 4096, kPlanThreads = 256;
+constexpr int kPlanBlocks = 512;  // of a kind, two a CU; more items go round, since every block sums all sequences up
 
 struct PlanArgs {
     int32_t *free_pages;
@@ -39,26 +39,38 @@ __device__ __forceinline__ Wish wish_of(const PlanArgs &A, int s) {
     return w;
 }
 
-// Exclusive sum over the block's threads of v; *total: of all.
-__device__ __forceinline__ int64_t block_before(int64_t v, int64_t *lds, int64_t *total) {
+struct Pair {
+    int64_t rows, pages;
+};
+
+// Exclusive sum over the block's threads of v; *total: of all. Once a kernel.
+__device__ __forceinline__ Pair block_before(Pair v, Pair *total) {
+    __shared__ Pair sums[kPlanThreads / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int64_t run = v;
+    Pair run = v;
 #pragma unroll
     for (int s = 1; s < 64; s <<= 1) {
-        const int64_t o = __shfl_up((long long)run, s);
-        if (lane >= s) run += o;
+        const int64_t r = __shfl_up((long long)run.rows, s), p = __shfl_up((long long)run.pages, s);
+        if (lane >= s) {
+            run.rows += r;
+            run.pages += p;
+        }
     }
+    if (lane == 63) sums[wave] = run;
     __syncthreads();
-    if (lane == 63) lds[wave] = run;
-    __syncthreads();
-    int64_t before = 0, all = 0;
+    Pair before{run.rows - v.rows, run.pages - v.pages}, all{0, 0};
 #pragma unroll
     for (int w = 0; w < kPlanThreads / 64; ++w) {
-        if (w < wave) before += lds[w];
-        all += lds[w];
+        const Pair s = sums[w];
+        if (w < wave) {
+            before.rows += s.rows;
+            before.pages += s.pages;
+        }
+        all.rows += s.rows;
+        all.pages += s.pages;
     }
     *total = all;
-    return before + run - v;
+    return before;
 }
 
 // The last s with start[s] <= i of an ascending start[0 .. n], for i < start[n].
@@ -71,70 +83,80 @@ __device__ __forceinline__ int owner(const int32_t *start, int n, int i) {
     return lo;
 }
 
-// Bound by its chain of dependent steps: count and lengths, two block sums, a search in LDS, a page, the stores.
-__global__ __launch_bounds__(kPlanThreads) void plan_chunk_kernel(PlanArgs A) {
+// Bound by its chain of dependent steps: count and lengths, a block sum, a search in LDS, a page, the stores. One
+// item a thread, the rows' blocks first, then the pages', then the sequences'.
+__global__ __launch_bounds__(kPlanThreads) void plan_chunk_kernel(PlanArgs A, int row_blocks, int page_blocks) {
     extern __shared__ int32_t plan_lds[];
-    __shared__ int64_t sums[kPlanThreads / 64];
     __shared__ int fit;
-    int32_t *start = plan_lds, *pages = plan_lds + A.seqs + 1;
+    int32_t *start = plan_lds, *pages = start + A.seqs + 1, *cached = pages + A.seqs + 1;
     const int t = threadIdx.x, per = (A.seqs + kPlanThreads - 1) / kPlanThreads;
     const int s0 = min(t * per, A.seqs), s1 = min(s0 + per, A.seqs);
     const int count = min(max(*A.count, 0), A.capacity);
     if (t == 0) fit = 0;
-    int64_t rows = 0, need = 0;
+    Pair mine{0, 0}, all;
     for (int s = s0; s < s1; ++s) {
         const Wish w = wish_of(A, s);
-        rows += w.rows;
-        need += w.need;
+        mine.rows += w.rows;
+        mine.pages += w.need;
+        cached[s] = w.cached;
     }
-    int64_t all;
-    int64_t r = block_before(rows, sums, &all), n = block_before(need, sums, &all);
-    int mine = 0;
+    Pair at = block_before(mine, &all);
+    int fits = 0;
     for (int s = s0; s < s1; ++s) {
         const Wish w = wish_of(A, s);
         // of a sequence that is not served nothing is read but whether it is
-        start[s] = (int)min(r, (int64_t)A.tokens);
-        pages[s] = (int)min(n, (int64_t)count);
-        r += w.rows;
-        n += w.need;
-        if (r <= A.tokens && n <= count) {
-            ++mine;
-            start[s + 1] = (int)r;  // the next thread writes the same, or is not served
-            pages[s + 1] = (int)n;
+        start[s] = (int)min(at.rows, (int64_t)A.tokens);
+        pages[s] = (int)min(at.pages, (int64_t)count);
+        at.rows += w.rows;
+        at.pages += w.need;
+        if (at.rows <= A.tokens && at.pages <= count) {
+            ++fits;
+            start[s + 1] = (int)at.rows;  // the next thread writes the same, or is not served
+            pages[s + 1] = (int)at.pages;
         }
     }
-    if (mine) atomicAdd(&fit, mine);
+    if (fits) atomicAdd(&fit, fits);
     __syncthreads();
     const int served = fit;
     const int total_rows = start[served], total_pages = pages[served], left = count - total_pages;
-    const int64_t stride = (int64_t)gridDim.x * kPlanThreads, first = (int64_t)blockIdx.x * kPlanThreads + t;
-    for (int64_t i = first; i < total_pages; i += stride) {
-        const int s = owner(pages, served, (int)i);
-        const Wish w = wish_of(A, s);
-        A.table[s * A.table_stride + w.held + ((int)i - pages[s])] = A.free_pages[left + i];
-    }
-    if (A.row_pos || A.row_slot || A.row_adapter)
-        for (int64_t i = first; i < A.tokens; i += stride) {
+    const int last = (1 << A.page_shift) - 1;
+    // where the new pages of served sequence s begin in its row of the table
+    auto first_new = [&](int s) {
+        const int then = (int)(((int64_t)cached[s] + (start[s + 1] - start[s]) + last) >> A.page_shift);
+        return then - (pages[s + 1] - pages[s]);
+    };
+    int block = blockIdx.x;
+    if (block < row_blocks) {
+        for (int64_t i = (int64_t)block * kPlanThreads + t; i < A.tokens; i += (int64_t)row_blocks * kPlanThreads) {
             int pos = -1, slot = -1, adapter = -2;
             if (i < total_rows) {
                 const int s = owner(start, served, (int)i);
-                const Wish w = wish_of(A, s);
-                pos = w.cached + ((int)i - start[s]);
-                adapter = A.seq_adapter ? A.seq_adapter[s] : -1;
+                adapter = A.seq_adapter && A.row_adapter ? A.seq_adapter[s] : -1;
+                pos = cached[s] + ((int)i - start[s]);
                 if (A.row_slot) {
-                    const int p = pos >> A.page_shift;
-                    const int page = p < w.held || p >= w.held + w.need ? A.table[s * A.table_stride + p]
-                                                                        : A.free_pages[left + pages[s] + (p - w.held)];
-                    if ((unsigned)page < (unsigned)A.num_pages)
-                        slot = (page << A.page_shift) + (pos & ((1 << A.page_shift) - 1));
+                    const int p = pos >> A.page_shift, from = first_new(s);
+                    // (a sequence's last page is its last new one, if it has any)
+                    const bool is_new = p >= from && pages[s + 1] > pages[s];
+                    const int page = is_new ? A.free_pages[left + pages[s] + (p - from)] : A.table[s * A.table_stride + p];
+                    if ((unsigned)page < (unsigned)A.num_pages) slot = (page << A.page_shift) + (pos & last);
                 }
             }
             if (A.row_pos) A.row_pos[i] = pos;
             if (A.row_slot) A.row_slot[i] = slot;
             if (A.row_adapter) A.row_adapter[i] = adapter;
         }
-    for (int64_t i = first; i < A.seqs; i += stride) {
-        const int s = (int)i;
+        return;
+    }
+    block -= row_blocks;
+    if (block < page_blocks) {
+        for (int64_t i = (int64_t)block * kPlanThreads + t; i < total_pages; i += (int64_t)page_blocks * kPlanThreads) {
+            const int s = owner(pages, served, (int)i);
+            A.table[s * A.table_stride + first_new(s) + ((int)i - pages[s])] = A.free_pages[left + i];
+        }
+        return;
+    }
+    block -= page_blocks;
+    for (int s = block * kPlanThreads + t; s < A.seqs; s += kPlanSeqs) {
         const Wish w = wish_of(A, s);
         const bool in = s < served;
         A.q_start[s + 1] = in ? start[s + 1] : total_rows;
@@ -142,7 +164,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_chunk_kernel(PlanArgs A) {
         if (A.held_out) A.held_out[s] = w.held + (in ? w.need : 0);
         if (A.last_row) A.last_row[s] = in && w.rows ? start[s + 1] - 1 : -1;
     }
-    if (first == 0) {
+    if (block == 0 && t == 0) {
         A.q_start[0] = 0;
         *A.free_left = left;
         *A.served = served;
@@ -164,23 +186,22 @@ __device__ __forceinline__ int2 range_of(const ReleaseArgs &A, int s) {
 
 __global__ __launch_bounds__(kPlanThreads) void release_pages_kernel(ReleaseArgs A) {
     extern __shared__ int32_t plan_lds[];
-    __shared__ int64_t sums[kPlanThreads / 64];
     int32_t *start = plan_lds;
     const int t = threadIdx.x, per = (A.seqs + kPlanThreads - 1) / kPlanThreads;
     const int s0 = min(t * per, A.seqs), s1 = min(s0 + per, A.seqs);
     const int count = min(max(*A.count, 0), A.capacity), room = A.capacity - count;
-    int64_t n = 0, all;
+    Pair n{0, 0}, all;
     for (int s = s0; s < s1; ++s) {
         const int2 r = range_of(A, s);
-        n += r.y - r.x;
+        n.pages += r.y - r.x;
     }
-    int64_t before = block_before(n, sums, &all);
+    int64_t before = block_before(n, &all).pages;
     for (int s = s0; s < s1; ++s) {
         const int2 r = range_of(A, s);
         start[s] = (int)min(before, (int64_t)room);
         before += r.y - r.x;
     }
-    const int total = (int)min(all, (int64_t)room);
+    const int total = (int)min(all.pages, (int64_t)room);
     if (t == 0) start[A.seqs] = total;
     __syncthreads();
     const int64_t stride = (int64_t)gridDim.x * kPlanThreads, first = (int64_t)blockIdx.x * kPlanThreads + t;
@@ -212,9 +233,9 @@ static int check_table(const char *who, const void *table, int table_pages, int6
     return G4_OK;
 }
 
-static unsigned plan_blocks(int64_t items) {
-    const int64_t n = (items + kPlanItems - 1) / kPlanItems;
-    return (unsigned)(n < 1 ? 1 : n > kPlanBlocks ? kPlanBlocks : n);
+static int plan_blocks(int64_t items) {
+    const int64_t n = (items + kPlanThreads - 1) / kPlanThreads;
+    return (int)(n < 1 ? 1 : n > kPlanBlocks ? kPlanBlocks : n);
 }
 
 }  // namespace g4
@@ -243,8 +264,12 @@ int g4_plan_chunk(const g4_free_pages *list, const int32_t *cached, const int32_
                table_stride ? table_stride : table_pages, q_start, kv_len, held_out, free_left, served, row_pos, row_slot,
                row_adapter, last_row, list->capacity, list->num_pages, __builtin_ctz(list->page_size), seqs, tokens, max_q,
                max_kv, table_pages};
-    const size_t lds = 2 * ((size_t)seqs + 1) * sizeof(int32_t);
-    hipLaunchKernelGGL(plan_chunk_kernel, dim3(plan_blocks(tokens)), dim3(kPlanThreads), lds, as_stream(stream), A);
+    const size_t lds = (3 * (size_t)seqs + 2) * sizeof(int32_t);
+    const bool per_row = row_pos || row_slot || row_adapter;
+    // a sequence's rows open a page each page_size of them, and one more; more pages (not held, though cached) go round
+    const int row_blocks = per_row ? plan_blocks(tokens) : 0, page_blocks = plan_blocks((int64_t)tokens / list->page_size + seqs);
+    hipLaunchKernelGGL(plan_chunk_kernel, dim3(row_blocks + page_blocks + plan_blocks(seqs)), dim3(kPlanThreads), lds,
+                       as_stream(stream), A, row_blocks, page_blocks);
     G4_LAUNCHED("plan_chunk_kernel");
     return G4_OK;
 }

@@ -54,7 +54,7 @@ __device__ __forceinline__ bool is_far(float x, const Cap &A) { return fabsf(x) 
 // 2^z: z = n + f, |f| <= 1/2, a polynomial in f (fitted like the softcap's, relative error 1.1e-12) and n into the
 // exponent; below 2^-1000 that (too small to count, and the exponent stays normal), and for a NaN.
 __device__ __forceinline__ double pow2(double z) {
-    z = z > -1000.0 ? z : -1000.0;
+    z = fmax(z, -1000.0);
     const double r = z + 0x1.8p52;  // n in the low word
     const double f = z - (r - 0x1.8p52);
     double e = 1.3259689002093833e-06;

@@ -21,8 +21,7 @@ typedef unsigned long long u64;
 constexpr int kSampleThreads = 256, kSampleWaves = kSampleThreads / 64;
 constexpr int kSampleUnit = 1024, kSamplePer = kSampleUnit / 64;  // a wave's range, and a lane's part of it
 constexpr int kSamplePart = kSampleWaves * kSampleUnit;
-constexpr int kWideThreads = 512, kWideWaves = kWideThreads / 64;  // of (2) and (3): a unit a wave
-constexpr int kBins = 1024, kBinsPer = kBins / kWideThreads;
+constexpr int kBins = 1024, kBinsPer = kBins / 64;
 constexpr int kList = 4096;  // entries; a row with more is read again
 constexpr int kFew = 64;     // entries that a wave orders by itself
 constexpr int kSub = 1024, kSubPer = kSub / kSampleThreads;  // ranges of one refinement step
@@ -59,7 +58,7 @@ struct SampleArgs {
     const float *top_p, *min_p, *u;
     CapArgs cap;
     int logit_rows, vocab, parts, units, shift, vec, cuts;  // cuts: top-k or top-p given
-    int spans;                   // blocks a row of (2) and (3)
+    int wide, spans;             // waves of a block of (2) and (3), a unit each, and blocks a row
     PartMax *stats;              // [rows][parts]
     Row *row;                    // [rows]
     Cuts *cut;                   // [rows]
@@ -84,7 +83,7 @@ __device__ __forceinline__ int unit_place(int j, int lane, int vec) {
     return vec ? (j / 4) * 256 + 4 * lane + j % 4 : j * 64 + lane;
 }
 
-// The lane's values of the wave's unit at x, `n` of which exist.
+// The lane's values of the wave's unit at x, `n` of which exist; a NaN is one.
 __device__ __forceinline__ void load_unit(const float *x, int n, int lane, int vec, float (&v)[kSamplePer]) {
     if (vec) {
 #pragma unroll
@@ -108,8 +107,6 @@ __device__ __forceinline__ void load_unit(const float *x, int n, int lane, int v
             v[j] = i < n ? x[i] : -INFINITY;
         }
     }
-#pragma unroll
-    for (int j = 0; j < kSamplePer; ++j) v[j] = clean(v[j]);
 }
 
 __device__ __forceinline__ void join_max(PartMax &a, float max, float min, int index) {
@@ -137,6 +134,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_max_kernel(SampleArgs A
         load_unit(x + base, A.vocab - base, lane, A.vec, v);
 #pragma unroll
         for (int j = 0; j < kSamplePer; ++j) {
+            v[j] = clean(v[j]);
             m.max = fmaxf(m.max, v[j]);
             m.min = fminf(m.min, v[j] > -INFINITY ? v[j] : INFINITY);
         }
@@ -213,7 +211,7 @@ __device__ __forceinline__ T uniform(const T &v) {
 // Under an infinite maximum a logit is as good as it, or nothing.
 __device__ __forceinline__ float seen(float x, const Row &R) { return R.inf ? (x == INFINITY ? 0.0f : -INFINITY) : x; }
 
-// y - top of a logit that is not past half the cap; for a -infinity that, or NaN.
+// y - top of a logit that is not past half the cap; for a NaN and a -infinity one of these two (no weight).
 template <bool CAP>
 __device__ __forceinline__ double near_distance(float x, const Row &R, const SampleArgs &A) {
     return (CAP ? near_cap((double)x, A.cap) : (double)x) - R.top;
@@ -228,9 +226,14 @@ __device__ __forceinline__ double distance(float x, const Row &R, const SampleAr
     }
     return y - R.top;
 }
+// The weight in steps (at most 2^51 and a little), rounded, above kNoSteps; its bits above kNoStepsBits are the integer.
+constexpr double kNoSteps = 0x1p52;
+constexpr u64 kNoStepsBits = 0x4330000000000000ull;
+__device__ __forceinline__ double raised_steps(double d, const Row &R, const SampleArgs &A) {
+    return pow2(__builtin_fma(d, R.slope, (double)A.shift)) + kNoSteps;
+}
 __device__ __forceinline__ u64 steps(double d, const Row &R, const SampleArgs &A) {
-    const double w = pow2(__builtin_fma(d, R.slope, (double)A.shift));  // at most 2^51 and a little
-    return (u64)__double_as_longlong(w + 0x1p52) & ((1ull << 52) - 1);
+    return (u64)__double_as_longlong(raised_steps(d, R, A)) - kNoStepsBits;
 }
 __device__ __forceinline__ int bin_of(double d, const Row &R) { return min(max((int)(-d * R.bins), 0), kBins - 1); }
 
@@ -270,16 +273,20 @@ __device__ __forceinline__ u64 block_run(u64 v, u64 *lds, u64 *total) {
     return before + v;
 }
 
-// Grid (spans, rows).
-template <bool CAP>
-__global__ __launch_bounds__(kWideThreads) void sample_weights_kernel(SampleArgs A) {
-    __shared__ u64 mass[kBins];
-    __shared__ uint32_t count[kBins];
-    __shared__ u64 ss[kWideWaves];
+struct Bin {
+    u64 mass;  // and kNoStepsBits for each token
+    uint32_t count, pad;
+};
+
+// Grid (spans, rows). Bound by issue: with a cap about 45 vector operations a logit, 27 of them 64-bit.
+template <bool CAP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void sample_weights_kernel(SampleArgs A) {
+    __shared__ Bin bins[kBins];
+    __shared__ u64 ss[WAVES];
     __shared__ Row shared_row;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, row = blockIdx.y;
     const float *x = row_of(A, row);
-    const int unit = blockIdx.x * kWideWaves + wave, base = unit * kSampleUnit;
+    const int unit = blockIdx.x * WAVES + wave, base = unit * kSampleUnit;
     float v[kSamplePer];
     load_unit(x + base, x ? A.vocab - base : 0, lane, A.vec, v);
     if (wave == 0) {  // once a block: as many operations as the weights of a unit
@@ -289,58 +296,71 @@ __global__ __launch_bounds__(kWideThreads) void sample_weights_kernel(SampleArgs
             if (blockIdx.x == 0) A.row[row] = R;
         }
     }
-    if (A.cuts) {
-#pragma unroll
-        for (int i = 0; i < kBinsPer; ++i) {
-            mass[i * kWideThreads + t] = 0;
-            count[i * kWideThreads + t] = 0;
-        }
-    }
+    if (A.cuts)
+        for (int i = t; i < kBins; i += 64 * WAVES) bins[i] = {0, 0, 0};
     __syncthreads();
     const Row R = uniform(shared_row);
     if (R.index < 0) return;
-    u64 all = 0, kept = 0;
-    auto add = [&](double d) {
-        const u64 w = steps(d, R, A);
-        all += w;
-        if (!R.filtered) {
-            kept += d >= R.d_min ? w : 0;
-        } else if (w) {
-            const int b = bin_of(d, R);
-            atomicAdd(&mass[b], w);
-            atomicAdd(&count[b], 1u);
-        }
-    };
-    uint32_t far = 0;  // few: past half the cap, one at a time
+    if (R.inf) {
 #pragma unroll
-    for (int j = 0; j < kSamplePer; ++j) {
-        const float xs = seen(v[j], R);
-        const bool f = CAP && is_far(xs, A.cap);
-        far |= f ? 1u << j : 0u;
-        add(f ? -INFINITY : near_distance<CAP>(xs, R, A));
+        for (int j = 0; j < kSamplePer; ++j) v[j] = seen(v[j], R);
     }
-    if (CAP)
-        for (; far; far &= far - 1) add(distance<CAP>(x[base + unit_place(__ffs(far) - 1, lane, A.vec)], R, A));
-    all = wave_sum(all);
-    if (lane == 0) ss[wave] = all;
-    if (!R.filtered) {
+    auto each = [&](auto add) {
+        uint32_t far = 0;  // places where a lane's logit is past half the cap: few, one at a time
+#pragma unroll
+        for (int j = 0; j < kSamplePer; ++j) {
+            float xs = v[j];
+            if (CAP) {
+                const bool f = is_far(xs, A.cap);
+                far |= __any(f) ? 1u << j : 0u;
+                xs = f ? -INFINITY : xs;
+            }
+            add(near_distance<CAP>(xs, R, A));
+        }
+        if (CAP)
+            for (; far; far &= far - 1) {
+                const int i = base + unit_place(__ffs(far) - 1, lane, A.vec);
+                const float xs = i < A.vocab ? x[i] : -INFINITY;
+                if (is_far(xs, A.cap)) add(distance<CAP>(xs, R, A));
+            }
+    };
+    u64 all = 0;
+    if (R.filtered) {
+        each([&](double d) {
+            const double w = raised_steps(d, R, A);
+            if (w > kNoSteps) {
+                Bin &b = bins[bin_of(d, R)];
+                atomicAdd(&b.mass, (u64)__double_as_longlong(w));
+                atomicAdd(&b.count, 1u);
+            }
+        });
+        __syncthreads();
+        for (int i = t; i < kBins; i += 64 * WAVES) {
+            const Bin b = bins[i];
+            if (!b.count) continue;
+            const u64 m = b.mass - b.count * kNoStepsBits;
+            all += m;
+            atomicAdd(&A.bin_mass[(int64_t)row * kBins + i], m);
+            atomicAdd(&A.bin_count[(int64_t)row * kBins + i], b.count);
+        }
+        all = wave_sum(all);
+    } else {
+        u64 kept = 0;
+        each([&](double d) {
+            const u64 w = steps(d, R, A);
+            all += w;
+            kept += d >= R.d_min ? w : 0;
+        });
+        all = wave_sum(all);
         kept = wave_sum(kept);
         if (lane == 0 && unit < A.units) A.unit_sums[(int64_t)row * A.units + unit] = kept;
     }
+    if (lane == 0) ss[wave] = all;
     __syncthreads();
-    if (t == 0) {
+    if (t) return;
 #pragma unroll
-        for (int w = 1; w < kWideWaves; ++w) all += ss[w];
-        A.span_sums[(int64_t)row * A.spans + blockIdx.x] = all;
-    }
-    if (!R.filtered) return;
-#pragma unroll
-    for (int i = 0; i < kBinsPer; ++i) {
-        const int b = i * kWideThreads + t;
-        if (!count[b]) continue;
-        atomicAdd(&A.bin_mass[(int64_t)row * kBins + b], mass[b]);
-        atomicAdd(&A.bin_count[(int64_t)row * kBins + b], count[b]);
-    }
+    for (int w = 1; w < WAVES; ++w) all += ss[w];
+    A.span_sums[(int64_t)row * A.spans + blockIdx.x] = all;
 }
 
 // A token is kept while the weight before it is under p * total: while it is under this.
@@ -360,72 +380,109 @@ __device__ __forceinline__ float least_of(const SampleArgs &A, const Row &R, int
     return z - 1e-3f * (fabsf(z) + cap);
 }
 
-// Grid (spans, rows): every block finds the bins of its row's cuts, then weighs its tokens above them.
-template <bool CAP>
-__global__ __launch_bounds__(kWideThreads) void sample_cut_kernel(SampleArgs A) {
-    __shared__ u64 sums[kWideWaves];
-    __shared__ Cuts C;
-    __shared__ u64 k_after;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, row = blockIdx.y;
-    const Row R = uniform(A.row[row]);
-    if (!R.filtered) return;  // (a row without a logit, too)
-    const float *x = row_of(A, row);
-    const int unit = blockIdx.x * kWideWaves + wave, base = unit * kSampleUnit;
-    u64 m[kBinsPer], n[kBinsPer], m_sum = 0, n_sum = 0;
+// Inclusive sum over a wave's lanes.
+template <class T>
+__device__ __forceinline__ T wave_run(T v) {
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        const T o = __shfl_up(v, s);
+        if ((int)(threadIdx.x & 63) >= s) v += o;
+    }
+    return v;
+}
+
+// The bins of a row's cuts, by one wave, the same in every lane; a lane has 16 bins.
+__device__ __forceinline__ Cuts find_cuts(const SampleArgs &A, const Row &R, int row) {
+    const int lane = threadIdx.x & 63;
+    const u64 *mass = A.bin_mass + (int64_t)row * kBins + lane * kBinsPer;
+    const uint32_t *count = A.bin_count + (int64_t)row * kBins + lane * kBinsPer;
+    u64 m[kBinsPer], m_sum = 0;
+    uint32_t n[kBinsPer], n_sum = 0;
 #pragma unroll
     for (int i = 0; i < kBinsPer; ++i) {
-        m[i] = A.bin_mass[(int64_t)row * kBins + t * kBinsPer + i];
-        n[i] = A.bin_count[(int64_t)row * kBins + t * kBinsPer + i];
+        m[i] = mass[i];
+        n[i] = count[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kBinsPer; ++i) {
         m_sum += m[i];
         n_sum += n[i];
     }
-    if (t == 0) {
-        C = {kBins, kBins, kBins, 0, 0, 0, 0.0f, 0.0f};
-        k_after = 0;
-    }
-    u64 m_all, n_all;
-    const u64 m_first = block_run<kWideThreads>(m_sum, sums, &m_all) - m_sum;
-    const u64 n_first = block_run<kWideThreads>(n_sum, sums, &n_all) - n_sum;
-    const bool by_k = R.k > 0 && (u64)R.k < n_all;
+    const u64 m_run = wave_run(m_sum), m_all = __shfl(m_run, 63), m_first = m_run - m_sum;
+    const uint32_t n_run = wave_run(n_sum), n_all = __shfl(n_run, 63), n_first = n_run - n_sum;
+    Cuts C{kBins, kBins, kBins, 0, 0, 0, 0.0f, 0.0f};
+    const bool by_k = R.k > 0 && (uint32_t)R.k < n_all;
+    u64 low_total = m_all, high_total = m_all;
     if (by_k) {
-        u64 mb = m_first, nb = n_first;
+        const uint32_t k = R.k;
+        const bool mine = n_first < k && k <= n_run;  // one lane
+        int bin = 0, rest = 0;
+        u64 mb = m_first, before = 0, after = 0;
+        uint32_t nb = n_first;
 #pragma unroll
         for (int i = 0; i < kBinsPer; ++i) {
-            if (nb < (u64)R.k && (u64)R.k <= nb + n[i]) {
-                C.k_bin = t * kBinsPer + i;
-                C.k_rest = R.k - (int)nb;
-                C.k_before = mb;
-                k_after = mb + m[i];
+            if (nb < k && k <= nb + n[i]) {
+                bin = lane * kBinsPer + i;
+                rest = (int)(k - nb);
+                before = mb;
+                after = mb + m[i];
             }
             mb += m[i];
             nb += n[i];
         }
+        const int at = __ffsll((long long)__ballot(mine)) - 1;
+        C.k_bin = __shfl(bin, at);
+        C.k_rest = __shfl(rest, at);
+        C.k_before = low_total = __shfl(before, at);
+        high_total = __shfl(after, at);
+        C.p_low = C.p_high = C.k_bin;
     }
-    __syncthreads();
     if (R.p < 1.0) {
         // the weight that top-k leaves lies between that above its bin and that with it
-        const u64 low = mass_target(R.p, by_k ? C.k_before : m_all), high = mass_target(R.p, by_k ? k_after : m_all);
-        u64 mb = m_first;
+        const u64 low = mass_target(R.p, low_total), high = mass_target(R.p, high_total);
+        int low_bin = 0, high_bin = 0;
+        u64 mb = m_first, before = 0;
 #pragma unroll
         for (int i = 0; i < kBinsPer; ++i) {
             if (mb < low && low <= mb + m[i]) {
-                C.p_low = t * kBinsPer + i;
-                C.p_before = mb;
+                low_bin = lane * kBinsPer + i;
+                before = mb;
             }
-            if (mb < high && high <= mb + m[i]) C.p_high = t * kBinsPer + i;
+            if (mb < high && high <= mb + m[i]) high_bin = lane * kBinsPer + i;
             mb += m[i];
         }
-    } else if (by_k && t == 0) {
-        C.p_low = C.p_high = C.k_bin;
+        const int low_at = __ffsll((long long)__ballot(m_first < low && low <= m_run)) - 1;
+        const int high_at = __ffsll((long long)__ballot(m_first < high && high <= m_run)) - 1;
+        C.p_low = __shfl(low_bin, low_at);
+        C.p_before = __shfl(before, low_at);
+        C.p_high = __shfl(high_bin, high_at);
+    }
+    C.least = least_of(A, R, max(C.p_high, by_k ? C.k_bin : 0));
+    return C;
+}
+
+// Grid (spans, rows): every block finds the bins of its row's cuts, then weighs its tokens above them.
+template <bool CAP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void sample_cut_kernel(SampleArgs A) {
+    __shared__ Cuts shared_cuts;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.y;
+    const int unit = blockIdx.x * WAVES + wave, base = unit * kSampleUnit;
+    const float top = unit < A.units ? A.unit_max[(int64_t)row * A.units + unit] : -INFINITY;
+    const Row R = uniform(A.row[row]);
+    if (!R.filtered) return;  // (a row without a logit, too)
+    const float *x = row_of(A, row);
+    if (wave == 0) {
+        const Cuts C = find_cuts(A, R, row);
+        if (lane == 0) {
+            shared_cuts = C;
+            if (blockIdx.x == 0) A.cut[row] = C;
+        }
     }
     __syncthreads();
-    Cuts c = uniform(C);
-    const int behind = max(c.p_high, c.k_bin < kBins ? c.k_bin : 0);
-    c.least = uniform(least_of(A, R, behind));
-    if (blockIdx.x == 0 && t == 0) A.cut[row] = c;
+    const Cuts c = uniform(shared_cuts);
     if (unit >= A.units) return;
     u64 sure = 0;
-    if (A.unit_max[(int64_t)row * A.units + unit] >= c.least) {
+    if (top >= c.least) {
         float v[kSamplePer];
         load_unit(x + base, A.vocab - base, lane, A.vec, v);
         uint32_t look = 0, in = 0;  // elements that may be in these bins, and those for the list
@@ -435,7 +492,7 @@ __global__ __launch_bounds__(kWideThreads) void sample_cut_kernel(SampleArgs A) 
 #pragma unroll
         for (int j = 0; j < kSamplePer; ++j) {
             if (!__any(look >> j & 1)) continue;
-            const float xs = seen(v[j], R);
+            const float xs = seen(clean(v[j]), R);
             const double d = distance<CAP>(xs, R, A);
             const u64 w = xs > -INFINITY ? steps(d, R, A) : 0;
             const int b = bin_of(d, R);
@@ -766,11 +823,13 @@ template <bool CAP>
 static int launch_sample(const SampleArgs &A, int rows, hipStream_t s) {
     hipLaunchKernelGGL(sample_max_kernel, dim3(A.parts, rows), dim3(kSampleThreads), 0, s, A);
     G4_LAUNCHED("sample_max_kernel");
-    const dim3 grid(A.spans, rows);
-    hipLaunchKernelGGL(sample_weights_kernel<CAP>, grid, dim3(kWideThreads), 0, s, A);
+    const dim3 grid(A.spans, rows), block(64 * A.wide);
+    if (A.wide == 4) hipLaunchKernelGGL((sample_weights_kernel<CAP, 4>), grid, block, 0, s, A);
+    else hipLaunchKernelGGL((sample_weights_kernel<CAP, 8>), grid, block, 0, s, A);
     G4_LAUNCHED("sample_weights_kernel");
     if (A.cuts) {
-        hipLaunchKernelGGL(sample_cut_kernel<CAP>, grid, dim3(kWideThreads), 0, s, A);
+        if (A.wide == 4) hipLaunchKernelGGL((sample_cut_kernel<CAP, 4>), grid, block, 0, s, A);
+        else hipLaunchKernelGGL((sample_cut_kernel<CAP, 8>), grid, block, 0, s, A);
         G4_LAUNCHED("sample_cut_kernel");
     }
     hipLaunchKernelGGL(sample_pick_kernel<CAP>, dim3(rows), dim3(kSampleThreads), 0, s, A);
@@ -834,7 +893,10 @@ int g4_sample_tokens(const float *logits, int logit_rows, int64_t logit_stride, 
     A.shift = 62 - bits < 51 ? 62 - bits : 51;
     A.vec = A.stride % 4 == 0 && ((uintptr_t)logits & 15) == 0;
     A.cuts = top_k || top_p;
-    A.spans = (A.units + kWideWaves - 1) / kWideWaves;  // at most parts
+    // 8 waves share a block's fixed work, the row's parameters, its histogram and its cuts; where that leaves CUs
+    // without a block, 4 have a SIMD each
+    A.wide = (int64_t)rows * ((A.units + 7) / 8) >= device_cu_count() ? 8 : 4;
+    A.spans = (A.units + A.wide - 1) / A.wide;  // at most parts
     A.stats = static_cast<PartMax *>(workspace);
     A.row = reinterpret_cast<Row *>(A.stats + (int64_t)rows * A.parts);
     A.cut = reinterpret_cast<Cuts *>(A.row + rows);

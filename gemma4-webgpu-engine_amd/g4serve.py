@@ -99,7 +99,18 @@ def _call_device(pages, chunk) -> int:
 
 
 def _packed(x, what, kinds, shape, device):
-    """The address of a contiguous operand of one of `kinds` and of `shape`."""
+    """The address of a contiguous operand of one of `kinds` and of `shape`. A call has up to 14 of them: what is in
+    order is found so by five questions, and what is not is named by _checked."""
+    try:
+        if (x.get_device() == device and _one_runtime and _kinds[x.dtype] in kinds and x.shape == shape
+                and x.is_contiguous()):
+            return x.data_ptr()
+    except (AttributeError, KeyError):  # a DeviceBuffer, or a type not met yet
+        pass
+    return _checked(x, what, kinds, shape, device)
+
+
+def _checked(x, what, kinds, shape, device):
     if _kind(x) not in kinds:
         raise g4.G4Error(1, f"{what} cannot be {x.dtype}")
     if x.shape != shape:
@@ -119,6 +130,11 @@ def _need_contiguous(x, what):
 
 def _workspace(x, device):
     """(address, bytes) of a workspace. One that is not contiguous may hold fewer bytes than it counts."""
+    try:
+        if x.get_device() == device and _one_runtime and x.is_contiguous():
+            return x.data_ptr(), x.nbytes
+    except AttributeError:
+        pass
     _need_contiguous(x, "the workspace")
     return _address(x, "workspace", device), x.nbytes
 
@@ -392,17 +408,23 @@ def plan_chunk(free, cached, rows, page_table, q_start, kv_len, free_left, serve
     device = _device()
     _need_device(free, device, "the free pages")
     at, seqs, width, stride = _table(page_table, device)
-    per_seq = [_optional(x, what, _I32, (seqs,), device) for x, what in (
-        (cached, "cached"), (rows, "rows"), (held, "held"), (seq_adapter, "seq_adapter"))]
-    per_row = [_optional(x, what, _I32, (tokens,), device) for x, what in (
-        (row_pos, "row_pos"), (row_slot, "row_slot"), (row_adapter, "row_adapter"))]
+    each, row, one = (seqs,), (tokens,), (1,)
     st = g4.lib().g4_plan_chunk(
-        free.ref, *per_seq, seqs, tokens, max_q, max_kv, at, width, stride, _packed(q_start, "q_start", _I32, (seqs + 1,), device),
-        _packed(kv_len, "kv_len", _I32, (seqs,), device), _optional(held_out, "held_out", _I32, (seqs,), device),
-        _packed(free_left, "free_left", _I32, (1,), device), _packed(served, "served", _I32, (1,), device), *per_row,
-        _optional(last_row, "last_row", _I32, (seqs,), device),
-        _stream(stream, device, *free.buffers, cached, rows, held, seq_adapter, page_table, q_start, kv_len, held_out, free_left,
-                served, row_pos, row_slot, row_adapter, last_row))
+        free.ref,
+        cached if cached is None else _packed(cached, "cached", _I32, each, device),
+        rows if rows is None else _packed(rows, "rows", _I32, each, device),
+        held if held is None else _packed(held, "held", _I32, each, device),
+        seq_adapter if seq_adapter is None else _packed(seq_adapter, "seq_adapter", _I32, each, device),
+        seqs, tokens, max_q, max_kv, at, width, stride,
+        _packed(q_start, "q_start", _I32, (seqs + 1,), device), _packed(kv_len, "kv_len", _I32, each, device),
+        held_out if held_out is None else _packed(held_out, "held_out", _I32, each, device),
+        _packed(free_left, "free_left", _I32, one, device), _packed(served, "served", _I32, one, device),
+        row_pos if row_pos is None else _packed(row_pos, "row_pos", _I32, row, device),
+        row_slot if row_slot is None else _packed(row_slot, "row_slot", _I32, row, device),
+        row_adapter if row_adapter is None else _packed(row_adapter, "row_adapter", _I32, row, device),
+        last_row if last_row is None else _packed(last_row, "last_row", _I32, each, device),
+        _stream(stream, device, page_table, q_start, kv_len, free_left, served, cached, rows, held, seq_adapter, held_out,
+                row_pos, row_slot, row_adapter, last_row, *free.buffers))
     if st:
         g4._check(st)
 
@@ -477,6 +499,12 @@ def adapter_workspace_bytes(adapters, tokens) -> int:
 
 def _matrix(x, what, tokens, width, device):
     """(address, kind, elements between rows) of [tokens][width], whose rows may lie apart."""
+    try:
+        if (x.get_device() == device and _one_runtime and x.shape == (tokens, width) and x.is_contiguous()
+                and _kinds[x.dtype] in _X_KINDS):
+            return x.data_ptr(), _kinds[x.dtype], width
+    except (AttributeError, KeyError):
+        pass
     kind = _kind(x)
     if kind not in _X_KINDS:
         raise g4.G4Error(1, f"{what} cannot be {x.dtype}")

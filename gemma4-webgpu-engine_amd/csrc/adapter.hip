@@ -2,10 +2,12 @@
 //   out[t] = base[t] + scale_a (x[t] A_a^T) B_a^T.
 //
 // The rows are grouped by adapter once a step (adapter_groups_kernel): a tile is up to 16 rows of one adapter, so that
-// a matrix instruction's other operand is that adapter's. Two launches a linear: (1) H = x A^T, a block per tile and
-// range of K, partial sums in f32; (2) out = base + scale H B^T, a block per tile and range of N, which adds up H's
-// partial sums. Both products transposed, the adapter's rows by the batch's: a lane then holds four consecutive
-// outputs of one row. Operands come straight from global memory, each used by one wave.
+// a matrix instruction's other operand is that adapter's. Both products are transposed, the adapter's rows by the
+// batch's: what a lane holds of H = x A^T, four ranks of one row, is its operand of the second product, and there it has
+// runs of consecutive outputs of one row. Operands come straight from global memory, each used by one wave.
+//
+// Few rows: one launch, every block computes its tile's H for itself. Many: H in f32 by tile pair and range of K, then
+// a block per tile and range of outputs, which adds up H's parts.
 #include "g4_internal.h"
 #include "../../include/g4serve.h"
 
@@ -15,18 +17,23 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
-constexpr int kAdThreads = 256, kAdWaves = 4;
 constexpr int kTile = 16;          // rows of a tile
-constexpr int kMaxRank = 128, kMaxAdapters = 4096;
+constexpr int kMaxRank = 128, kMaxAdapters = 4096, kMaxK = 1 << 23;  // an adapter's A has less than 2^31 elements
 constexpr int kMaxTokens = 1 << 19;  // a grid has a row of blocks per tile
 constexpr int kGroupThreads = 1024;
+// What blocks of a single launch may read of x and A together, over and over, from the L2s: up to there it takes less
+// than the second launch and H's way through memory.
+constexpr int64_t kFusedBytes = 24 << 20;
+// And the matrix unit's time for a block's H in cycles of a SIMD; exact f32 products take 16 times that of f16.
+constexpr int64_t kFusedCycles = 5000;
 
-// groups: the header, the tiles, then the rows by adapter.
+// groups: the header, then the tiles.
 struct GroupHeader {
     int tiles, tokens, adapters, pad;
 };
 struct GroupTile {
-    int adapter, first, rows, pad;  // adapter -1: none; rows order[first ..]
+    int adapter, first, rows, pad;  // adapter -1: none; first: rows in the tiles before it
+    int row[kTile];                 // here and not in a list of their own: a load less on every block's way
 };
 
 static int64_t max_tiles(int64_t tokens, int64_t adapters) {
@@ -34,33 +41,46 @@ static int64_t max_tiles(int64_t tokens, int64_t adapters) {
 }
 static_assert(kMaxTokens / kTile + kMaxAdapters + 1 <= 65535, "tiles of a grid");
 static size_t groups_bytes_of(int64_t tokens, int64_t adapters) {
-    return sizeof(GroupHeader) + max_tiles(tokens, adapters) * sizeof(GroupTile) + tokens * sizeof(int32_t);
+    return sizeof(GroupHeader) + max_tiles(tokens, adapters) * sizeof(GroupTile);
 }
 
 // One block. Where a row stands in its group changes no result.
 __global__ __launch_bounds__(kGroupThreads) void adapter_groups_kernel(const int32_t *row_adapter, int tokens, int adapters,
-                                                                       GroupHeader *header, GroupTile *tiles,
-                                                                       int32_t *order) {
-    extern __shared__ int32_t group_lds[];  // [adapters + 1] counts, then places; group 0: no adapter
+                                                                       GroupHeader *header, GroupTile *tiles) {
+    extern __shared__ int32_t group_lds[];  // group 0: no adapter
     __shared__ int2 sums[kGroupThreads / 64];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, groups = adapters + 1;
-    for (int i = t; i < groups; i += kGroupThreads) group_lds[i] = 0;
+    int32_t *count = group_lds, *first_tile = group_lds + groups;
+    for (int i = t; i < groups; i += kGroupThreads) count[i] = 0;
     __syncthreads();
     auto group_of = [&](int row) {
         const int a = row < tokens ? row_adapter[row] : -2;
         return a == -2 ? -1 : (unsigned)a < (unsigned)adapters ? a + 1 : 0;
     };
-    for (int row = t; row < tokens; row += kGroupThreads) {
-        const int g = group_of(row);
-        if (g >= 0) atomicAdd(&group_lds[g], 1);
-    }
+    // a wave's rows of one group are counted together, and stand together
+    auto place = [&](int g) {
+        int mine = 0;
+        unsigned long long left = __ballot(g >= 0);
+        while (left) {
+            const int leader = __ffsll((long long)left) - 1;
+            const unsigned long long same = __ballot(g == __shfl(g, leader));
+            if (same >> lane & 1) {
+                int at = 0;
+                if (lane == leader) at = atomicAdd(&count[g], (int)__popcll(same));
+                mine = __shfl(at, leader) + __popcll(same & ((1ull << lane) - 1));
+            }
+            left &= ~same;
+        }
+        return mine;
+    };
+    for (int row = t; row - lane < tokens; row += kGroupThreads) place(group_of(row));
     __syncthreads();
-    // every group's first row and first tile; a thread has a run of groups
+    // every group's first tile and first row; a thread has a run of groups
     const int per = (groups + kGroupThreads - 1) / kGroupThreads, g0 = min(t * per, groups), g1 = min(g0 + per, groups);
     int2 mine = make_int2(0, 0);
     for (int g = g0; g < g1; ++g) {
-        mine.x += group_lds[g];
-        mine.y += (group_lds[g] + kTile - 1) / kTile;
+        mine.x += count[g];
+        mine.y += (count[g] + kTile - 1) / kTile;
     }
     int2 run = mine;
 #pragma unroll
@@ -83,28 +103,22 @@ __global__ __launch_bounds__(kGroupThreads) void adapter_groups_kernel(const int
         all += sums[w].y;
     }
     for (int g = g0; g < g1; ++g) {
-        const int n = group_lds[g];
-        group_lds[g] = at.x;
-        for (int i = 0; i < n; i += kTile) tiles[at.y++] = {g - 1, at.x + i, min(n - i, kTile), 0};
+        const int n = count[g];
+        count[g] = 0;
+        first_tile[g] = at.y;
+        for (int i = 0; i < n; i += kTile) {
+            GroupTile &T = tiles[at.y++];
+            T.adapter = g - 1;
+            T.first = at.x + i;
+            T.rows = min(n - i, kTile);
+        }
         at.x += n;
     }
     if (t == 0) *header = {all, tokens, adapters, 0};
     __syncthreads();
     for (int row = t; row - lane < tokens; row += kGroupThreads) {
-        const int g = group_of(row);
-        // a wave's rows of one group stand together
-        unsigned long long left = __ballot(g >= 0);
-        while (left) {
-            const int leader = __ffsll((long long)left) - 1;
-            const unsigned long long same = __ballot(g == __shfl(g, leader));
-            if (same >> lane & 1) {
-                int place = 0;
-                if (lane == leader) place = atomicAdd(&group_lds[g], (int)__popcll(same));
-                place = __shfl(place, leader);
-                order[place + __popcll(same & ((1ull << lane) - 1))] = row;
-            }
-            left &= ~same;
-        }
+        const int g = group_of(row), i = place(g);
+        if (g >= 0) tiles[first_tile[g] + i / kTile].row[i % kTile] = row;
     }
 }
 
@@ -116,22 +130,31 @@ struct AdapterArgs {
     int max_rank, rank16, k, n, tokens, count;  // rank16: max_rank in whole 16s, H's row
     const GroupHeader *header;
     const GroupTile *tiles;
-    const int32_t *order;
-    const void *x;
-    int64_t x_stride;
-    const void *base;
-    int64_t base_stride;
-    float x_scale, base_scale, out_scale;
+    const void *x, *base;
     void *out;
-    int64_t out_stride;
-    int splits, range, vec;  // K in `splits` ranges of `range`; vec: four outputs may be moved at once
-    float *h;                // [splits][tokens][rank16]
+    int64_t x_stride, base_stride, out_stride;
+    float x_scale, base_scale, out_scale;
+    int base_kind, out_kind;
+    int splits, k_range, n_range, vec;  // K in `splits` ranges; vec: eight outputs may be moved at once
+    float *h;                           // [splits][tokens][rank16]
 };
 
 // How many tiles there are: none in groups of another batch, whose rows are not these.
 __device__ __forceinline__ int tiles_of(const AdapterArgs &A) {
     const GroupHeader h = *A.header;
     return h.tokens == A.tokens && h.adapters == A.count ? h.tiles : 0;
+}
+
+// What a block needs to know of a tile; there is room for every block's, also where there are fewer tiles.
+struct Tile {
+    int index, adapter, first, rows;
+};
+__device__ __forceinline__ Tile tile_of(const AdapterArgs &A, int index) {
+    const GroupTile &T = A.tiles[index];
+    return {index, T.adapter, T.first, T.rows};
+}
+__device__ __forceinline__ int64_t row_of(const AdapterArgs &A, const Tile &T, int col) {
+    return A.tiles[T.index].row[min(col, T.rows - 1)];
 }
 
 __device__ __forceinline__ int rank_of(const AdapterArgs &A, int adapter) {
@@ -177,227 +200,422 @@ __device__ __forceinline__ f4 product<G4_KIND_F32>(h8 a, const XLoad<G4_KIND_F32
     return c;
 }
 
-// Grid (splits, tiles): a range of K of a tile's H; the block's waves take steps of 32 in turn and add up in LDS. RT:
-// the pool's rank in tiles of 16.
-template <int XK, int RT>
-__global__ __launch_bounds__(kAdThreads) void adapter_shrink_kernel(AdapterArgs A) {
-    __shared__ f4 part[kAdWaves][RT][64];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 15, group = lane >> 4;
-    if ((int)blockIdx.y >= tiles_of(A)) return;
-    const GroupTile T = A.tiles[blockIdx.y];
-    if (T.adapter < 0) return;
-    const int rank = rank_of(A, T.adapter);
-    const int64_t row = A.order[T.first + min(col, T.rows - 1)];
-    const _Float16 *a = A.a + T.adapter * A.a_stride;
-    f4 acc[RT];
+// Steps of shrink that are loaded at once: what 150 registers hold (less what else is on its way), at most 8.
+constexpr int unroll_of(int xk, int rt, int mt, int less) {
+    const int step = mt * (xk == G4_KIND_F32 ? 8 : 4) + 4 * rt, n = (150 - less) / step;
+    return n < 1 ? 1 : n > 8 ? 8 : n;
+}
+
+// acc[i][r] += the products over the wave's part of [k0, k1), a run of whole lines of the rows, in steps of 32: tile i's
+// rows by A's rows 16 r ..; RT: the pool's rank in tiles. UNROLL steps are loaded before the first is used; rows of A
+// behind the adapter's rank are loaded, so that the rank comes with them and not before, and replaced.
+template <int XK, int RT, int MT, int WAVES, int UNROLL>
+__device__ __forceinline__ void shrink(const AdapterArgs &A, const _Float16 *a, int rank, const int64_t (&row)[MT], int k0,
+                                       int k1, int wave, f4 (&acc)[MT][RT]) {
+    const int lane = threadIdx.x & 63, col = lane & 15, group = lane >> 4;
+    const int part = ((k1 - k0 + WAVES - 1) / WAVES + 63) / 64 * 64, from = k0 + wave * part, end = min(from + part, k1);
+#pragma unroll 1
+    for (int k = from; k < end; k += 32 * UNROLL) {
+        XLoad<XK> x[UNROLL][MT];
+        h8 w[UNROLL][RT];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) acc[r] = f4{};
-    const int k0 = blockIdx.x * A.range, k1 = min(k0 + A.range, A.k);
-    for (int k = k0 + 32 * wave; k < k1; k += 32 * kAdWaves) {
-        const int at = k + 8 * group;
-        const bool in = at < k1;
-        XLoad<XK> x;
-        x.load(A.x, row * A.x_stride + at, in);
+        for (int u = 0; u < UNROLL; ++u) {
+            const int at = k + 32 * u + 8 * group;
+            const bool in = at < end;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            h8 w{};
-            if (in && 16 * r + col < rank) w = *reinterpret_cast<const h8 *>(a + (int64_t)(16 * r + col) * A.k + at);
-            acc[r] = product<XK>(w, x, acc[r]);
+            for (int i = 0; i < MT; ++i) x[u][i].load(A.x, row[i] * A.x_stride + at, in);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                w[u][r] = h8{};
+                if (in && 16 * r + col < A.max_rank) w[u][r] = *reinterpret_cast<const h8 *>(a + (16 * r + col) * A.k + at);
+            }
         }
-    }
 #pragma unroll
-    for (int r = 0; r < RT; ++r) part[wave][r][lane] = acc[r];
-    __syncthreads();
-    for (int i = t; i < RT * 64; i += kAdThreads) {
-        const int r = i >> 6, l = i & 63;
-        f4 s = part[0][r][l];
+        for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
-        for (int w = 1; w < kAdWaves; ++w) s += part[w][r][l];
-        if ((l & 15) < T.rows)
-            *reinterpret_cast<f4 *>(A.h + ((int64_t)blockIdx.x * A.tokens + T.first + (l & 15)) * A.rank16 + 16 * r +
-                                    4 * (l >> 4)) = s;
+            for (int r = 0; r < RT; ++r) {
+                const h8 v = 16 * r + col < rank ? w[u][r] : h8{};
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[i][r] = product<XK>(v, x[u][i], acc[i][r]);
+            }
     }
 }
 
-template <int KIND>
-__device__ __forceinline__ f4 load4(const void *p, int64_t at, int n, bool vec, float scale) {
-    f4 y{};
-    if (KIND == G4_KIND_I8) {
-        const int8_t *q = static_cast<const int8_t *>(p) + at;
+__device__ __forceinline__ f4 multiply(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f4 multiply(h4 a, h4 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
+
+// Eight consecutive elements of a row of `kind`, `n` of which exist (one at least), as they come: packed (vec), or each in
+// a word of its own. Nothing waits for them here.
+struct Raw8 {
+    u32x4 a, b;  // whole vectors in every branch: an array that branches fill in part would be kept in memory
+    __device__ __forceinline__ void load(const void *p, int kind, int64_t at, int n, bool vec) {
+        b = u32x4{};
         if (vec) {
-            const uint32_t c = *reinterpret_cast<const uint32_t *>(q);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = (float)(int8_t)(c >> (8 * e)) * scale;
+            if (kind == G4_KIND_F32) {
+                const u32x4 *q = reinterpret_cast<const u32x4 *>(static_cast<const float *>(p) + at);
+                a = q[0];
+                b = q[1];
+            } else if (kind == G4_KIND_F16) {
+                a = *reinterpret_cast<const u32x4 *>(static_cast<const _Float16 *>(p) + at);
+            } else {
+                const uint2 c = *reinterpret_cast<const uint2 *>(static_cast<const int8_t *>(p) + at);
+                a = u32x4{c.x, c.y, 0, 0};
+            }
+        } else if (kind == G4_KIND_F32) {
+            words(static_cast<const uint32_t *>(p) + at, n);
+        } else if (kind == G4_KIND_F16) {
+            words(static_cast<const uint16_t *>(p) + at, n);
         } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e < n) y[e] = (float)q[e] * scale;
-        }
-    } else if (KIND == G4_KIND_F16) {
-        const _Float16 *q = static_cast<const _Float16 *>(p) + at;
-        if (vec) {
-            const h4 c = *reinterpret_cast<const h4 *>(q);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = (float)c[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e < n) y[e] = (float)q[e];
-        }
-    } else {
-        const float *q = static_cast<const float *>(p) + at;
-        if (vec) {
-            y = *reinterpret_cast<const f4 *>(q);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e < n) y[e] = q[e];
+            words(static_cast<const uint8_t *>(p) + at, n);
         }
     }
-    return y;
-}
+    template <class T>
+    __device__ __forceinline__ void words(const T *p, int n) {
+        a = u32x4{p[0], p[min(1, n - 1)], p[min(2, n - 1)], p[min(3, n - 1)]};
+        b = u32x4{p[min(4, n - 1)], p[min(5, n - 1)], p[min(6, n - 1)], p[min(7, n - 1)]};
+    }
+    __device__ __forceinline__ void values(int kind, bool vec, float scale, float (&y)[8]) const {
+        if (kind == G4_KIND_F32) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(e < 4 ? a[e % 4] : b[e % 4]);
+        } else if (kind == G4_KIND_F16) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t h = vec ? a[e / 2] >> (16 * (e % 2)) : e < 4 ? a[e % 4] : b[e % 4];
+                y[e] = (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                y[e] = (float)(int8_t)(vec ? a[e / 4] >> (8 * (e % 4)) : e < 4 ? a[e % 4] : b[e % 4]) * scale;
+        }
+    }
+};
 
-template <int KIND>
-__device__ __forceinline__ void store4(void *p, int64_t at, int n, bool vec, f4 y, float snap) {
-    if (KIND == G4_KIND_I8) {
+__device__ __forceinline__ void store8(void *p, int kind, int64_t at, int n, bool vec, const float (&v)[8], float snap) {
+    if (kind == G4_KIND_I8) {
         int8_t *q = static_cast<int8_t *>(p) + at;
-        uint32_t c = 0;
+        uint2 c = make_uint2(0, 0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c |= (uint32_t)(uint8_t)srq_code_i(y[e], snap) << (8 * e);
+        for (int e = 0; e < 8; ++e) (e < 4 ? c.x : c.y) |= (uint32_t)(uint8_t)srq_code_i(v[e], snap) << (8 * (e % 4));
         if (vec) {
-            *reinterpret_cast<uint32_t *>(q) = c;
+            *reinterpret_cast<uint2 *>(q) = c;
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (e < n) q[e] = (int8_t)(c >> (8 * e));
+            for (int e = 0; e < 8; ++e)
+                if (e < n) q[e] = (int8_t)((e < 4 ? c.x : c.y) >> (8 * (e % 4)));
         }
         return;
     }
-    if (snap != 0.0f) {
+    float y[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = srq_code_f(y[e], snap) * snap;
-    }
-    if (KIND == G4_KIND_F16) {
+    for (int e = 0; e < 8; ++e) y[e] = snap != 0.0f ? srq_code_f(v[e], snap) * snap : v[e];
+    if (kind == G4_KIND_F16) {
         _Float16 *q = static_cast<_Float16 *>(p) + at;
-        h4 c;
+        h8 c;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c[e] = (_Float16)y[e];
+        for (int e = 0; e < 8; ++e) c[e] = (_Float16)y[e];
         if (vec) {
-            *reinterpret_cast<h4 *>(q) = c;
+            *reinterpret_cast<h8 *>(q) = c;
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 8; ++e)
                 if (e < n) q[e] = c[e];
         }
     } else {
         float *q = static_cast<float *>(p) + at;
         if (vec) {
-            *reinterpret_cast<f4 *>(q) = y;
+            reinterpret_cast<f4 *>(q)[0] = f4{y[0], y[1], y[2], y[3]};
+            reinterpret_cast<f4 *>(q)[1] = f4{y[4], y[5], y[6], y[7]};
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 8; ++e)
                 if (e < n) q[e] = y[e];
         }
     }
 }
 
-constexpr int kNTiles = 4;                            // tiles of 16 outputs a wave has
-constexpr int kNBlock = kAdWaves * kNTiles * kTile;  // outputs a block has
+constexpr int kOutWaves = 8, kOutThreads = 64 * kOutWaves;  // of a block that writes outputs
+constexpr int kWaveN = 64, kBlockN = kOutWaves * kWaveN;    // outputs of a wave, and of a block, at a time
 
-// Grid (ranges of N, tiles).
-template <int BK, int OK, int RT>
-__global__ __launch_bounds__(kAdThreads) void adapter_expand_kernel(AdapterArgs A) {
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 15, group = lane >> 4;
-    if ((int)blockIdx.y >= tiles_of(A)) return;
-    const GroupTile T = A.tiles[blockIdx.y];
-    const bool some = col < T.rows;
-    const int64_t row = A.order[T.first + min(col, T.rows - 1)];
-    const int n0 = blockIdx.x * kNBlock + wave * (kNTiles * kTile);
-    f4 acc[kNTiles];
+// A wave's 64 outputs of a tile's rows. Tile j of the product has the outputs n0 + 32 (j / 2) + 8 q + 4 (j % 2) + e,
+// q its row's group and e its place there, so that a lane has eight consecutive outputs in each pair of tiles.
+template <int RT>
+struct Expand {
+    // A lane's ranks of a product: eight consecutive ones of 32, or four of 16 where there are no more.
+    static constexpr int kRanks = RT == 1 ? 4 : 8, kSteps = RT == 1 ? 1 : RT / 2;
+    typedef _Float16 hr __attribute__((ext_vector_type(kRanks)));
+    hr w[kSteps][4];
+    Raw8 raw[2];
+    int n0;
+
+    // Loads what does not depend on H.
+    __device__ __forceinline__ void load(const AdapterArgs &A, const Tile &T, const _Float16 *b, int64_t row, int n) {
+        const int lane = threadIdx.x & 63, col = lane & 15, group = lane >> 4;
+        n0 = n;
 #pragma unroll
-    for (int j = 0; j < kNTiles; ++j) acc[j] = f4{};
-    float scale = 0.0f;
-    if (T.adapter >= 0) {
-        const int rank = rank_of(A, T.adapter);
-        scale = (A.scales ? A.scales[T.adapter] : 1.0f) * A.x_scale;
-        const _Float16 *b = A.b + T.adapter * A.b_stride;
-        const float *h = A.h + (int64_t)(T.first + min(col, T.rows - 1)) * A.rank16;
+        for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            const int at = 16 * r + 4 * group;  // the lane's ranks at .. at + 3
-            if (16 * r >= rank) break;
-            f4 y{};
-            for (int s = 0; s < A.splits; ++s)
-                y += *reinterpret_cast<const f4 *>(h + (int64_t)s * A.tokens * A.rank16 + at);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = at + e < rank ? y[e] : 0.0f;  // (an infinite x leaves NaN there)
-#pragma unroll
-            for (int j = 0; j < kNTiles; ++j) {
-                const int n = n0 + 16 * j + col;
-                h4 w{};
-                if (n < A.n && at < rank) w = *reinterpret_cast<const h4 *>(b + (int64_t)n * A.max_rank + at);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(at + e < rank ? (float)w[e] : 0.0f, y[e], acc[j], 0, 0, 0);
+            for (int j = 0; j < 4; ++j) {
+                const int at = kRanks * (4 * s + group), out = n0 + 32 * (j / 2) + 8 * (col / 4) + 4 * (j % 2) + col % 4;
+                w[s][j] = hr{};
+                if (at < A.max_rank && out < A.n) w[s][j] = *reinterpret_cast<const hr *>(b + (int64_t)out * A.max_rank + at);
             }
+        if (!A.base || col >= T.rows) return;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const int out = n0 + 32 * p + 8 * group, left = A.n - out;
+            if (left > 0) raw[p].load(A.base, A.base_kind, row * A.base_stride + out, left, A.vec);
         }
     }
-    if (!some) return;
+
+    // h: the tile's H in LDS, as the first product leaves it, [rank tile][lane], a lane's four ranks of its row. H enters the
+    // product as the sum of two f16 values, relative to the row's largest: off by 2^-23 of itself, as by two roundings to
+    // f32.
+    __device__ __forceinline__ void finish(const AdapterArgs &A, const Tile &T, const f4 *h, int rank, float scale, int64_t row) {
+        const int lane = threadIdx.x & 63, col = lane & 15, group = lane >> 4;
+        f4 acc[4] = {f4{}, f4{}, f4{}, f4{}};
+        if (rank > 0) {
+            float v[kSteps][kRanks];
+            float top = 0.0f;
 #pragma unroll
-    for (int j = 0; j < kNTiles; ++j) {
-        const int n = n0 + 16 * j + 4 * group, left = A.n - n;
-        if (left <= 0) continue;
-        f4 y{};
-        if (A.base) y = load4<BK>(A.base, row * A.base_stride + n, left, A.vec, A.base_scale);
-        if (T.adapter >= 0) {
+            for (int s = 0; s < kSteps; ++s) {
+                const int at = kRanks * (4 * s + group);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] += scale * acc[j][e];
+                for (int e = 0; e < kRanks; e += 4) {
+                    const f4 o = at + e < rank ? h[(at + e) / 16 * 64 + (at + e) / 4 % 4 * 16 + col] : f4{};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        // (an infinite x leaves NaN behind the rank)
+                        v[s][e + i] = at + e + i < rank ? o[i] : 0.0f;
+                        top = fmaxf(top, fabsf(v[s][e + i]));
+                    }
+                }
+            }
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            // the largest to [2^14, 2^15) of f16's 65504
+            int up = 141 - (int)(__float_as_uint(top) >> 23);
+            up = min(max(up, -120), 120);
+            const float to = __uint_as_float((uint32_t)(127 + up) << 23);
+            scale *= __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                if (4 * kRanks * s >= rank) break;
+                hr hi, lo;
+#pragma unroll
+                for (int e = 0; e < kRanks; ++e) {
+                    const float o = v[s][e] * to;
+                    hi[e] = (_Float16)o;
+                    lo[e] = (_Float16)(o - (float)hi[e]);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    hr b = w[s][j];
+#pragma unroll
+                    for (int e = 0; e < kRanks; ++e) b[e] = kRanks * (4 * s + group) + e < rank ? b[e] : (_Float16)0.0f;
+                    acc[j] = multiply(b, hi, acc[j]);
+                    acc[j] = multiply(b, lo, acc[j]);
+                }
+            }
         }
-        store4<OK>(A.out, row * A.out_stride + n, left, A.vec, y, A.out_scale);
+        if (col >= T.rows) return;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const int out = n0 + 32 * p + 8 * group, left = A.n - out;
+            if (left <= 0) continue;
+            float y[8] = {};
+            if (A.base) raw[p].values(A.base_kind, A.vec, A.base_scale, y);
+            if (rank > 0) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] += scale * acc[2 * p + e / 4][e % 4];
+            }
+            store8(A.out, A.out_kind, row * A.out_stride + out, left, A.vec, y, A.out_scale);
+        }
+    }
+};
+
+__device__ __forceinline__ float scale_of(const AdapterArgs &A, int adapter) {
+    return adapter < 0 ? 0.0f : (A.scales ? A.scales[adapter] : 1.0f) * A.x_scale;
+}
+
+// Grid (ranges of outputs, tiles): H, then the outputs.
+template <int XK, int RT>
+__global__ __launch_bounds__(kOutThreads) void adapter_fused_kernel(AdapterArgs A) {
+    __shared__ f4 part[kOutWaves][RT * 64];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 15;
+    const Tile T = tile_of(A, blockIdx.y);
+    const int tiles = tiles_of(A);
+    if ((int)blockIdx.y >= tiles) return;
+    const int64_t row[1] = {row_of(A, T, col)};
+    const int rank = T.adapter < 0 ? 0 : rank_of(A, T.adapter);
+    const float scale = scale_of(A, T.adapter);
+    const _Float16 *b = A.b + max(T.adapter, 0) * A.b_stride;
+    const int end = min((int)(blockIdx.x + 1) * A.n_range, A.n);
+    int n = blockIdx.x * A.n_range + wave * kWaveN;
+    Expand<RT> E;
+    E.load(A, T, b, row[0], n);
+    if (rank > 0) {
+        f4 acc[1][RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) acc[0][r] = f4{};
+        shrink<XK, RT, 1, kOutWaves, unroll_of(XK, RT, 1, 8 * RT)>(A, A.a + T.adapter * A.a_stride, rank, row, 0, A.k, wave, acc);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) part[wave][r * 64 + lane] = acc[0][r];
+        __syncthreads();
+        for (int i = t; i < RT * 64; i += kOutThreads) {
+            f4 s = part[0][i];
+#pragma unroll
+            for (int w = 1; w < kOutWaves; ++w) s += part[w][i];
+            part[0][i] = s;
+        }
+        __syncthreads();
+    }
+    while (true) {
+        E.finish(A, T, part[0], rank, scale, row[0]);
+        n += kBlockN;
+        if (n - wave * kWaveN >= end) return;
+        E.load(A, T, b, row[0], n);
     }
 }
 
-// Ranges of K: blocks for every CU a few times, each with some steps of 32 for each of its waves.
-static int adapter_splits(int k, int tokens) {
-    const int tiles = (tokens + kTile - 1) / kTile, most = (k + 32 * kAdWaves - 1) / (32 * kAdWaves);
-    int want = (1024 + tiles - 1) / tiles;
-    if (want > 16) want = 16;
-    return want < most ? want : most;
+constexpr int kHWaves = 4, kHThreads = 64 * kHWaves;  // of a block that makes a part of H
+
+// Grid (splits, pairs of tiles): a range of K of the tiles' H. Two tiles of one adapter share its rows of A.
+template <int XK, int RT>
+__global__ __launch_bounds__(kHThreads) void adapter_shrink_kernel(AdapterArgs A) {
+    __shared__ f4 part[kHWaves][2 * RT * 64];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 15;
+    const int first = 2 * blockIdx.y, tiles = min(tiles_of(A) - first, 2);
+    if (tiles <= 0) return;
+    const Tile T0 = tile_of(A, first), T1 = tile_of(A, tiles > 1 ? first + 1 : first);
+    const int k0 = blockIdx.x * A.k_range, k1 = min(k0 + A.k_range, A.k);
+    f4 acc[2][RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) acc[0][r] = acc[1][r] = f4{};
+    const int64_t row[2] = {row_of(A, T0, col), row_of(A, T1, col)};
+    if (T0.adapter == T1.adapter) {
+        if (T0.adapter < 0) return;
+        shrink<XK, RT, 2, kHWaves, unroll_of(XK, RT, 2, 0)>(A, A.a + T0.adapter * A.a_stride, rank_of(A, T0.adapter), row, k0, k1,
+                                                            wave, acc);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int adapter = i ? T1.adapter : T0.adapter;
+            if (adapter < 0) continue;
+            const int64_t one[1] = {row[i]};
+            f4 mine[1][RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) mine[0][r] = f4{};
+            shrink<XK, RT, 1, kHWaves, unroll_of(XK, RT, 2, 0)>(A, A.a + adapter * A.a_stride, rank_of(A, adapter), one, k0, k1,
+                                                                wave, mine);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) acc[i][r] = mine[0][r];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) part[wave][(i * RT + r) * 64 + lane] = acc[i][r];
+    __syncthreads();
+    for (int i = t; i < tiles * RT * 64; i += kHThreads) {
+        const bool second = i >= RT * 64;
+        const int r = i / 64 % RT, l = i & 63, place = (second ? T1.first : T0.first) + (l & 15);
+        f4 s = part[0][i];
+#pragma unroll
+        for (int w = 1; w < kHWaves; ++w) s += part[w][i];
+        if ((l & 15) < (second ? T1.rows : T0.rows) && 16 * r < A.rank16)
+            *reinterpret_cast<f4 *>(A.h + ((int64_t)blockIdx.x * A.tokens + place) * A.rank16 + 16 * r + 4 * (l >> 4)) = s;
+    }
+}
+
+// Grid (ranges of outputs, tiles).
+// (128 registers: two blocks a CU)
+template <int RT>
+__global__ __launch_bounds__(kOutThreads, RT <= 4 ? 4 : 2) void adapter_expand_kernel(AdapterArgs A) {
+    __shared__ f4 h[RT * 64];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 15;
+    const Tile T = tile_of(A, blockIdx.y);
+    const int tiles = tiles_of(A);
+    if ((int)blockIdx.y >= tiles) return;
+    const int64_t row = row_of(A, T, col);
+    const int rank = T.adapter < 0 ? 0 : rank_of(A, T.adapter);
+    const float scale = scale_of(A, T.adapter);
+    const _Float16 *b = A.b + max(T.adapter, 0) * A.b_stride;
+    const int end = min((int)(blockIdx.x + 1) * A.n_range, A.n);
+    int n = blockIdx.x * A.n_range + wave * kWaveN;
+    Expand<RT> E;
+    E.load(A, T, b, row, n);
+    if (rank > 0) {
+        for (int i = t; i < RT * 64; i += kOutThreads) {
+            const int r = i >> 6, l = i & 63;
+            if (16 * r >= A.rank16) break;
+            const float *p = A.h + (int64_t)(T.first + min(l & 15, T.rows - 1)) * A.rank16 + 16 * r + 4 * (l >> 4);
+            f4 s{};
+#pragma unroll 8
+            for (int j = 0; j < A.splits; ++j) s += *reinterpret_cast<const f4 *>(p + (int64_t)j * A.tokens * A.rank16);
+            h[i] = s;
+        }
+        __syncthreads();
+    }
+    while (true) {
+        E.finish(A, T, h, rank, scale, row);
+        n += kBlockN;
+        if (n - wave * kWaveN >= end) return;
+        E.load(A, T, b, row, n);
+    }
+}
+
+// How a call is run: in one launch (splits 0), or with H's parts of `splits` ranges of K.
+static int adapter_splits(const g4_adapters *D, int tokens, int x_size) {
+    const int64_t tiles = max_tiles(tokens, D->count), ranges = (D->n + 2 * kBlockN - 1) / (2 * kBlockN);
+    const int64_t again = tiles * ranges * D->k * (2 * D->max_rank + kTile * x_size);
+    const int64_t cycles = (D->k / 32) * ((D->max_rank + 15) / 16) * (x_size == 4 ? 256 : 16) / 4;
+    if (again <= kFusedBytes && cycles <= kFusedCycles) return 0;
+    const int64_t pairs = (tiles + 1) / 2, most = (D->k + 32 * kHWaves - 1) / (32 * kHWaves);
+    int64_t want = 512 / pairs;  // two blocks a CU at once
+    want = want < 1 ? 1 : want > 16 ? 16 : want;
+    return (int)(want < most ? want : most);
+}
+
+template <int XK>
+static int launch_fused(const AdapterArgs &A, dim3 grid, hipStream_t s) {
+    const dim3 block(kOutThreads);
+    if (A.rank16 <= 16) hipLaunchKernelGGL((adapter_fused_kernel<XK, 1>), grid, block, 0, s, A);
+    else if (A.rank16 <= 32) hipLaunchKernelGGL((adapter_fused_kernel<XK, 2>), grid, block, 0, s, A);
+    else if (A.rank16 <= 64) hipLaunchKernelGGL((adapter_fused_kernel<XK, 4>), grid, block, 0, s, A);
+    else hipLaunchKernelGGL((adapter_fused_kernel<XK, 8>), grid, block, 0, s, A);
+    G4_LAUNCHED("adapter_fused_kernel");
+    return G4_OK;
 }
 
 template <int XK>
 static int launch_shrink(const AdapterArgs &A, dim3 grid, hipStream_t s) {
-    switch (A.rank16 / 16) {
-#define G4_RT(n) case n: hipLaunchKernelGGL((adapter_shrink_kernel<XK, n>), grid, dim3(kAdThreads), 0, s, A); break
-        G4_RT(1); G4_RT(2); G4_RT(3); G4_RT(4); G4_RT(5); G4_RT(6); G4_RT(7); G4_RT(8);
-#undef G4_RT
-    }
+    const dim3 block(kHThreads);
+    if (A.rank16 <= 16) hipLaunchKernelGGL((adapter_shrink_kernel<XK, 1>), grid, block, 0, s, A);
+    else if (A.rank16 <= 32) hipLaunchKernelGGL((adapter_shrink_kernel<XK, 2>), grid, block, 0, s, A);
+    else if (A.rank16 <= 64) hipLaunchKernelGGL((adapter_shrink_kernel<XK, 4>), grid, block, 0, s, A);
+    else hipLaunchKernelGGL((adapter_shrink_kernel<XK, 8>), grid, block, 0, s, A);
     G4_LAUNCHED("adapter_shrink_kernel");
     return G4_OK;
 }
 
-template <int BK, int OK>
 static int launch_expand(const AdapterArgs &A, dim3 grid, hipStream_t s) {
-    if (A.rank16 <= 32)
-        hipLaunchKernelGGL((adapter_expand_kernel<BK, OK, 2>), grid, dim3(kAdThreads), 0, s, A);
-    else
-        hipLaunchKernelGGL((adapter_expand_kernel<BK, OK, kMaxRank / 16>), grid, dim3(kAdThreads), 0, s, A);
+    const dim3 block(kOutThreads);
+    if (A.rank16 <= 16) hipLaunchKernelGGL(adapter_expand_kernel<1>, grid, block, 0, s, A);
+    else if (A.rank16 <= 32) hipLaunchKernelGGL(adapter_expand_kernel<2>, grid, block, 0, s, A);
+    else if (A.rank16 <= 64) hipLaunchKernelGGL(adapter_expand_kernel<4>, grid, block, 0, s, A);
+    else hipLaunchKernelGGL(adapter_expand_kernel<8>, grid, block, 0, s, A);
     G4_LAUNCHED("adapter_expand_kernel");
     return G4_OK;
-}
-template <int BK>
-static int launch_expand_out(const AdapterArgs &A, int ok, dim3 grid, hipStream_t s) {
-    if (ok == G4_KIND_I8) return launch_expand<BK, G4_KIND_I8>(A, grid, s);
-    if (ok == G4_KIND_F16) return launch_expand<BK, G4_KIND_F16>(A, grid, s);
-    return launch_expand<BK, G4_KIND_F32>(A, grid, s);
 }
 
 static int check_adapters(const char *who, const g4_adapters *D) {
     if (!D || !D->a || !D->b) return set_error(G4_ERR_INVALID, "%s needs the adapters' A and B", who);
     if (D->count <= 0 || D->count > kMaxAdapters)
         return set_error(G4_ERR_INVALID, "%s: %d adapters (1 to %d)", who, D->count, kMaxAdapters);
-    if (D->k <= 0 || D->k % 8 || D->n <= 0)
-        return set_error(G4_ERR_INVALID, "%s: k %d, n %d (k a multiple of 8)", who, D->k, D->n);
+    if (D->k <= 0 || D->k % 8 || D->k > kMaxK || D->n <= 0)
+        return set_error(G4_ERR_INVALID, "%s: k %d, n %d (k a multiple of 8 up to %d)", who, D->k, D->n, kMaxK);
     if (D->max_rank <= 0 || D->max_rank % 8 || D->max_rank > kMaxRank)
         return set_error(G4_ERR_INVALID, "%s: max_rank %d is not a multiple of 8 up to %d", who, D->max_rank, kMaxRank);
     if (((uintptr_t)D->a | (uintptr_t)D->b) & 15) return set_error(G4_ERR_INVALID, "%s: A and B must be 16-byte aligned", who);
@@ -433,16 +651,17 @@ int g4_adapter_groups(const int32_t *row_adapter, int tokens, int adapters, void
     if ((uintptr_t)groups & 15) return set_error(G4_ERR_INVALID, "adapter-groups: groups must be 16-byte aligned");
     GroupHeader *h = static_cast<GroupHeader *>(groups);
     GroupTile *tiles = reinterpret_cast<GroupTile *>(h + 1);
-    hipLaunchKernelGGL(adapter_groups_kernel, dim3(1), dim3(kGroupThreads), (adapters + 1) * sizeof(int32_t),
-                       as_stream(stream), row_adapter, tokens, adapters, h, tiles,
-                       reinterpret_cast<int32_t *>(tiles + max_tiles(tokens, adapters)));
+    hipLaunchKernelGGL(adapter_groups_kernel, dim3(1), dim3(kGroupThreads), 2 * (adapters + 1) * sizeof(int32_t),
+                       as_stream(stream), row_adapter, tokens, adapters, h, tiles);
     G4_LAUNCHED("adapter_groups_kernel");
     return G4_OK;
 }
 
 size_t g4_adapter_workspace_bytes(const g4_adapters *adapters, int tokens) {
     if (check_adapters("adapter-linear", adapters) || tokens <= 0 || tokens > kMaxTokens) return 0;
-    return (size_t)adapter_splits(adapters->k, tokens) * tokens * ((adapters->max_rank + 15) / 16 * 16) * sizeof(float);
+    // the most that any type of x takes; one launch takes none
+    const int splits = adapter_splits(adapters, tokens, 4);
+    return splits ? (size_t)splits * tokens * ((adapters->max_rank + 15) / 16 * 16) * sizeof(float) : 16;
 }
 
 int g4_adapter_linear(const g4_adapters *adapters, const void *groups, size_t groups_bytes, int tokens, const void *x,
@@ -488,32 +707,39 @@ int g4_adapter_linear(const g4_adapters *adapters, const void *groups, size_t gr
     A.b_stride = D->b_stride ? D->b_stride : (int64_t)D->n * D->max_rank;
     A.header = static_cast<const GroupHeader *>(groups);
     A.tiles = reinterpret_cast<const GroupTile *>(A.header + 1);
-    A.order = reinterpret_cast<const int32_t *>(A.tiles + tiles);
     A.x = x;
     A.x_stride = xs;
     A.x_scale = x_kind == G4_KIND_I8 ? x_scale : 1.0f;
     A.base = base;
+    A.base_kind = base ? base_kind : G4_KIND_F32;
     A.base_stride = bs;
     A.base_scale = base_scale;
     A.out = out;
+    A.out_kind = out_kind;
     A.out_stride = os;
     A.out_scale = out_scale;
-    A.splits = adapter_splits(D->k, tokens);
-    A.range = ((D->k + A.splits - 1) / A.splits + 31) / 32 * 32;
-    A.vec = D->n % 4 == 0 && os % 4 == 0 && (!base || bs % 4 == 0) &&
-            ((uintptr_t)out % (4 * kind_size(out_kind))) == 0 && (!base || (uintptr_t)base % (4 * kind_size(base_kind)) == 0);
+    A.splits = adapter_splits(D, tokens, kind_size(x_kind));
+    A.vec = D->n % 8 == 0 && os % 8 == 0 && (!base || bs % 8 == 0) && ((uintptr_t)out & 15) == 0 && ((uintptr_t)base & 15) == 0;
     A.h = static_cast<float *>(workspace);
     hipStream_t s = as_stream(stream);
-    const dim3 grid(A.splits, (unsigned)tiles);
+    // ranges of outputs: a block of two rounds where that leaves a block for every other CU
+    const int64_t rounds = tiles * ((D->n + 2 * kBlockN - 1) / (2 * kBlockN)) >= device_cu_count() / 2 ? 2 : 1;
+    A.n_range = (int)(rounds * kBlockN);
+    const dim3 out_grid((unsigned)((D->n + A.n_range - 1) / A.n_range), (unsigned)tiles);
+    if (A.splits == 0) {
+        if (x_kind == G4_KIND_I8) return launch_fused<G4_KIND_I8>(A, out_grid, s);
+        if (x_kind == G4_KIND_F16) return launch_fused<G4_KIND_F16>(A, out_grid, s);
+        return launch_fused<G4_KIND_F32>(A, out_grid, s);
+    }
+    A.k_range = ((D->k + A.splits - 1) / A.splits + 31) / 32 * 32;
+    A.n_range = kBlockN;
+    const dim3 grid(A.splits, (unsigned)((tiles + 1) / 2));
     int st;
     if (x_kind == G4_KIND_I8) st = launch_shrink<G4_KIND_I8>(A, grid, s);
     else if (x_kind == G4_KIND_F16) st = launch_shrink<G4_KIND_F16>(A, grid, s);
     else st = launch_shrink<G4_KIND_F32>(A, grid, s);
     if (st) return st;
-    const dim3 out_grid((unsigned)((D->n + kNBlock - 1) / kNBlock), (unsigned)tiles);
-    if (base && base_kind == G4_KIND_I8) return launch_expand_out<G4_KIND_I8>(A, out_kind, out_grid, s);
-    if (base && base_kind == G4_KIND_F16) return launch_expand_out<G4_KIND_F16>(A, out_kind, out_grid, s);
-    return launch_expand_out<G4_KIND_F32>(A, out_kind, out_grid, s);
+    return launch_expand(A, dim3((unsigned)((D->n + kBlockN - 1) / kBlockN), (unsigned)tiles), s);
 }
 
 }  // extern "C"

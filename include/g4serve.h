@@ -204,8 +204,8 @@ int g4_release_pages(const g4_free_pages *list, const int32_t *page_table, int t
  * Low-rank adapters of one linear, f16: adapter i adds scales[i] * (x A_i^T) B_i^T to its rows.
  * A_i = a + i * a_stride, [max_rank][k]; B_i = b + i * b_stride, [n][max_rank] (strides in elements, 0: packed). ranks
  * (NULL: max_rank for all): adapter i has ranks[i] (clamped to [0, max_rank]) rows of A_i and columns of B_i; what lies
- * behind them is not used, whatever it holds. k and max_rank multiples of 8, max_rank up to 128, at most 4096 adapters; a and
- * b 16-byte aligned, the strides multiples of 8.
+ * behind them is not used, whatever it holds. k and max_rank multiples of 8, k up to 2^23 and max_rank to 128; at most 4096
+ * adapters; a and b 16-byte aligned, the strides multiples of 8.
  */
 typedef struct g4_adapters {
     const void *a, *b;

@@ -39,7 +39,9 @@ class Case:
 
     def want(self):
         """(out, bound) before the output's type: sums of n products in f32 are n + 2 roundings off of the sum of
-        magnitudes (in any order), H's error goes through B, and each step of the epilogue adds one."""
+        magnitudes (in any order), H's error goes through B, H's two f16 values are 2^-23 off (two roundings more) or,
+        by the smaller one's last place under the row's largest, 2^-38 of that, and each step of the epilogue adds
+        one."""
         u = 2.0 ** -24
         x = self.x.astype(np.float64) * (float(self.x_scale) if self.kinds[0] == "i8" else 1.0)
         y = np.zeros((len(self.ids), self.n))
@@ -54,7 +56,8 @@ class Case:
             h = x[rows] @ a.T
             h_off = (self.k + 2) * u * (np.abs(x[rows]) @ np.abs(a).T)
             d = s * (h @ b.T)
-            bound[rows] += s * ((h_off + (m + 2) * u * np.abs(h)) @ np.abs(b).T) + 4 * u * (np.abs(d) + np.abs(y[rows]))
+            h_off = h_off + (m + 4) * u * np.abs(h) + 2.0 ** -38 * np.abs(h).max(1, keepdims=True, initial=0)
+            bound[rows] += s * (h_off @ np.abs(b).T) + 4 * u * (np.abs(d) + np.abs(y[rows]))
             y[rows] += d
         return y, bound
 
@@ -159,6 +162,19 @@ def test_batches(gpu, tokens, runs, adapters):
     c.check()
 
 
+@pytest.mark.parametrize("rank", [8, 32, 40, 128])
+@pytest.mark.parametrize("x", ["f32", "f16", "i8"])
+def test_long_batches(gpu, x, rank):
+    """Enough rows and sizes for H to go through memory: pairs of tiles of one adapter and of two, none, odd sizes."""
+    r = np.random.default_rng(rank)
+    for t, k, n, base, out in ((700, 6144, 1500, "f32", "f16"), (1300, 4104, 2056, "f16", "f32")):
+        ids = np.concatenate([[2] * 41, np.sort(r.integers(-2, 5, t - 60)), [0] * 19])
+        c = Case(ids, adapters=5, k=k, n=n, rank=rank, x=x, base=base, out=out, ranks=[rank, 3, rank, 0, rank - 5]).upload()
+        assert c.ws.nbytes > t * rank * 4  # there is an H
+        c.call()
+        c.check()
+
+
 def test_ids(gpu):
     """No adapter (-1, and ids out of range), no row (-2); none at all, all of one."""
     for ids in ([-1, -2, 0, 99, 3, -7, -2, 2 ** 31 - 1], [-1] * 5, [-2] * 5, [3] * 40, list(range(4)) * 9):
@@ -224,22 +240,23 @@ def test_a_bad_row_stays_alone(gpu):
     c.check(good)
 
 
-def test_a_row_does_not_depend_on_its_batch(gpu):
+@pytest.mark.parametrize("t,k,n", [(41, 512, 64), (1000, 6144, 1024)])
+def test_a_row_does_not_depend_on_its_batch(gpu, t, k, n):
     """The same row in another place, among other adapters, of as many tokens: the same bits."""
     r = np.random.default_rng(8)
-    c = Case([2] + [0] * 40, k=512).upload()
+    c = Case([2] + [0] * (t - 1), k=k, n=n).upload()
     c.call()
     g4.synchronize()
     one = c.out.download()[0]
-    d = Case(list(r.integers(0, 4, 30)) + [2] + [1] * 10, k=512)
+    d = Case(list(r.integers(0, 4, t - 11)) + [2] + [1] * 10, k=k, n=n)
     d.a, d.b, d.scales = c.a, c.b, c.scales
-    d.x[30], d.base[30] = c.x[0], c.base[0]
+    d.x[t - 11], d.base[t - 11] = c.x[0], c.base[0]
     d.upload()
     for _ in range(3):
         gs.adapter_groups(d.d_ids, d.groups, 4)
         d.call()
         g4.synchronize()
-        assert np.array_equal(d.out.download()[30], one)
+        assert np.array_equal(d.out.download()[t - 11], one)
 
 
 def test_replays(gpu):

@@ -86,6 +86,7 @@ def test_adapter_refusals(g4):
         expect(g4, lambda: call(p), 1, text)
         expect(g4, lambda: gs.adapter_workspace_bytes(p, 6), 1, "no such call")
     expect(g4, lambda: call(pool(h(4, 16, 252)), x=Fake((6, 252), F)), 1, "k a multiple of 8")
+    expect(g4, lambda: call(pool(h(1, 16, (1 << 23) + 8), h(1, 64, 16)), x=Fake((6, (1 << 23) + 8), F)), 1, "up to 8388608")
     expect(g4, lambda: call(x=Fake((6, 128), F)), 1, "x has shape [6, 128]")
     expect(g4, lambda: call(x=Fake((6, 256), I)), 1, "x cannot be int32")
     expect(g4, lambda: call(x=Strided((6, 256), F, (257, 1))), 1, "x must be 16-byte aligned, its rows too")
@@ -95,7 +96,7 @@ def test_adapter_refusals(g4):
     expect(g4, lambda: call(out=Fake((6, 64), np.float16)), 1, "out can be base only with its type and stride")
     expect(g4, lambda: call(out=Strided((6, 64), F, (80, 1))), 1, "out can be base only with its type and stride")
     expect(g4, lambda: call(g=Fake((16,), np.uint8)), 1, "groups 16 B <")
-    expect(g4, lambda: call(ws=Fake((16,), np.uint8)), 1, "workspace 16 B <")
+    expect(g4, lambda: call(ws=Fake((8,), np.uint8)), 1, "workspace 8 B <")
     expect(g4, lambda: call(ws=Strided((1 << 24,), np.uint8, (0,))), 1, "the workspace must be contiguous")
     expect(g4, lambda: call(g=Fake((1 << 20,), np.uint8, 0x1008)), 1, "16-byte aligned")
     expect(g4, lambda: g4._check(g4.lib().g4_adapter_linear(pool().ref, 0x1000, 1 << 20, 6, 0x1000, 3, 0, 1.0, 0x1000, 0, 0, 1.0, 0x1000,

@@ -273,6 +273,10 @@ __device__ __forceinline__ u64 block_run(u64 v, u64 *lds, u64 *total) {
     return before + v;
 }
 
+// The bin that stands at place i of a row's histogram in memory: a lane's 16 consecutive bins lie 64 apart, so that a
+// wave's loads of them are of whole lines. (Loads of 128 bytes a lane stalled on each other's lines: 12 us.)
+__device__ __forceinline__ int bin_at(int i) { return i % 64 * kBinsPer + i / 64; }
+
 struct Bin {
     u64 mass;  // and kNoStepsBits for each token
     uint32_t count, pad;
@@ -336,7 +340,7 @@ __global__ __launch_bounds__(64 * WAVES) void sample_weights_kernel(SampleArgs A
         });
         __syncthreads();
         for (int i = t; i < kBins; i += 64 * WAVES) {
-            const Bin b = bins[i];
+            const Bin b = bins[bin_at(i)];
             if (!b.count) continue;
             const u64 m = b.mass - b.count * kNoStepsBits;
             all += m;
@@ -391,18 +395,27 @@ __device__ __forceinline__ T wave_run(T v) {
     return v;
 }
 
-// The bins of a row's cuts, by one wave, the same in every lane; a lane has 16 bins.
-__device__ __forceinline__ Cuts find_cuts(const SampleArgs &A, const Row &R, int row) {
-    const int lane = threadIdx.x & 63;
-    const u64 *mass = A.bin_mass + (int64_t)row * kBins + lane * kBinsPer;
-    const uint32_t *count = A.bin_count + (int64_t)row * kBins + lane * kBinsPer;
-    u64 m[kBinsPer], m_sum = 0;
-    uint32_t n[kBinsPer], n_sum = 0;
+// A lane's 16 bins of a row.
+struct LaneBins {
+    u64 m[kBinsPer];
+    uint32_t n[kBinsPer];
+    __device__ __forceinline__ void load(const SampleArgs &A, int row) {
+        const int64_t at = (int64_t)row * kBins + (threadIdx.x & 63);
 #pragma unroll
-    for (int i = 0; i < kBinsPer; ++i) {
-        m[i] = mass[i];
-        n[i] = count[i];
+        for (int i = 0; i < kBinsPer; ++i) {
+            m[i] = A.bin_mass[at + 64 * i];
+            n[i] = A.bin_count[at + 64 * i];
+        }
     }
+};
+
+// The bins of a row's cuts, by one wave, the same in every lane.
+__device__ __forceinline__ Cuts find_cuts(const SampleArgs &A, const Row &R, const LaneBins &B) {
+    const int lane = threadIdx.x & 63;
+    const auto &m = B.m;
+    const auto &n = B.n;
+    u64 m_sum = 0;
+    uint32_t n_sum = 0;
 #pragma unroll
     for (int i = 0; i < kBinsPer; ++i) {
         m_sum += m[i];
@@ -461,18 +474,85 @@ __device__ __forceinline__ Cuts find_cuts(const SampleArgs &A, const Row &R, int
     return C;
 }
 
-// Grid (spans, rows): every block finds the bins of its row's cuts, then weighs its tokens above them.
+// Four rows a block, a wave each: for calls of many blocks, each of which would do it again.
+__global__ __launch_bounds__(kSampleThreads) void sample_find_kernel(SampleArgs A, int rows) {
+    const int row = blockIdx.x * kSampleWaves + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    LaneBins B;
+    B.load(A, row);
+    const Row R = uniform(A.row[row]);
+    if (!R.filtered) return;
+    const Cuts C = find_cuts(A, R, B);
+    if ((threadIdx.x & 63) == 0) A.cut[row] = C;
+}
+
+// A wave's unit of a row with cuts: the weight above them, and what lies in their bins to the list. v: its logits, at x.
+template <bool CAP>
+__device__ __forceinline__ u64 cut_unit(const SampleArgs &A, const Row &R, const Cuts &c, int row, const float *x, int base,
+                                        const float (&v)[kSamplePer]) {
+    const int lane = threadIdx.x & 63;
+    u64 sure = 0;
+    uint32_t look = 0, far = 0, in = 0;  // places where a lane's token may be in these bins or above; past half the cap; a
+                                         // lane's for the list
+    int many = 0;
+    auto take = [&](int j, double d, bool real) {
+        const u64 w = real ? steps(d, R, A) : 0;
+        const int b = bin_of(d, R);
+        if (b < c.p_low && d >= R.d_min) sure += w;
+        const bool mine = w && ((b >= c.p_low && b <= c.p_high) || b == c.k_bin);
+        in |= mine ? 1u << j : 0u;
+        many += __popcll(__ballot(mine));
+    };
+#pragma unroll
+    for (int j = 0; j < kSamplePer; ++j) {
+        look |= __any(v[j] >= c.least) ? 1u << j : 0u;
+        far |= CAP && __any(is_far(v[j], A.cap) && v[j] >= c.least) ? 1u << j : 0u;
+    }
+#pragma unroll
+    for (int j = 0; j < kSamplePer; ++j) {
+        if (!(look >> j & 1)) continue;
+        const float xs = seen(clean(v[j]), R);
+        take(j, near_distance<CAP>(xs, R, A), xs > -INFINITY && !(CAP && is_far(xs, A.cap)));
+    }
+    if (CAP)
+        for (; far; far &= far - 1) {
+            const int j = __ffs(far) - 1, i = base + unit_place(j, lane, A.vec);
+            const float xs = i < A.vocab ? x[i] : -INFINITY;
+            take(j, distance<CAP>(xs, R, A), is_far(xs, A.cap));
+        }
+    if (many) {
+        uint32_t at = 0;
+        if (lane == 0) at = atomicAdd(&A.listed[row], (uint32_t)many);
+        at = __shfl(at, 0);
+#pragma unroll
+        for (int j = 0; j < kSamplePer; ++j) {
+            const bool mine = in >> j & 1;
+            const u64 who = __ballot(mine);
+            const uint32_t place = at + __popcll(who & ((1ull << lane) - 1));
+            if (mine && place < (uint32_t)kList)
+                A.list[(int64_t)row * kList + place] = order_key(seen(v[j], R), base + unit_place(j, lane, A.vec));
+            at += __popcll(who);
+        }
+    }
+    return wave_sum(sure);
+}
+
+// Grid (spans, rows): a block finds its row's cuts itself, its logits on their way.
 template <bool CAP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void sample_cut_kernel(SampleArgs A) {
     __shared__ Cuts shared_cuts;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.y;
     const int unit = blockIdx.x * WAVES + wave, base = unit * kSampleUnit;
+    const float *x = row_of(A, row);
     const float top = unit < A.units ? A.unit_max[(int64_t)row * A.units + unit] : -INFINITY;
+    float v[kSamplePer];
+    load_unit(x + base, x ? A.vocab - base : 0, lane, A.vec, v);
+    LaneBins B;
+    if (wave == 0) B.load(A, row);
     const Row R = uniform(A.row[row]);
     if (!R.filtered) return;  // (a row without a logit, too)
-    const float *x = row_of(A, row);
     if (wave == 0) {
-        const Cuts C = find_cuts(A, R, row);
+        const Cuts C = find_cuts(A, R, B);
         if (lane == 0) {
             shared_cuts = C;
             if (blockIdx.x == 0) A.cut[row] = C;
@@ -481,43 +561,32 @@ __global__ __launch_bounds__(64 * WAVES) void sample_cut_kernel(SampleArgs A) {
     __syncthreads();
     const Cuts c = uniform(shared_cuts);
     if (unit >= A.units) return;
+    const u64 sure = top >= c.least ? cut_unit<CAP>(A, R, c, row, x, base, v) : 0;
+    if (lane == 0) A.unit_sums[(int64_t)row * A.units + unit] = sure;
+}
+
+// Grid (spans of kCutSpan units a wave, rows), behind sample_find_kernel: units that do not reach up to the cuts are not
+// read.
+constexpr int kCutSpan = 4;
+template <bool CAP>
+__global__ __launch_bounds__(kSampleThreads) void sample_cut_found_kernel(SampleArgs A) {
+    const int lane = threadIdx.x & 63, row = blockIdx.y;
+    const int first = (blockIdx.x * kSampleWaves + (threadIdx.x >> 6)) * kCutSpan;
+    const Row R = uniform(A.row[row]);
+    const Cuts c = uniform(A.cut[row]);
+    if (!R.filtered || first >= A.units) return;
+    const float *x = row_of(A, row);
+    const float top = lane < kCutSpan && first + lane < A.units ? A.unit_max[(int64_t)row * A.units + first + lane] : -INFINITY;
     u64 sure = 0;
-    if (top >= c.least) {
+#pragma unroll 1
+    for (u64 left = __ballot(top >= c.least && lane < kCutSpan && first + lane < A.units); left; left &= left - 1) {
+        const int i = __ffsll((long long)left) - 1, base = (first + i) * kSampleUnit;
         float v[kSamplePer];
         load_unit(x + base, A.vocab - base, lane, A.vec, v);
-        uint32_t look = 0, in = 0;  // elements that may be in these bins, and those for the list
-#pragma unroll
-        for (int j = 0; j < kSamplePer; ++j) look |= v[j] >= c.least ? 1u << j : 0u;
-        int many = 0;
-#pragma unroll
-        for (int j = 0; j < kSamplePer; ++j) {
-            if (!__any(look >> j & 1)) continue;
-            const float xs = seen(clean(v[j]), R);
-            const double d = distance<CAP>(xs, R, A);
-            const u64 w = xs > -INFINITY ? steps(d, R, A) : 0;
-            const int b = bin_of(d, R);
-            if (b < c.p_low && d >= R.d_min) sure += w;
-            const bool mine = w && ((b >= c.p_low && b <= c.p_high) || b == c.k_bin);
-            in |= mine ? 1u << j : 0u;
-            many += __popcll(__ballot(mine));
-        }
-        if (many) {
-            uint32_t at = 0;
-            if (lane == 0) at = atomicAdd(&A.listed[row], (uint32_t)many);
-            at = __shfl(at, 0);
-#pragma unroll
-            for (int j = 0; j < kSamplePer; ++j) {
-                const bool mine = in >> j & 1;
-                const u64 who = __ballot(mine);
-                const uint32_t place = at + __popcll(who & ((1ull << lane) - 1));
-                if (mine && place < (uint32_t)kList)
-                    A.list[(int64_t)row * kList + place] = order_key(seen(v[j], R), base + unit_place(j, lane, A.vec));
-                at += __popcll(who);
-            }
-        }
-        sure = wave_sum(sure);
+        const u64 sum = cut_unit<CAP>(A, R, c, row, x, base, v);
+        if (lane == i) sure = sum;
     }
-    if (lane == 0) A.unit_sums[(int64_t)row * A.units + unit] = sure;
+    if (lane < kCutSpan && first + lane < A.units) A.unit_sums[(int64_t)row * A.units + first + lane] = sure;
 }
 
 __device__ __forceinline__ float logit_of(u64 key) {
@@ -566,17 +635,22 @@ __device__ __forceinline__ u64 wave_cut(u64 key, u64 w, bool is, bool by_p, u64 
     return lane64(key, j);
 }
 
+constexpr int kCache = 2048;  // entries that the last kernel's block holds in LDS
+constexpr u64 kNearK = 1ull << 63, kNearP = 1ull << 62, kNearKept = 1ull << 61, kNearW = (1ull << 53) - 1;
+
 struct PickShared {
-    u64 extra[kMaxVocab / kSampleUnit];  // of the units, from a list of more than kFew
+    u64 key[kCache], w[kCache];  // the list; w: and the kNear bits
     u64 mass[kSub];
     uint32_t count[kSub];
-    u64 sums[kSampleWaves];
+    u64 sums[2][kSampleWaves];
     u64 few_key[kFew], few_w[kFew];
-    u64 high, low, before, mass_before;
+    u64 high[2], low[2];  // keys among top-k's tokens and top-p's
+    u64 before, mass_before;
     uint32_t at, count_at, few;
 };
 
-// What a block looks its row's cuts up in where a wave cannot: the list, or where that overflowed the row.
+// What a block looks its row's cuts up in where a wave cannot: the list in LDS, the list, or, where that overflowed, the
+// row.
 template <bool CAP>
 struct Search {
     const SampleArgs &A;
@@ -587,9 +661,9 @@ struct Search {
     const u64 *list;
     int n;
 
-    // All of them with f. Both loops take one element a thread at a time: lists of more than kFew are rare.
+    // Every token of the cuts' bins with f(key, w and bits), from where it lies.
     template <class F>
-    __device__ __forceinline__ void each(F f) {
+    __device__ __forceinline__ void each_given(F f) {
         const bool whole = n > kList;
         const int end = whole ? A.vocab : n;
         for (int i = threadIdx.x; i < end; i += kSampleThreads) {
@@ -601,34 +675,61 @@ struct Search {
                 key = list[i];
             }
             const Near e = near_of<CAP>(A, R, C, key);
-            if (e.k || e.p) f(e);
+            f(i, key, e.w | (e.k ? kNearK : 0) | (e.p ? kNearP : 0) | (e.kept ? kNearKept : 0));
         }
+    }
+    template <class F>
+    __device__ __forceinline__ void each(F f) {
+        if (n <= kCache) {
+            for (int i = threadIdx.x; i < n; i += kSampleThreads) f(S.key[i], S.w[i]);
+        } else {
+            each_given([&](int, u64 key, u64 w) { f(key, w); });
+        }
+    }
+    // First of all: the list to LDS, and the ranges of keys.
+    __device__ __forceinline__ void begin() {
+        const int t = threadIdx.x;
+        if (t < 2) {
+            S.high[t] = 0;
+            S.low[t] = ~0ull;
+        }
+        __syncthreads();
+        u64 high[2] = {0, 0}, low[2] = {~0ull, ~0ull};
+        each_given([&](int i, u64 key, u64 w) {
+            if (n <= kCache) {
+                S.key[i] = key;
+                S.w[i] = w;
+            }
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const bool is = w & (p ? kNearP : kNearK);
+                high[p] = is && key > high[p] ? key : high[p];
+                low[p] = is && key < low[p] ? key : low[p];
+            }
+        });
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+#pragma unroll
+            for (int s = 32; s; s >>= 1) {
+                const u64 h = __shfl_xor(high[p], s), l = __shfl_xor(low[p], s);
+                high[p] = h > high[p] ? h : high[p];
+                low[p] = l < low[p] ? l : low[p];
+            }
+            if ((t & 63) == 0) {
+                atomicMax(&S.high[p], high[p]);
+                atomicMin(&S.low[p], low[p]);
+            }
+        }
+        __syncthreads();
     }
 
     // As wave_cut, among top-p's (by_p) or top-k's tokens with a key of at least `least`. Each step splits the range of
     // keys in 1024, until a wave can order what is left.
     __device__ u64 refine(bool by_p, u64 least, u64 target, u64 *mass) {
-        const int t = threadIdx.x, lane = t & 63;
-        __syncthreads();
-        if (t == 0) {
-            S.high = 0;
-            S.low = ~0ull;
-        }
-        __syncthreads();
-        u64 hi = 0, lo = ~0ull;
-        each([&](const Near &e) {
-            if (!(by_p ? e.p : e.k) || e.key < least) return;
-            hi = e.key > hi ? e.key : hi;
-            lo = e.key < lo ? e.key : lo;
-        });
-        if (hi) {
-            atomicMax(&S.high, hi);
-            atomicMin(&S.low, lo);
-        }
-        __syncthreads();
-        hi = S.high;
-        lo = S.low;
-        u64 mass_sum = 0;
+        const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+        const u64 bit = by_p ? kNearP : kNearK;
+        u64 hi = S.high[by_p], lo = S.low[by_p], mass_sum = 0;
+        lo = lo < least ? least : lo;
         while (true) {
             const int bits = 64 - __clzll((long long)((hi - lo) | 1)), sh = bits > 10 ? bits - 10 : 0;
 #pragma unroll
@@ -638,21 +739,39 @@ struct Search {
                 S.few = 0;
             }
             __syncthreads();
-            each([&](const Near &e) {
-                if (!(by_p ? e.p : e.k) || e.key < lo || e.key > hi) return;
-                atomicAdd(&S.mass[(hi - e.key) >> sh], e.w);
-                atomicAdd(&S.count[(hi - e.key) >> sh], 1u);
+            each([&](u64 key, u64 w) {
+                if (!(w & bit) || key < lo || key > hi) return;
+                atomicAdd(&S.mass[(hi - key) >> sh], w & kNearW);
+                atomicAdd(&S.count[(hi - key) >> sh], 1u);
             });
             __syncthreads();
-            u64 m[kSubPer], c[kSubPer], m_sum = 0, c_sum = 0, m_all, c_all;
+            u64 m[kSubPer], c[kSubPer], m_run = 0, c_run = 0;
 #pragma unroll
             for (int i = 0; i < kSubPer; ++i) {
                 m[i] = S.mass[t * kSubPer + i];
                 c[i] = S.count[t * kSubPer + i];
-                m_sum += m[i];
-                c_sum += c[i];
+                m_run += m[i];
+                c_run += c[i];
             }
-            u64 m_run = block_run(m_sum, S.sums, &m_all) - m_sum, c_run = block_run(c_sum, S.sums, &c_all) - c_sum;
+            const u64 m_mine = m_run, c_mine = c_run;
+            m_run = wave_run(m_run);
+            c_run = wave_run(c_run);
+            if (lane == 63) {
+                S.sums[0][wave] = m_run;
+                S.sums[1][wave] = c_run;
+            }
+            __syncthreads();
+            m_run -= m_mine;
+            c_run -= c_mine;
+            u64 m_all = 0;
+#pragma unroll
+            for (int o = 0; o < kSampleWaves; ++o) {
+                m_all += S.sums[0][o];
+                if (o < wave) {
+                    m_run += S.sums[0][o];
+                    c_run += S.sums[1][o];
+                }
+            }
 #pragma unroll
             for (int i = 0; i < kSubPer; ++i) {
                 const u64 run = by_p ? m_run : c_run, one = by_p ? m[i] : c[i];
@@ -669,6 +788,7 @@ struct Search {
             const uint32_t at = S.at, left = S.count_at;
             if (at == kSub) {
                 *mass = mass_sum + m_all;
+                __syncthreads();
                 return lo;
             }
             target -= S.before;
@@ -676,30 +796,46 @@ struct Search {
             hi -= (u64)at << sh;
             const u64 width = (1ull << sh) - 1;
             lo = hi - lo > width ? hi - width : lo;
-            __syncthreads();
-            if (left > kFew) continue;  // (a range of one key holds one token)
-            each([&](const Near &e) {
-                if (!(by_p ? e.p : e.k) || e.key < lo || e.key > hi) return;
+            if (left > kFew) {  // (a range of one key holds one token)
+                __syncthreads();
+                continue;
+            }
+            each([&](u64 key, u64 w) {
+                if (!(w & bit) || key < lo || key > hi) return;
                 const uint32_t place = atomicAdd(&S.few, 1u);
-                S.few_key[place] = e.key;
-                S.few_w[place] = e.w;
+                S.few_key[place] = key;
+                S.few_w[place] = w & kNearW;
             });
             __syncthreads();
             const bool is = lane < (int)left;
             u64 rest = 0;
             const u64 cut = wave_cut(is ? S.few_key[lane] : 0, is ? S.few_w[lane] : 0, is, by_p, target, &rest);
             *mass = mass_sum + rest;
+            __syncthreads();
             return cut;
         }
     }
 };
 
-// One block per row.
+// One block per row. Dynamic LDS: a sum a unit, of the list's weights where that has more than kFew.
 template <bool CAP>
 __global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(SampleArgs A) {
+    extern __shared__ u64 extra[];
     __shared__ PickShared S;
     const int t = threadIdx.x, lane = t & 63, row = blockIdx.x;
     const float *x = row_of(A, row);
+    // all that may be asked for, at once; of a row without cuts the last three are not used
+    const float u = A.u[row];
+    const u64 *list = A.list + (int64_t)row * kList;
+    const uint32_t n = A.listed[row];
+    const u64 first_key = list[lane];
+    const Cuts C = uniform(A.cut[row]);
+    u64 all = 0;
+    for (int c = lane; c < A.spans; c += 64) all += A.span_sums[(int64_t)row * A.spans + c];
+    const u64 *units = A.unit_sums + (int64_t)row * A.units;
+    const int per = (A.units + kSampleThreads - 1) / kSampleThreads, u0 = min(t * per, A.units), u1 = min(u0 + per, A.units);
+    u64 mine = 0;
+    for (int i = u0; i < u1; ++i) mine += units[i];
     const Row R = uniform(A.row[row]);
     if (R.index < 0) {
         if (t == 0) {
@@ -708,15 +844,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(SampleArgs 
         }
         return;
     }
-    // every wave by itself: the sum of all weights
-    u64 all = 0;
-    for (int c = lane; c < A.spans; c += 64) all += A.span_sums[(int64_t)row * A.spans + c];
-    const u64 *units = A.unit_sums + (int64_t)row * A.units;
-    const int per = (A.units + kSampleThreads - 1) / kSampleThreads, u0 = min(t * per, A.units), u1 = min(u0 + per, A.units);
-    u64 mine = 0;
-    if (!R.greedy)
-        for (int i = u0; i < u1; ++i) mine += units[i];
-    all = wave_sum(all);
+    all = wave_sum(all);  // every wave by itself
     if (R.greedy) {
         if (t == 0) {
             A.tokens[row] = R.index;
@@ -725,46 +853,42 @@ __global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(SampleArgs 
         return;
     }
     u64 cut = 0;  // the last kept key
-    bool spread = false;  // the list's weights are in S.extra
+    bool spread = false;  // the list's weights are in `extra`
     Near e{0, 0, false, false, false};
     u64 few = 0;  // lanes with an element that is kept
-    if (R.filtered) {
-        const Cuts C = uniform(A.cut[row]);
-        if (C.p_low < kBins) {
-            const uint32_t n = A.listed[row];
-            const u64 *list = A.list + (int64_t)row * kList;
-            u64 mass = all;
-            if (n <= kFew) {
-                e = near_of<CAP>(A, R, C, lane < (int)n ? list[lane] : 0);
-                if (C.k_bin < kBins) {
-                    cut = wave_cut(e.key, e.w, e.k, false, C.k_rest, &mass);
-                    mass += C.k_before;
-                }
-                if (R.p < 1.0)
-                    cut = wave_cut(e.key, e.w, e.p && e.key >= cut, true, mass_target(R.p, mass) - C.p_before, &mass);
-                few = __ballot((e.k || e.p) && e.key >= cut && e.kept);
-                for (u64 left = few; left; left &= left - 1) {
-                    const int j = __ffsll((long long)left) - 1;
-                    const int unit = (int)(~(uint32_t)__builtin_amdgcn_readlane((int)e.key, j) / kSampleUnit);
-                    const u64 w = lane64(e.w, j);
-                    mine += unit >= u0 && unit < u1 ? w : 0;
-                }
-            } else {
-                Search<CAP> L{A, R, C, x, S, list, (int)min(n, (uint32_t)kList + 1)};
-                if (C.k_bin < kBins) {
-                    cut = L.refine(false, 0, C.k_rest, &mass);
-                    mass += C.k_before;
-                }
-                if (R.p < 1.0) cut = L.refine(true, cut, mass_target(R.p, mass) - C.p_before, &mass);
-                for (int i = t; i < A.units; i += kSampleThreads) S.extra[i] = 0;
-                __syncthreads();
-                L.each([&](const Near &o) {
-                    if (o.key >= cut && o.kept) atomicAdd(&S.extra[~(uint32_t)o.key / kSampleUnit], o.w);
-                });
-                __syncthreads();
-                spread = true;
-                for (int i = u0; i < u1; ++i) mine += S.extra[i];
+    if (R.filtered && C.p_low < kBins) {
+        u64 mass = all;
+        if (n <= kFew) {
+            e = near_of<CAP>(A, R, C, lane < (int)n ? first_key : 0);
+            if (C.k_bin < kBins) {
+                cut = wave_cut(e.key, e.w, e.k, false, C.k_rest, &mass);
+                mass += C.k_before;
             }
+            if (R.p < 1.0)
+                cut = wave_cut(e.key, e.w, e.p && e.key >= cut, true, mass_target(R.p, mass) - C.p_before, &mass);
+            few = __ballot((e.k || e.p) && e.key >= cut && e.kept);
+            for (u64 left = few; left; left &= left - 1) {
+                const int j = __ffsll((long long)left) - 1;
+                const int unit = (int)(~(uint32_t)__builtin_amdgcn_readlane((int)e.key, j) / kSampleUnit);
+                const u64 w = lane64(e.w, j);
+                mine += unit >= u0 && unit < u1 ? w : 0;
+            }
+        } else {
+            Search<CAP> L{A, R, C, x, S, list, (int)min(n, (uint32_t)kList + 1)};
+            for (int i = t; i < A.units; i += kSampleThreads) extra[i] = 0;
+            L.begin();
+            if (C.k_bin < kBins) {
+                cut = L.refine(false, 0, C.k_rest, &mass);
+                mass += C.k_before;
+            }
+            if (R.p < 1.0) cut = L.refine(true, cut, mass_target(R.p, mass) - C.p_before, &mass);
+            L.each([&](u64 key, u64 w) {
+                if (key >= cut && (w & (kNearK | kNearP)) && (w & kNearKept))
+                    atomicAdd(&extra[~(uint32_t)key / kSampleUnit], w & kNearW);
+            });
+            __syncthreads();
+            spread = true;
+            for (int i = u0; i < u1; ++i) mine += extra[i];
         }
     }
     // the unit, then the token, where the running sum passes u of the total
@@ -773,13 +897,13 @@ __global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(SampleArgs 
         S.at = 0;
         S.before = 0;
     }
-    u64 run = block_run(mine, S.sums, &total) - mine;
-    const float uf = fminf(fmaxf(A.u[row], 0.0f), 0x1.fffffep-1f);  // NaN: 0
+    u64 run = block_run(mine, S.sums[0], &total) - mine;
+    const float uf = fminf(fmaxf(u, 0.0f), 0x1.fffffep-1f);  // NaN: 0
     u64 target = (u64)((double)uf * (double)total);
     const bool here = run <= target && target < run + mine;  // one thread
     if (__any(here)) {
         for (int i = u0; i < u1; ++i) {
-            u64 w = units[i] + (spread ? S.extra[i] : 0);
+            u64 w = units[i] + (spread ? extra[i] : 0);
             for (u64 left = few; left; left &= left - 1) {
                 const int j = __ffsll((long long)left) - 1;
                 if ((int)(~(uint32_t)__builtin_amdgcn_readlane((int)e.key, j) / kSampleUnit) == i) w += lane64(e.w, j);
@@ -805,7 +929,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(SampleArgs 
         w[i] = v > -INFINITY && d[i] >= R.d_min && order_key(v, id) >= cut ? steps(d[i], R, A) : 0;
         mine += w[i];
     }
-    run = block_run(mine, S.sums, &total) - mine;
+    run = block_run(mine, S.sums[1], &total) - mine;
     if (run <= target && target < run + mine) {
 #pragma unroll
         for (int i = 0; i < kUnitPer; ++i) {
@@ -827,12 +951,19 @@ static int launch_sample(const SampleArgs &A, int rows, hipStream_t s) {
     if (A.wide == 4) hipLaunchKernelGGL((sample_weights_kernel<CAP, 4>), grid, block, 0, s, A);
     else hipLaunchKernelGGL((sample_weights_kernel<CAP, 8>), grid, block, 0, s, A);
     G4_LAUNCHED("sample_weights_kernel");
-    if (A.cuts) {
+    if (A.cuts && (int64_t)A.spans * rows >= 16 * device_cu_count()) {
+        hipLaunchKernelGGL(sample_find_kernel, dim3((rows + kSampleWaves - 1) / kSampleWaves), dim3(kSampleThreads), 0, s, A,
+                           rows);
+        G4_LAUNCHED("sample_find_kernel");
+        const int per = kSampleWaves * kCutSpan;
+        hipLaunchKernelGGL(sample_cut_found_kernel<CAP>, dim3((A.units + per - 1) / per, rows), dim3(kSampleThreads), 0, s, A);
+        G4_LAUNCHED("sample_cut_found_kernel");
+    } else if (A.cuts) {
         if (A.wide == 4) hipLaunchKernelGGL((sample_cut_kernel<CAP, 4>), grid, block, 0, s, A);
         else hipLaunchKernelGGL((sample_cut_kernel<CAP, 8>), grid, block, 0, s, A);
         G4_LAUNCHED("sample_cut_kernel");
     }
-    hipLaunchKernelGGL(sample_pick_kernel<CAP>, dim3(rows), dim3(kSampleThreads), 0, s, A);
+    hipLaunchKernelGGL(sample_pick_kernel<CAP>, dim3(rows), dim3(kSampleThreads), A.units * sizeof(u64), s, A);
     G4_LAUNCHED("sample_pick_kernel");
     return G4_OK;
 }

@@ -200,6 +200,26 @@ def test_ends_of_the_arguments(gpu):
     both(logits, u, temperature=np.array(t, np.float32), top_k=k, top_p=np.array(p, np.float32), min_p=np.array(m, np.float32))
 
 
+def test_largest_vocabulary(gpu):
+    r = np.random.default_rng(12)
+    vocab = 1 << 22
+    logits = np.round(3 * r.standard_normal((3, vocab)), 2).astype(np.float32)
+    both(logits, [0.3, 0.7, 0.99], temperature=[1.0, 2.0, 0.5], top_k=[0, 3000000, 5000], top_p=[0.9, 0.99, 1.0], cap=30.0)
+
+
+def test_many_rows(gpu):
+    """Enough blocks for the cuts to be found by a kernel of their own."""
+    r = np.random.default_rng(13)
+    rows, vocab = 200, 70001
+    logits = (3 * r.standard_normal((rows, vocab))).astype(np.float32)
+    logits[::2, r.integers(0, vocab, 20)] += 15
+    logits[5] = np.nan
+    logits[9] = -np.inf
+    logits[20:24] = np.round(logits[20:24])
+    for cap in (0.0, 30.0):
+        both(logits, numbers(r, rows), cap=cap, **mixed(r, rows, vocab))
+
+
 def test_row_index_and_strides(gpu):
     """Several requests of one row, rows that no request has, an index outside; rows apart, aligned and not."""
     r = np.random.default_rng(6)

@@ -26,6 +26,7 @@ constexpr int kList = 4096;  // entries; a row with more is read again
 constexpr int kFew = 64;     // entries that a wave orders by itself
 constexpr int kSub = 1024, kSubPer = kSub / kSampleThreads;  // ranges of one refinement step
 constexpr int kUnitPer = kSampleUnit / kSampleThreads;
+constexpr int kLineWords = 32;
 constexpr int kMaxVocab = 1 << 22;
 
 struct PartMax {
@@ -66,7 +67,7 @@ struct SampleArgs {
     u64 *bin_mass;               // [rows][kBins]
     u64 *list;                   // [rows][kList]
     uint32_t *bin_count;         // [rows][kBins]
-    uint32_t *listed;            // [rows]
+    uint32_t *listed;            // [rows], kLineWords apart: rows' counters on lines of their own
     float *unit_max;             // [rows][units]
     int32_t *tokens;
     float *logprobs;
@@ -151,7 +152,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_max_kernel(SampleArgs A
             A.bin_mass[(int64_t)row * kBins + i] = 0;
             A.bin_count[(int64_t)row * kBins + i] = 0;
         }
-        if (part == 0 && t == 0) A.listed[row] = 0;
+        if (part == 0 && t == 0) A.listed[(int64_t)row * kLineWords] = 0;
     }
     __syncthreads();
     if (t) return;
@@ -235,7 +236,12 @@ __device__ __forceinline__ double raised_steps(double d, const Row &R, const Sam
 __device__ __forceinline__ u64 steps(double d, const Row &R, const SampleArgs &A) {
     return (u64)__double_as_longlong(raised_steps(d, R, A)) - kNoStepsBits;
 }
-__device__ __forceinline__ int bin_of(double d, const Row &R) { return min(max((int)(-d * R.bins), 0), kBins - 1); }
+// (The conversion takes what is below 0, a rounding, and a NaN to 0, and what is too large to the largest.)
+__device__ __forceinline__ int bin_of(double d, const Row &R) {
+    uint32_t b;
+    asm("v_cvt_u32_f64 %0, %1" : "=v"(b) : "v"(-d * R.bins));
+    return (int)min(b, (uint32_t)kBins - 1);
+}
 
 // Order of tokens: logit down, then id up, as a number (0: none).
 __device__ __forceinline__ u64 order_key(float x, int id) {
@@ -282,9 +288,18 @@ struct Bin {
     uint32_t count, pad;
 };
 
+// Four rows a block, a wave each: for calls of many blocks, each of which would do it again.
+__global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs A, int rows) {
+    const int row = blockIdx.x * kSampleWaves + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const Row R = row_params(A, row);
+    if ((threadIdx.x & 63) == 0) A.row[row] = R;
+}
+
 // Grid (spans, rows). Bound by issue: with a cap about 45 vector operations a logit, 27 of them 64-bit.
-template <bool CAP, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void sample_weights_kernel(SampleArgs A) {
+// READY: the rows' parameters are there (sample_row_kernel).
+template <bool CAP, int WAVES, bool READY>
+__global__ __launch_bounds__(64 * WAVES, 8) void sample_weights_kernel(SampleArgs A) {
     __shared__ Bin bins[kBins];
     __shared__ u64 ss[WAVES];
     __shared__ Row shared_row;
@@ -293,7 +308,10 @@ __global__ __launch_bounds__(64 * WAVES) void sample_weights_kernel(SampleArgs A
     const int unit = blockIdx.x * WAVES + wave, base = unit * kSampleUnit;
     float v[kSamplePer];
     load_unit(x + base, x ? A.vocab - base : 0, lane, A.vec, v);
-    if (wave == 0) {  // once a block: as many operations as the weights of a unit
+    Row given;
+    if (READY) {
+        given = A.row[row];
+    } else if (wave == 0) {  // once a block: as many operations as the weights of a unit
         const Row R = row_params(A, row);
         if (lane == 0) {
             shared_row = R;
@@ -303,7 +321,7 @@ __global__ __launch_bounds__(64 * WAVES) void sample_weights_kernel(SampleArgs A
     if (A.cuts)
         for (int i = t; i < kBins; i += 64 * WAVES) bins[i] = {0, 0, 0};
     __syncthreads();
-    const Row R = uniform(shared_row);
+    const Row R = uniform(READY ? given : shared_row);
     if (R.index < 0) return;
     if (R.inf) {
 #pragma unroll
@@ -316,8 +334,9 @@ __global__ __launch_bounds__(64 * WAVES) void sample_weights_kernel(SampleArgs A
             float xs = v[j];
             if (CAP) {
                 const bool f = is_far(xs, A.cap);
-                far |= __any(f) ? 1u << j : 0u;
+                far |= __ballot(f) ? 1u << j : 0u;
                 xs = f ? -INFINITY : xs;
+                asm("" : "+v"(xs));  // chosen here, in 32 bits, and not behind the conversion
             }
             add(near_distance<CAP>(xs, R, A));
         }
@@ -330,12 +349,14 @@ __global__ __launch_bounds__(64 * WAVES) void sample_weights_kernel(SampleArgs A
     };
     u64 all = 0;
     if (R.filtered) {
+        uint32_t one = 1;
+        asm("" : "+v"(one));  // kept, and not made again for each logit
         each([&](double d) {
             const double w = raised_steps(d, R, A);
             if (w > kNoSteps) {
                 Bin &b = bins[bin_of(d, R)];
                 atomicAdd(&b.mass, (u64)__double_as_longlong(w));
-                atomicAdd(&b.count, 1u);
+                atomicAdd(&b.count, one);
             }
         });
         __syncthreads();
@@ -505,8 +526,8 @@ __device__ __forceinline__ u64 cut_unit(const SampleArgs &A, const Row &R, const
     };
 #pragma unroll
     for (int j = 0; j < kSamplePer; ++j) {
-        look |= __any(v[j] >= c.least) ? 1u << j : 0u;
-        far |= CAP && __any(is_far(v[j], A.cap) && v[j] >= c.least) ? 1u << j : 0u;
+        look |= __ballot(v[j] >= c.least) ? 1u << j : 0u;
+        far |= CAP && __ballot(is_far(v[j], A.cap) && v[j] >= c.least) ? 1u << j : 0u;
     }
 #pragma unroll
     for (int j = 0; j < kSamplePer; ++j) {
@@ -522,7 +543,7 @@ __device__ __forceinline__ u64 cut_unit(const SampleArgs &A, const Row &R, const
         }
     if (many) {
         uint32_t at = 0;
-        if (lane == 0) at = atomicAdd(&A.listed[row], (uint32_t)many);
+        if (lane == 0) at = atomicAdd(&A.listed[(int64_t)row * kLineWords], (uint32_t)many);
         at = __shfl(at, 0);
 #pragma unroll
         for (int j = 0; j < kSamplePer; ++j) {
@@ -567,9 +588,9 @@ __global__ __launch_bounds__(64 * WAVES) void sample_cut_kernel(SampleArgs A) {
 
 // Grid (spans of kCutSpan units a wave, rows), behind sample_find_kernel: units that do not reach up to the cuts are not
 // read.
-constexpr int kCutSpan = 4;
+constexpr int kCutSpan = 2;
 template <bool CAP>
-__global__ __launch_bounds__(kSampleThreads) void sample_cut_found_kernel(SampleArgs A) {
+__global__ __launch_bounds__(kSampleThreads, 5) void sample_cut_found_kernel(SampleArgs A) {
     const int lane = threadIdx.x & 63, row = blockIdx.y;
     const int first = (blockIdx.x * kSampleWaves + (threadIdx.x >> 6)) * kCutSpan;
     const Row R = uniform(A.row[row]);
@@ -827,7 +848,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(SampleArgs 
     // all that may be asked for, at once; of a row without cuts the last three are not used
     const float u = A.u[row];
     const u64 *list = A.list + (int64_t)row * kList;
-    const uint32_t n = A.listed[row];
+    const uint32_t n = A.listed[(int64_t)row * kLineWords];
     const u64 first_key = list[lane];
     const Cuts C = uniform(A.cut[row]);
     u64 all = 0;
@@ -947,13 +968,20 @@ template <bool CAP>
 static int launch_sample(const SampleArgs &A, int rows, hipStream_t s) {
     hipLaunchKernelGGL(sample_max_kernel, dim3(A.parts, rows), dim3(kSampleThreads), 0, s, A);
     G4_LAUNCHED("sample_max_kernel");
-    const dim3 grid(A.spans, rows), block(64 * A.wide);
-    if (A.wide == 4) hipLaunchKernelGGL((sample_weights_kernel<CAP, 4>), grid, block, 0, s, A);
-    else hipLaunchKernelGGL((sample_weights_kernel<CAP, 8>), grid, block, 0, s, A);
+    const dim3 grid(A.spans, rows), block(64 * A.wide), by_row((rows + kSampleWaves - 1) / kSampleWaves);
+    const bool many = (int64_t)A.spans * rows >= 16 * device_cu_count();
+    if (many) {
+        hipLaunchKernelGGL(sample_row_kernel, by_row, dim3(kSampleThreads), 0, s, A, rows);
+        G4_LAUNCHED("sample_row_kernel");
+        hipLaunchKernelGGL((sample_weights_kernel<CAP, 8, true>), grid, block, 0, s, A);
+    } else if (A.wide == 4) {
+        hipLaunchKernelGGL((sample_weights_kernel<CAP, 4, false>), grid, block, 0, s, A);
+    } else {
+        hipLaunchKernelGGL((sample_weights_kernel<CAP, 8, false>), grid, block, 0, s, A);
+    }
     G4_LAUNCHED("sample_weights_kernel");
-    if (A.cuts && (int64_t)A.spans * rows >= 16 * device_cu_count()) {
-        hipLaunchKernelGGL(sample_find_kernel, dim3((rows + kSampleWaves - 1) / kSampleWaves), dim3(kSampleThreads), 0, s, A,
-                           rows);
+    if (A.cuts && many) {
+        hipLaunchKernelGGL(sample_find_kernel, by_row, dim3(kSampleThreads), 0, s, A, rows);
         G4_LAUNCHED("sample_find_kernel");
         const int per = kSampleWaves * kCutSpan;
         hipLaunchKernelGGL(sample_cut_found_kernel<CAP>, dim3((A.units + per - 1) / per, rows), dim3(kSampleThreads), 0, s, A);
@@ -981,7 +1009,7 @@ size_t g4_sample_workspace_bytes(int rows, int64_t vocab) {
     if (rows <= 0 || rows > 65535 || vocab <= 0 || vocab > kMaxVocab) return 0;
     const size_t row = (size_t)sample_parts(vocab) * (sizeof(PartMax) + sizeof(u64)) +
                        (size_t)sample_units(vocab) * (sizeof(u64) + sizeof(float)) + kBins * (sizeof(u64) + sizeof(uint32_t)) +
-                       kList * sizeof(u64) + sizeof(Row) + sizeof(Cuts) + sizeof(uint32_t);
+                       kList * sizeof(u64) + sizeof(Row) + sizeof(Cuts) + kLineWords * sizeof(uint32_t);
     return rows * row;
 }
 
@@ -1037,7 +1065,7 @@ int g4_sample_tokens(const float *logits, int logit_rows, int64_t logit_stride, 
     A.list = A.bin_mass + (int64_t)rows * kBins;
     A.bin_count = reinterpret_cast<uint32_t *>(A.list + (int64_t)rows * kList);
     A.listed = A.bin_count + (int64_t)rows * kBins;
-    A.unit_max = reinterpret_cast<float *>(A.listed + rows);
+    A.unit_max = reinterpret_cast<float *>(A.listed + (int64_t)rows * kLineWords);
     A.tokens = tokens;
     A.logprobs = logprobs;
     hipStream_t s = as_stream(stream);

@@ -4,10 +4,13 @@
 // The rows are grouped by adapter once a step (adapter_groups_kernel): a tile is up to 16 rows of one adapter, so that
 // a matrix instruction's other operand is that adapter's. Both products are transposed, the adapter's rows by the
 // batch's: what a lane holds of H = x A^T, four ranks of one row, is its operand of the second product, and there it has
-// runs of consecutive outputs of one row. Operands come straight from global memory, each used by one wave.
+// runs of consecutive outputs of one row.
 //
 // Few rows: one launch, every block computes its tile's H for itself. Many: H in f32 by tile pair and range of K, then
 // a block per tile and range of outputs, which adds up H's parts.
+//
+// A, x and B come to LDS in whole lines. A matrix instruction's operands straight from memory are 16 rows' 64 bytes a
+// load, which a CU's first-level cache gives at 16 bytes a cycle; whole lines at 58.
 #include "g4_internal.h"
 #include "../../include/g4serve.h"
 
@@ -161,84 +164,170 @@ __device__ __forceinline__ int rank_of(const AdapterArgs &A, int adapter) {
     return A.ranks ? min(max(A.ranks[adapter], 0), A.max_rank) : A.max_rank;
 }
 
-// Eight elements of x from `at` on as f32 or, where the type is exact in it, f16.
+// Eight elements of x as f32 or, where the type is exact in it, f16.
 template <int XK>
-struct XLoad {
+struct XPart {
     h8 v;
-    __device__ __forceinline__ void load(const void *x, int64_t at, bool in) {
-        v = h8{};
-        if (!in) return;
-        if (XK == G4_KIND_F16) {
-            v = *reinterpret_cast<const h8 *>(static_cast<const _Float16 *>(x) + at);
-        } else {
-            const uint2 c = *reinterpret_cast<const uint2 *>(static_cast<const int8_t *>(x) + at);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = (_Float16)(float)(int8_t)((e < 4 ? c.x : c.y) >> (8 * (e % 4)));
-        }
-    }
 };
 template <>
-struct XLoad<G4_KIND_F32> {
+struct XPart<G4_KIND_F32> {
     f4 v[2];
-    __device__ __forceinline__ void load(const void *x, int64_t at, bool in) {
-        v[0] = v[1] = f4{};
-        if (!in) return;
-        const f4 *p = reinterpret_cast<const f4 *>(static_cast<const float *>(x) + at);
-        v[0] = p[0];
-        v[1] = p[1];
-    }
 };
 
 template <int XK>
-__device__ __forceinline__ f4 product(h8 a, const XLoad<XK> &x, f4 c) {
+__device__ __forceinline__ f4 product(h8 a, const XPart<XK> &x, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, x.v, c, 0, 0, 0);
 }
 template <>
-__device__ __forceinline__ f4 product<G4_KIND_F32>(h8 a, const XLoad<G4_KIND_F32> &x, f4 c) {
+__device__ __forceinline__ f4 product<G4_KIND_F32>(h8 a, const XPart<G4_KIND_F32> &x, f4 c) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32((float)a[e], x.v[e / 4][e % 4], c, 0, 0, 0);
     return c;
 }
 
-// Steps of shrink that are loaded at once: what 150 registers hold (less what else is on its way), at most 8.
-constexpr int unroll_of(int xk, int rt, int mt, int less) {
-    const int step = mt * (xk == G4_KIND_F32 ? 8 : 4) + 4 * rt, n = (150 - less) / step;
-    return n < 1 ? 1 : n > 8 ? 8 : n;
+// 16 (4) bytes a lane from memory to LDS at lds + 16 (4) * lane. Through asm, with waits of the kernel's own: the compiler
+// would wait for every load before the next LDS read. Nothing else here uses M0.
+__device__ __forceinline__ void dma16(const void *src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src) : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(const void *src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+                 :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(src) : "memory", "m0");
+}
+// At most N of the wave's loads are still on their way.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    static_assert(N >= 0 && N < 64, "vmcnt holds 6 bits");
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+}
+// Every wave's LDS reads and writes are done, and what each has waited for is there.
+__device__ __forceinline__ void block_meet() {
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void *p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p;
 }
 
-// acc[i][r] += the products over the wave's part of [k0, k1), a run of whole lines of the rows, in steps of 32: tile i's
-// rows by A's rows 16 r ..; RT: the pool's rank in tiles. UNROLL steps are loaded before the first is used; rows of A
-// behind the adapter's rank are loaded, so that the rank comes with them and not before, and replaced.
-template <int XK, int RT, int MT, int WAVES, int UNROLL>
-__device__ __forceinline__ void shrink(const AdapterArgs &A, const _Float16 *a, int rank, const int64_t (&row)[MT], int k0,
-                                       int k1, int wave, f4 (&acc)[MT][RT]) {
-    const int lane = threadIdx.x & 63, col = lane & 15, group = lane >> 4;
-    const int part = ((k1 - k0 + WAVES - 1) / WAVES + 63) / 64 * 64, from = k0 + wave * part, end = min(from + part, k1);
-#pragma unroll 1
-    for (int k = from; k < end; k += 32 * UNROLL) {
-        XLoad<XK> x[UNROLL][MT];
-        h8 w[UNROLL][RT];
+constexpr int kWaves = 8, kAdThreads = 64 * kWaves;
+constexpr int kChunk = 32 * kWaves;  // of K: a step of a matrix instruction for each wave
+
+// The ring through which chunks of A's and x's rows come: row r of A's 16 RT at 512 r, of x's 16 MT at X + r * XROW. A
+// row's units of 16 bytes stand at their number XOR (r % 8), for reads of one unit of eight rows at a time.
+template <int XK, int RT, int MT, int ROOM>
+struct Ring {
+    static constexpr int XROW = kChunk * (XK == G4_KIND_F32 ? 4 : XK == G4_KIND_F16 ? 2 : 1);
+    static constexpr int X = RT * 16 * kChunk * 2, BYTES = X + MT * 16 * XROW;
+    static constexpr int SLOTS = ROOM / BYTES < 8 ? ROOM / BYTES : 8;
+    static constexpr int XLOADS = XK == G4_KIND_F16 ? MT : 2 * MT, LOADS = RT + XLOADS;  // of a wave and chunk
+    static_assert(SLOTS >= 2 && (SLOTS - 2) * LOADS < 64, "one chunk is read, others are on their way");
+};
+
+// acc[i][r] += tile i's rows by A's rows r0 + 16 r .. over [k0, k1), a wave taking 32 of each chunk's 256. row: the rows of
+// x of the lane's column. Loads never leave the matrices: places behind their ends read the last unit or row, and
+// enter as 0.
+template <int XK, int RT, int MT, int ROOM>
+__device__ __forceinline__ void shrink(const AdapterArgs &A, const _Float16 *a, int rank, int r0, const int (&row)[MT], int k0,
+                                       int k1, char *lds, f4 (&acc)[MT][RT]) {
+    typedef Ring<XK, RT, MT, ROOM> G;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
+    const uint32_t lds0 = lds_address(lds);
+    const int chunks = (k1 - k0 + kChunk - 1) / kChunk;
+    if (chunks <= 0) return;
+    // A's rows come by pairs; the lane's row and element of a chunk in each of its wave's loads
+    const char *from[RT], *xfrom[G::XLOADS];
+    int at[RT], xat[G::XLOADS];
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int at = k + 32 * u + 8 * group;
-            const bool in = at < end;
+    for (int i = 0; i < RT; ++i) {
+        const int r = 2 * (wave * RT + i) + lane / 32;
+        from[i] = reinterpret_cast<const char *>(a + (int64_t)min(r0 + r, A.max_rank - 1) * A.k);
+        at[i] = 8 * (lane % 32 ^ r % 8);
+    }
 #pragma unroll
-            for (int i = 0; i < MT; ++i) x[u][i].load(A.x, row[i] * A.x_stride + at, in);
+    for (int i = 0; i < G::XLOADS; ++i) {
+        const int r = XK == G4_KIND_F16 ? 2 * (wave * MT + i) + lane / 32 : wave * 2 * MT + i;
+        int token = row[0];
+        if (MT == 1) {
+            token = __shfl(row[0], r % 16);
+        } else {
+            const int t0 = __shfl(row[0], r % 16), t1 = __shfl(row[MT - 1], r % 16);
+            token = r < 16 ? t0 : t1;
+        }
+        xfrom[i] = static_cast<const char *>(A.x) + token * A.x_stride * (G::XROW / kChunk);
+        xat[i] = XK == G4_KIND_F16 ? 8 * (lane % 32 ^ r % 8) : XK == G4_KIND_F32 ? 4 * (lane ^ r % 8)
+                                                                                 : 16 * (lane / 4 ^ r % 8) + 4 * (lane % 4);
+    }
+    auto issue = [&](int c) {
+        const uint32_t slot = lds0 + c % G::SLOTS * G::BYTES;
+        const int k = k0 + c * kChunk;
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                w[u][r] = h8{};
-                if (in && 16 * r + col < A.max_rank) w[u][r] = *reinterpret_cast<const h8 *>(a + (16 * r + col) * A.k + at);
+        for (int i = 0; i < RT; ++i) dma16(from[i] + 2 * (int64_t)min(k + at[i], A.k - 8), slot + (wave * RT + i) * 1024);
+#pragma unroll
+        for (int i = 0; i < G::XLOADS; ++i) {
+            if (XK == G4_KIND_I8) {
+                dma4(xfrom[i] + min(k + xat[i], A.k - 4), slot + G::X + (wave * 2 * MT + i) * 256);
+            } else if (XK == G4_KIND_F16) {
+                dma16(xfrom[i] + 2 * (int64_t)min(k + xat[i], A.k - 8), slot + G::X + (wave * MT + i) * 1024);
+            } else {
+                dma16(xfrom[i] + 4 * (int64_t)min(k + xat[i], A.k - 4), slot + G::X + (wave * 2 * MT + i) * 1024);
+            }
+        }
+    };
+    for (int c = 0; c < min(G::SLOTS - 1, chunks); ++c) issue(c);
+    for (int c = 0; c < chunks; ++c) {
+        if (c + G::SLOTS - 2 < chunks) wait_loads<(G::SLOTS - 2) * G::LOADS>();
+        else wait_loads<0>();
+        block_meet();  // chunk c is there, and chunk c - 1 has been read
+        if (c + G::SLOTS - 1 < chunks) issue(c + G::SLOTS - 1);
+        const char *slot = lds + c % G::SLOTS * G::BYTES;
+        const bool in = k0 + c * kChunk + 32 * wave + 8 * group < k1;
+        XPart<XK> x[MT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const char *p = slot + G::X + (16 * i + col) * G::XROW;
+            if constexpr (XK == G4_KIND_F32) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const f4 v = *reinterpret_cast<const f4 *>(p + ((8 * wave + 2 * group + e) ^ col % 8) * 16);
+                    x[i].v[e] = in ? v : f4{};
+                }
+            } else if constexpr (XK == G4_KIND_F16) {
+                const h8 v = *reinterpret_cast<const h8 *>(p + ((4 * wave + group) ^ col % 8) * 16);
+                x[i].v = in ? v : h8{};
+            } else {
+                uint2 q = *reinterpret_cast<const uint2 *>(p + ((2 * wave + group / 2) ^ col % 8) * 16 + group % 2 * 8);
+                if (!in) q = make_uint2(0, 0);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[i].v[e] = (_Float16)(float)(int8_t)((e < 4 ? q.x : q.y) >> (8 * (e % 4)));
             }
         }
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
+        for (int r = 0; r < RT; ++r) {
+            const h8 v = *reinterpret_cast<const h8 *>(slot + (16 * r + col) * (kChunk * 2) + ((4 * wave + group) ^ col % 8) * 16);
+            const h8 w = in && r0 + 16 * r + col < rank ? v : h8{};
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const h8 v = 16 * r + col < rank ? w[u][r] : h8{};
-#pragma unroll
-                for (int i = 0; i < MT; ++i) acc[i][r] = product<XK>(v, x[u][i], acc[i][r]);
-            }
+            for (int i = 0; i < MT; ++i) acc[i][r] = product<XK>(w, x[i], acc[i][r]);
+        }
     }
+    block_meet();  // the ring is free
+}
+
+// The block's sum of the waves' acc, each tile's and rank tile's f4 by lane, at `part`.
+template <int N>
+__device__ __forceinline__ void sum_waves(const f4 (&acc)[N], f4 *part) {
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[(wave * N + i) * 64 + lane] = acc[i];
+    __syncthreads();
+    for (int i = t; i < N * 64; i += kAdThreads) {
+        f4 s = part[i];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) s += part[w * N * 64 + i];
+        part[i] = s;
+    }
+    __syncthreads();
 }
 
 __device__ __forceinline__ f4 multiply(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -335,8 +424,25 @@ __device__ __forceinline__ void store8(void *p, int kind, int64_t at, int n, boo
     }
 }
 
-constexpr int kOutWaves = 8, kOutThreads = 64 * kOutWaves;  // of a block that writes outputs
-constexpr int kWaveN = 64, kBlockN = kOutWaves * kWaveN;    // outputs of a wave, and of a block, at a time
+constexpr int kWaveN = 64, kBlockN = kWaves * kWaveN;  // outputs of a wave, and of a block, at a time
+
+// B's rows n0 .. n0 + 511 at `lds`, max_rank halves each; loads of whole lines (see Ring). A row's units of 16 bytes
+// stand at their number XOR unit_xor(row): a product's lanes read one unit of rows 0-3 and 8-11 at a time.
+__device__ __forceinline__ int unit_xor(int row, int units) {
+    return units == 8 || units == 16 ? (row & 3) | (row >> 1 & 4)
+           : units == 4              ? (row >> 1 & 1) | (row >> 2 & 2)
+           : units == 2              ? row >> 3 & 1
+                                     : 0;
+}
+__device__ __forceinline__ void load_b(const AdapterArgs &A, const _Float16 *b, int n0, char *lds) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, units = A.max_rank / 8;
+    const uint32_t lds0 = lds_address(lds), by_units = 0xffffffffu / units + 1;
+    for (int i = 0; i < units; ++i) {
+        const int place = (wave * units + i) * 64 + lane, row = units == 1 ? place : (int)__umulhi(place, by_units);
+        const int unit = (place - row * units) ^ unit_xor(row, units);
+        dma16(b + (int64_t)min(n0 + row, A.n - 1) * A.max_rank + 8 * unit, lds0 + (wave * units + i) * 1024);
+    }
+}
 
 // A wave's 64 outputs of a tile's rows. Tile j of the product has the outputs n0 + 32 (j / 2) + 8 q + 4 (j % 2) + e,
 // q its row's group and e its place there, so that a lane has eight consecutive outputs in each pair of tiles.
@@ -345,22 +451,13 @@ struct Expand {
     // A lane's ranks of a product: eight consecutive ones of 32, or four of 16 where there are no more.
     static constexpr int kRanks = RT == 1 ? 4 : 8, kSteps = RT == 1 ? 1 : RT / 2;
     typedef _Float16 hr __attribute__((ext_vector_type(kRanks)));
-    hr w[kSteps][4];
     Raw8 raw[2];
     int n0;
 
-    // Loads what does not depend on H.
-    __device__ __forceinline__ void load(const AdapterArgs &A, const Tile &T, const _Float16 *b, int64_t row, int n) {
+    // Loads the wave's part of base.
+    __device__ __forceinline__ void load(const AdapterArgs &A, const Tile &T, int64_t row, int n) {
         const int lane = threadIdx.x & 63, col = lane & 15, group = lane >> 4;
         n0 = n;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int at = kRanks * (4 * s + group), out = n0 + 32 * (j / 2) + 8 * (col / 4) + 4 * (j % 2) + col % 4;
-                w[s][j] = hr{};
-                if (at < A.max_rank && out < A.n) w[s][j] = *reinterpret_cast<const hr *>(b + (int64_t)out * A.max_rank + at);
-            }
         if (!A.base || col >= T.rows) return;
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
@@ -369,11 +466,12 @@ struct Expand {
         }
     }
 
-    // h: the tile's H in LDS, as the first product leaves it, [rank tile][lane], a lane's four ranks of its row. H enters the
-    // product as the sum of two f16 values, relative to the row's largest: off by 2^-23 of itself, as by two roundings to
-    // f32.
-    __device__ __forceinline__ void finish(const AdapterArgs &A, const Tile &T, const f4 *h, int rank, float scale, int64_t row) {
-        const int lane = threadIdx.x & 63, col = lane & 15, group = lane >> 4;
+    // h: the tile's H in LDS, as the first product leaves it, [rank tile][lane], a lane's four ranks of its row; b: of
+    // load_b. H enters the product as the sum of two f16 values, relative to the row's largest: off by 2^-23 of itself,
+    // as by two roundings to f32.
+    __device__ __forceinline__ void finish(const AdapterArgs &A, const Tile &T, const f4 *h, const char *b, int rank, float scale,
+                                           int64_t row) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
         f4 acc[4] = {f4{}, f4{}, f4{}, f4{}};
         if (rank > 0) {
             float v[kSteps][kRanks];
@@ -399,9 +497,11 @@ struct Expand {
             up = min(max(up, -120), 120);
             const float to = __uint_as_float((uint32_t)(127 + up) << 23);
             scale *= __uint_as_float((uint32_t)(127 - up) << 23);
+            const int units = A.max_rank / 8;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 if (4 * kRanks * s >= rank) break;
+                const int at = kRanks * (4 * s + group);
                 hr hi, lo;
 #pragma unroll
                 for (int e = 0; e < kRanks; ++e) {
@@ -411,11 +511,14 @@ struct Expand {
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    hr b = w[s][j];
+                    const int r = wave * kWaveN + 32 * (j / 2) + 8 * (col / 4) + 4 * (j % 2) + col % 4;
+                    hr w{};
+                    if (at < A.max_rank)
+                        w = *reinterpret_cast<const hr *>(b + (r * units + (at / 8 ^ unit_xor(r, units))) * 16 + at % 8 * 2);
 #pragma unroll
-                    for (int e = 0; e < kRanks; ++e) b[e] = kRanks * (4 * s + group) + e < rank ? b[e] : (_Float16)0.0f;
-                    acc[j] = multiply(b, hi, acc[j]);
-                    acc[j] = multiply(b, lo, acc[j]);
+                    for (int e = 0; e < kRanks; ++e) w[e] = at + e < rank ? w[e] : (_Float16)0.0f;
+                    acc[j] = multiply(w, hi, acc[j]);
+                    acc[j] = multiply(w, lo, acc[j]);
                 }
             }
         }
@@ -439,53 +542,60 @@ __device__ __forceinline__ float scale_of(const AdapterArgs &A, int adapter) {
     return adapter < 0 ? 0.0f : (A.scales ? A.scales[adapter] : 1.0f) * A.x_scale;
 }
 
-// Grid (ranges of outputs, tiles): H, then the outputs.
+constexpr int kLds = 144 << 10;  // what a block takes of a CU's 160 KB
+
+// Grid (ranges of outputs, tiles): H, then the outputs, in rounds of 512.
 template <int XK, int RT>
-__global__ __launch_bounds__(kOutThreads) void adapter_fused_kernel(AdapterArgs A) {
-    __shared__ f4 part[kOutWaves][RT * 64];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 15;
+__global__ __launch_bounds__(kAdThreads) void adapter_fused_kernel(AdapterArgs A) {
+    constexpr int kRoom = kLds - RT * 16 * kBlockN * 2;
+    typedef Ring<XK, RT, 1, kRoom> G;
+    __shared__ __align__(1024) char lds[G::SLOTS * G::BYTES], b_lds[RT * 16 * kBlockN * 2];
+    static_assert(G::SLOTS * G::BYTES >= kWaves * RT * 64 * (int)sizeof(f4), "the waves' sums take the ring's place");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15;
     const Tile T = tile_of(A, blockIdx.y);
     const int tiles = tiles_of(A);
     if ((int)blockIdx.y >= tiles) return;
-    const int64_t row[1] = {row_of(A, T, col)};
-    const int rank = T.adapter < 0 ? 0 : rank_of(A, T.adapter);
-    const float scale = scale_of(A, T.adapter);
+    const int row[1] = {(int)row_of(A, T, col)};
+    const bool some = T.adapter >= 0;
     const _Float16 *b = A.b + max(T.adapter, 0) * A.b_stride;
     const int end = min((int)(blockIdx.x + 1) * A.n_range, A.n);
-    int n = blockIdx.x * A.n_range + wave * kWaveN;
+    int n = blockIdx.x * A.n_range;
     Expand<RT> E;
-    E.load(A, T, b, row[0], n);
-    if (rank > 0) {
+    E.load(A, T, row[0], n + wave * kWaveN);
+    if (some) load_b(A, b, n, b_lds);
+    const int rank = some ? rank_of(A, T.adapter) : 0;
+    const float scale = scale_of(A, T.adapter);
+    f4 *const h = reinterpret_cast<f4 *>(lds);
+    if (some) {
         f4 acc[1][RT];
 #pragma unroll
         for (int r = 0; r < RT; ++r) acc[0][r] = f4{};
-        shrink<XK, RT, 1, kOutWaves, unroll_of(XK, RT, 1, 8 * RT)>(A, A.a + T.adapter * A.a_stride, rank, row, 0, A.k, wave, acc);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) part[wave][r * 64 + lane] = acc[0][r];
-        __syncthreads();
-        for (int i = t; i < RT * 64; i += kOutThreads) {
-            f4 s = part[0][i];
-#pragma unroll
-            for (int w = 1; w < kOutWaves; ++w) s += part[w][i];
-            part[0][i] = s;
-        }
-        __syncthreads();
+        shrink<XK, RT, 1, kRoom>(A, A.a + T.adapter * A.a_stride, rank, 0, row, 0, A.k, lds, acc);
+        sum_waves<RT>(acc[0], h);
     }
     while (true) {
-        E.finish(A, T, part[0], rank, scale, row[0]);
+        E.finish(A, T, h, b_lds, rank, scale, row[0]);
         n += kBlockN;
-        if (n - wave * kWaveN >= end) return;
-        E.load(A, T, b, row[0], n);
+        if (n >= end) return;
+        E.load(A, T, row[0], n + wave * kWaveN);
+        if (some) {
+            block_meet();
+            load_b(A, b, n, b_lds);
+            wait_loads<0>();
+            block_meet();
+        }
     }
 }
 
-constexpr int kHWaves = 4, kHThreads = 64 * kHWaves;  // of a block that makes a part of H
-
-// Grid (splits, pairs of tiles): a range of K of the tiles' H. Two tiles of one adapter share its rows of A.
+// Grid (splits, pairs of tiles, ranks by 64): a range of K of the tiles' H. Two tiles of one adapter share its rows of A.
 template <int XK, int RT>
-__global__ __launch_bounds__(kHThreads) void adapter_shrink_kernel(AdapterArgs A) {
-    __shared__ f4 part[kHWaves][2 * RT * 64];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 15;
+__global__ __launch_bounds__(kAdThreads) void adapter_shrink_kernel(AdapterArgs A) {
+    typedef Ring<XK, RT, 2, kLds> G;
+    typedef Ring<XK, RT, 1, kLds> One;
+    constexpr int kRing = G::SLOTS * G::BYTES > One::SLOTS * One::BYTES ? G::SLOTS * G::BYTES : One::SLOTS * One::BYTES;
+    constexpr int kSums = kWaves * 2 * RT * 64 * (int)sizeof(f4);
+    __shared__ __align__(1024) char lds[kRing > kSums ? kRing : kSums];
+    const int t = threadIdx.x, lane = t & 63, col = lane & 15, r0 = 64 * blockIdx.z;
     const int first = 2 * blockIdx.y, tiles = min(tiles_of(A) - first, 2);
     if (tiles <= 0) return;
     const Tile T0 = tile_of(A, first), T1 = tile_of(A, tiles > 1 ? first + 1 : first);
@@ -493,61 +603,58 @@ __global__ __launch_bounds__(kHThreads) void adapter_shrink_kernel(AdapterArgs A
     f4 acc[2][RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) acc[0][r] = acc[1][r] = f4{};
-    const int64_t row[2] = {row_of(A, T0, col), row_of(A, T1, col)};
+    const int row[2] = {(int)row_of(A, T0, col), (int)row_of(A, T1, col)};
     if (T0.adapter == T1.adapter) {
         if (T0.adapter < 0) return;
-        shrink<XK, RT, 2, kHWaves, unroll_of(XK, RT, 2, 0)>(A, A.a + T0.adapter * A.a_stride, rank_of(A, T0.adapter), row, k0, k1,
-                                                            wave, acc);
+        shrink<XK, RT, 2, kLds>(A, A.a + T0.adapter * A.a_stride, rank_of(A, T0.adapter), r0, row, k0, k1, lds, acc);
     } else {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int adapter = i ? T1.adapter : T0.adapter;
             if (adapter < 0) continue;
-            const int64_t one[1] = {row[i]};
+            const int alone[1] = {row[i]};
             f4 mine[1][RT];
 #pragma unroll
             for (int r = 0; r < RT; ++r) mine[0][r] = f4{};
-            shrink<XK, RT, 1, kHWaves, unroll_of(XK, RT, 2, 0)>(A, A.a + adapter * A.a_stride, rank_of(A, adapter), one, k0, k1,
-                                                                wave, mine);
+            shrink<XK, RT, 1, kLds>(A, A.a + adapter * A.a_stride, rank_of(A, adapter), r0, alone, k0, k1, lds, mine);
 #pragma unroll
             for (int r = 0; r < RT; ++r) acc[i][r] = mine[0][r];
         }
     }
+    f4 both[2 * RT];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) part[wave][(i * RT + r) * 64 + lane] = acc[i][r];
-    __syncthreads();
-    for (int i = t; i < tiles * RT * 64; i += kHThreads) {
+    for (int r = 0; r < RT; ++r) {
+        both[r] = acc[0][r];
+        both[RT + r] = acc[1][r];
+    }
+    f4 *const part = reinterpret_cast<f4 *>(lds);
+    sum_waves<2 * RT>(both, part);
+    for (int i = t; i < tiles * RT * 64; i += kAdThreads) {
         const bool second = i >= RT * 64;
-        const int r = i / 64 % RT, l = i & 63, place = (second ? T1.first : T0.first) + (l & 15);
-        f4 s = part[0][i];
-#pragma unroll
-        for (int w = 1; w < kHWaves; ++w) s += part[w][i];
-        if ((l & 15) < (second ? T1.rows : T0.rows) && 16 * r < A.rank16)
-            *reinterpret_cast<f4 *>(A.h + ((int64_t)blockIdx.x * A.tokens + place) * A.rank16 + 16 * r + 4 * (l >> 4)) = s;
+        const int r = r0 + i / 64 % RT * 16, l = i & 63, place = (second ? T1.first : T0.first) + (l & 15);
+        if ((l & 15) < (second ? T1.rows : T0.rows) && r < A.rank16)
+            *reinterpret_cast<f4 *>(A.h + ((int64_t)blockIdx.x * A.tokens + place) * A.rank16 + r + 4 * (l >> 4)) = part[i];
     }
 }
 
-// Grid (ranges of outputs, tiles).
-// (128 registers: two blocks a CU)
+// Grid (ranges of 512 outputs, tiles).
 template <int RT>
-__global__ __launch_bounds__(kOutThreads, RT <= 4 ? 4 : 2) void adapter_expand_kernel(AdapterArgs A) {
+__global__ __launch_bounds__(kAdThreads) void adapter_expand_kernel(AdapterArgs A) {
     __shared__ f4 h[RT * 64];
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 15;
+    __shared__ __align__(1024) char b_lds[RT * 16 * kBlockN * 2];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, col = lane & 15, n = blockIdx.x * kBlockN;
     const Tile T = tile_of(A, blockIdx.y);
     const int tiles = tiles_of(A);
     if ((int)blockIdx.y >= tiles) return;
     const int64_t row = row_of(A, T, col);
-    const int rank = T.adapter < 0 ? 0 : rank_of(A, T.adapter);
-    const float scale = scale_of(A, T.adapter);
-    const _Float16 *b = A.b + max(T.adapter, 0) * A.b_stride;
-    const int end = min((int)(blockIdx.x + 1) * A.n_range, A.n);
-    int n = blockIdx.x * A.n_range + wave * kWaveN;
+    const bool some = T.adapter >= 0;
+    if (some) load_b(A, A.b + T.adapter * A.b_stride, n, b_lds);
     Expand<RT> E;
-    E.load(A, T, b, row, n);
-    if (rank > 0) {
-        for (int i = t; i < RT * 64; i += kOutThreads) {
+    E.load(A, T, row, n + wave * kWaveN);
+    const int rank = some ? rank_of(A, T.adapter) : 0;
+    const float scale = scale_of(A, T.adapter);
+    if (some) {
+        for (int i = t; i < RT * 64; i += kAdThreads) {
             const int r = i >> 6, l = i & 63;
             if (16 * r >= A.rank16) break;
             const float *p = A.h + (int64_t)(T.first + min(l & 15, T.rows - 1)) * A.rank16 + 16 * r + 4 * (l >> 4);
@@ -556,14 +663,10 @@ __global__ __launch_bounds__(kOutThreads, RT <= 4 ? 4 : 2) void adapter_expand_k
             for (int j = 0; j < A.splits; ++j) s += *reinterpret_cast<const f4 *>(p + (int64_t)j * A.tokens * A.rank16);
             h[i] = s;
         }
-        __syncthreads();
+        wait_loads<0>();
+        block_meet();
     }
-    while (true) {
-        E.finish(A, T, h, rank, scale, row);
-        n += kBlockN;
-        if (n - wave * kWaveN >= end) return;
-        E.load(A, T, b, row, n);
-    }
+    E.finish(A, T, h, b_lds, rank, scale, row);
 }
 
 // How a call is run: in one launch (splits 0), or with H's parts of `splits` ranges of K.
@@ -571,37 +674,36 @@ static int adapter_splits(const g4_adapters *D, int tokens, int x_size) {
     const int64_t tiles = max_tiles(tokens, D->count), ranges = (D->n + 2 * kBlockN - 1) / (2 * kBlockN);
     const int64_t again = tiles * ranges * D->k * (2 * D->max_rank + kTile * x_size);
     const int64_t cycles = (D->k / 32) * ((D->max_rank + 15) / 16) * (x_size == 4 ? 256 : 16) / 4;
-    if (again <= kFusedBytes && cycles <= kFusedCycles) return 0;
-    const int64_t pairs = (tiles + 1) / 2, most = (D->k + 32 * kHWaves - 1) / (32 * kHWaves);
-    int64_t want = 512 / pairs;  // two blocks a CU at once
+    const bool fits = D->max_rank <= (x_size == 4 ? 32 : 64);
+    if (fits && again <= kFusedBytes && cycles <= kFusedCycles) return 0;
+    const int64_t pairs = (tiles + 1) / 2, most = (D->k + kChunk - 1) / kChunk;
+    int64_t want = device_cu_count() / (pairs * ((D->max_rank + 63) / 64));  // a block a CU at once
     want = want < 1 ? 1 : want > 16 ? 16 : want;
     return (int)(want < most ? want : most);
 }
 
 template <int XK>
 static int launch_fused(const AdapterArgs &A, dim3 grid, hipStream_t s) {
-    const dim3 block(kOutThreads);
+    const dim3 block(kAdThreads);
     if (A.rank16 <= 16) hipLaunchKernelGGL((adapter_fused_kernel<XK, 1>), grid, block, 0, s, A);
     else if (A.rank16 <= 32) hipLaunchKernelGGL((adapter_fused_kernel<XK, 2>), grid, block, 0, s, A);
-    else if (A.rank16 <= 64) hipLaunchKernelGGL((adapter_fused_kernel<XK, 4>), grid, block, 0, s, A);
-    else hipLaunchKernelGGL((adapter_fused_kernel<XK, 8>), grid, block, 0, s, A);
+    else if constexpr (XK != G4_KIND_F32) hipLaunchKernelGGL((adapter_fused_kernel<XK, 4>), grid, block, 0, s, A);
     G4_LAUNCHED("adapter_fused_kernel");
     return G4_OK;
 }
 
 template <int XK>
 static int launch_shrink(const AdapterArgs &A, dim3 grid, hipStream_t s) {
-    const dim3 block(kHThreads);
+    const dim3 block(kAdThreads);
     if (A.rank16 <= 16) hipLaunchKernelGGL((adapter_shrink_kernel<XK, 1>), grid, block, 0, s, A);
     else if (A.rank16 <= 32) hipLaunchKernelGGL((adapter_shrink_kernel<XK, 2>), grid, block, 0, s, A);
-    else if (A.rank16 <= 64) hipLaunchKernelGGL((adapter_shrink_kernel<XK, 4>), grid, block, 0, s, A);
-    else hipLaunchKernelGGL((adapter_shrink_kernel<XK, 8>), grid, block, 0, s, A);
+    else hipLaunchKernelGGL((adapter_shrink_kernel<XK, 4>), grid, block, 0, s, A);
     G4_LAUNCHED("adapter_shrink_kernel");
     return G4_OK;
 }
 
 static int launch_expand(const AdapterArgs &A, dim3 grid, hipStream_t s) {
-    const dim3 block(kOutThreads);
+    const dim3 block(kAdThreads);
     if (A.rank16 <= 16) hipLaunchKernelGGL(adapter_expand_kernel<1>, grid, block, 0, s, A);
     else if (A.rank16 <= 32) hipLaunchKernelGGL(adapter_expand_kernel<2>, grid, block, 0, s, A);
     else if (A.rank16 <= 64) hipLaunchKernelGGL(adapter_expand_kernel<4>, grid, block, 0, s, A);
@@ -731,9 +833,8 @@ int g4_adapter_linear(const g4_adapters *adapters, const void *groups, size_t gr
         if (x_kind == G4_KIND_F16) return launch_fused<G4_KIND_F16>(A, out_grid, s);
         return launch_fused<G4_KIND_F32>(A, out_grid, s);
     }
-    A.k_range = ((D->k + A.splits - 1) / A.splits + 31) / 32 * 32;
-    A.n_range = kBlockN;
-    const dim3 grid(A.splits, (unsigned)((tiles + 1) / 2));
+    A.k_range = ((D->k + A.splits - 1) / A.splits + kChunk - 1) / kChunk * kChunk;
+    const dim3 grid(A.splits, (unsigned)((tiles + 1) / 2), (unsigned)((D->max_rank + 63) / 64));
     int st;
     if (x_kind == G4_KIND_I8) st = launch_shrink<G4_KIND_I8>(A, grid, s);
     else if (x_kind == G4_KIND_F16) st = launch_shrink<G4_KIND_F16>(A, grid, s);

@@ -24,11 +24,13 @@ constexpr int kTile = 16;          // rows of a tile
 constexpr int kMaxRank = 128, kMaxAdapters = 4096, kMaxK = 1 << 23;  // an adapter's A has less than 2^31 elements
 constexpr int kMaxTokens = 1 << 19;  // a grid has a row of blocks per tile
 constexpr int kGroupThreads = 1024;
-// What blocks of a single launch may read of x and A together, over and over, from the L2s: up to there it takes less
-// than the second launch and H's way through memory.
-constexpr int64_t kFusedBytes = 24 << 20;
-// And the matrix unit's time for a block's H in cycles of a SIMD; exact f32 products take 16 times that of f16.
-constexpr int64_t kFusedCycles = 5000;
+// One launch, where every block makes its tile's H again, saves the second launch and H's way through memory, 2 to 3.5 us.
+// It pays up to these bounds (in one launch and in two):
+//   blocks a CU: f16 x, K 1536, N 6144, rank 32, 256 rows (396 blocks) 8.2 and 11.6 us; 512 rows (588) 15.7 and 13.7
+//   row pairs that a wave loads: f16, 1 row, rank 32, K 3584 (42) 9.8 and 10.4 us; K 6144 (72) 12.7 and 9.3
+//   cycles of a SIMD's matrix unit, where f32 x takes 16 times f16's: 64 rows, K 1536, rank 32 (6144) 12.1 and 12.5 us;
+//   K 2048, rank 24 (8192) 13.3 and 11.5
+constexpr int kFusedBlocks = 2, kFusedLoads = 48, kFusedCycles = 6500;
 
 // groups: the header, then the tiles.
 struct GroupHeader {
@@ -138,7 +140,7 @@ struct AdapterArgs {
     int64_t x_stride, base_stride, out_stride;
     float x_scale, base_scale, out_scale;
     int base_kind, out_kind;
-    int splits, k_range, n_range, vec;  // K in `splits` ranges; vec: eight outputs may be moved at once
+    int splits, k_range, vec;  // K in `splits` ranges; vec: eight outputs may be moved at once
     float *h;                           // [splits][tokens][rank16]
 };
 
@@ -275,12 +277,7 @@ __device__ __forceinline__ void shrink(const AdapterArgs &A, const _Float16 *a, 
             }
         }
     };
-    for (int c = 0; c < min(G::SLOTS - 1, chunks); ++c) issue(c);
-    for (int c = 0; c < chunks; ++c) {
-        if (c + G::SLOTS - 2 < chunks) wait_loads<(G::SLOTS - 2) * G::LOADS>();
-        else wait_loads<0>();
-        block_meet();  // chunk c is there, and chunk c - 1 has been read
-        if (c + G::SLOTS - 1 < chunks) issue(c + G::SLOTS - 1);
+    auto multiply_chunk = [&](int c) {
         const char *slot = lds + c % G::SLOTS * G::BYTES;
         const bool in = k0 + c * kChunk + 32 * wave + 8 * group < k1;
         XPart<XK> x[MT];
@@ -309,6 +306,21 @@ __device__ __forceinline__ void shrink(const AdapterArgs &A, const _Float16 *a, 
             const h8 w = in && r0 + 16 * r + col < rank ? v : h8{};
 #pragma unroll
             for (int i = 0; i < MT; ++i) acc[i][r] = product<XK>(w, x[i], acc[i][r]);
+        }
+    };
+    if (chunks <= G::SLOTS) {  // all at once, and one wait
+        for (int c = 0; c < chunks; ++c) issue(c);
+        wait_loads<0>();
+        block_meet();
+        for (int c = 0; c < chunks; ++c) multiply_chunk(c);
+    } else {
+        for (int c = 0; c < G::SLOTS - 1; ++c) issue(c);
+        for (int c = 0; c < chunks; ++c) {
+            if (c + G::SLOTS - 2 < chunks) wait_loads<(G::SLOTS - 2) * G::LOADS>();
+            else wait_loads<0>();
+            block_meet();  // chunk c is there, and chunk c - 1 has been read
+            if (c + G::SLOTS - 1 < chunks) issue(c + G::SLOTS - 1);
+            multiply_chunk(c);
         }
     }
     block_meet();  // the ring is free
@@ -424,7 +436,7 @@ __device__ __forceinline__ void store8(void *p, int kind, int64_t at, int n, boo
     }
 }
 
-constexpr int kWaveN = 64, kBlockN = kWaves * kWaveN;  // outputs of a wave, and of a block, at a time
+constexpr int kWaveN = 64, kBlockN = kWaves * kWaveN;  // outputs of a wave, and of a block
 
 // B's rows n0 .. n0 + 511 at `lds`, max_rank halves each; loads of whole lines (see Ring). A row's units of 16 bytes
 // stand at their number XOR unit_xor(row): a product's lanes read one unit of rows 0-3 and 8-11 at a time.
@@ -544,7 +556,7 @@ __device__ __forceinline__ float scale_of(const AdapterArgs &A, int adapter) {
 
 constexpr int kLds = 144 << 10;  // what a block takes of a CU's 160 KB
 
-// Grid (ranges of outputs, tiles): H, then the outputs, in rounds of 512.
+// Grid (ranges of 512 outputs, tiles): H, then the outputs.
 template <int XK, int RT>
 __global__ __launch_bounds__(kAdThreads) void adapter_fused_kernel(AdapterArgs A) {
     constexpr int kRoom = kLds - RT * 16 * kBlockN * 2;
@@ -558,8 +570,7 @@ __global__ __launch_bounds__(kAdThreads) void adapter_fused_kernel(AdapterArgs A
     const int row[1] = {(int)row_of(A, T, col)};
     const bool some = T.adapter >= 0;
     const _Float16 *b = A.b + max(T.adapter, 0) * A.b_stride;
-    const int end = min((int)(blockIdx.x + 1) * A.n_range, A.n);
-    int n = blockIdx.x * A.n_range;
+    const int n = blockIdx.x * kBlockN;
     Expand<RT> E;
     E.load(A, T, row[0], n + wave * kWaveN);
     if (some) load_b(A, b, n, b_lds);
@@ -573,18 +584,7 @@ __global__ __launch_bounds__(kAdThreads) void adapter_fused_kernel(AdapterArgs A
         shrink<XK, RT, 1, kRoom>(A, A.a + T.adapter * A.a_stride, rank, 0, row, 0, A.k, lds, acc);
         sum_waves<RT>(acc[0], h);
     }
-    while (true) {
-        E.finish(A, T, h, b_lds, rank, scale, row[0]);
-        n += kBlockN;
-        if (n >= end) return;
-        E.load(A, T, row[0], n + wave * kWaveN);
-        if (some) {
-            block_meet();
-            load_b(A, b, n, b_lds);
-            wait_loads<0>();
-            block_meet();
-        }
-    }
+    E.finish(A, T, h, b_lds, rank, scale, row[0]);
 }
 
 // Grid (splits, pairs of tiles, ranks by 64): a range of K of the tiles' H. Two tiles of one adapter share its rows of A.
@@ -671,15 +671,17 @@ __global__ __launch_bounds__(kAdThreads) void adapter_expand_kernel(AdapterArgs 
 
 // How a call is run: in one launch (splits 0), or with H's parts of `splits` ranges of K.
 static int adapter_splits(const g4_adapters *D, int tokens, int x_size) {
-    const int64_t tiles = max_tiles(tokens, D->count), ranges = (D->n + 2 * kBlockN - 1) / (2 * kBlockN);
-    const int64_t again = tiles * ranges * D->k * (2 * D->max_rank + kTile * x_size);
-    const int64_t cycles = (D->k / 32) * ((D->max_rank + 15) / 16) * (x_size == 4 ? 256 : 16) / 4;
-    const bool fits = D->max_rank <= (x_size == 4 ? 32 : 64);
-    if (fits && again <= kFusedBytes && cycles <= kFusedCycles) return 0;
-    const int64_t pairs = (tiles + 1) / 2, most = (D->k + kChunk - 1) / kChunk;
+    const int64_t tiles = max_tiles(tokens, D->count), blocks = tiles * ((D->n + kBlockN - 1) / kBlockN);
+    const int64_t ranks = (D->max_rank + 15) / 16, room = ranks > 2 ? 4 : ranks;  // by 16, and what a kernel has of them
+    const int64_t chunks = (D->k + kChunk - 1) / kChunk, loads = chunks * (room + (x_size == 2 ? 1 : 2));
+    const int64_t cycles = (int64_t)(D->k / 32) * room * (x_size == 4 ? 256 : 16) / 4;
+    if (ranks <= (x_size == 4 ? 2 : 4) && blocks <= kFusedBlocks * device_cu_count() && loads <= kFusedLoads &&
+        cycles <= kFusedCycles)
+        return 0;
+    const int64_t pairs = (tiles + 1) / 2;
     int64_t want = device_cu_count() / (pairs * ((D->max_rank + 63) / 64));  // a block a CU at once
     want = want < 1 ? 1 : want > 16 ? 16 : want;
-    return (int)(want < most ? want : most);
+    return (int)(want < chunks ? want : chunks);
 }
 
 template <int XK>
@@ -824,10 +826,7 @@ int g4_adapter_linear(const g4_adapters *adapters, const void *groups, size_t gr
     A.vec = D->n % 8 == 0 && os % 8 == 0 && (!base || bs % 8 == 0) && ((uintptr_t)out & 15) == 0 && ((uintptr_t)base & 15) == 0;
     A.h = static_cast<float *>(workspace);
     hipStream_t s = as_stream(stream);
-    // ranges of outputs: a block of two rounds where that leaves a block for every other CU
-    const int64_t rounds = tiles * ((D->n + 2 * kBlockN - 1) / (2 * kBlockN)) >= device_cu_count() / 2 ? 2 : 1;
-    A.n_range = (int)(rounds * kBlockN);
-    const dim3 out_grid((unsigned)((D->n + A.n_range - 1) / A.n_range), (unsigned)tiles);
+    const dim3 out_grid((unsigned)((D->n + kBlockN - 1) / kBlockN), (unsigned)tiles);
     if (A.splits == 0) {
         if (x_kind == G4_KIND_I8) return launch_fused<G4_KIND_I8>(A, out_grid, s);
         if (x_kind == G4_KIND_F16) return launch_fused<G4_KIND_F16>(A, out_grid, s);
@@ -840,7 +839,7 @@ int g4_adapter_linear(const g4_adapters *adapters, const void *groups, size_t gr
     else if (x_kind == G4_KIND_F16) st = launch_shrink<G4_KIND_F16>(A, grid, s);
     else st = launch_shrink<G4_KIND_F32>(A, grid, s);
     if (st) return st;
-    return launch_expand(A, dim3((unsigned)((D->n + kBlockN - 1) / kBlockN), (unsigned)tiles), s);
+    return launch_expand(A, out_grid, s);
 }
 
 }  // extern "C"

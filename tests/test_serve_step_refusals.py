@@ -1,5 +1,7 @@
 """What the plan, the release, the adapters and the sampling refuse before anything is launched (no device needed)."""
 import ctypes
+import sys
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
@@ -146,3 +148,37 @@ def test_struct_layout(g4):
     assert ctypes.sizeof(gs.FreePagesStruct) == 2 * 8 + 3 * 4 + 4
     assert ctypes.sizeof(gs.AdaptersStruct) == 4 * 8 + 4 * 4 + 2 * 8
     assert gs.AdaptersStruct.a_stride.offset == 48 and gs.FreePagesStruct.page_size.offset == 24
+
+
+def test_tensors_are_used_on_torchs_current_stream(g4, monkeypatch):
+    """Without a stream argument, where any operand is a tensor; DeviceBuffers alone go to the default stream."""
+    class Tensor(Fake):
+        is_cuda = True
+        data_ptr = lambda self: self.ptr
+        get_device = lambda self: 0
+        stride = lambda self: tuple(int(np.prod(self.shape[i + 1:])) for i in range(len(self.shape)))
+        is_contiguous = lambda self: True
+
+    names = ("g4_plan_chunk", "g4_release_pages", "g4_adapter_groups", "g4_adapter_linear", "g4_sample_tokens")
+    seen = []
+    library = type("Library", (), dict.fromkeys(names, staticmethod(lambda *a: seen.append(a[-1]) or 0)))
+    cuda = SimpleNamespace(is_initialized=lambda: True, current_device=lambda: 0)
+    monkeypatch.setitem(sys.modules, "torch", SimpleNamespace(cuda=cuda, _C=SimpleNamespace(_cuda_getCurrentRawStream=lambda d: 0x77)))
+    monkeypatch.setattr(gs.g4, "lib", lambda: library)
+    monkeypatch.setattr(gs, "_one_runtime", True, raising=False)
+
+    def calls(kind, **kw):
+        f, ws = free(), Fake((1 << 24,), np.uint8)
+        p = gs.Adapters(Fake((4, 16, 256), np.float16), Fake((4, 64, 16), np.float16))
+        gs.plan_chunk(f, i32(3), i32(3), i32(3, 4), i32(4), i32(3), i32(1), i32(1), tokens=9, max_q=4, max_kv=60,
+                      last_row=kind((3,), I), **kw)
+        gs.release_pages(f, i32(3, 4), kind((3,), I), i32(3), i32(1), **kw)
+        gs.adapter_groups(i32(6), kind((1 << 20,), np.uint8), 4, **kw)
+        gs.adapter_linear(p, ws, Fake((6, 256), F), None, kind((6, 64), F), ws, **kw)
+        gs.sample_tokens(Fake((3, 99), F), Fake((3,), F), i32(3), None, ws, min_p=kind((3,), F), **kw)
+
+    calls(Tensor)
+    calls(Fake)
+    calls(Tensor, stream=0)
+    calls(Tensor, stream=5)
+    assert seen == [0x77] * 5 + [None] * 5 + [0] * 5 + [5] * 5

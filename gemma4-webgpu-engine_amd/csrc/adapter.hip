@@ -21,7 +21,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 16;          // rows of a tile
-constexpr int kMaxRank = 128, kMaxAdapters = 4096, kMaxK = 1 << 23;  // an adapter's A has less than 2^31 elements
+constexpr int kMaxRank = 128, kMaxAdapters = 4096, kMaxK = 1 << 23, kMaxN = 1 << 30;  // rows are counted in 32 bits
 constexpr int kMaxTokens = 1 << 19;  // a grid has a row of blocks per tile
 constexpr int kGroupThreads = 1024;
 // One launch, where every block makes its tile's H again, saves the second launch and H's way through memory, 2 to 3.5 us.
@@ -718,8 +718,8 @@ static int check_adapters(const char *who, const g4_adapters *D) {
     if (!D || !D->a || !D->b) return set_error(G4_ERR_INVALID, "%s needs the adapters' A and B", who);
     if (D->count <= 0 || D->count > kMaxAdapters)
         return set_error(G4_ERR_INVALID, "%s: %d adapters (1 to %d)", who, D->count, kMaxAdapters);
-    if (D->k <= 0 || D->k % 8 || D->k > kMaxK || D->n <= 0)
-        return set_error(G4_ERR_INVALID, "%s: k %d, n %d (k a multiple of 8 up to %d)", who, D->k, D->n, kMaxK);
+    if (D->k <= 0 || D->k % 8 || D->k > kMaxK || D->n <= 0 || D->n > kMaxN)
+        return set_error(G4_ERR_INVALID, "%s: k %d, n %d (k a multiple of 8 up to %d, n up to %d)", who, D->k, D->n, kMaxK, kMaxN);
     if (D->max_rank <= 0 || D->max_rank % 8 || D->max_rank > kMaxRank)
         return set_error(G4_ERR_INVALID, "%s: max_rank %d is not a multiple of 8 up to %d", who, D->max_rank, kMaxRank);
     if (((uintptr_t)D->a | (uintptr_t)D->b) & 15) return set_error(G4_ERR_INVALID, "%s: A and B must be 16-byte aligned", who);
@@ -795,6 +795,7 @@ int g4_adapter_linear(const g4_adapters *adapters, const void *groups, size_t gr
     const size_t need = g4_adapter_workspace_bytes(D, tokens);
     if (!workspace || workspace_bytes < need)
         return set_error(G4_ERR_INVALID, "adapter-linear: workspace %zu B < %zu B", workspace_bytes, need);
+    if (out == x) return set_error(G4_ERR_INVALID, "adapter-linear: out cannot be x, which every block of a row reads");
     const int64_t tiles = max_tiles(tokens, D->count);
     AdapterArgs A{};
     A.a = static_cast<const _Float16 *>(D->a);

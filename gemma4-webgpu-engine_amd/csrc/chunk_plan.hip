@@ -258,8 +258,10 @@ int g4_plan_chunk(const g4_free_pages *list, const int32_t *cached, const int32_
     if ((int64_t)table_pages * list->page_size < max_kv)
         return set_error(G4_ERR_INVALID, "plan-chunk: %d table pages of %d slots do not hold max_kv %d positions", table_pages,
                          list->page_size, max_kv);
-    if (free_left == list->count || kv_len == cached || (held && held_out == held))
-        return set_error(G4_ERR_INVALID, "plan-chunk: free_left, kv_len and held_out cannot be the arrays they are made from");
+    for (const int32_t *in : {list->count, cached, rows, held, seq_adapter})
+        for (const int32_t *out : {q_start, kv_len, held_out, free_left, served, row_pos, row_slot, row_adapter, last_row})
+            if (in && in == out)
+                return set_error(G4_ERR_INVALID, "plan-chunk: outputs cannot be the arrays they are made from");
     PlanArgs A{list->pages, list->count, cached, rows, held, seq_adapter, page_table,
                table_stride ? table_stride : table_pages, q_start, kv_len, held_out, free_left, served, row_pos, row_slot,
                row_adapter, last_row, list->capacity, list->num_pages, __builtin_ctz(list->page_size), seqs, tokens, max_q,

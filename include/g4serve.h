@@ -181,7 +181,7 @@ typedef struct g4_free_pages {
  * without rows: the row of g4_sample_tokens), and of each of the `tokens` rows its position row_pos, its cache slot
  * row_slot (page * page_size + position % page_size, -1 on an absent page) and its adapter row_adapter
  * (seq_adapter[s], -1 where that is NULL). Rows behind the last sequence: -1, -1 and -2.
- * free_left must not be the free list's count, kv_len not cached and held_out not held: those are read throughout.
+ * No output may be the free list's count, cached, rows, held or seq_adapter: those are read throughout.
  * At most 4096 sequences, and num_pages * page_size below 2^31.
  */
 int g4_plan_chunk(const g4_free_pages *list, const int32_t *cached, const int32_t *rows, const int32_t *held,
@@ -204,8 +204,8 @@ int g4_release_pages(const g4_free_pages *list, const int32_t *page_table, int t
  * Low-rank adapters of one linear, f16: adapter i adds scales[i] * (x A_i^T) B_i^T to its rows.
  * A_i = a + i * a_stride, [max_rank][k]; B_i = b + i * b_stride, [n][max_rank] (strides in elements, 0: packed). ranks
  * (NULL: max_rank for all): adapter i has ranks[i] (clamped to [0, max_rank]) rows of A_i and columns of B_i; what lies
- * behind them is not used, whatever it holds. k and max_rank multiples of 8, k up to 2^23 and max_rank to 128; at most 4096
- * adapters; a and b 16-byte aligned, the strides multiples of 8.
+ * behind them is not used, whatever it holds. k and max_rank multiples of 8, k up to 2^23, max_rank to 128 and n to 2^30;
+ * at most 4096 adapters; a and b 16-byte aligned, the strides multiples of 8.
  */
 typedef struct g4_adapters {
     const void *a, *b;
@@ -231,9 +231,10 @@ size_t g4_adapter_groups_bytes(int tokens, int adapters);
  * linear gave: f32, f16, or int8 codes times base_scale, or NULL (zeros). out: f32, f16, or int8 codes on out_scale;
  * out_scale != 0 snaps f32 and f16 outputs to that grid too, as g4_linear does (a f32 output code * out_scale; the
  * quotient's clamp takes a NaN to -128). Rows start x_stride, base_stride and out_stride elements apart (0: packed); x 16-byte
- * aligned, x_stride a multiple of 16 bytes (codes: of 8). out may be base, of the same type and stride. groups: of
- * g4_adapter_groups, for the same tokens and number of adapters.
- * Products are exact (f16 and f32 values in f32), added up in f32, as is x A^T, which is not rounded in between.
+ * aligned, x_stride a multiple of 16 bytes (codes: of 8). out may be base, of the same type and stride, and not x.
+ * groups: of g4_adapter_groups, for the same tokens and number of adapters (of others: nothing is written).
+ * x A^T is made of exact products, added up in f32, and enters the second product with 23 bits, relative to its row's
+ * largest value; that product's sums are f32 too.
  * workspace: g4_adapter_workspace_bytes(...) bytes, 16-byte aligned.
  */
 int g4_adapter_linear(const g4_adapters *adapters, const void *groups, size_t groups_bytes, int tokens, const void *x,

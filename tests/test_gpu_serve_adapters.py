@@ -127,6 +127,19 @@ def test_inner_sizes(gpu, k, x):
     c.check()
 
 
+@pytest.mark.parametrize("rank", [16, 32, 64, 128])
+@pytest.mark.parametrize("x", ["f32", "f16", "i8"])
+def test_chunks_of_k(gpu, x, rank):
+    """K about whole chunks of 256, and about as many as a block holds at once; long rows of zeros too."""
+    for k in (248, 256, 264, 768, 1288, 2040, 2048, 2056, 2304, 2568):
+        c = Case(ids_of(np.random.default_rng(k), 21, 3), adapters=3, k=k, n=40, x=x, rank=rank)
+        c.x[5] = 0
+        c.x[6, :-1] = 0
+        c.upload()
+        c.call()
+        c.check()
+
+
 @pytest.mark.parametrize("rank", [8, 16, 24, 32, 40, 64, 72, 96, 104, 128])
 def test_ranks(gpu, rank):
     """The pool's rank, and adapters of less, of none and of a rank out of range."""
@@ -145,7 +158,7 @@ def test_rank_past_the_pool_is_the_pools(gpu):
     c.check()
 
 
-@pytest.mark.parametrize("n", [1, 3, 15, 16, 17, 255, 256, 257, 2048, 6145])
+@pytest.mark.parametrize("n", [1, 3, 15, 16, 17, 255, 256, 257, 504, 511, 512, 513, 1032, 2048, 6145])
 def test_outer_sizes(gpu, n):
     c = Case(ids_of(np.random.default_rng(3), 21, 4), n=n, x="i8").upload()
     c.call()
@@ -221,6 +234,34 @@ def test_strides(gpu):
             wide = views[2].base.download()
             assert (wide[:, n:] == 5).all()
             c.check(wide[:, :n])
+
+
+def test_far_rows(gpu):
+    """Rows past 2^31 elements: x, base and out a row apart, and two adapters."""
+    far = (1 << 31) + 64
+    c = Case([1, 0], adapters=2, k=256, n=64, rank=16, x="i8", base="i8", out="i8", out_scale=0.03).upload()
+    views = []
+    for host in (c.x, c.base, np.full((2, 64), 77, np.int8)):
+        room = g4.DeviceBuffer.empty((far + host.shape[1],), np.int8)
+        for i in range(2):
+            row = np.ascontiguousarray(host[i])
+            g4._check(g4.lib().g4_memcpy_h2d(room.ptr + i * far, row.ctypes.data, row.nbytes, None))
+        views.append(View(room, 0, host.shape, (far, 1), np.int8))
+    pools = []
+    for host in (c.a, c.b):
+        room = g4.DeviceBuffer.empty((far + host[0].size,), np.float16)
+        for i in range(2):
+            one = np.ascontiguousarray(host[i])
+            g4._check(g4.lib().g4_memcpy_h2d(room.ptr + 2 * i * far, one.ctypes.data, one.nbytes, None))
+        pools.append(View(room, 0, host.shape, (far, host.shape[2], 1), np.float16))
+    c.adapters = gs.Adapters(*pools, dev(c.scales))
+    c.call(out=views[2], x=views[0], base=views[1])
+    g4.synchronize()
+    got = np.zeros((2, 64), np.int8)
+    for i in range(2):
+        g4._check(g4.lib().g4_memcpy_d2h(got[i].ctypes.data, views[2].ptr + i * far, 64, None))
+    g4.synchronize()
+    c.check(got)
 
 
 def test_a_bad_row_stays_alone(gpu):

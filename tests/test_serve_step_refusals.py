@@ -40,6 +40,15 @@ def test_plan_refusals(g4):
     expect(g4, lambda: call(kv_len=i32(3, ptr=0x2000)), 1, "cannot be the arrays they are made from")
     expect(g4, lambda: call(held=i32(3), held_out=i32(3)), 1, "cannot be the arrays they are made from")
     expect(g4, lambda: call(row_pos=i32(8)), 1, "row_pos has shape [8], expected [9]")
+    apart = lambda i, *shape: i32(*shape, ptr=0x10000 * (i + 1))
+    outs = dict(q_start=4, kv_len=3, free_left=1, served=1, held_out=3, row_pos=9, row_slot=9, row_adapter=9, last_row=3)
+    for i, at in enumerate(outs):
+        for j, name in enumerate(("cached", "rows", "held", "seq_adapter", "count")):
+            to = {n: apart(m, size) for m, (n, size) in enumerate(outs.items())}
+            given = {n: apart(20 + m, 3) for m, n in enumerate(("cached", "rows", "held", "seq_adapter"))}
+            to[at] = i32(outs[at], ptr=0x9000 if name == "count" else 0x10000 * (21 + j))
+            expect(g4, lambda: gs.plan_chunk(free(), page_table=i32(3, 4), tokens=9, max_q=4, max_kv=60, **to, **given), 1,
+                   "cannot be the arrays they are made from")
     n = 4097
     expect(g4, lambda: gs.plan_chunk(free(), i32(n, ptr=0x2000), i32(n), i32(n, 4), i32(n + 1), i32(n), i32(1), i32(1), tokens=9,
                                      max_q=4, max_kv=60), 5, "4097 sequences in one call (at most 4096)")
@@ -89,6 +98,8 @@ def test_adapter_refusals(g4):
         expect(g4, lambda: gs.adapter_workspace_bytes(p, 6), 1, "no such call")
     expect(g4, lambda: call(pool(h(4, 16, 252)), x=Fake((6, 252), F)), 1, "k a multiple of 8")
     expect(g4, lambda: call(pool(h(1, 16, (1 << 23) + 8), h(1, 64, 16)), x=Fake((6, (1 << 23) + 8), F)), 1, "up to 8388608")
+    wide = pool(Fake((1, 16, 256), np.float16), Fake((1, (1 << 30) + 1, 16), np.float16))
+    expect(g4, lambda: call(wide, base=None, out=Fake((6, (1 << 30) + 1), F, 0x5000)), 1, "n up to 1073741824")
     expect(g4, lambda: call(x=Fake((6, 128), F)), 1, "x has shape [6, 128]")
     expect(g4, lambda: call(x=Fake((6, 256), I)), 1, "x cannot be int32")
     expect(g4, lambda: call(x=Strided((6, 256), F, (257, 1))), 1, "x must be 16-byte aligned, its rows too")
@@ -97,6 +108,7 @@ def test_adapter_refusals(g4):
     expect(g4, lambda: call(out=Fake((6, 64), np.int8, 0x5000)), 1, "int8 output codes need a calibrated outScale")
     expect(g4, lambda: call(out=Fake((6, 64), np.float16)), 1, "out can be base only with its type and stride")
     expect(g4, lambda: call(out=Strided((6, 64), F, (80, 1))), 1, "out can be base only with its type and stride")
+    expect(g4, lambda: call(), 1, "out cannot be x")
     expect(g4, lambda: call(g=Fake((16,), np.uint8)), 1, "groups 16 B <")
     expect(g4, lambda: call(ws=Fake((8,), np.uint8)), 1, "workspace 8 B <")
     expect(g4, lambda: call(ws=Strided((1 << 24,), np.uint8, (0,))), 1, "the workspace must be contiguous")

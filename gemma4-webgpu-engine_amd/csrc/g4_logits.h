@@ -25,10 +25,12 @@ __device__ __forceinline__ double fma_k(double a, double b, double k) {
 // row's maximum, the bulk of its sums and the judged logits all go through the same two, so that the maximum's
 // exponent is 0 and no other's is above: at a temperature of 1e-12 a difference of 1e-13 would count. (Neither falls
 // as x grows: below half the cap the values of neighbouring f32 logits are 2^-25 of them apart and 2^-44 off.)
+// first: the polynomial's first coefficient, which a loop may keep in a vector register.
+constexpr double kNearCapFirst = 0.00039943422382545215;
 template <class Cap>
-__device__ __forceinline__ double near_cap(double x, const Cap &A) {
+__device__ __forceinline__ double near_cap(double x, const Cap &A, double first = kNearCapFirst) {
     const double t = x * x * A.inv_cap2;
-    double c = 0.00039943422382545215;
+    double c = first;
     c = fma_k(c, t, -0.0013843999024647944);
     c = fma_k(c, t, 0.0035776163994480498);
     c = fma_k(c, t, -0.008861575554686911);

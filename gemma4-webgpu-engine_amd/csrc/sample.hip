@@ -45,6 +45,7 @@ struct Cuts {
 // What a row's weights are made with.
 struct Row {
     double top, slope, d_min, bins;  // weight 2^((y - top) slope), kept from d_min on, bin (top - y) bins
+    double d_low;                    // below this a weight is far below a step
     double inv_t, p;
     int index, k;                // the first maximum (-1: no logit)
     int greedy, filtered, inf, pad;  // inf: the maximum is +infinity, whose like share all weight
@@ -59,7 +60,7 @@ struct SampleArgs {
     const float *top_p, *min_p, *u;
     CapArgs cap;
     int logit_rows, vocab, parts, units, shift, vec, cuts;  // cuts: top-k or top-p given
-    int wide, spans;             // waves of a block of (2) and (3), a unit each, and blocks a row
+    int wide, spans, many;       // waves of a block of (2) and (3), blocks a row, and whether there are many
     PartMax *stats;              // [rows][parts]
     Row *row;                    // [rows]
     Cuts *cut;                   // [rows]
@@ -186,6 +187,7 @@ __device__ __forceinline__ Row row_params(const SampleArgs &A, int row) {
     R.k = k < A.vocab ? k : 0;
     R.p = pf < 1.0f ? (double)pf : 1.0;  // NaN: off
     R.filtered = !R.greedy && m.index >= 0 && (R.k > 0 || R.p < 1.0);
+    R.d_low = -1000.0 / R.slope;
     R.bins = 0.0;
     if (R.filtered && !R.inf) {
         // the bins reach from the top to the lowest logit, or to where weights round to no step
@@ -209,13 +211,38 @@ __device__ __forceinline__ T uniform(const T &v) {
     return __builtin_bit_cast(T, a);
 }
 
+// The same of what an earlier kernel left in memory, by scalar loads.
+template <class T>
+__device__ __forceinline__ T uniform_at(const T *p) {
+    struct Words {
+        int w[sizeof(T) / 4];
+    };
+    const auto *from = (const __attribute__((address_space(4))) int *)(uintptr_t)p;
+    Words a;
+#pragma unroll
+    for (size_t i = 0; i < sizeof(T) / 4; ++i) a.w[i] = from[i];
+    return __builtin_bit_cast(T, a);
+}
+
 // Under an infinite maximum a logit is as good as it, or nothing.
 __device__ __forceinline__ float seen(float x, const Row &R) { return R.inf ? (x == INFINITY ? 0.0f : -INFINITY) : x; }
 
+// The polynomials' first coefficients.
+constexpr double kPowFirst = 1.3259689002093833e-06;
+struct Firsts {
+    double cap = kNearCapFirst, pow = kPowFirst;
+};
+// The same kept in vector registers: a step has a place for one scalar operand, and they would be made for each logit.
+__device__ __forceinline__ Firsts firsts() {
+    Firsts F;
+    asm("" : "+v"(F.cap), "+v"(F.pow));
+    return F;
+}
+
 // y - top of a logit that is not past half the cap; for a NaN and a -infinity one of these two (no weight).
 template <bool CAP>
-__device__ __forceinline__ double near_distance(float x, const Row &R, const SampleArgs &A) {
-    return (CAP ? near_cap((double)x, A.cap) : (double)x) - R.top;
+__device__ __forceinline__ double near_distance(float x, const Row &R, const SampleArgs &A, Firsts F = {}) {
+    return (CAP ? near_cap((double)x, A.cap, F.cap) : (double)x) - R.top;
 }
 // And of any.
 template <bool CAP>
@@ -230,18 +257,35 @@ __device__ __forceinline__ double distance(float x, const Row &R, const SampleAr
 // The weight in steps (at most 2^51 and a little), rounded, above kNoSteps; its bits above kNoStepsBits are the integer.
 constexpr double kNoSteps = 0x1p52;
 constexpr u64 kNoStepsBits = 0x4330000000000000ull;
-__device__ __forceinline__ double raised_steps(double d, const Row &R, const SampleArgs &A) {
-    return pow2(__builtin_fma(d, R.slope, (double)A.shift)) + kNoSteps;
+// 2^(d slope + shift) as pow2 of g4_logits.h makes it, with fewer steps: the integer part comes from one fused product, and d
+// is bounded where that is (a NaN too).
+__device__ __forceinline__ double raised_steps(double d, const Row &R, const SampleArgs &A, Firsts F = {}) {
+    d = fmax(d, R.d_low);
+    const double magic = 0x1.8p52 + A.shift, r = __builtin_fma(d, R.slope, magic);  // n + shift in the low word
+    const double f = __builtin_fma(d, R.slope, -(r - magic));
+    double e = F.pow;
+    e = fma_k(e, f, 1.531008106933654e-05);
+    e = fma_k(e, f, 0.00015403433582607232);
+    e = fma_k(e, f, 0.0013333450560096254);
+    e = fma_k(e, f, 0.009618129194093111);
+    e = fma_k(e, f, 0.05550410941217064);
+    e = fma_k(e, f, 0.24022650695640319);
+    e = fma_k(e, f, 0.6931471805459295);
+    e = fma_k(e, f, 1.0000000000000135);
+    return __hiloint2double(__double2hiint(e) + (int)((uint32_t)__double2loint(r) << 20), __double2loint(e)) + kNoSteps;
 }
-__device__ __forceinline__ u64 steps(double d, const Row &R, const SampleArgs &A) {
-    return (u64)__double_as_longlong(raised_steps(d, R, A)) - kNoStepsBits;
+__device__ __forceinline__ u64 steps(double d, const Row &R, const SampleArgs &A, Firsts F = {}) {
+    return (u64)__double_as_longlong(raised_steps(d, R, A, F)) - kNoStepsBits;
 }
-// (The conversion takes what is below 0, a rounding, and a NaN to 0, and what is too large to the largest.)
-__device__ __forceinline__ int bin_of(double d, const Row &R) {
+// (The conversion takes what is below 0, a rounding, and a NaN to 0, and what is too large to the largest.) A weight above
+// no step is more than half of one, its d above -(shift + 1) ln 2 t, and no d is below the lowest logit's: the number is
+// below kBins, whose share of the range is a bin more than bins counts on.
+__device__ __forceinline__ uint32_t bin_number(double d, const Row &R) {
     uint32_t b;
     asm("v_cvt_u32_f64 %0, %1" : "=v"(b) : "v"(-d * R.bins));
-    return (int)min(b, (uint32_t)kBins - 1);
+    return b;
 }
+__device__ __forceinline__ int bin_of(double d, const Row &R) { return (int)min(bin_number(d, R), (uint32_t)kBins - 1); }
 
 // Order of tokens: logit down, then id up, as a number (0: none).
 __device__ __forceinline__ u64 order_key(float x, int id) {
@@ -257,7 +301,6 @@ __device__ __forceinline__ u64 wave_sum(u64 v) {
 }
 
 // Inclusive sum over the block's threads; *total: of all.
-template <int THREADS = kSampleThreads>
 __device__ __forceinline__ u64 block_run(u64 v, u64 *lds, u64 *total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -270,7 +313,7 @@ __device__ __forceinline__ u64 block_run(u64 v, u64 *lds, u64 *total) {
     __syncthreads();
     u64 before = 0, all = 0;
 #pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) {
+    for (int w = 0; w < kSampleWaves; ++w) {
         const u64 s = lds[w];
         if (w < wave) before += s;
         all += s;
@@ -308,10 +351,7 @@ __global__ __launch_bounds__(64 * WAVES, 8) void sample_weights_kernel(SampleArg
     const int unit = blockIdx.x * WAVES + wave, base = unit * kSampleUnit;
     float v[kSamplePer];
     load_unit(x + base, x ? A.vocab - base : 0, lane, A.vec, v);
-    Row given;
-    if (READY) {
-        given = A.row[row];
-    } else if (wave == 0) {  // once a block: as many operations as the weights of a unit
+    if (!READY && wave == 0) {  // once a block: as many operations as the weights of a unit
         const Row R = row_params(A, row);
         if (lane == 0) {
             shared_row = R;
@@ -321,44 +361,63 @@ __global__ __launch_bounds__(64 * WAVES, 8) void sample_weights_kernel(SampleArg
     if (A.cuts)
         for (int i = t; i < kBins; i += 64 * WAVES) bins[i] = {0, 0, 0};
     __syncthreads();
-    const Row R = uniform(READY ? given : shared_row);
+    const Row R = READY ? uniform_at(A.row + row) : uniform(shared_row);
     if (R.index < 0) return;
+    const Firsts F = firsts();
+    auto each = [&](auto add) {
+        float most = 0.0f;
+        if (CAP) {
+#pragma unroll
+            for (int j = 0; j < kSamplePer; ++j) most = fmaxf(most, fabsf(v[j]));
+        }
+        uint32_t far = 0;  // places where a lane's logit is past half the cap: few, one at a time
+        if (CAP && __any(most > A.cap.half_cap)) {
+#pragma unroll
+            for (int j = 0; j < kSamplePer; ++j) {
+                const bool f = is_far(v[j], A.cap);
+                far |= __ballot(f) ? 1u << j : 0u;
+                v[j] = f ? -INFINITY : v[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kSamplePer; ++j) {
+            float xs = v[j];
+            asm("" : "+v"(xs));  // one after the other: all at once they would not fit the registers
+            add(near_distance<CAP>(xs, R, A, F));
+        }
+        for (; far; far &= far - 1) {
+            const int i = base + unit_place(__ffs(far) - 1, lane, A.vec);
+            const float xs = i < A.vocab ? x[i] : -INFINITY;
+            if (is_far(xs, A.cap)) add(distance<CAP>(xs, R, A));
+        }
+    };
     if (R.inf) {
 #pragma unroll
         for (int j = 0; j < kSamplePer; ++j) v[j] = seen(v[j], R);
     }
-    auto each = [&](auto add) {
-        uint32_t far = 0;  // places where a lane's logit is past half the cap: few, one at a time
-#pragma unroll
-        for (int j = 0; j < kSamplePer; ++j) {
-            float xs = v[j];
-            if (CAP) {
-                const bool f = is_far(xs, A.cap);
-                far |= __ballot(f) ? 1u << j : 0u;
-                xs = f ? -INFINITY : xs;
-                asm("" : "+v"(xs));  // chosen here, in 32 bits, and not behind the conversion
-            }
-            add(near_distance<CAP>(xs, R, A));
-        }
-        if (CAP)
-            for (; far; far &= far - 1) {
-                const int i = base + unit_place(__ffs(far) - 1, lane, A.vec);
-                const float xs = i < A.vocab ? x[i] : -INFINITY;
-                if (is_far(xs, A.cap)) add(distance<CAP>(xs, R, A));
-            }
-    };
     u64 all = 0;
     if (R.filtered) {
         uint32_t one = 1;
         asm("" : "+v"(one));  // kept, and not made again for each logit
         each([&](double d) {
-            const double w = raised_steps(d, R, A);
-            if (w > kNoSteps) {
-                Bin &b = bins[bin_of(d, R)];
+            const double w = raised_steps(d, R, A, F);
+            if (w > kNoSteps) {  // a weight of no step would be past the last bin, no other is
+                Bin &b = bins[bin_number(d, R)];
                 atomicAdd(&b.mass, (u64)__double_as_longlong(w));
                 atomicAdd(&b.count, one);
             }
         });
+    } else {
+        u64 kept = 0;
+        each([&](double d) {
+            const u64 w = steps(d, R, A, F);
+            all += w;
+            kept += d >= R.d_min ? w : 0;
+        });
+        kept = wave_sum(kept);
+        if (lane == 0 && unit < A.units) A.unit_sums[(int64_t)row * A.units + unit] = kept;
+    }
+    if (R.filtered) {
         __syncthreads();
         for (int i = t; i < kBins; i += 64 * WAVES) {
             const Bin b = bins[bin_at(i)];
@@ -368,18 +427,8 @@ __global__ __launch_bounds__(64 * WAVES, 8) void sample_weights_kernel(SampleArg
             atomicAdd(&A.bin_mass[(int64_t)row * kBins + i], m);
             atomicAdd(&A.bin_count[(int64_t)row * kBins + i], b.count);
         }
-        all = wave_sum(all);
-    } else {
-        u64 kept = 0;
-        each([&](double d) {
-            const u64 w = steps(d, R, A);
-            all += w;
-            kept += d >= R.d_min ? w : 0;
-        });
-        all = wave_sum(all);
-        kept = wave_sum(kept);
-        if (lane == 0 && unit < A.units) A.unit_sums[(int64_t)row * A.units + unit] = kept;
     }
+    all = wave_sum(all);
     if (lane == 0) ss[wave] = all;
     __syncthreads();
     if (t) return;
@@ -497,11 +546,11 @@ __device__ __forceinline__ Cuts find_cuts(const SampleArgs &A, const Row &R, con
 
 // Four rows a block, a wave each: for calls of many blocks, each of which would do it again.
 __global__ __launch_bounds__(kSampleThreads) void sample_find_kernel(SampleArgs A, int rows) {
-    const int row = blockIdx.x * kSampleWaves + (threadIdx.x >> 6);
+    const int row = blockIdx.x * kSampleWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (row >= rows) return;
     LaneBins B;
     B.load(A, row);
-    const Row R = uniform(A.row[row]);
+    const Row R = uniform_at(A.row + row);
     if (!R.filtered) return;
     const Cuts C = find_cuts(A, R, B);
     if ((threadIdx.x & 63) == 0) A.cut[row] = C;
@@ -570,7 +619,7 @@ __global__ __launch_bounds__(64 * WAVES) void sample_cut_kernel(SampleArgs A) {
     load_unit(x + base, x ? A.vocab - base : 0, lane, A.vec, v);
     LaneBins B;
     if (wave == 0) B.load(A, row);
-    const Row R = uniform(A.row[row]);
+    const Row R = uniform_at(A.row + row);
     if (!R.filtered) return;  // (a row without a logit, too)
     if (wave == 0) {
         const Cuts C = find_cuts(A, R, B);
@@ -593,8 +642,8 @@ template <bool CAP>
 __global__ __launch_bounds__(kSampleThreads, 5) void sample_cut_found_kernel(SampleArgs A) {
     const int lane = threadIdx.x & 63, row = blockIdx.y;
     const int first = (blockIdx.x * kSampleWaves + (threadIdx.x >> 6)) * kCutSpan;
-    const Row R = uniform(A.row[row]);
-    const Cuts c = uniform(A.cut[row]);
+    const Row R = uniform_at(A.row + row);
+    const Cuts c = uniform_at(A.cut + row);
     if (!R.filtered || first >= A.units) return;
     const float *x = row_of(A, row);
     const float top = lane < kCutSpan && first + lane < A.units ? A.unit_max[(int64_t)row * A.units + first + lane] : -INFINITY;
@@ -850,14 +899,14 @@ __global__ __launch_bounds__(kSampleThreads) void sample_pick_kernel(SampleArgs 
     const u64 *list = A.list + (int64_t)row * kList;
     const uint32_t n = A.listed[(int64_t)row * kLineWords];
     const u64 first_key = list[lane];
-    const Cuts C = uniform(A.cut[row]);
+    const Cuts C = uniform_at(A.cut + row);
     u64 all = 0;
     for (int c = lane; c < A.spans; c += 64) all += A.span_sums[(int64_t)row * A.spans + c];
     const u64 *units = A.unit_sums + (int64_t)row * A.units;
     const int per = (A.units + kSampleThreads - 1) / kSampleThreads, u0 = min(t * per, A.units), u1 = min(u0 + per, A.units);
     u64 mine = 0;
     for (int i = u0; i < u1; ++i) mine += units[i];
-    const Row R = uniform(A.row[row]);
+    const Row R = uniform_at(A.row + row);
     if (R.index < 0) {
         if (t == 0) {
             A.tokens[row] = -1;
@@ -969,8 +1018,7 @@ static int launch_sample(const SampleArgs &A, int rows, hipStream_t s) {
     hipLaunchKernelGGL(sample_max_kernel, dim3(A.parts, rows), dim3(kSampleThreads), 0, s, A);
     G4_LAUNCHED("sample_max_kernel");
     const dim3 grid(A.spans, rows), block(64 * A.wide), by_row((rows + kSampleWaves - 1) / kSampleWaves);
-    const bool many = (int64_t)A.spans * rows >= 16 * device_cu_count();
-    if (many) {
+    if (A.many) {
         hipLaunchKernelGGL(sample_row_kernel, by_row, dim3(kSampleThreads), 0, s, A, rows);
         G4_LAUNCHED("sample_row_kernel");
         hipLaunchKernelGGL((sample_weights_kernel<CAP, 8, true>), grid, block, 0, s, A);
@@ -980,7 +1028,7 @@ static int launch_sample(const SampleArgs &A, int rows, hipStream_t s) {
         hipLaunchKernelGGL((sample_weights_kernel<CAP, 8, false>), grid, block, 0, s, A);
     }
     G4_LAUNCHED("sample_weights_kernel");
-    if (A.cuts && many) {
+    if (A.cuts && A.many) {
         hipLaunchKernelGGL(sample_find_kernel, by_row, dim3(kSampleThreads), 0, s, A, rows);
         G4_LAUNCHED("sample_find_kernel");
         const int per = kSampleWaves * kCutSpan;
@@ -1056,6 +1104,7 @@ int g4_sample_tokens(const float *logits, int logit_rows, int64_t logit_stride, 
     // without a block, 4 have a SIMD each
     A.wide = (int64_t)rows * ((A.units + 7) / 8) >= device_cu_count() ? 8 : 4;
     A.spans = (A.units + A.wide - 1) / A.wide;  // at most parts
+    A.many = (int64_t)rows * A.spans > 4 * device_cu_count();
     A.stats = static_cast<PartMax *>(workspace);
     A.row = reinterpret_cast<Row *>(A.stats + (int64_t)rows * A.parts);
     A.cut = reinterpret_cast<Cuts *>(A.row + rows);

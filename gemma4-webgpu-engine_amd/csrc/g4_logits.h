@@ -7,12 +7,6 @@
 
 namespace g4 {
 
-// What the softcap needs of a cap; the functions below take anything with these members.
-struct CapArgs {
-    double cap, inv_cap2;
-    float half_cap;  // a little less than half the cap
-};
-
 // a b + k with k in scalar registers (the compiler would copy it to vector ones first, two moves a step).
 __device__ __forceinline__ double fma_k(double a, double b, double k) {
     double r;
@@ -25,7 +19,8 @@ __device__ __forceinline__ double fma_k(double a, double b, double k) {
 // row's maximum, the bulk of its sums and the judged logits all go through the same two, so that the maximum's
 // exponent is 0 and no other's is above: at a temperature of 1e-12 a difference of 1e-13 would count. (Neither falls
 // as x grows: below half the cap the values of neighbouring f32 logits are 2^-25 of them apart and 2^-44 off.)
-// first: the polynomial's first coefficient, which a loop may keep in a vector register.
+// first: the polynomial's first coefficient, which a loop may keep in a vector register. Cap: cap, inv_cap2 and half_cap, a
+// little less than half the cap.
 constexpr double kNearCapFirst = 0.00039943422382545215;
 template <class Cap>
 __device__ __forceinline__ double near_cap(double x, const Cap &A, double first = kNearCapFirst) {

@@ -51,6 +51,12 @@ struct Row {
     int greedy, filtered, inf, pad;  // inf: the maximum is +infinity, whose like share all weight
 };
 
+// (half_cap: a little less than half the cap)
+struct CapArgs {
+    double cap, inv_cap, inv_cap2;
+    float half_cap;
+};
+
 struct SampleArgs {
     const float *logits;
     int64_t stride;
@@ -162,6 +168,34 @@ __global__ __launch_bounds__(kSampleThreads) void sample_max_kernel(SampleArgs A
     A.stats[(int64_t)row * A.parts + part] = m;
 }
 
+// The softcap past half the cap, cap - 2 cap / (e^(2 |x| / cap) + 1), 1e-14 of the cap off, where the library's exponential
+// would hold twenty registers through the loops around it: 2^z as n + f, |f| <= 1/2, by the series to f^11.
+__device__ __forceinline__ double far_logit(float x, const CapArgs &A) {
+    const double z = fmin(fabs((double)x) * A.inv_cap * (2 * 1.4426950408889634074), 1000.0);
+    const double r = z + 0x1.8p52, f = z - (r - 0x1.8p52);
+    double e = 4.44553827187081e-10;
+    e = fma_k(e, f, 7.054911620801121e-09);
+    e = fma_k(e, f, 1.0178086009239696e-07);
+    e = fma_k(e, f, 1.3215486790144305e-06);
+    e = fma_k(e, f, 1.5252733804059838e-05);
+    e = fma_k(e, f, 0.00015403530393381606);
+    e = fma_k(e, f, 0.0013333558146428441);
+    e = fma_k(e, f, 0.009618129107628477);
+    e = fma_k(e, f, 0.055504108664821576);
+    e = fma_k(e, f, 0.2402265069591007);
+    e = fma_k(e, f, 0.6931471805599453);
+    e = fma_k(e, f, 1.0);
+    e = __hiloint2double(__double2hiint(e) + (int)((uint32_t)__double2loint(r) << 20), __double2loint(e)) + 1.0;
+    double q = __builtin_amdgcn_rcp(e);
+    q *= __builtin_fma(-e, q, 2.0);
+    q *= __builtin_fma(-e, q, 2.0);
+    return copysign(__builtin_fma(-2.0 * A.cap, q, A.cap), (double)x);
+}
+__device__ __forceinline__ double capped(float x, const CapArgs &A) {
+    if (A.cap == 0.0) return x;
+    return fabsf(x) > A.half_cap ? far_logit(x, A) : near_cap((double)x, A);
+}
+
 // By one wave, the same in every lane.
 __device__ __forceinline__ Row row_params(const SampleArgs &A, int row) {
     const int lane = threadIdx.x & 63;
@@ -181,7 +215,7 @@ __device__ __forceinline__ Row row_params(const SampleArgs &A, int row) {
     R.inv_t = 1.0 / t;
     R.slope = R.inv_t * 1.4426950408889634074;
     R.inf = A.cap.cap == 0.0 && m.max == INFINITY;
-    R.top = R.inf || m.index < 0 ? 0.0 : softcap64(m.max, A.cap);
+    R.top = R.inf || m.index < 0 ? 0.0 : capped(m.max, A.cap);
     R.d_min = -INFINITY;
     if (mf > 0.0f) R.d_min = mf >= 1.0f ? 0.0 : log((double)mf) * t;
     R.k = k < A.vocab ? k : 0;
@@ -191,7 +225,7 @@ __device__ __forceinline__ Row row_params(const SampleArgs &A, int row) {
     R.bins = 0.0;
     if (R.filtered && !R.inf) {
         // the bins reach from the top to the lowest logit, or to where weights round to no step
-        const double range = fmin(R.top - softcap64(m.min, A.cap), (A.shift + 1) * 0.69314718055994530942 * t);
+        const double range = fmin(R.top - capped(m.min, A.cap), (A.shift + 1) * 0.69314718055994530942 * t);
         if (range > 0.0) R.bins = fmin((kBins - 1) * __builtin_amdgcn_rcp(range), 1e300);
     }
     R.pad = 0;
@@ -250,7 +284,7 @@ __device__ __forceinline__ double distance(float x, const Row &R, const SampleAr
     double y = x;
     if (CAP) {
         y = near_cap(y, A.cap);
-        if (is_far(x, A.cap)) y = far_cap(x, A.cap.cap);
+        if (is_far(x, A.cap)) y = far_logit(x, A.cap);
     }
     return y - R.top;
 }
@@ -326,11 +360,6 @@ __device__ __forceinline__ u64 block_run(u64 v, u64 *lds, u64 *total) {
 // wave's loads of them are of whole lines. (Loads of 128 bytes a lane stalled on each other's lines: 12 us.)
 __device__ __forceinline__ int bin_at(int i) { return i % 64 * kBinsPer + i / 64; }
 
-struct Bin {
-    u64 mass;  // and kNoStepsBits for each token
-    uint32_t count, pad;
-};
-
 // Four rows a block, a wave each: for calls of many blocks, each of which would do it again.
 __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs A, int rows) {
     const int row = blockIdx.x * kSampleWaves + (threadIdx.x >> 6);
@@ -343,7 +372,8 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs A
 // READY: the rows' parameters are there (sample_row_kernel).
 template <bool CAP, int WAVES, bool READY>
 __global__ __launch_bounds__(64 * WAVES, 8) void sample_weights_kernel(SampleArgs A) {
-    __shared__ Bin bins[kBins];
+    __shared__ u64 mass[kBins];        // (16 bytes a bin with its count: a wave's atomics in more conflicts, 4 us of 105)
+    __shared__ uint32_t count[kBins];  // where there is a top-k
     __shared__ u64 ss[WAVES];
     __shared__ Row shared_row;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, row = blockIdx.y;
@@ -359,7 +389,7 @@ __global__ __launch_bounds__(64 * WAVES, 8) void sample_weights_kernel(SampleArg
         }
     }
     if (A.cuts)
-        for (int i = t; i < kBins; i += 64 * WAVES) bins[i] = {0, 0, 0};
+        for (int i = t; i < kBins; i += 64 * WAVES) mass[i] = 0, count[i] = 0;
     __syncthreads();
     const Row R = READY ? uniform_at(A.row + row) : uniform(shared_row);
     if (R.index < 0) return;
@@ -402,9 +432,9 @@ __global__ __launch_bounds__(64 * WAVES, 8) void sample_weights_kernel(SampleArg
         each([&](double d) {
             const double w = raised_steps(d, R, A, F);
             if (w > kNoSteps) {  // a weight of no step would be past the last bin, no other is
-                Bin &b = bins[bin_number(d, R)];
-                atomicAdd(&b.mass, (u64)__double_as_longlong(w));
-                atomicAdd(&b.count, one);
+                const uint32_t b = bin_number(d, R);
+                atomicAdd(&mass[b], (u64)__double_as_longlong(w) - kNoStepsBits);
+                if (R.k) atomicAdd(&count[b], one);
             }
         });
     } else {
@@ -420,12 +450,11 @@ __global__ __launch_bounds__(64 * WAVES, 8) void sample_weights_kernel(SampleArg
     if (R.filtered) {
         __syncthreads();
         for (int i = t; i < kBins; i += 64 * WAVES) {
-            const Bin b = bins[bin_at(i)];
-            if (!b.count) continue;
-            const u64 m = b.mass - b.count * kNoStepsBits;
+            const u64 m = mass[bin_at(i)];
+            if (!m) continue;
             all += m;
             atomicAdd(&A.bin_mass[(int64_t)row * kBins + i], m);
-            atomicAdd(&A.bin_count[(int64_t)row * kBins + i], b.count);
+            if (R.k) atomicAdd(&A.bin_count[(int64_t)row * kBins + i], count[bin_at(i)]);
         }
     }
     all = wave_sum(all);
@@ -1090,7 +1119,7 @@ int g4_sample_tokens(const float *logits, int logit_rows, int64_t logit_stride, 
     A.top_p = top_p;
     A.min_p = min_p;
     A.u = u;
-    A.cap = {cap, cap > 0.0f ? 1.0 / ((double)cap * cap) : 0.0, 0.4999999f * cap};
+    A.cap = {cap, cap > 0.0f ? 1.0 / cap : 0.0, cap > 0.0f ? 1.0 / ((double)cap * cap) : 0.0, 0.4999999f * cap};
     A.logit_rows = logit_rows;
     A.vocab = (int)vocab;
     A.parts = (int)sample_parts(vocab);

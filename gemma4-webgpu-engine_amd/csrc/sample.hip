@@ -591,27 +591,36 @@ __device__ __forceinline__ u64 cut_unit(const SampleArgs &A, const Row &R, const
                                         const float (&v)[kSamplePer]) {
     const int lane = threadIdx.x & 63;
     u64 sure = 0;
-    uint32_t look = 0, far = 0, in = 0;  // places where a lane's token may be in these bins or above; past half the cap; a
-                                         // lane's for the list
+    uint32_t far = 0, in = 0;  // places where a lane's token is past half the cap, and may count; a lane's for the list
     int many = 0;
+    const int low = min(c.p_low, c.k_bin), wide = max(c.p_high, c.k_bin < kBins ? c.k_bin : 0) - low;
     auto take = [&](int j, double d, bool real) {
-        const u64 w = real ? steps(d, R, A) : 0;
         const int b = bin_of(d, R);
+        const u64 w = real ? steps(d, R, A) : 0;
         if (b < c.p_low && d >= R.d_min) sure += w;
-        const bool mine = w && ((b >= c.p_low && b <= c.p_high) || b == c.k_bin);
-        in |= mine ? 1u << j : 0u;
-        many += __popcll(__ballot(mine));
+        if (__any((uint32_t)(b - low) <= (uint32_t)wide)) {  // few: the cuts' bins are narrow
+            const bool mine = w && ((b >= c.p_low && b <= c.p_high) || b == c.k_bin);
+            in |= mine ? 1u << j : 0u;
+            many += __popcll(__ballot(mine));
+        }
     };
+    float most = 0.0f;
+    if (CAP) {
 #pragma unroll
-    for (int j = 0; j < kSamplePer; ++j) {
-        look |= __ballot(v[j] >= c.least) ? 1u << j : 0u;
-        far |= CAP && __ballot(is_far(v[j], A.cap) && v[j] >= c.least) ? 1u << j : 0u;
+        for (int j = 0; j < kSamplePer; ++j) most = fmaxf(most, fabsf(v[j]));
     }
+    const bool some = CAP && __any(most > A.cap.half_cap);
 #pragma unroll
     for (int j = 0; j < kSamplePer; ++j) {
-        if (!(look >> j & 1)) continue;
+        if (!__any(v[j] >= c.least)) continue;
         const float xs = seen(clean(v[j]), R);
-        take(j, near_distance<CAP>(xs, R, A), xs > -INFINITY && !(CAP && is_far(xs, A.cap)));
+        bool real = xs > -INFINITY;
+        if (some) {
+            const bool f = is_far(xs, A.cap);
+            far |= __any(f && v[j] >= c.least) ? 1u << j : 0u;
+            real = real && !f;
+        }
+        take(j, near_distance<CAP>(xs, R, A), real);
     }
     if (CAP)
         for (; far; far &= far - 1) {
@@ -664,28 +673,22 @@ __global__ __launch_bounds__(64 * WAVES) void sample_cut_kernel(SampleArgs A) {
     if (lane == 0) A.unit_sums[(int64_t)row * A.units + unit] = sure;
 }
 
-// Grid (spans of kCutSpan units a wave, rows), behind sample_find_kernel: units that do not reach up to the cuts are not
-// read.
-constexpr int kCutSpan = 2;
+// Grid (units by 4, rows), behind sample_find_kernel: units that do not reach up to the cuts are not read.
 template <bool CAP>
-__global__ __launch_bounds__(kSampleThreads, 5) void sample_cut_found_kernel(SampleArgs A) {
+__global__ __launch_bounds__(kSampleThreads, 8) void sample_cut_found_kernel(SampleArgs A) {
     const int lane = threadIdx.x & 63, row = blockIdx.y;
-    const int first = (blockIdx.x * kSampleWaves + (threadIdx.x >> 6)) * kCutSpan;
+    const int unit = blockIdx.x * kSampleWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), base = unit * kSampleUnit;
     const Row R = uniform_at(A.row + row);
     const Cuts c = uniform_at(A.cut + row);
-    if (!R.filtered || first >= A.units) return;
+    if (!R.filtered || unit >= A.units) return;
     const float *x = row_of(A, row);
-    const float top = lane < kCutSpan && first + lane < A.units ? A.unit_max[(int64_t)row * A.units + first + lane] : -INFINITY;
     u64 sure = 0;
-#pragma unroll 1
-    for (u64 left = __ballot(top >= c.least && lane < kCutSpan && first + lane < A.units); left; left &= left - 1) {
-        const int i = __ffsll((long long)left) - 1, base = (first + i) * kSampleUnit;
+    if (uniform_at(A.unit_max + (int64_t)row * A.units + unit) >= c.least) {
         float v[kSamplePer];
         load_unit(x + base, A.vocab - base, lane, A.vec, v);
-        const u64 sum = cut_unit<CAP>(A, R, c, row, x, base, v);
-        if (lane == i) sure = sum;
+        sure = cut_unit<CAP>(A, R, c, row, x, base, v);
     }
-    if (lane < kCutSpan && first + lane < A.units) A.unit_sums[(int64_t)row * A.units + first + lane] = sure;
+    if (lane == 0) A.unit_sums[(int64_t)row * A.units + unit] = sure;
 }
 
 __device__ __forceinline__ float logit_of(u64 key) {
@@ -1060,8 +1063,8 @@ static int launch_sample(const SampleArgs &A, int rows, hipStream_t s) {
     if (A.cuts && A.many) {
         hipLaunchKernelGGL(sample_find_kernel, by_row, dim3(kSampleThreads), 0, s, A, rows);
         G4_LAUNCHED("sample_find_kernel");
-        const int per = kSampleWaves * kCutSpan;
-        hipLaunchKernelGGL(sample_cut_found_kernel<CAP>, dim3((A.units + per - 1) / per, rows), dim3(kSampleThreads), 0, s, A);
+        const dim3 by_unit((A.units + kSampleWaves - 1) / kSampleWaves, rows);
+        hipLaunchKernelGGL(sample_cut_found_kernel<CAP>, by_unit, dim3(kSampleThreads), 0, s, A);
         G4_LAUNCHED("sample_cut_found_kernel");
     } else if (A.cuts) {
         if (A.wide == 4) hipLaunchKernelGGL((sample_cut_kernel<CAP, 4>), grid, block, 0, s, A);

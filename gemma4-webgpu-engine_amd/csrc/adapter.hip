@@ -10,7 +10,12 @@
 // a block per tile and range of outputs, which adds up H's parts.
 //
 // A, x and B come to LDS in whole lines. A matrix instruction's operands straight from memory are 16 rows' 64 bytes a
-// load, which a CU's first-level cache gives at 16 bytes a cycle; whole lines at 58.
+// load, which a CU's first-level cache gives at 16 bytes a cycle; whole lines at 58 (2048 rows, K 6144, N 1536, rank 64: 27
+// us, and 20.4).
+//
+// Bound, of one launch: a chain of loads (tile, rows, x and A, B beside them), the product, the stores: 6.6 us for a row of
+// K 1536, N 2048, rank 16; of two: the first reads x and A once a pair of tiles, a CU its 0.4 MB in 10.2 us of that case, the
+// second reads base and writes, 19 MB in 10.9 us, most of it the chain's.
 #include "g4_internal.h"
 #include "../../include/g4serve.h"
 
@@ -31,6 +36,9 @@ constexpr int kGroupThreads = 1024;
 //   cycles of a SIMD's matrix unit, where f32 x takes 16 times f16's: 64 rows, K 1536, rank 32 (6144) 12.1 and 12.5 us;
 //   K 2048, rank 24 (8192) 13.3 and 11.5
 constexpr int kFusedBlocks = 2, kFusedLoads = 48, kFusedCycles = 6500;
+// Two launches: the ranges of K whose parts of H the second one adds up. 1 row, K 6144, rank 64, f16: 4 ranges 14.4 us, 8 12.3,
+// 16 12.7. f32's products take longer: 64 rows, 8 ranges 22.6, 16 20.4.
+constexpr int kSplits = 8, kSplitsF32 = 16;
 
 // groups: the header, then the tiles.
 struct GroupHeader {
@@ -679,9 +687,11 @@ static int adapter_splits(const g4_adapters *D, int tokens, int x_size) {
         cycles <= kFusedCycles)
         return 0;
     const int64_t pairs = (tiles + 1) / 2;
+    const int64_t most = x_size == 4 ? kSplitsF32 : kSplits;
     int64_t want = device_cu_count() / (pairs * ((D->max_rank + 63) / 64));  // a block a CU at once
-    want = want < 1 ? 1 : want > 16 ? 16 : want;
-    return (int)(want < chunks ? want : chunks);
+    want = want < 1 ? 1 : want > most ? most : want;
+    const int64_t each = (chunks + want - 1) / want;
+    return (int)((chunks + each - 1) / each);
 }
 
 template <int XK>
@@ -833,7 +843,7 @@ int g4_adapter_linear(const g4_adapters *adapters, const void *groups, size_t gr
         if (x_kind == G4_KIND_F16) return launch_fused<G4_KIND_F16>(A, out_grid, s);
         return launch_fused<G4_KIND_F32>(A, out_grid, s);
     }
-    A.k_range = ((D->k + A.splits - 1) / A.splits + kChunk - 1) / kChunk * kChunk;
+    A.k_range = ((D->k + kChunk - 1) / kChunk + A.splits - 1) / A.splits * kChunk;
     const dim3 grid(A.splits, (unsigned)((tiles + 1) / 2), (unsigned)((D->max_rank + 63) / 64));
     int st;
     if (x_kind == G4_KIND_I8) st = launch_shrink<G4_KIND_I8>(A, grid, s);

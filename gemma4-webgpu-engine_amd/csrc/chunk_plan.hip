@@ -10,7 +10,9 @@
 namespace g4 {
 
 constexpr int kPlanSeqs = 4096, kPlanThreads = 256;
-constexpr int kPlanBlocks = 512;  // of a kind, two a CU; more items go round, since every block sums all sequences up
+// Blocks of a kind, two a CU; more items go round, since every block sums all sequences up (1000 requests that
+// give back a page each, of 1024: 9.6 us a call, 15.3 with 4000 blocks).
+constexpr int kPlanBlocks = 512;
 
 struct PlanArgs {
     int32_t *free_pages;
@@ -83,8 +85,9 @@ __device__ __forceinline__ int owner(const int32_t *start, int n, int i) {
     return lo;
 }
 
-// Bound by its chain of dependent steps: count and lengths, a block sum, a search in LDS, a page, the stores. One
-// item a thread, the rows' blocks first, then the pages', then the sequences'.
+// Bound by its chain of dependent steps: count and lengths, a block sum, a search in LDS, a page, the stores (256 requests
+// of 1 to 8 rows 6.4 us, 64 prompts of up to 2048 6.2). One item a thread, the rows' blocks first, then the pages', then
+// the sequences'.
 __global__ __launch_bounds__(kPlanThreads) void plan_chunk_kernel(PlanArgs A, int row_blocks, int page_blocks) {
     extern __shared__ int32_t plan_lds[];
     __shared__ int fit;
@@ -184,6 +187,8 @@ __device__ __forceinline__ int2 range_of(const ReleaseArgs &A, int s) {
     return make_int2(a, max(min(A.last[s], A.table_pages), a));
 }
 
+// Bound by its chain: count, ranges, a block sum, a search, an entry, the store. 16 requests of 256 pages 3.2 us, 1000 of which
+// each gives back one 4.9.
 __global__ __launch_bounds__(kPlanThreads) void release_pages_kernel(ReleaseArgs A) {
     extern __shared__ int32_t plan_lds[];
     int32_t *start = plan_lds;

@@ -212,7 +212,7 @@ __device__ __forceinline__ Row row_params(const SampleArgs &A, int row) {
     Row R;
     R.index = m.index;
     R.greedy = !(tf > 0.0f);
-    const double t = R.greedy ? 1.0 : tf;
+    const double t = R.greedy ? 1.0 : fmin((double)tf, 0x1p127);  // (an infinite one: -infinity / t would be NaN)
     R.inv_t = 1.0 / t;
     R.slope = R.inv_t * 1.4426950408889634074;
     R.inf = A.cap.cap == 0.0 && m.max == INFINITY;

@@ -200,6 +200,18 @@ def test_ends_of_the_arguments(gpu):
     both(logits, u, temperature=np.array(t, np.float32), top_k=k, top_p=np.array(p, np.float32), min_p=np.array(m, np.float32))
 
 
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("t", [np.inf, 3.4e38, 1e-45])
+def test_temperatures_at_the_ends_with_masked_tokens(gpu, t, cap):
+    """Every filter, rows with -infinity and NaN among the logits, and units that end inside a vocabulary."""
+    r = np.random.default_rng(14)
+    logits = (4 * r.standard_normal((6, 2500))).astype(np.float32)
+    logits[1::2, r.integers(0, 2500, 900)] = -np.inf
+    logits[2, ::3] = np.nan
+    for params in ({}, {"min_p": [0.5] * 6}, {"top_k": [40] * 6}, {"top_p": [0.7] * 6}, {"top_k": [900] * 6, "top_p": [0.3] * 6}):
+        both(logits, [0.0, 0.2, 0.5, 0.7, 0.9, LAST], cap=cap, temperature=[t] * 6, **params)
+
+
 def test_largest_vocabulary(gpu):
     r = np.random.default_rng(12)
     vocab = 1 << 22

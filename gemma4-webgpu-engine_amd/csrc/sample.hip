@@ -212,13 +212,13 @@ __device__ __forceinline__ Row row_params(const SampleArgs &A, int row) {
     Row R;
     R.index = m.index;
     R.greedy = !(tf > 0.0f);
-    const double t = R.greedy ? 1.0 : fmin((double)tf, 0x1p127);  // (an infinite one: -infinity / t would be NaN)
+    const double t = R.greedy ? 1.0 : fmin((double)tf, 0x1p200);  // (past all differences; -infinity / infinity would be NaN)
     R.inv_t = 1.0 / t;
     R.slope = R.inv_t * 1.4426950408889634074;
     R.inf = A.cap.cap == 0.0 && m.max == INFINITY;
     R.top = R.inf || m.index < 0 ? 0.0 : capped(m.max, A.cap);
     R.d_min = -INFINITY;
-    if (mf > 0.0f) R.d_min = mf >= 1.0f ? 0.0 : log((double)mf) * t;
+    if (mf > 0.0f && tf < INFINITY) R.d_min = mf >= 1.0f ? 0.0 : log((double)mf) * t;  // (an infinite one makes all alike)
     R.k = k < A.vocab ? k : 0;
     R.p = pf < 1.0f ? (double)pf : 1.0;  // NaN: off
     R.filtered = !R.greedy && m.index >= 0 && (R.k > 0 || R.p < 1.0);

@@ -522,7 +522,7 @@ def _matrix(x, what, tokens, width, device):
 def adapter_linear(adapters, groups, x, base, out, workspace, x_scale=1.0, base_scale=1.0, out_scale=0.0, stream=None):
     """g4_adapter_linear: out = base + scale * (x A^T) B^T with each row's adapter. x [tokens][k] and base (or None)
     [tokens][n]: f32, f16 or int8 codes on x_scale / base_scale; out f32, f16, or int8 codes on out_scale; out may be
-    base. groups: of adapter_groups, for as many tokens."""
+    base, not x. groups: of adapter_groups, for as many tokens."""
     device = _device()
     _need_device(adapters, device, "the adapters")
     tokens = int(x.shape[0])

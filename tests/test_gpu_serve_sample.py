@@ -163,8 +163,8 @@ def test_crowded_bins(gpu):
         both(logits, numbers(r, 12), temperature=[t] * 12, top_k=[k] * 12, top_p=[p] * 12, min_p=[0.0, 1e-4] * 6)
 
 
-@pytest.mark.parametrize("cap", [0.0, 30.0])
-def test_masked_and_infinite_logits(gpu, cap):
+def odd_rows():
+    """Rows of 5000 logits with masks, infinities and NaN."""
     r = np.random.default_rng(3)
     vocab = 5000
     x = (3 * r.standard_normal((12, vocab))).astype(np.float32)
@@ -181,10 +181,27 @@ def test_masked_and_infinite_logits(gpu, cap):
     x[8, 17] = np.inf
     x[8, 18:] = np.nan
     x[9] = 0.0
+    return x
+
+
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_masked_and_infinite_logits(gpu, cap):
+    x = odd_rows()
     for params in ({}, dict(top_k=[3] * 12), dict(top_p=[0.7] * 12), dict(top_k=[700] * 12, top_p=[0.5] * 12, min_p=[0.1] * 12),
                    dict(temperature=[0.0] * 12)):
         for u in (0.0, 0.4, LAST):
             both(x, np.full(12, u, np.float32), cap=cap, **params)
+
+
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_masked_and_infinite_logits_of_many_rows(gpu, cap):
+    """Enough requests for the parameters and the cuts to be found by kernels of their own, many of them on one row of
+    logits."""
+    r = np.random.default_rng(15)
+    n = 1200
+    index = r.integers(-1, 13, n).astype(np.int32)
+    both(odd_rows(), numbers(r, n), cap=cap, index=index, **mixed(r, n, 5000))
+    both(odd_rows(), numbers(r, n), cap=cap, index=index, top_p=r.choice([0.1, 0.9, 1.0], n), temperature=r.choice([0.01, 1, np.inf], n))
 
 
 def test_ends_of_the_arguments(gpu):
@@ -208,7 +225,7 @@ def test_temperatures_at_the_ends_with_masked_tokens(gpu, t, cap):
     logits = (4 * r.standard_normal((6, 2500))).astype(np.float32)
     logits[1::2, r.integers(0, 2500, 900)] = -np.inf
     logits[2, ::3] = np.nan
-    for params in ({}, {"min_p": [0.5] * 6}, {"top_k": [40] * 6}, {"top_p": [0.7] * 6}, {"top_k": [900] * 6, "top_p": [0.3] * 6}):
+    for params in ({}, {"min_p": [0.5] * 6}, {"min_p": [1.0] * 6}, {"top_k": [40] * 6}, {"top_p": [0.7] * 6}, {"top_k": [900] * 6, "top_p": [0.3] * 6}):
         both(logits, [0.0, 0.2, 0.5, 0.7, 0.9, LAST], cap=cap, temperature=[t] * 6, **params)
 
 

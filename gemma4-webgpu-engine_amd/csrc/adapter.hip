@@ -529,6 +529,7 @@ struct Expand {
                     hi[e] = (_Float16)o;
                     lo[e] = (_Float16)(o - (float)hi[e]);
                 }
+                if (__any(top == INFINITY)) lo = top == INFINITY ? hr{} : lo;  // an infinite H stays one
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int r = wave * kWaveN + 32 * (j / 2) + 8 * (col / 4) + 4 * (j % 2) + col % 4;

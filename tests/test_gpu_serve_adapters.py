@@ -281,6 +281,27 @@ def test_a_bad_row_stays_alone(gpu):
     c.check(good)
 
 
+@pytest.mark.parametrize("rank", [8, 72])
+def test_infinities_are_those_of_the_formula(gpu, rank):
+    """An infinite x, and sums that pass f32: outputs of their sign, NaN where the formula has one."""
+    c = Case([0, 0, 1, 1, 2], adapters=3, rank=rank, ranks=[1, 2, rank], x="f32", out="f32", k=64, n=40)
+    c.b[0, ::7, 0] = 0
+    c.x[0, 3], c.x[2, 5] = np.inf, -np.inf
+    c.x[1] = np.float32(3e38) * np.sign(c.a[0, 0]).astype(np.float32)
+    c.x[4, 9] = np.nan
+    c.upload()
+    c.call()
+    g4.synchronize()
+    got = c.out.download()
+    with np.errstate(all="ignore"):
+        for i, a in enumerate(c.ids):
+            m = c.ranks[a]
+            h = np.array([np.float32((c.x[i].astype(np.float64) * c.a[a, r]).sum()) for r in range(m)], np.float64)
+            want = (c.base[i] + float(c.scales[a]) * (h * c.b[a, :, :m].astype(np.float64)).sum(1)).astype(np.float32)
+            there = ~np.isfinite(want)
+            assert np.array_equal(np.isnan(want), np.isnan(got[i])) and np.array_equal(want[there], got[i][there], equal_nan=True), i
+
+
 @pytest.mark.parametrize("t,k,n", [(41, 512, 64), (1000, 6144, 1024)])
 def test_a_row_does_not_depend_on_its_batch(gpu, t, k, n):
     """The same row in another place, among other adapters, of as many tokens: the same bits."""

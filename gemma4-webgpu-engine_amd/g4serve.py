@@ -39,7 +39,12 @@ def _kind(x):
 def _device() -> int:
     """The current device, which torch tensors have to be on (asked once a call)."""
     torch = sys.modules.get("torch")
-    return torch.cuda.current_device() if torch is not None and torch.cuda.is_initialized() else 0
+    if torch is None or not torch.cuda.is_initialized():
+        return 0
+    try:
+        return torch._C._cuda_getDevice()
+    except AttributeError:  # the same, a little slower
+        return torch.cuda.current_device()
 
 
 _one_runtime = None
@@ -83,12 +88,15 @@ def _address(x, what, device):
 def _stream(stream, device, *operands):
     """The handle to launch on."""
     torch = sys.modules.get("torch")
-    if stream is not None or torch is None or not any(hasattr(x, "data_ptr") for x in operands):
+    if stream is not None or torch is None:
         return stream
-    try:
-        return torch._C._cuda_getCurrentRawStream(device)
-    except AttributeError:  # the same, some microseconds slower
-        return torch.cuda.current_stream(device).cuda_stream
+    for x in operands:
+        if hasattr(x, "data_ptr"):
+            try:
+                return torch._C._cuda_getCurrentRawStream(device)
+            except AttributeError:  # the same, some microseconds slower
+                return torch.cuda.current_stream(device).cuda_stream
+    return None
 
 
 def _call_device(pages, chunk) -> int:
@@ -370,6 +378,13 @@ def _optional(x, what, kinds, shape, device):
 
 def _table(page_table, device):
     """(address, sequences, pages, elements between rows) of a page table."""
+    try:
+        if (page_table.get_device() == device and _one_runtime and page_table.dim() == 2 and page_table.is_contiguous()
+                and _kinds[page_table.dtype] == g4.KIND_I32):
+            seqs, width = page_table.shape
+            return page_table.data_ptr(), seqs, width, width
+    except (AttributeError, KeyError):
+        pass
     if len(page_table.shape) != 2:
         raise g4.G4Error(1, f"page_table has shape {list(page_table.shape)}, expected [seqs][pages]")
     seqs, width = (int(n) for n in page_table.shape)

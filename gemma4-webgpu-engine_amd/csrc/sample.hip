@@ -27,6 +27,7 @@ constexpr int kFew = 64;     // entries that a wave orders by itself
 constexpr int kSub = 1024, kSubPer = kSub / kSampleThreads;  // ranges of one refinement step
 constexpr int kUnitPer = kSampleUnit / kSampleThreads;
 constexpr int kLineWords = 32;
+constexpr int kWideRow = 128;  // units
 constexpr int kMaxVocab = 1 << 22;
 
 struct PartMax {
@@ -66,7 +67,7 @@ struct SampleArgs {
     const float *top_p, *min_p, *u;
     CapArgs cap;
     int logit_rows, vocab, parts, units, shift, vec, cuts;  // cuts: top-k or top-p given
-    int wide, spans, many;       // waves of a block of (2) and (3), blocks a row, and whether there are many
+    int wide, share, spans, many;  // waves of a block of (2) and (3), those of a unit, blocks a row, whether there are many
     PartMax *stats;              // [rows][parts]
     Row *row;                    // [rows]
     Cuts *cut;                   // [rows]
@@ -91,11 +92,12 @@ __device__ __forceinline__ int unit_place(int j, int lane, int vec) {
     return vec ? (j / 4) * 256 + 4 * lane + j % 4 : j * 64 + lane;
 }
 
-// The lane's values of the wave's unit at x, `n` of which exist; a NaN is one.
-__device__ __forceinline__ void load_unit(const float *x, int n, int lane, int vec, float (&v)[kSamplePer]) {
+// The lane's values of the wave's unit, or quarter of one, at x, `n` of which exist; a NaN is one.
+template <int PER>
+__device__ __forceinline__ void load_unit(const float *x, int n, int lane, int vec, float (&v)[PER]) {
     if (vec) {
 #pragma unroll
-        for (int j = 0; j < kSamplePer; j += 4) {
+        for (int j = 0; j < PER; j += 4) {
             const int i = unit_place(j, lane, 1);
             if (i + 4 <= n) {
                 const float4 y = *reinterpret_cast<const float4 *>(x + i);
@@ -110,7 +112,7 @@ __device__ __forceinline__ void load_unit(const float *x, int n, int lane, int v
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < kSamplePer; ++j) {
+        for (int j = 0; j < PER; ++j) {
             const int i = unit_place(j, lane, 0);
             v[j] = i < n ? x[i] : -INFINITY;
         }
@@ -361,6 +363,17 @@ __device__ __forceinline__ u64 block_run(u64 v, u64 *lds, u64 *total) {
 // wave's loads of them are of whole lines. (Loads of 128 bytes a lane stalled on each other's lines: 12 us.)
 __device__ __forceinline__ int bin_at(int i) { return i % 64 * kBinsPer + i / 64; }
 
+// The sums of units that waves of a block share.
+template <int WAVES, int SHARE>
+__device__ __forceinline__ void put_unit_sums(const SampleArgs &A, int row, const u64 *sums) {
+    const int t = threadIdx.x, unit = blockIdx.x * (WAVES / SHARE) + t;
+    if (t >= WAVES / SHARE || unit >= A.units) return;
+    u64 all = 0;
+#pragma unroll
+    for (int w = 0; w < SHARE; ++w) all += sums[t * SHARE + w];
+    A.unit_sums[(int64_t)row * A.units + unit] = all;
+}
+
 // Four rows a block, a wave each: for calls of many blocks, each of which would do it again (5.4 us).
 __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs A, int rows) {
     const int row = blockIdx.x * kSampleWaves + (threadIdx.x >> 6);
@@ -370,18 +383,20 @@ __global__ __launch_bounds__(kSampleThreads) void sample_row_kernel(SampleArgs A
 }
 
 // Grid (spans, rows). Bound by issue: with a cap 41 vector operations a logit, 27 of them 64-bit, which keep the vector
-// units busy for 75% of 105 us (256 rows of 262144); the atomics keep LDS busy for half of it. One row: 8.7 us, a chain.
+// units busy for 75% of 105 us (256 rows of 262144); the atomics keep LDS busy for half of it. One row: 7.2 us, a chain.
+// SHARE: waves that share a unit, a quarter each.
 // READY: the rows' parameters are there (sample_row_kernel).
-template <bool CAP, int WAVES, bool READY>
+template <bool CAP, int WAVES, int SHARE, bool READY>
 __global__ __launch_bounds__(64 * WAVES, 8) void sample_weights_kernel(SampleArgs A) {
     __shared__ u64 mass[kBins];        // (16 bytes a bin with its count: a wave's atomics in more conflicts, 4 us of 105)
     __shared__ uint32_t count[kBins];  // where there is a top-k
-    __shared__ u64 ss[WAVES];
+    __shared__ u64 ss[WAVES], ks[WAVES];
+    constexpr int kPer = kSamplePer / SHARE;
     __shared__ Row shared_row;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, row = blockIdx.y;
     const float *x = row_of(A, row);
-    const int unit = blockIdx.x * WAVES + wave, base = unit * kSampleUnit;
-    float v[kSamplePer];
+    const int place = blockIdx.x * WAVES + wave, unit = place / SHARE, base = place * (kSampleUnit / SHARE);
+    float v[kPer];
     load_unit(x + base, x ? A.vocab - base : 0, lane, A.vec, v);
     if (!READY && wave == 0) {  // once a block: as many operations as the weights of a unit
         const Row R = row_params(A, row);
@@ -400,19 +415,19 @@ __global__ __launch_bounds__(64 * WAVES, 8) void sample_weights_kernel(SampleArg
         float most = 0.0f;
         if (CAP) {
 #pragma unroll
-            for (int j = 0; j < kSamplePer; ++j) most = fmaxf(most, fabsf(v[j]));
+            for (int j = 0; j < kPer; ++j) most = fmaxf(most, fabsf(v[j]));
         }
         uint32_t far = 0;  // places where a lane's logit is past half the cap: few, one at a time
         if (CAP && __any(most > A.cap.half_cap)) {
 #pragma unroll
-            for (int j = 0; j < kSamplePer; ++j) {
+            for (int j = 0; j < kPer; ++j) {
                 const bool f = is_far(v[j], A.cap);
                 far |= __ballot(f) ? 1u << j : 0u;
                 v[j] = f ? -INFINITY : v[j];
             }
         }
 #pragma unroll
-        for (int j = 0; j < kSamplePer; ++j) {
+        for (int j = 0; j < kPer; ++j) {
             float xs = v[j];
             asm("" : "+v"(xs));  // one after the other: all at once they would not fit the registers
             add(near_distance<CAP>(xs, R, A, F));
@@ -425,7 +440,7 @@ __global__ __launch_bounds__(64 * WAVES, 8) void sample_weights_kernel(SampleArg
     };
     if (R.inf) {
 #pragma unroll
-        for (int j = 0; j < kSamplePer; ++j) v[j] = seen(v[j], R);
+        for (int j = 0; j < kPer; ++j) v[j] = seen(v[j], R);
     }
     u64 all = 0;
     if (R.filtered) {
@@ -447,7 +462,8 @@ __global__ __launch_bounds__(64 * WAVES, 8) void sample_weights_kernel(SampleArg
             kept += d >= R.d_min ? w : 0;
         });
         kept = wave_sum(kept);
-        if (lane == 0 && unit < A.units) A.unit_sums[(int64_t)row * A.units + unit] = kept;
+        if (SHARE == 1 && lane == 0 && unit < A.units) A.unit_sums[(int64_t)row * A.units + unit] = kept;
+        if (SHARE > 1 && lane == 0) ks[wave] = kept;
     }
     if (R.filtered) {
         __syncthreads();
@@ -462,6 +478,7 @@ __global__ __launch_bounds__(64 * WAVES, 8) void sample_weights_kernel(SampleArg
     all = wave_sum(all);
     if (lane == 0) ss[wave] = all;
     __syncthreads();
+    if (SHARE > 1 && !R.filtered) put_unit_sums<WAVES, SHARE>(A, row, ks);
     if (t) return;
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) all += ss[w];
@@ -588,9 +605,9 @@ __global__ __launch_bounds__(kSampleThreads) void sample_find_kernel(SampleArgs 
 }
 
 // A wave's unit of a row with cuts: the weight above them, and what lies in their bins to the list. v: its logits, at x.
-template <bool CAP>
+template <bool CAP, int PER>
 __device__ __forceinline__ u64 cut_unit(const SampleArgs &A, const Row &R, const Cuts &c, int row, const float *x, int base,
-                                        const float (&v)[kSamplePer]) {
+                                        const float (&v)[PER]) {
     const int lane = threadIdx.x & 63;
     u64 sure = 0;
     uint32_t far = 0, in = 0;  // places where a lane's token is past half the cap, and may count; a lane's for the list
@@ -609,11 +626,11 @@ __device__ __forceinline__ u64 cut_unit(const SampleArgs &A, const Row &R, const
     float most = 0.0f;
     if (CAP) {
 #pragma unroll
-        for (int j = 0; j < kSamplePer; ++j) most = fmaxf(most, fabsf(v[j]));
+        for (int j = 0; j < PER; ++j) most = fmaxf(most, fabsf(v[j]));
     }
     const bool some = CAP && __any(most > A.cap.half_cap);
 #pragma unroll
-    for (int j = 0; j < kSamplePer; ++j) {
+    for (int j = 0; j < PER; ++j) {
         if (!__any(v[j] >= c.least)) continue;
         const float xs = seen(clean(v[j]), R);
         bool real = xs > -INFINITY;
@@ -635,7 +652,7 @@ __device__ __forceinline__ u64 cut_unit(const SampleArgs &A, const Row &R, const
         if (lane == 0) at = atomicAdd(&A.listed[(int64_t)row * kLineWords], (uint32_t)many);
         at = __shfl(at, 0);
 #pragma unroll
-        for (int j = 0; j < kSamplePer; ++j) {
+        for (int j = 0; j < PER; ++j) {
             const bool mine = in >> j & 1;
             const u64 who = __ballot(mine);
             const uint32_t place = at + __popcll(who & ((1ull << lane) - 1));
@@ -647,15 +664,16 @@ __device__ __forceinline__ u64 cut_unit(const SampleArgs &A, const Row &R, const
     return wave_sum(sure);
 }
 
-// Grid (spans, rows): a block finds its row's cuts itself, its logits on their way. One row 6.1 us, 32 rows of 262144 11.6.
-template <bool CAP, int WAVES>
+// Grid (spans, rows): a block finds its row's cuts itself, its logits on their way. One row 5.2 us, 32 rows of 262144 11.6.
+template <bool CAP, int WAVES, int SHARE>
 __global__ __launch_bounds__(64 * WAVES) void sample_cut_kernel(SampleArgs A) {
     __shared__ Cuts shared_cuts;
+    __shared__ u64 ss[WAVES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.y;
-    const int unit = blockIdx.x * WAVES + wave, base = unit * kSampleUnit;
+    const int place = blockIdx.x * WAVES + wave, unit = place / SHARE, base = place * (kSampleUnit / SHARE);
     const float *x = row_of(A, row);
     const float top = unit < A.units ? A.unit_max[(int64_t)row * A.units + unit] : -INFINITY;
-    float v[kSamplePer];
+    float v[kSamplePer / SHARE];
     load_unit(x + base, x ? A.vocab - base : 0, lane, A.vec, v);
     LaneBins B;
     if (wave == 0) B.load(A, row);
@@ -670,9 +688,15 @@ __global__ __launch_bounds__(64 * WAVES) void sample_cut_kernel(SampleArgs A) {
     }
     __syncthreads();
     const Cuts c = uniform(shared_cuts);
-    if (unit >= A.units) return;
-    const u64 sure = top >= c.least ? cut_unit<CAP>(A, R, c, row, x, base, v) : 0;
-    if (lane == 0) A.unit_sums[(int64_t)row * A.units + unit] = sure;
+    if (SHARE == 1 && unit >= A.units) return;
+    const u64 sure = unit < A.units && top >= c.least ? cut_unit<CAP>(A, R, c, row, x, base, v) : 0;
+    if (SHARE == 1) {
+        if (lane == 0) A.unit_sums[(int64_t)row * A.units + unit] = sure;
+        return;
+    }
+    if (lane == 0) ss[wave] = sure;
+    __syncthreads();
+    put_unit_sums<WAVES, SHARE>(A, row, ss);
 }
 
 // Grid (units by 4, rows), behind sample_find_kernel: units that do not reach up to the cuts are not read. 256 rows of
@@ -1057,11 +1081,13 @@ static int launch_sample(const SampleArgs &A, int rows, hipStream_t s) {
     if (A.many) {
         hipLaunchKernelGGL(sample_row_kernel, by_row, dim3(kSampleThreads), 0, s, A, rows);
         G4_LAUNCHED("sample_row_kernel");
-        hipLaunchKernelGGL((sample_weights_kernel<CAP, 8, true>), grid, block, 0, s, A);
-    } else if (A.wide == 4) {
-        hipLaunchKernelGGL((sample_weights_kernel<CAP, 4, false>), grid, block, 0, s, A);
+        hipLaunchKernelGGL((sample_weights_kernel<CAP, 8, 1, true>), grid, block, 0, s, A);
+    } else if (A.wide == 16) {
+        hipLaunchKernelGGL((sample_weights_kernel<CAP, 16, 4, false>), grid, block, 0, s, A);
+    } else if (A.share == 4) {
+        hipLaunchKernelGGL((sample_weights_kernel<CAP, 8, 4, false>), grid, block, 0, s, A);
     } else {
-        hipLaunchKernelGGL((sample_weights_kernel<CAP, 8, false>), grid, block, 0, s, A);
+        hipLaunchKernelGGL((sample_weights_kernel<CAP, 8, 1, false>), grid, block, 0, s, A);
     }
     G4_LAUNCHED("sample_weights_kernel");
     if (A.cuts && A.many) {
@@ -1071,8 +1097,9 @@ static int launch_sample(const SampleArgs &A, int rows, hipStream_t s) {
         hipLaunchKernelGGL(sample_cut_found_kernel<CAP>, by_unit, dim3(kSampleThreads), 0, s, A);
         G4_LAUNCHED("sample_cut_found_kernel");
     } else if (A.cuts) {
-        if (A.wide == 4) hipLaunchKernelGGL((sample_cut_kernel<CAP, 4>), grid, block, 0, s, A);
-        else hipLaunchKernelGGL((sample_cut_kernel<CAP, 8>), grid, block, 0, s, A);
+        if (A.wide == 16) hipLaunchKernelGGL((sample_cut_kernel<CAP, 16, 4>), grid, block, 0, s, A);
+        else if (A.share == 4) hipLaunchKernelGGL((sample_cut_kernel<CAP, 8, 4>), grid, block, 0, s, A);
+        else hipLaunchKernelGGL((sample_cut_kernel<CAP, 8, 1>), grid, block, 0, s, A);
         G4_LAUNCHED("sample_cut_kernel");
     }
     hipLaunchKernelGGL(sample_pick_kernel<CAP>, dim3(rows), dim3(kSampleThreads), A.units * sizeof(u64), s, A);
@@ -1091,8 +1118,8 @@ extern "C" {
 
 size_t g4_sample_workspace_bytes(int rows, int64_t vocab) {
     if (rows <= 0 || rows > 65535 || vocab <= 0 || vocab > kMaxVocab) return 0;
-    const size_t row = (size_t)sample_parts(vocab) * (sizeof(PartMax) + sizeof(u64)) +
-                       (size_t)sample_units(vocab) * (sizeof(u64) + sizeof(float)) + kBins * (sizeof(u64) + sizeof(uint32_t)) +
+    const size_t row = (size_t)sample_parts(vocab) * sizeof(PartMax) +
+                       (size_t)sample_units(vocab) * (2 * sizeof(u64) + sizeof(float)) + kBins * (sizeof(u64) + sizeof(uint32_t)) +
                        kList * sizeof(u64) + sizeof(Row) + sizeof(Cuts) + kLineWords * sizeof(uint32_t);
     return rows * row;
 }
@@ -1136,18 +1163,21 @@ int g4_sample_tokens(const float *logits, int logit_rows, int64_t logit_stride, 
     A.shift = 62 - bits < 51 ? 62 - bits : 51;
     A.vec = A.stride % 4 == 0 && ((uintptr_t)logits & 15) == 0;
     A.cuts = top_k || top_p;
-    // 8 waves share a block's fixed work, the row's parameters, its histogram and its cuts; where that leaves CUs
-    // without a block, 4 have a SIMD each: 8 rows of 262144 (256 blocks) 34.4 us and by 4 waves 35.6, 32 rows of 32003 (128)
-    // 36.5 and 35.2. More blocks than are there at once would each make the row's parameters and cuts: two launches more,
-    // 64 rows (2048 blocks) 88 us and without 93, 32 rows (1024) 61 and 56
-    A.wide = (int64_t)rows * ((A.units + 7) / 8) >= device_cu_count() ? 8 : 4;
-    A.spans = (A.units + A.wide - 1) / A.wide;  // at most parts
-    A.many = (int64_t)rows * A.spans > 4 * device_cu_count();
+    // A block's waves have its fixed work together, the row's parameters, its histogram and its cuts. Where a wave a unit would
+    // leave SIMDs with few, four share one: 1 row of 262144 21.3 us, a wave a unit 24.1; 32 rows of 32003 30.3 and 36.2;
+    // 6 rows of 262144 (1536 units) 32-45 and 34; 2000 rows of 1024 62 and 88. In a wide row by 16 waves a block, since each
+    // block adds to the row's histogram: 1 row of 262144 21.3 us, 8 waves 23.1; 32 rows of 32003 30.3 and 31.0.
+    A.share = (int64_t)rows * A.units <= 4 * device_cu_count() || A.units <= 2 ? 4 : 1;
+    A.wide = A.share == 4 && A.units >= kWideRow ? 16 : 8;
+    A.spans = (A.units * A.share + A.wide - 1) / A.wide;  // at most units
+    // More blocks than are there at once would each make the row's parameters and cuts: two launches more, 64 rows (2048
+    // blocks) 88 us and without 93, 32 rows (1024) 61 and 56
+    A.many = A.share == 1 && (int64_t)rows * A.spans > 4 * device_cu_count();
     A.stats = static_cast<PartMax *>(workspace);
     A.row = reinterpret_cast<Row *>(A.stats + (int64_t)rows * A.parts);
     A.cut = reinterpret_cast<Cuts *>(A.row + rows);
     A.span_sums = reinterpret_cast<u64 *>(A.cut + rows);
-    A.unit_sums = A.span_sums + (int64_t)rows * A.parts;
+    A.unit_sums = A.span_sums + (int64_t)rows * A.units;
     A.bin_mass = A.unit_sums + (int64_t)rows * A.units;
     A.list = A.bin_mass + (int64_t)rows * kBins;
     A.bin_count = reinterpret_cast<uint32_t *>(A.list + (int64_t)rows * kList);

@@ -139,6 +139,21 @@ def test_rows(gpu, rows):
     both(logits, numbers(r, rows), cap=20.0, **mixed(r, rows, 3001))
 
 
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("vocab", [131072, 200003, 262144])
+@pytest.mark.parametrize("rows", [1, 4])
+def test_few_wide_rows(gpu, rows, vocab, cap):
+    """A unit shared by four waves, in blocks of sixteen; every kind of filter, peaked and flat rows, far logits, masks."""
+    r = np.random.default_rng(rows + vocab)
+    for i in range(6):
+        logits = ((0.5, 4.0)[i % 2] * r.standard_normal((rows, vocab))).astype(np.float32)
+        logits[:, r.integers(0, vocab, 30)] += 14
+        logits[:, r.integers(0, vocab, 5000)] = (-np.inf, np.nan, -3.4e38)[i % 3]
+        both(logits, r.random(rows).astype(np.float32), cap=cap, **mixed(r, rows, vocab))
+    both(logits, [LAST] * rows, cap=cap)
+    both(logits, [0.5] * rows, cap=cap, min_p=[0.01] * rows, temperature=[2.0] * rows)
+
+
 @pytest.mark.parametrize("vocab", [3000, 262144])
 def test_ties(gpu, vocab):
     """Logits on a coarse grid (a quantised head), all alike, or all alike but one: cuts go by the lower id, and more

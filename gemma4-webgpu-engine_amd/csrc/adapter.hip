@@ -70,19 +70,21 @@ __global__ __launch_bounds__(kGroupThreads) void adapter_groups_kernel(const int
         const int a = row < tokens ? row_adapter[row] : -2;
         return a == -2 ? -1 : (unsigned)a < (unsigned)adapters ? a + 1 : 0;
     };
-    // a wave's rows of one group are counted together, and stand together
+    // Where many of a wave's rows have the first one's group, as in a prompt, those are counted together: additions to one
+    // address wait for each other (2048 rows of 4 groups in runs 5.1 us and each row by itself 7.3; all others so: 4096
+    // rows of 64 groups at random 6.4 us, group by group 50).
     auto place = [&](int g) {
         int mine = 0;
-        unsigned long long left = __ballot(g >= 0);
-        while (left) {
-            const int leader = __ffsll((long long)left) - 1;
-            const unsigned long long same = __ballot(g == __shfl(g, leader));
-            if (same >> lane & 1) {
-                int at = 0;
-                if (lane == leader) at = atomicAdd(&count[g], (int)__popcll(same));
-                mine = __shfl(at, leader) + __popcll(same & ((1ull << lane) - 1));
-            }
-            left &= ~same;
+        const unsigned long long real = __ballot(g >= 0);
+        if (!real) return 0;
+        const int leader = __ffsll((long long)real) - 1;
+        unsigned long long same = __ballot(g == __builtin_amdgcn_readlane(g, leader));
+        if (__popcll(same) < 16) same = 0;
+        if (same >> lane & 1) {
+            if (lane == leader) mine = atomicAdd(&count[g], (int)__popcll(same));
+            mine = __builtin_amdgcn_readlane(mine, leader) + (int)__popcll(same & ((1ull << lane) - 1));
+        } else if (g >= 0) {
+            mine = atomicAdd(&count[g], 1);
         }
         return mine;
     };

@@ -1170,8 +1170,8 @@ int g4_sample_tokens(const float *logits, int logit_rows, int64_t logit_stride, 
     A.share = (int64_t)rows * A.units <= 4 * device_cu_count() || A.units <= 2 ? 4 : 1;
     A.wide = A.share == 4 && A.units >= kWideRow ? 16 : 8;
     A.spans = (A.units * A.share + A.wide - 1) / A.wide;  // at most units
-    // More blocks than are there at once would each make the row's parameters and cuts: two launches more, 64 rows (2048
-    // blocks) 88 us and without 93, 32 rows (1024) 61 and 56
+    // More blocks than are there at once would each make the row's parameters and cuts: two launches more, 56 rows (1792
+    // blocks) 71.3 us and without 75.5, 32 rows (1024) 55.2 and 51.5
     A.many = A.share == 1 && (int64_t)rows * A.spans > 4 * device_cu_count();
     A.stats = static_cast<PartMax *>(workspace);
     A.row = reinterpret_cast<Row *>(A.stats + (int64_t)rows * A.parts);

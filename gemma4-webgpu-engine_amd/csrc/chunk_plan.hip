@@ -3,16 +3,18 @@
 //
 // No block waits for another: each computes the prefix sums of all sequences (at most 4096, a few loads a
 // thread) into LDS and finds its items' sequences there by binary search. That is why a call's counts are
-// read from other arrays than it writes.
+// read from other arrays than it writes. Release counts the pages in front of a block's entries in the same way.
 #include "g4_internal.h"
 #include "../../include/g4serve.h"
 
 namespace g4 {
 
 constexpr int kPlanSeqs = 4096, kPlanThreads = 256;
-// Blocks of a kind, two a CU; more items go round, since every block sums all sequences up (1000 requests that
-// give back a page each, of 1024: 9.6 us a call, 15.3 with 4000 blocks).
+// Blocks of a kind, two a CU; more items go round, since every block sums all sequences up.
 constexpr int kPlanBlocks = 512;
+// Release: 512 threads a block start and meet sooner than 1024 (16 requests of up to 256 pages 4.0 and 5.1 us replayed), and read
+// nearly as fast (1024 of up to 1024 pages 46.6 and 40.2).
+constexpr int kReleaseLog = 9, kReleaseThreads = 1 << kReleaseLog, kReleaseBlocks = 256;
 
 struct PlanArgs {
     int32_t *free_pages;
@@ -46,8 +48,9 @@ struct Pair {
 };
 
 // Exclusive sum over the block's threads of v; *total: of all. Once a kernel.
+template <int THREADS>
 __device__ __forceinline__ Pair block_before(Pair v, Pair *total) {
-    __shared__ Pair sums[kPlanThreads / 64];
+    __shared__ Pair sums[THREADS / 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     Pair run = v;
 #pragma unroll
@@ -62,7 +65,7 @@ __device__ __forceinline__ Pair block_before(Pair v, Pair *total) {
     __syncthreads();
     Pair before{run.rows - v.rows, run.pages - v.pages}, all{0, 0};
 #pragma unroll
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
+    for (int w = 0; w < THREADS / 64; ++w) {
         const Pair s = sums[w];
         if (w < wave) {
             before.rows += s.rows;
@@ -76,7 +79,8 @@ __device__ __forceinline__ Pair block_before(Pair v, Pair *total) {
 }
 
 // The last s with start[s] <= i of an ascending start[0 .. n], for i < start[n].
-__device__ __forceinline__ int owner(const int32_t *start, int n, int i) {
+template <class T>
+__device__ __forceinline__ int owner(const T *start, int n, T i) {
     int lo = 0, hi = n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -103,7 +107,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_chunk_kernel(PlanArgs A, in
         mine.pages += w.need;
         cached[s] = w.cached;
     }
-    Pair at = block_before(mine, &all);
+    Pair at = block_before<kPlanThreads>(mine, &all);
     int fits = 0;
     for (int s = s0; s < s1; ++s) {
         const Wish w = wish_of(A, s);
@@ -133,7 +137,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_chunk_kernel(PlanArgs A, in
         for (int64_t i = (int64_t)block * kPlanThreads + t; i < A.tokens; i += (int64_t)row_blocks * kPlanThreads) {
             int pos = -1, slot = -1, adapter = -2;
             if (i < total_rows) {
-                const int s = owner(start, served, (int)i);
+                const int s = owner(start, served, (int32_t)i);
                 adapter = A.seq_adapter && A.row_adapter ? A.seq_adapter[s] : -1;
                 pos = cached[s] + ((int)i - start[s]);
                 if (A.row_slot) {
@@ -153,7 +157,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_chunk_kernel(PlanArgs A, in
     block -= row_blocks;
     if (block < page_blocks) {
         for (int64_t i = (int64_t)block * kPlanThreads + t; i < total_pages; i += (int64_t)page_blocks * kPlanThreads) {
-            const int s = owner(pages, served, (int)i);
+            const int s = owner(pages, served, (int32_t)i);
             A.table[s * A.table_stride + first_new(s) + ((int)i - pages[s])] = A.free_pages[left + i];
         }
         return;
@@ -179,7 +183,7 @@ struct ReleaseArgs {
     const int32_t *count, *table, *first, *last;
     int64_t table_stride;
     int32_t *count_out;
-    int capacity, seqs, table_pages;
+    int capacity, num_pages, seqs, table_pages;
 };
 
 __device__ __forceinline__ int2 range_of(const ReleaseArgs &A, int s) {
@@ -187,34 +191,101 @@ __device__ __forceinline__ int2 range_of(const ReleaseArgs &A, int s) {
     return make_int2(a, max(min(A.last[s], A.table_pages), a));
 }
 
-// Bound by its chain: count, ranges, a block sum, a search, an entry, the store. 16 requests of 256 pages 3.2 us, 1000 of which
-// each gives back one 4.9.
-__global__ __launch_bounds__(kPlanThreads) void release_pages_kernel(ReleaseArgs A) {
-    extern __shared__ int32_t plan_lds[];
-    int32_t *start = plan_lds;
-    const int t = threadIdx.x, per = (A.seqs + kPlanThreads - 1) / kPlanThreads;
+// 2^grid_log blocks have equal runs of the ranges' entries, a tile of an entry a thread at a time. Absent entries are left
+// out, so where a block's pages go depends on how many of those stand in front of its own: it reads all that do. Bound by its
+// chain, count, ranges, a block sum, a search, an entry, those in front, a block sum, the store: 16 requests of 170 pages
+// 4.0 us replayed, 1000 of which most give back one 5.0; past some 50000 pages by the last block's reads (100074 pages
+// 10 us, 655842 46; 3.4 and 9.1 if nobody looked for absent ones).
+__global__ __launch_bounds__(kReleaseThreads) void release_pages_kernel(ReleaseArgs A, int grid_log) {
+    extern __shared__ int64_t release_lds[];
+    __shared__ int wave_absent[kReleaseThreads / 64], wave_pages[kReleaseThreads / 64];
+    int64_t *start = release_lds;  // of each request's entries among all
+    int32_t *from = reinterpret_cast<int32_t *>(start + A.seqs + 1);
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, per = (A.seqs + kReleaseThreads - 1) / kReleaseThreads;
     const int s0 = min(t * per, A.seqs), s1 = min(s0 + per, A.seqs);
-    const int count = min(max(*A.count, 0), A.capacity), room = A.capacity - count;
+    const int count = min(max(*A.count, 0), A.capacity);
     Pair n{0, 0}, all;
     for (int s = s0; s < s1; ++s) {
         const int2 r = range_of(A, s);
+        from[s] = r.x;
+        start[s] = n.pages;
         n.pages += r.y - r.x;
     }
-    int64_t before = block_before(n, &all).pages;
-    for (int s = s0; s < s1; ++s) {
-        const int2 r = range_of(A, s);
-        start[s] = (int)min(before, (int64_t)room);
-        before += r.y - r.x;
-    }
-    const int total = (int)min(all.pages, (int64_t)room);
+    const int64_t before = block_before<kReleaseThreads>(n, &all).pages, total = all.pages;
+    for (int s = s0; s < s1; ++s) start[s] += before;
     if (t == 0) start[A.seqs] = total;
     __syncthreads();
-    const int64_t stride = (int64_t)gridDim.x * kPlanThreads, first = (int64_t)blockIdx.x * kPlanThreads + t;
-    for (int64_t i = first; i < total; i += stride) {
-        const int s = owner(start, A.seqs, (int)i);
-        A.free_pages[count + i] = A.table[s * A.table_stride + range_of(A, s).x + ((int)i - start[s])];
+    const int64_t tiles = (total + kReleaseThreads - 1) / kReleaseThreads;
+    const int64_t run = ((tiles + (1 << grid_log) - 1) >> grid_log) * kReleaseThreads;
+    const int64_t begin = blockIdx.x * run, end = min(begin + run, total);
+    if (begin >= total && (blockIdx.x || total)) return;
+    auto page_at = [&](int64_t i) {
+        if (i >= end) return -1;
+        const int s = owner(start, A.seqs, i);
+        return A.table[s * A.table_stride + from[s] + (i - start[s])];
+    };
+    auto is_page = [&](int page) { return (unsigned)page < (unsigned)A.num_pages; };
+    int page = page_at(begin + t);
+    int absent = 0;  // in front
+    if (begin) {
+        // a request's entries by 2^group_log threads: what there is for each, or for its average number to be four loads
+        int group_log = 0;
+        while (group_log < kReleaseLog &&
+               ((A.seqs << (group_log + 1)) <= kReleaseThreads || ((int64_t)A.seqs << (group_log + 5)) <= total))
+            ++group_log;
+        const int rows = owner(start, A.seqs, begin - 1) + 1;
+        const uint32_t step = 4 << group_log, mine = 4 * (t & ((1 << group_log) - 1));
+        for (int s = t >> group_log; s < rows; s += kReleaseThreads >> group_log) {
+            const uint32_t len = (uint32_t)(min(begin, start[s + 1]) - start[s]);
+            const int32_t *row = A.table + s * A.table_stride + from[s];
+            if (len < 4) {
+                for (uint32_t i = mine; i < len; ++i) absent += !is_page(row[i]);
+                continue;
+            }
+            for (uint32_t i = mine; i < len; i += 4 * step) {
+                int32_t e[4][4];
+                uint32_t most = 0;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)  // the last four where fewer are left
+                    __builtin_memcpy(e[u], row + min(i + u * step, len - 4), sizeof e[u]);
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) most = max(most, (uint32_t)e[u][j]);
+                if (is_page(most)) continue;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)  // (what is not this thread's is not counted)
+                        absent += min(i + u * step, len - 4) + j >= i + u * step && !is_page(e[u][j]);
+            }
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) absent += __shfl_xor(absent, o);
     }
-    if (first == 0) *A.count_out = count + total;
+    if (lane == 0) wave_absent[wave] = absent;
+    int64_t at = count + begin;
+    for (int64_t i = begin; i < end; i += kReleaseThreads) {
+        const bool is = is_page(page);
+        const unsigned long long who = __ballot(is);
+        if (lane == 0) wave_pages[wave] = __popcll(who);
+        __syncthreads();
+        int waves_before = 0, tile = 0;
+#pragma unroll
+        for (int w = 0; w < kReleaseThreads / 64; ++w) {
+            if (i == begin) at -= wave_absent[w];
+            waves_before += w < wave ? wave_pages[w] : 0;
+            tile += wave_pages[w];
+        }
+        const int64_t to = at + waves_before + __popcll(who & ((1ull << lane) - 1));
+        if (is && to < A.capacity) A.free_pages[to] = page;
+        at += tile;
+        if (i + kReleaseThreads < end) {
+            page = page_at(i + kReleaseThreads + t);
+            __syncthreads();
+        }
+    }
+    if (t == 0 && end == total) *A.count_out = (int)min(at, (int64_t)A.capacity);
 }
 
 static int check_list(const char *who, const g4_free_pages *L) {
@@ -289,10 +360,12 @@ int g4_release_pages(const g4_free_pages *list, const int32_t *page_table, int t
     if (count_out == list->count)
         return set_error(G4_ERR_INVALID, "release-pages: count_out cannot be the list's count");
     ReleaseArgs A{list->pages, list->count, page_table, first, last, table_stride ? table_stride : table_pages, count_out,
-                  list->capacity, seqs, table_pages};
+                  list->capacity, list->num_pages, seqs, table_pages};
     const int64_t most = (int64_t)seqs * table_pages;
-    hipLaunchKernelGGL(release_pages_kernel, dim3(plan_blocks(most < list->capacity ? most : list->capacity)),
-                       dim3(kPlanThreads), ((size_t)seqs + 1) * sizeof(int32_t), as_stream(stream), A);
+    int grid_log = 0;
+    while ((1 << grid_log) < kReleaseBlocks && ((int64_t)kReleaseThreads << grid_log) < most) ++grid_log;
+    const size_t lds = ((size_t)seqs + 1) * sizeof(int64_t) + (size_t)seqs * sizeof(int32_t);
+    hipLaunchKernelGGL(release_pages_kernel, dim3(1 << grid_log), dim3(kReleaseThreads), lds, as_stream(stream), A, grid_log);
     G4_LAUNCHED("release_pages_kernel");
     return G4_OK;
 }

@@ -446,7 +446,7 @@ def plan_chunk(free, cached, rows, page_table, q_start, kv_len, free_left, serve
 
 def release_pages(free, page_table, first, last, count_out, stream=None):
     """g4_release_pages: entries first[s] .. last[s] - 1 (int32 [seqs]) of every sequence's row of page_table back to the
-    free pages; count_out int32 [1] is the new count."""
+    free pages, but for absent ones; count_out int32 [1] is the new count."""
     device = _device()
     _need_device(free, device, "the free pages")
     at, seqs, width, stride = _table(page_table, device)

@@ -193,7 +193,8 @@ int g4_plan_chunk(const g4_free_pages *list, const int32_t *cached, const int32_
 /*
  * Pages back to the free list: entries first[s] .. last[s] - 1 of every sequence's row of page_table (clamped to
  * [0, table_pages]; a finished request's all, or those that a window has left behind) are appended to the free pages, by
- * sequence, then by position; count_out is the new count. Entries that would pass the list's capacity are dropped.
+ * sequence, then by position; count_out is the new count. Absent entries, outside [0, num_pages), are left out, and
+ * pages that would pass the list's capacity dropped.
  * page_table stays as it is: its user no longer counts these pages as held. An entry must not be released
  * twice, nor one that two sequences share. count_out must not be the list's count. At most 4096 sequences.
  */

@@ -495,6 +495,7 @@ struct Expand {
                                            int64_t row) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
         f4 acc[4] = {f4{}, f4{}, f4{}, f4{}};
+        float back = 1.0f;
         if (rank > 0) {
             float v[kSteps][kRanks];
             float top = 0.0f;
@@ -518,7 +519,7 @@ struct Expand {
             int up = 141 - (int)(__float_as_uint(top) >> 23);
             up = min(max(up, -120), 120);
             const float to = __uint_as_float((uint32_t)(127 + up) << 23);
-            scale *= __uint_as_float((uint32_t)(127 - up) << 23);
+            back = __uint_as_float((uint32_t)(127 - up) << 23);
             const int units = A.max_rank / 8;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
@@ -554,7 +555,7 @@ struct Expand {
             if (A.base) raw[p].values(A.base_kind, A.vec, A.base_scale, y);
             if (rank > 0) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] += scale * acc[2 * p + e / 4][e % 4];
+                for (int e = 0; e < 8; ++e) y[e] += scale * (acc[2 * p + e / 4][e % 4] * back);  // (scale * back may be out of range)
             }
             store8(A.out, A.out_kind, row * A.out_stride + out, left, A.vec, y, A.out_scale);
         }

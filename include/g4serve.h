@@ -171,8 +171,10 @@ typedef struct g4_free_pages {
 /*
  * The plan of a chunk from the requests' lengths: the arrays of g4_chunk, the pages of the new positions, and where
  * each row goes. Sequence s has c = cached[s] positions (clamped to [0, max_kv]) and asks for n = rows[s] new ones
- * (clamped to [0, min(max_q, max_kv - c)]). It holds held[s] pages, the first entries of its row of page_table (held
- * NULL: those that c positions need), and needs max(0, ceil((c + n) / page_size) - held[s]) more where n > 0.
+ * (clamped to [0, min(max_q, max_kv - c)]). held[s] entries of its row of page_table have been given, from the first on
+ * (held NULL: those that c positions need), and it needs max(0, ceil((c + n) / page_size) - held[s]) more where n > 0, which
+ * go behind them. Entry p / page_size is position p's whatever went back in the meantime: pages that a window has left
+ * behind stay counted in held, and only a request that ended has its held set back.
  * Sequences are served in order, while their rows fit into `tokens` and their pages into the free ones: from the first
  * that does not fit on, all get no rows and no pages in this chunk. served: how many fit.
  * The pages given are the last ones of the free list, in the list's order: by sequence, then by position.
@@ -192,11 +194,13 @@ int g4_plan_chunk(const g4_free_pages *list, const int32_t *cached, const int32_
 
 /*
  * Pages back to the free list: entries first[s] .. last[s] - 1 of every sequence's row of page_table (clamped to
- * [0, table_pages]; a finished request's all, or those that a window has left behind) are appended to the free pages, by
- * sequence, then by position; count_out is the new count. Absent entries, outside [0, num_pages), are left out, and
- * pages that would pass the list's capacity dropped.
- * page_table stays as it is: its user no longer counts these pages as held. An entry must not be released
- * twice, nor one that two sequences share. count_out must not be the list's count. At most 4096 sequences.
+ * [0, table_pages]) are appended to the free pages, by sequence, then by position; count_out is the new count. Absent
+ * entries, outside [0, num_pages), are left out, and pages that would pass the list's capacity dropped.
+ * page_table and held stay as they are. An entry must not be released twice, nor one that two sequences share, nor one behind
+ * held[s], where an earlier request's may still stand. So the user keeps, a request, the entry that the next release begins at:
+ * 0 at first; a window that no later row reaches behind position p gives back up to p / page_size, which is the next first;
+ * a finished request gives back up to held[s], and both are 0 again.
+ * count_out must not be the list's count, which is the one that the plan or release before has left. At most 4096 sequences.
  */
 int g4_release_pages(const g4_free_pages *list, const int32_t *page_table, int table_pages, int64_t table_stride,
                      const int32_t *first, const int32_t *last, int seqs, int32_t *count_out, void *stream);

@@ -1,4 +1,4 @@
-"""Release of pages with absent entries among them."""
+"""Pages that come and go: absent entries among released ones, and windows that move between plans."""
 import numpy as np
 import pytest
 
@@ -81,6 +81,60 @@ def test_rows_of_very_different_lengths(gpu):
     table[::3, ::5] = -1
     last = np.where(np.arange(600) % 200 == 77, 1700, r.integers(0, 3, 600))
     check_release(table, np.zeros(600), last, np.full(1 << 20, -1, np.int32), 0, 1 << 20)
+
+
+def test_a_moving_window(gpu):
+    """Pages go back from behind a window while requests grow, and the rest when they finish. held counts the entries that
+    a row was ever given, whatever went back from its front, so the next page goes behind the last; what went back is
+    the program's own count, and the next release begins there. Every page is held once or free once at all times."""
+    r = np.random.default_rng(4)
+    seqs, page, width, total, window = 5, 8, 40, 60, 40
+    free, table = dev(r.permutation(total).astype(np.int32)), dev(np.full((seqs, width), -1, np.int32))
+    counts = [dev(np.array([total], np.int32)), dev(np.zeros(1, np.int32))]
+    lists = [gs.FreePages(free, c, total, page) for c in counts]
+    held = [dev(np.zeros(seqs, np.int32)) for _ in range(2)]
+    z = lambda n: dev(np.zeros(n, np.int32))
+    q_start, kv_len, served, slots = z(seqs + 1), z(seqs), z(1), z(64)
+    lens, gone, now = np.zeros(seqs, np.int32), np.zeros(seqs, np.int32), 0
+    content = {}  # what a slot holds: (request's number, position)
+    number = list(range(seqs))
+    finished = 0
+    for step in range(60):
+        rows = np.where(lens == 0, r.integers(1, 13, seqs), r.integers(0, 9, seqs)).astype(np.int32)
+        rows = np.minimum(rows, page * width - lens)
+        h = step % 2
+        gs.plan_chunk(lists[now], dev(lens), dev(rows), table, q_start, kv_len, counts[1 - now], served, tokens=64, max_q=16,
+                      max_kv=page * width, held=held[h], held_out=held[1 - h], row_slot=slots)
+        now = 1 - now
+        g4.synchronize()
+        start, new, have, t = q_start.download(), kv_len.download(), held[1 - h].download(), table.download()
+        at = slots.download()
+        assert served.download()[0] == seqs
+        for s in range(seqs):
+            for i, p in enumerate(range(lens[s], new[s])):
+                assert at[start[s] + i] == t[s, p // page] * page + p % page
+                content[int(at[start[s] + i])] = (number[s], p)
+            # what the window sees of the request, from its earliest row of the next chunk, is still its own
+            for p in range(max(0, new[s] - window), new[s]):
+                assert content[int(t[s, p // page]) * page + p % page] == (number[s], p), (step, s, p)
+        lens = new
+        done = (lens > 100) & (r.random(seqs) < 0.3) | (lens > page * width - 20)
+        last = np.where(done, have, np.maximum(lens - window, 0) // page).astype(np.int32)
+        assert (gone <= last).all() and (have >= -(-lens // page)).all()
+        gs.release_pages(lists[now], table, dev(gone), dev(last), counts[1 - now])
+        now = 1 - now
+        g4.synchronize()
+        gone = np.where(done, 0, last).astype(np.int32)
+        have = np.where(done, 0, have).astype(np.int32)
+        held[1 - h].upload(have)
+        left = int(counts[now].download()[0])
+        mine = [int(p) for s in range(seqs) for p in t[s, gone[s]:have[s]]]
+        assert sorted(mine + [int(p) for p in free.download()[:left]]) == list(range(total)), step
+        lens = np.where(done, 0, lens).astype(np.int32)
+        for s in np.nonzero(done)[0]:
+            number[s] += seqs
+            finished += 1
+    assert finished > 3
 
 
 def test_release_replayed(gpu):

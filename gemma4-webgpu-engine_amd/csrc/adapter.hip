@@ -810,6 +810,8 @@ int g4_adapter_linear(const g4_adapters *adapters, const void *groups, size_t gr
     if (!workspace || workspace_bytes < need)
         return set_error(G4_ERR_INVALID, "adapter-linear: workspace %zu B < %zu B", workspace_bytes, need);
     if (out == x) return set_error(G4_ERR_INVALID, "adapter-linear: out cannot be x, which every block of a row reads");
+    if ((uintptr_t)groups < (uintptr_t)workspace + need && (uintptr_t)workspace < (uintptr_t)groups + need_groups)
+        return set_error(G4_ERR_INVALID, "adapter-linear: groups and workspace overlap");
     const int64_t tiles = max_tiles(tokens, D->count);
     AdapterArgs A{};
     A.a = static_cast<const _Float16 *>(D->a);

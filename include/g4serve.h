@@ -240,7 +240,7 @@ size_t g4_adapter_groups_bytes(int tokens, int adapters);
  * groups: of g4_adapter_groups, for the same tokens and number of adapters (of others: nothing is written).
  * x A^T is made of exact products, added up in f32, and enters the second product with 23 bits, relative to its row's
  * largest value; that product's sums are f32 too.
- * workspace: g4_adapter_workspace_bytes(...) bytes, 16-byte aligned.
+ * workspace: g4_adapter_workspace_bytes(...) bytes, 16-byte aligned, apart from groups, which are read throughout.
  */
 int g4_adapter_linear(const g4_adapters *adapters, const void *groups, size_t groups_bytes, int tokens, const void *x,
                       int x_kind, int64_t x_stride, float x_scale, const void *base, int base_kind, int64_t base_stride,

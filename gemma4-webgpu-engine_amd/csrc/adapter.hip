@@ -14,8 +14,10 @@
 // us, and 20.4).
 //
 // Bound, of one launch: a chain of loads (tile, rows, x and A, B beside them), the product, the stores: 6.6 us for a row of
-// K 1536, N 2048, rank 16; of two: the first reads x and A once a pair of tiles, a CU its 0.4 MB in 10.2 us of that case, the
-// second reads base and writes, 19 MB in 10.9 us, most of it the chain's.
+// K 1536, N 2048, rank 16. Of two, at those 2048 rows: the first takes 10.2 us by its waits, 56% of its waves' cycles (the
+// matrix units are busy for 4%, LDS for 9%, and a CU's 0.4 MB would come in 3 us): header, tile and rows one after the other,
+// then chunks of 48 KB, two on their way at a time; the second reads base and writes, 19 MB in 11 us, most of it the
+// chain's.
 #include "g4_internal.h"
 #include "../../include/g4serve.h"
 
@@ -681,7 +683,10 @@ __global__ __launch_bounds__(kAdThreads) void adapter_expand_kernel(AdapterArgs 
     E.finish(A, T, h, b_lds, rank, scale, row);
 }
 
-// How a call is run: in one launch (splits 0), or with H's parts of `splits` ranges of K.
+// How a call is run: in one launch (splits 0), or with H's parts of `splits` ranges of K. By the most tiles that the rows can
+// make of the pool's adapters: how many they make is known on the device only. Rows of few adapters of a large pool pay for
+// it: 512 rows of 4, K 6144, N 1536, rank 64 take 15.1 us of a pool of 4, 17.0 of 64, 26.3 of 256 or more (one range of K);
+// 2048 rows 24.5, 24.4, 30.8; 64 rows of 16, K 1536, N 6144, rank 32 8.9 us of 16, 11.1 of 64 or more (two launches).
 static int adapter_splits(const g4_adapters *D, int tokens, int x_size) {
     const int64_t tiles = max_tiles(tokens, D->count), blocks = tiles * ((D->n + kBlockN - 1) / kBlockN);
     const int64_t ranks = (D->max_rank + 15) / 16, room = ranks > 2 ? 4 : ranks;  // by 16, and what a kernel has of them
